@@ -25,6 +25,8 @@
  *   5. The seven templates: embedded gfx950 code objects, launcher-owned
  *      geometry and one entry point per template (the symbols and memref
  *      argument lists of lib/dsl/kernels/<name>.cpp).
+ *   8. Sequence caches: the operators of a decoder's serving step over a
+ *      paged cache of keys and values. No counterpart in the reference.
  */
 #ifndef KHRT_H
 #define KHRT_H
@@ -372,6 +374,157 @@ KHRT_API int khrt_bench_metric(const char *formula, const double *args, int narg
  * counts as the triad (three streams of n floats). The rows' rate column is
  * work * 1000 / ms / 1e9. */
 KHRT_API int khrt_bench_row_work(const char *kernel, const char *shape, double *work, int *is_flops);
+
+/* ---- 8. Sequence caches -------------------------------------------------- */
+/* A serving step of a decoder over a paged cache: write the new tokens' keys
+ * and values (kh_qk_norm_rope), attend over the cache (kh_paged_attention), add
+ * up the attention that each entry received (kh_paged_weights), and keep only
+ * the entries that received most (kh_paged_evict). All are asynchronous on
+ * `stream`, allocate nothing, take device pointers, and may be captured into a
+ * graph; what a captured graph uses (workspaces included) is its own until it
+ * has been replayed.
+ *
+ * Element types: fp32, fp16 and bf16; products, sums, norms and softmax
+ * statistics are in 32 bits. head_dim is a multiple of 8 up to 256. Rows of
+ * head_dim elements are contiguous; pointers to them are 16-byte aligned and
+ * strides (in elements) multiples of 16 bytes. Anything else the host can see
+ * is refused with KHRT_E_INVALID before any device work.
+ *
+ * What lies in device memory is brought into range by the kernels: a length is
+ * clamped to what its table row can hold, a start to [0, tokens], and an entry
+ * whose page number is not in [0, pages) is one that nobody sees and nobody
+ * writes. */
+#define KHRT_F32 0
+#define KHRT_F16 1
+#define KHRT_BF16 2
+
+/* Keys and values of `pages` pages of `page_size` entries. Head h of the entry
+ * in slot t of page p starts at k + p k_page_stride + t k_slot_stride +
+ * h k_head_stride (v alike): [pages, page_size, kv_heads, head_dim],
+ * [pages, kv_heads, page_size, head_dim] and interleaved layouts are all
+ * strides. Offsets are 64 bits wide. */
+typedef struct kh_paged_cache {
+  void *k, *v;
+  int64_t k_page_stride, k_slot_stride, k_head_stride;
+  int64_t v_page_stride, v_slot_stride, v_head_stride;
+  int64_t pages, page_size, kv_heads, head_dim;
+  int32_t dtype;
+} kh_paged_cache;
+
+/* Entry j of sequence s lies in slot j % page_size of page
+ * pages[s row_stride + j / page_size]; the sequence has lens[s] entries.
+ * Sequences may share pages that a call only reads. max_len: the longest
+ * length the caller expects, 0 if unknown (the whole row); it sizes the launch
+ * and changes no result but its rounding. */
+typedef struct kh_page_table {
+  const int32_t *pages, *lens;
+  int64_t row_stride, seqs, width, max_len;
+} kh_page_table;
+
+/* Rows of q[tokens, q_heads, head_dim] and k[tokens, kv_heads, head_dim] are
+ * divided by sqrt(mean square + eps) and multiplied by the weights (norm != 0;
+ * null weights are ones), then the pairs (i, i + rotary_dim/2), or (2i, 2i + 1)
+ * where interleaved, i < rotary_dim/2, are rotated by positions[t]
+ * inv_freq[i] (formed in 64 bits). Tokens are q_stride, k_stride, v_stride
+ * elements apart, so q, k and v may be parts of one projection's output.
+ * q_out may be q and k_out k (in place, the same strides). k_out may be null
+ * where there is a cache. cache.k null: no cache, and v, slots are not used.
+ * With a cache the rotated k and v itself go to its slot slots[t] =
+ * page * page_size + slot; a token whose slot is not in the cache (-1 for
+ * padding) writes nothing there. Two tokens with the same slot: either's rows,
+ * in part. kv_heads, head_dim and dtype are the cache's fields (set also where
+ * there is none). rotary_dim is a multiple of 8, 0 to head_dim. */
+typedef struct kh_qk_norm_rope_args {
+  const void *q, *k, *v;
+  void *q_out, *k_out;
+  const void *q_gamma, *k_gamma; /* [head_dim], of the rows' type */
+  const float *inv_freq;         /* [rotary_dim / 2] */
+  const int64_t *positions;      /* [tokens] */
+  const int64_t *slots;          /* [tokens] */
+  int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+  kh_paged_cache cache;
+  int64_t tokens, q_heads, rotary_dim;
+  int32_t interleaved, norm;
+  float eps;
+} kh_qk_norm_rope_args;
+KHRT_API int kh_qk_norm_rope(const kh_qk_norm_rope_args *args, void *stream);
+
+/* out[t, h] = sum_j softmax_j(scale q[t, h] . k_j) v_j for the new tokens of
+ * ragged sequences: those of sequence s are tokens q_starts[s] ..
+ * q_starts[s + 1] - 1 of q[tokens, q_heads, head_dim], and its last entries in
+ * the cache. A token sees the entries up to its own, with window > 0 the last
+ * `window` of them. Head h reads kv head h / (q_heads / kv_heads). lse[t, h]
+ * (fp32, may be null) is the natural log of the sum of exponentials. A token
+ * that sees nothing (an empty cache, a sequence with fewer entries than new
+ * tokens, absent pages) gives zeros and -inf; tokens outside every sequence are
+ * left as they were. Infinities and NaN in entries that a token does not see
+ * do not reach it. out must not be q.
+ *
+ * workspace (16-byte aligned, may be null): with it a long sequence is split
+ * over several workgroups. More than
+ * kh_paged_attention_workspace reports is not used, less means fewer splits.
+ * Its contents need no preparation; calls that overlap in time need one
+ * each. */
+typedef struct kh_paged_attention_args {
+  kh_paged_cache cache;
+  kh_page_table table;
+  const void *q;
+  void *out;
+  float *lse;
+  const int32_t *q_starts; /* [seqs + 1] */
+  int64_t q_stride, out_stride;
+  int64_t tokens, q_heads, window;
+  float scale;
+} kh_paged_attention_args;
+KHRT_API int kh_paged_attention_workspace(const kh_paged_attention_args *args, size_t *bytes);
+KHRT_API int kh_paged_attention(const kh_paged_attention_args *args, void *workspace, size_t workspace_bytes,
+                                void *stream);
+
+/* weights[s, h, j] = (entry j is not one of the new tokens ? weights_in[s, h, j] : 0)
+ *   + sum over the new tokens that see it and the query heads of kv head h
+ *     of exp(scale q . k_j - lse)
+ * for j < lens[s]; behind that the row is left as it was. lse is the attention's
+ * of the same tokens (-inf: adds nothing). weights_in null: zeros; it may be
+ * weights itself. Both have the strides given, at least lens[s] floats a row.
+ * The order of the sums is fixed: a repeated call gives the same bits. */
+typedef struct kh_paged_weights_args {
+  kh_paged_cache cache;
+  kh_page_table table;
+  const void *q;
+  const float *lse;
+  const int32_t *q_starts;
+  int64_t q_stride;
+  const float *weights_in;
+  float *weights;
+  int64_t weights_seq_stride, weights_head_stride;
+  int64_t tokens, q_heads, window;
+  float scale;
+} kh_paged_weights_args;
+KHRT_API int kh_paged_weights(const kh_paged_weights_args *args, void *stream);
+
+/* For each sequence and kv head: of n = lens[s] > budget entries the `recent`
+ * newest and the budget - recent others of largest weight (equal weights: the
+ * lowest index first; NaN above all) are kept, in order; with n <= budget all
+ * are. Entry i of those goes to entry i of the table kept_pages[seqs,
+ * kept_width] over the same cache, its weight to weights[s, h, i], and
+ * kept_lens[s] = min(n, budget). The caller's to see to: pages of kept_pages are
+ * in it once, and no sequence of the call reads them (the source's pages may be
+ * shared, and can be freed afterwards). The arrays written must not be those
+ * read. workspace: kh_paged_evict_workspace bytes, 16-byte aligned. */
+typedef struct kh_paged_evict_args {
+  kh_paged_cache cache;
+  kh_page_table table;
+  const int32_t *kept_pages;
+  int64_t kept_row_stride, kept_width;
+  int32_t *kept_lens;
+  const float *weights_in;
+  int64_t in_seq_stride, in_head_stride;
+  float *weights;
+  int64_t seq_stride, head_stride;
+  int64_t budget, recent;
+} kh_paged_evict_args;
+KHRT_API int kh_paged_evict_workspace(const kh_paged_evict_args *args, size_t *bytes);
+KHRT_API int kh_paged_evict(const kh_paged_evict_args *args, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

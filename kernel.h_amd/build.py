@@ -49,16 +49,21 @@ OBJ = os.path.join(BUILD, "obj")
 # tune cache names it, and `kernelh tune` evaluates them through the runtime.
 TUNE_PARTS = 4
 VARIANTS = {f"gemm_tune{p}": ("gemm_tune", [f"-DKH_GEMM_TUNE_PART={p}"]) for p in range(TUNE_PARTS)}
+# Sequence-cache operators: csrc/kernels/<base>.hip once per element type
+# (KH_ELEM of kh_elem.h). paged_evict moves bytes and needs one build.
+ELEMENTS = {"f32": 0, "f16": 1, "bf16": 2}
+TYPED = ["qk_norm_rope", "paged_attention", "paged_weights"]
+VARIANTS |= {f"{b}_{t}": (b, [f"-DKH_ELEM={e}"]) for b in TYPED for t, e in ELEMENTS.items()}
 # Product code objects embedded in libkhrt.so (order = kh_embed.S order).
 PRODUCT = ["vecadd", "fused_gelu", "softmax", "layernorm", "scan", "gemm", "attention", "util", "roofline",
-           *VARIANTS]
+           "paged_evict", *VARIANTS]
 # Test fixtures, built here so that no GPU run compiles anything:
 #   tests/fixtures/<name>.hip -> co/<name>.hsaco, loaded by tests through
 #     khrt_module_load_data (never embedded in the runtime);
 #   tests/cpp/<name>.cpp -> build/<name>, C++ programs over include/khrt.hpp
 #     and over the reference-side Backend binding.
 TDIR = os.path.join(REPO, "tests")
-PROBES = ["mfma_probe"]
+PROBES = ["mfma_probe", "mfma16_probe"]
 #   csrc/kernels/<base>.hip with test-only defines -> co/<name>.hsaco, also
 #     loaded by tests only: scan with a short bounded wait, so that a test can
 #     make its give-up paths run (every kernel still exits normally).

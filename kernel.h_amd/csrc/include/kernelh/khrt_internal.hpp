@@ -31,6 +31,12 @@ int current_device();
 int verified_launch(void *function, khrt_dim3 grid, khrt_dim3 block, size_t shared, void *stream,
                     void **params, size_t nparams);
 
+// Launches `symbol` (a string that lives as long as the process: it is
+// compared by address) of the embedded code object `co` on the current device,
+// verified on its first launch and by its grid alone after that.
+int launch_embedded(const char *co, const char *symbol, khrt_dim3 grid, khrt_dim3 block, void *stream, void **params,
+                    size_t nparams);
+
 // Packs memref descriptors into 8-byte slots (LaunchArgs::add_memref).
 class LaunchArgs {
  public:

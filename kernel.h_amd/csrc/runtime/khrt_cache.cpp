@@ -1,0 +1,351 @@
+// The sequence-cache operators behind the C-ABI (khrt.h, group 8): the checks
+// of what the host can see, the launch geometry, and the kernels' parameters.
+#include "kernelh/khrt_internal.hpp"
+#include "kh_paged.h"
+#include "kh_tiles.h"
+
+#include <algorithm>
+#include <cmath>
+#include <exception>
+#include <string>
+
+namespace {
+
+int bad(const char *op, const std::string &what) { return khrt::fail(KHRT_E_INVALID, std::string(op) + ": " + what); }
+
+// Nothing thrown below leaves a C entry point.
+template <class Call>
+int guarded(const char *op, Call &&call) {
+  try {
+    return call();
+  } catch (const std::exception &e) {
+    try {
+      return bad(op, e.what());
+    } catch (...) {
+      return KHRT_E_INVALID;
+    }
+  } catch (...) {
+    return KHRT_E_INVALID;
+  }
+}
+
+constexpr int64_t kMaxPageSize = int64_t(1) << 20;
+constexpr int64_t kMaxStride = int64_t(1) << 40;   // of tables and weights
+constexpr int64_t kMaxSpan = int64_t(1) << 59;     // elements that a stride covers: three such offsets fit 64 bits in bytes
+constexpr int64_t kMaxRows = int64_t(1) << 30;     // tokens x heads
+constexpr int64_t kMaxPairs = int64_t(1) << 20;    // sequences x kv heads
+constexpr int64_t kCapacity = (int64_t(1) << 31) - (int64_t(1) << 16);  // entries of a sequence
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int element_bytes(int32_t dtype) { return dtype == KHRT_F32 ? 4 : 2; }
+
+bool aligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// A stride over `extent` rows: not negative, 16 bytes' worth, and for rows that
+// are written (least > 0) no shorter than the row where there is a next one.
+bool stride_ok(int64_t stride, int64_t extent, int element, int64_t least) {
+  if (extent <= 1) return stride >= 0 && stride <= kMaxSpan;
+  return stride >= least && stride <= kMaxSpan / extent && stride % (16 / element) == 0;
+}
+
+// The fields that describe rows, of a cache that may have none.
+int check_rows(const char *op, const kh_paged_cache &c) {
+  if (c.dtype != KHRT_F32 && c.dtype != KHRT_F16 && c.dtype != KHRT_BF16)
+    return bad(op, "dtype must be KHRT_F32, KHRT_F16 or KHRT_BF16 (got " + std::to_string(c.dtype) + ")");
+  if (c.head_dim <= 0 || c.head_dim > 256 || c.head_dim % 8 != 0)
+    return bad(op, "head_dim must be a multiple of 8 up to 256 (got " + std::to_string(c.head_dim) + ")");
+  if (c.kv_heads <= 0 || c.kv_heads > 65535) return bad(op, "kv_heads must be in [1, 65535]");
+  return 0;
+}
+
+int check_cache(const char *op, const kh_paged_cache &c, bool written) {
+  if (int rc = check_rows(op, c)) return rc;
+  if (c.k == nullptr || c.v == nullptr) return bad(op, "null cache");
+  if (c.pages <= 0 || c.pages > INT32_MAX) return bad(op, "pages must be in [1, 2^31)");
+  if (c.page_size <= 0 || c.page_size > kMaxPageSize) return bad(op, "page_size must be in [1, 2^20]");
+  const int e = element_bytes(c.dtype);
+  const int64_t least = written ? c.head_dim : 0;
+  for (const bool is_v : {false, true}) {
+    if (!aligned(is_v ? c.v : c.k)) return bad(op, "the cache must be 16-byte aligned");
+    if (!stride_ok(is_v ? c.v_page_stride : c.k_page_stride, c.pages, e, least) ||
+        !stride_ok(is_v ? c.v_slot_stride : c.k_slot_stride, c.page_size, e, least) ||
+        !stride_ok(is_v ? c.v_head_stride : c.k_head_stride, c.kv_heads, e, least))
+      return bad(op, written ? "cache strides must be multiples of 16 bytes and hold a row"
+                             : "cache strides must be multiples of 16 bytes, not negative");
+  }
+  return 0;
+}
+
+int check_table(const char *op, const kh_page_table &t, const kh_paged_cache &c) {
+  if (t.pages == nullptr || t.lens == nullptr) return bad(op, "null page table");
+  if (t.seqs <= 0 || t.width <= 0 || t.width > INT32_MAX) return bad(op, "seqs and width must be positive");
+  if (t.row_stride < 0 || t.row_stride > kMaxStride) return bad(op, "the table's row stride must not be negative");
+  if (t.seqs > kMaxPairs || t.seqs * c.kv_heads > kMaxPairs) return bad(op, "more than 2^20 pairs of sequence and kv head");
+  if (t.max_len < 0) return bad(op, "max_len must not be negative");
+  return 0;
+}
+
+KhCache device_cache(const kh_paged_cache &c) {
+  return KhCache{c.k, c.v, c.k_page_stride, c.k_slot_stride, c.k_head_stride, c.v_page_stride, c.v_slot_stride,
+                 c.v_head_stride, static_cast<int32_t>(c.pages), static_cast<int32_t>(c.page_size),
+                 static_cast<int32_t>(c.kv_heads), static_cast<int32_t>(c.head_dim),
+                 kh_div_by(static_cast<uint32_t>(c.page_size))};
+}
+
+int64_t capacity_of(int64_t width, int64_t page_size) { return std::min(width * page_size, kCapacity); }
+
+KhTable device_table(const kh_page_table &t, const kh_paged_cache &c) {
+  return KhTable{t.pages, t.lens, t.row_stride, static_cast<int32_t>(t.seqs), static_cast<int32_t>(t.width),
+                 static_cast<int32_t>(capacity_of(t.width, c.page_size))};
+}
+
+// The longest sequence that a launch is sized for.
+int64_t expected_len(const kh_page_table &t, const kh_paged_cache &c) {
+  const int64_t all = capacity_of(t.width, c.page_size);
+  return t.max_len > 0 ? std::min(t.max_len, all) : all;
+}
+
+int check_tokens(const char *op, int64_t tokens, int64_t q_heads, const kh_paged_cache &c) {
+  if (tokens <= 0 || q_heads <= 0) return bad(op, "tokens and q_heads must be positive");
+  if (tokens > kMaxRows || q_heads > 65535 || tokens * (q_heads + 2 * c.kv_heads) > kMaxRows)
+    return bad(op, "more than 2^30 rows");
+  return 0;
+}
+
+int check_queries(const char *op, const void *q, int64_t q_stride, int64_t tokens, int64_t q_heads, int64_t window,
+                  float scale, const kh_paged_cache &c) {
+  if (int rc = check_tokens(op, tokens, q_heads, c)) return rc;
+  if (q_heads % c.kv_heads != 0) return bad(op, "q_heads must be a multiple of kv_heads");
+  if (!aligned(q)) return bad(op, "q must be 16-byte aligned");
+  if (!stride_ok(q_stride, tokens, element_bytes(c.dtype), 0)) return bad(op, "q_stride must be a multiple of 16 bytes, not negative");
+  if (window < 0 || window > INT32_MAX) return bad(op, "window must be in [0, 2^31)");
+  if (!std::isfinite(scale)) return bad(op, "scale must be finite");
+  return 0;
+}
+
+// Code objects and symbols by element type.
+struct Symbol {
+  const char *co, *name;
+};
+#define KH_BY_TYPE(base, suffix)                                                              \
+  {                                                                                           \
+    {#base "_f32", #base suffix "_f32"}, {#base "_f16", #base suffix "_f16"}, {#base "_bf16", #base suffix "_bf16"} \
+  }
+const Symbol kRope[3][3] = {KH_BY_TYPE(qk_norm_rope, "_8"), KH_BY_TYPE(qk_norm_rope, "_16"),
+                            KH_BY_TYPE(qk_norm_rope, "_32")};
+const Symbol kAttention[3][3] = {KH_BY_TYPE(paged_attention, "_64"), KH_BY_TYPE(paged_attention, "_128"),
+                                 KH_BY_TYPE(paged_attention, "_256")};
+const Symbol kJoin[3] = KH_BY_TYPE(paged_attention, "_join");
+const Symbol kWeights[3][3] = {KH_BY_TYPE(paged_weights, "_64"), KH_BY_TYPE(paged_weights, "_128"),
+                               KH_BY_TYPE(paged_weights, "_256")};
+const Symbol kChoose = {"paged_evict", "paged_evict_choose"};
+const Symbol kMove = {"paged_evict", "paged_evict_move"};
+
+// Which of the kernels' widths holds head_dim: 64, 128 or 256.
+int width_of(int64_t head_dim) { return head_dim <= 64 ? 0 : head_dim <= 128 ? 1 : 2; }
+
+template <class Params>
+int launch(const Symbol &s, int64_t x, int64_t y, unsigned threads, Params &p, void *stream) {
+  void *params[] = {&p};
+  return khrt::launch_embedded(s.co, s.name, khrt_dim3{static_cast<unsigned>(x), static_cast<unsigned>(y), 1},
+                               khrt_dim3{threads, 1, 1}, stream, params, 1);
+}
+
+int check_attention(const char *op, const kh_paged_attention_args &a) {
+  if (int rc = check_cache(op, a.cache, false)) return rc;
+  if (int rc = check_table(op, a.table, a.cache)) return rc;
+  if (!a.q || !a.out || !a.q_starts) return bad(op, "null buffer");
+  if (int rc = check_queries(op, a.q, a.q_stride, a.tokens, a.q_heads, a.window, a.scale, a.cache)) return rc;
+  if (!aligned(a.out)) return bad(op, "out must be 16-byte aligned");
+  if (!stride_ok(a.out_stride, a.tokens, element_bytes(a.cache.dtype), a.q_heads * a.cache.head_dim))
+    return bad(op, "out_stride must be a multiple of 16 bytes and hold a token");
+  if (a.out == a.q) return bad(op, "out must not be q");
+  return 0;
+}
+
+// How a launch of paged_attention spreads over the chip.
+struct AttentionPlan {
+  int64_t row_tiles, splits, split_keys;
+  size_t bytes;  // of workspace that the splits take
+};
+
+AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_bytes) {
+  AttentionPlan p;
+  const int64_t group = a.q_heads / a.cache.kv_heads, pairs = a.table.seqs * a.cache.kv_heads;
+  p.row_tiles = std::min<int64_t>(ceil_div(ceil_div(a.tokens, a.table.seqs) * group, 16), 65535);
+  int64_t len = expected_len(a.table, a.cache);
+  // With a window nobody looks further back than the window and the new tokens.
+  if (a.window > 0) len = std::min(len, a.window + a.tokens);
+  const int64_t rows = a.tokens * a.q_heads;
+  const size_t per_split = static_cast<size_t>(rows) * (2 + static_cast<size_t>(a.cache.head_dim)) * sizeof(float);
+  int64_t splits = std::min(ceil_div(4 * KH_GEMM_CUS, pairs * p.row_tiles), ceil_div(len, 256));
+  splits = std::min<int64_t>(splits, static_cast<int64_t>(workspace_bytes / per_split));
+  p.splits = std::max<int64_t>(splits, 1);
+  p.split_keys = std::max<int64_t>(ceil_div(ceil_div(len, p.splits), 128) * 128, 128);
+  p.splits = std::min(p.splits, ceil_div(len, p.split_keys));
+  p.bytes = p.splits > 1 ? static_cast<size_t>(p.splits) * per_split : 0;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kh_qk_norm_rope(const kh_qk_norm_rope_args *args, void *stream) {
+  const char *op = "qk_norm_rope";
+  return guarded(op, [&] {
+    if (args == nullptr) return bad(op, "null arguments");
+    const kh_qk_norm_rope_args &a = *args;
+    const kh_paged_cache &c = a.cache;
+    const bool cached = c.k != nullptr;
+    if (int rc = cached ? check_cache(op, c, true) : check_rows(op, c)) return rc;
+    if (int rc = check_tokens(op, a.tokens, a.q_heads, c)) return rc;
+    if (!a.q || !a.k || !a.q_out || (!a.k_out && !cached) || (cached && (!a.v || !a.slots))) return bad(op, "null buffer");
+    if (a.rotary_dim < 0 || a.rotary_dim > c.head_dim || a.rotary_dim % 8 != 0)
+      return bad(op, "rotary_dim must be a multiple of 8 up to head_dim");
+    if (a.rotary_dim > 0 && (!a.inv_freq || !a.positions)) return bad(op, "null inv_freq or positions");
+    if (!(a.eps >= 0.0f) || !std::isfinite(a.eps)) return bad(op, "eps must be finite and not negative");
+    for (const void *p : {a.q, a.k, cached ? a.v : nullptr, static_cast<const void *>(a.q_out),
+                          static_cast<const void *>(a.k_out), a.q_gamma, a.k_gamma})
+      if (!aligned(p)) return bad(op, "buffers must be 16-byte aligned");
+    const int e = element_bytes(c.dtype);
+    const int64_t q_row = a.q_heads * c.head_dim, k_row = c.kv_heads * c.head_dim;
+    if (!stride_ok(a.q_stride, a.tokens, e, 0) || !stride_ok(a.k_stride, a.tokens, e, 0) ||
+        (cached && !stride_ok(a.v_stride, a.tokens, e, 0)))
+      return bad(op, "strides must be multiples of 16 bytes, not negative");
+    if (!stride_ok(a.q_out_stride, a.tokens, e, q_row) || (a.k_out != nullptr && !stride_ok(a.k_out_stride, a.tokens, e, k_row)))
+      return bad(op, "output strides must be multiples of 16 bytes and hold a token");
+    if ((a.q_out == a.q && a.q_out_stride != a.q_stride) || (a.k_out == a.k && a.k_out_stride != a.k_stride))
+      return bad(op, "in place, input and output strides must be the same");
+
+    const int lanes = c.head_dim <= 64 ? 8 : c.head_dim <= 128 ? 16 : 32;
+    // Heads of a token are shared out over waves until the chip has some
+    // sixteen of them to a CU.
+    const int64_t steps = ceil_div(a.q_heads + 2 * c.kv_heads, 64 / lanes);
+    const int64_t parts = std::clamp<int64_t>(ceil_div(16 * KH_GEMM_CUS, a.tokens), 1, steps);
+    KhRopeParams p{a.q, a.k, a.v, a.q_out, a.k_out, a.q_gamma, a.k_gamma, a.inv_freq, a.positions, a.slots, c.k, c.v,
+                   a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride, c.k_page_stride, c.k_slot_stride,
+                   c.k_head_stride, c.v_page_stride, c.v_slot_stride, c.v_head_stride, cached ? c.pages * c.page_size : 0,
+                   static_cast<int32_t>(c.page_size), static_cast<int32_t>(a.tokens), static_cast<int32_t>(a.q_heads),
+                   static_cast<int32_t>(c.kv_heads), static_cast<int32_t>(c.head_dim), static_cast<int32_t>(a.rotary_dim),
+                   a.interleaved != 0, a.norm != 0, static_cast<int32_t>(parts), a.eps};
+    return launch(kRope[lanes / 16][c.dtype], ceil_div(a.tokens * parts, 4), 1, 256, p, stream);
+  });
+}
+
+int kh_paged_attention_workspace(const kh_paged_attention_args *args, size_t *bytes) {
+  const char *op = "paged_attention_workspace";
+  return guarded(op, [&] {
+    if (args == nullptr || bytes == nullptr) return bad(op, "null argument");
+    if (int rc = check_attention(op, *args)) return rc;
+    *bytes = attention_plan(*args, SIZE_MAX / 2).bytes;
+    return 0;
+  });
+}
+
+int kh_paged_attention(const kh_paged_attention_args *args, void *workspace, size_t workspace_bytes, void *stream) {
+  const char *op = "paged_attention";
+  return guarded(op, [&] {
+    if (args == nullptr) return bad(op, "null arguments");
+    const kh_paged_attention_args &a = *args;
+    if (int rc = check_attention(op, a)) return rc;
+    if (!aligned(workspace)) return bad(op, "workspace must be 16-byte aligned");
+    const AttentionPlan plan = attention_plan(a, workspace != nullptr ? workspace_bytes : 0);
+    const int64_t rows = a.tokens * a.q_heads, group = a.q_heads / a.cache.kv_heads;
+    float *ml = static_cast<float *>(workspace);
+    // Joined parts are read 16 bytes at a time: they come first.
+    KhAttentionParams p{device_cache(a.cache), device_table(a.table, a.cache), a.q, a.out, a.lse, a.q_starts,
+                        ml != nullptr ? ml + plan.splits * rows * a.cache.head_dim : nullptr, ml, a.q_stride, a.out_stride,
+                        static_cast<int32_t>(a.tokens), static_cast<int32_t>(a.q_heads), static_cast<int32_t>(group),
+                        static_cast<int32_t>(a.window), static_cast<int32_t>(plan.splits),
+                        static_cast<int32_t>(plan.split_keys), kh_div_by(static_cast<uint32_t>(group)),
+                        a.scale * 1.44269504088896340736f};
+    if (int rc = launch(kAttention[width_of(a.cache.head_dim)][a.cache.dtype],
+                        a.cache.kv_heads * a.table.seqs * plan.splits, plan.row_tiles, 256, p, stream))
+      return rc;
+    if (plan.splits == 1) return 0;
+    return launch(kJoin[a.cache.dtype], ceil_div(rows, 4), 1, 256, p, stream);
+  });
+}
+
+int kh_paged_weights(const kh_paged_weights_args *args, void *stream) {
+  const char *op = "paged_weights";
+  return guarded(op, [&] {
+    if (args == nullptr) return bad(op, "null arguments");
+    const kh_paged_weights_args &a = *args;
+    if (int rc = check_cache(op, a.cache, false)) return rc;
+    if (int rc = check_table(op, a.table, a.cache)) return rc;
+    if (!a.q || !a.lse || !a.q_starts || !a.weights) return bad(op, "null buffer");
+    if (int rc = check_queries(op, a.q, a.q_stride, a.tokens, a.q_heads, a.window, a.scale, a.cache)) return rc;
+    if (a.weights_seq_stride < 0 || a.weights_head_stride < 0 || a.weights_seq_stride > kMaxStride ||
+        a.weights_head_stride > kMaxStride || (a.cache.kv_heads > 1 && a.weights_head_stride == 0) ||
+        (a.table.seqs > 1 && a.weights_seq_stride == 0))
+      return bad(op, "strides of weights must be positive");
+    const int64_t group = a.q_heads / a.cache.kv_heads;
+    KhWeightsParams p{device_cache(a.cache), device_table(a.table, a.cache), a.q, a.lse, a.q_starts, a.weights_in, a.weights,
+                      a.q_stride, a.weights_seq_stride, a.weights_head_stride, static_cast<int32_t>(a.tokens),
+                      static_cast<int32_t>(a.q_heads), static_cast<int32_t>(group), static_cast<int32_t>(a.window),
+                      kh_div_by(static_cast<uint32_t>(group)), a.scale * 1.44269504088896340736f};
+    const int64_t y = std::min<int64_t>(ceil_div(expected_len(a.table, a.cache), 128), 65535);
+    return launch(kWeights[width_of(a.cache.head_dim)][a.cache.dtype], a.cache.kv_heads * a.table.seqs, y, 256, p, stream);
+  });
+}
+
+static int check_evict(const char *op, const kh_paged_evict_args &a) {
+  if (int rc = check_cache(op, a.cache, true)) return rc;
+  if (int rc = check_table(op, a.table, a.cache)) return rc;
+  if (!a.kept_pages || !a.kept_lens || !a.weights_in || !a.weights) return bad(op, "null buffer");
+  if (a.budget <= 0 || a.budget > kCapacity) return bad(op, "budget must be positive");
+  if (a.recent < 0 || a.recent > a.budget) return bad(op, "recent must be in [0, budget]");
+  if (a.kept_width <= 0 || a.kept_width > INT32_MAX || a.kept_row_stride < 0 || a.kept_row_stride > kMaxStride ||
+      (a.table.seqs > 1 && a.kept_row_stride < a.kept_width))
+    return bad(op, "kept_width must be positive and rows of kept_pages not overlap");
+  if (a.kept_width * a.cache.page_size < a.budget) return bad(op, "kept_pages must hold budget entries");
+  if (a.kept_pages == a.table.pages || a.kept_lens == a.table.lens || a.weights == a.weights_in)
+    return bad(op, "what is written must not be what is read");
+  const int64_t pairs[][2] = {{a.in_seq_stride, a.table.seqs}, {a.in_head_stride, a.cache.kv_heads},
+                              {a.seq_stride, a.table.seqs}, {a.head_stride, a.cache.kv_heads}};
+  for (const auto &s : pairs)
+    if (s[0] < 0 || s[0] > kMaxStride) return bad(op, "strides of weights must not be negative");
+  if ((a.table.seqs > 1 && a.seq_stride < a.budget) || (a.cache.kv_heads > 1 && a.head_stride < a.budget))
+    return bad(op, "rows of weights must hold budget entries");
+  return 0;
+}
+
+static size_t evict_bytes(const kh_paged_evict_args &a) {
+  return static_cast<size_t>(a.table.seqs * a.cache.kv_heads) * static_cast<size_t>(a.budget) * sizeof(int32_t);
+}
+
+int kh_paged_evict_workspace(const kh_paged_evict_args *args, size_t *bytes) {
+  const char *op = "paged_evict_workspace";
+  return guarded(op, [&] {
+    if (args == nullptr || bytes == nullptr) return bad(op, "null argument");
+    if (int rc = check_evict(op, *args)) return rc;
+    *bytes = evict_bytes(*args);
+    return 0;
+  });
+}
+
+int kh_paged_evict(const kh_paged_evict_args *args, void *workspace, size_t workspace_bytes, void *stream) {
+  const char *op = "paged_evict";
+  return guarded(op, [&] {
+    if (args == nullptr) return bad(op, "null arguments");
+    const kh_paged_evict_args &a = *args;
+    if (int rc = check_evict(op, a)) return rc;
+    if (workspace == nullptr || workspace_bytes < evict_bytes(a))
+      return bad(op, "workspace of " + std::to_string(evict_bytes(a)) + " bytes needed");
+    if (!aligned(workspace)) return bad(op, "workspace must be 16-byte aligned");
+    KhEvictParams p{device_cache(a.cache), device_table(a.table, a.cache), a.kept_pages, a.kept_lens, a.weights_in, a.weights,
+                    static_cast<int32_t *>(workspace), a.kept_row_stride, a.in_seq_stride, a.in_head_stride, a.seq_stride,
+                    a.head_stride, static_cast<int32_t>(a.kept_width), static_cast<int32_t>(a.budget),
+                    static_cast<int32_t>(a.recent), element_bytes(a.cache.dtype)};
+    const int64_t pairs = a.cache.kv_heads * a.table.seqs;
+    if (int rc = launch(kChoose, pairs, 1, 1024, p, stream)) return rc;
+    const int64_t pieces = a.budget * (a.cache.head_dim * element_bytes(a.cache.dtype) / 16);
+    const int64_t y = std::clamp<int64_t>(ceil_div(pieces, 256 * 4), 1, std::max<int64_t>(1, 16 * KH_GEMM_CUS / pairs));
+    return launch(kMove, pairs, std::min<int64_t>(y, 65535), 256, p, stream);
+  });
+}
+
+}  // extern "C"

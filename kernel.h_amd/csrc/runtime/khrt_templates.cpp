@@ -43,6 +43,12 @@ KH_DECLARE_CO(gemm_tune0)
 KH_DECLARE_CO(gemm_tune1)
 KH_DECLARE_CO(gemm_tune2)
 KH_DECLARE_CO(gemm_tune3)
+// Sequence-cache operators, one per element type.
+#define KH_DECLARE_TYPED(name) KH_DECLARE_CO(name##_f32) KH_DECLARE_CO(name##_f16) KH_DECLARE_CO(name##_bf16)
+KH_DECLARE_TYPED(qk_norm_rope)
+KH_DECLARE_TYPED(paged_attention)
+KH_DECLARE_TYPED(paged_weights)
+KH_DECLARE_CO(paged_evict)
 static_assert(KH_GEMM_TUNE_PARTS == 4, "one code object per part of the tune list");
 
 namespace {
@@ -63,6 +69,9 @@ const CodeObject kCodeObjects[] = {
     {"gemm_tune1", kh_co_gemm_tune1, kh_co_gemm_tune1_end},
     {"gemm_tune2", kh_co_gemm_tune2, kh_co_gemm_tune2_end},
     {"gemm_tune3", kh_co_gemm_tune3, kh_co_gemm_tune3_end},
+#define KH_CO(name) {#name, kh_co_##name, kh_co_##name##_end}
+#define KH_TYPED_CO(name) KH_CO(name##_f32), KH_CO(name##_f16), KH_CO(name##_bf16)
+    KH_TYPED_CO(qk_norm_rope), KH_TYPED_CO(paged_attention), KH_TYPED_CO(paged_weights), KH_CO(paged_evict),
 };
 
 struct KernelResources {
@@ -768,6 +777,24 @@ int launch_template(Kind kind, StackArgs &args, const Dims &d, void *stream) {
 int bad(const char *what) { return khrt::fail(KHRT_E_INVALID, what); }
 
 }  // namespace
+
+int khrt::launch_embedded(const char *co, const char *symbol, khrt_dim3 grid, khrt_dim3 block, void *stream,
+                          void **params, size_t nparams) {
+  if (int rc = khrt::ensure_device()) return rc;
+  const int dev = khrt::current_device();
+  const Ready *known = find_ready(symbol, dev, block.x);
+  if (known != nullptr && grid.x <= known->max_grid[0] && grid.y <= known->max_grid[1] && grid.z <= known->max_grid[2]) {
+    return khrt_launch_raw(known->fn, grid, block, 0, stream, params);
+  }
+  Ready r{symbol, dev, block.x, nullptr, 0, {0, 0, 0}};
+  if (int rc = get_function(co, symbol, &r.fn)) return rc;
+  khrt_device_limits live;
+  if (int rc = khrt_live_limits(&live)) return rc;
+  for (int i = 0; i < 3; ++i) r.max_grid[i] = live.max_grid_dim[i];
+  if (int rc = khrt::verified_launch(r.fn, grid, block, 0, stream, params, nparams)) return rc;
+  if (known == nullptr) add_ready(r);
+  return 0;
+}
 
 extern "C" {
 

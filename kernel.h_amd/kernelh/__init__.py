@@ -100,6 +100,63 @@ class GemmCandidate(ctypes.Structure):
                 ("k_split", ctypes.c_int32), ("product", ctypes.c_int32)]
 
 
+# Element types of the sequence-cache operators.
+F32, F16, BF16 = 0, 1, 2
+
+
+class PagedCache(ctypes.Structure):
+    """kh_paged_cache: keys and values in pages. Pointers are integers; strides are in elements."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_page_stride", ctypes.c_int64), ("k_slot_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+                ("v_page_stride", ctypes.c_int64), ("v_slot_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+                ("pages", ctypes.c_int64), ("page_size", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("head_dim", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
+class PageTable(ctypes.Structure):
+    """kh_page_table: the pages and the length of each sequence."""
+    _fields_ = [("pages", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("row_stride", ctypes.c_int64),
+                ("seqs", ctypes.c_int64), ("width", ctypes.c_int64), ("max_len", ctypes.c_int64)]
+
+
+class QkNormRope(ctypes.Structure):
+    """Arguments of qk_norm_rope (kh_qk_norm_rope_args)."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+                ("q_gamma", ctypes.c_void_p), ("k_gamma", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+                ("positions", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
+                ("q_out_stride", ctypes.c_int64), ("k_out_stride", ctypes.c_int64), ("cache", PagedCache),
+                ("tokens", ctypes.c_int64), ("q_heads", ctypes.c_int64), ("rotary_dim", ctypes.c_int64),
+                ("interleaved", ctypes.c_int32), ("norm", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+class PagedAttention(ctypes.Structure):
+    """Arguments of paged_attention (kh_paged_attention_args)."""
+    _fields_ = [("cache", PagedCache), ("table", PageTable), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("lse", ctypes.c_void_p), ("q_starts", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
+                ("out_stride", ctypes.c_int64), ("tokens", ctypes.c_int64), ("q_heads", ctypes.c_int64),
+                ("window", ctypes.c_int64), ("scale", ctypes.c_float)]
+
+
+class PagedWeights(ctypes.Structure):
+    """Arguments of paged_weights (kh_paged_weights_args)."""
+    _fields_ = [("cache", PagedCache), ("table", PageTable), ("q", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("q_starts", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("weights_in", ctypes.c_void_p),
+                ("weights", ctypes.c_void_p), ("weights_seq_stride", ctypes.c_int64),
+                ("weights_head_stride", ctypes.c_int64), ("tokens", ctypes.c_int64), ("q_heads", ctypes.c_int64),
+                ("window", ctypes.c_int64), ("scale", ctypes.c_float)]
+
+
+class PagedEvict(ctypes.Structure):
+    """Arguments of paged_evict (kh_paged_evict_args)."""
+    _fields_ = [("cache", PagedCache), ("table", PageTable), ("kept_pages", ctypes.c_void_p),
+                ("kept_row_stride", ctypes.c_int64), ("kept_width", ctypes.c_int64), ("kept_lens", ctypes.c_void_p),
+                ("weights_in", ctypes.c_void_p), ("in_seq_stride", ctypes.c_int64), ("in_head_stride", ctypes.c_int64),
+                ("weights", ctypes.c_void_p), ("seq_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("budget", ctypes.c_int64), ("recent", ctypes.c_int64)]
+
+
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
@@ -173,6 +230,12 @@ SIGNATURES = {
     "kh_roofline_triad": (_i, [_vp, _vp, _vp, _i64, _vp]),
     "kh_roofline_copy": (_i, [_vp, _vp, _i64, _vp]),
     "kh_roofline_mfma": (_i, [_vp, _i64, _i64, _vp]),
+    "kh_qk_norm_rope": (_i, [ctypes.POINTER(QkNormRope), _vp]),
+    "kh_paged_attention_workspace": (_i, [ctypes.POINTER(PagedAttention), ctypes.POINTER(_sz)]),
+    "kh_paged_attention": (_i, [ctypes.POINTER(PagedAttention), _vp, _sz, _vp]),
+    "kh_paged_weights": (_i, [ctypes.POINTER(PagedWeights), _vp]),
+    "kh_paged_evict_workspace": (_i, [ctypes.POINTER(PagedEvict), ctypes.POINTER(_sz)]),
+    "kh_paged_evict": (_i, [ctypes.POINTER(PagedEvict), _vp, _sz, _vp]),
     "khrt_bench_metric": (_i, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double), _i, ctypes.POINTER(ctypes.c_double)]),
     "khrt_bench_row_work": (_i, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),
                                  ctypes.POINTER(_i)]),
@@ -622,6 +685,41 @@ def attention(Q, K, V, O, batch: int, heads: int, seq: int, head_dim: int, strea
         rc = lib.kh_attention(_ptr(Q), _ptr(K), _ptr(V), _ptr(O), batch, heads, seq, head_dim, _ptr(stream))
     if rc:
         check(rc)
+
+
+# ------------------------------------------------------------------ sequence caches
+# One structure of arguments per operator (khrt.h, group 8, says what each
+# field means); a program that repeats a call may keep its structure and change
+# fields. `args` is passed by reference; the call copies what it needs.
+
+def qk_norm_rope(args: QkNormRope, stream=None) -> None:
+    check(lib.kh_qk_norm_rope(args, _ptr(stream)))
+
+
+def paged_attention_workspace(args: PagedAttention) -> int:
+    """Bytes with which paged_attention splits these sequences as far as it pays."""
+    n = ctypes.c_size_t()
+    check(lib.kh_paged_attention_workspace(args, ctypes.byref(n)))
+    return n.value
+
+
+def paged_attention(args: PagedAttention, workspace=None, workspace_bytes: int = 0, stream=None) -> None:
+    check(lib.kh_paged_attention(args, _ptr(workspace), workspace_bytes, _ptr(stream)))
+
+
+def paged_weights(args: PagedWeights, stream=None) -> None:
+    check(lib.kh_paged_weights(args, _ptr(stream)))
+
+
+def paged_evict_workspace(args: PagedEvict) -> int:
+    """Bytes that paged_evict needs."""
+    n = ctypes.c_size_t()
+    check(lib.kh_paged_evict_workspace(args, ctypes.byref(n)))
+    return n.value
+
+
+def paged_evict(args: PagedEvict, workspace, workspace_bytes: int, stream=None) -> None:
+    check(lib.kh_paged_evict(args, _ptr(workspace), workspace_bytes, _ptr(stream)))
 
 
 def roofline_triad(a, b, c, n: int, stream=None) -> None:
