@@ -402,7 +402,7 @@ KHRT_API int khrt_bench_row_work(const char *kernel, const char *shape, double *
  * in slot t of page p starts at k + p k_page_stride + t k_slot_stride +
  * h k_head_stride (v alike): [pages, page_size, kv_heads, head_dim],
  * [pages, kv_heads, page_size, head_dim] and interleaved layouts are all
- * strides. Offsets are 64 bits wide. */
+ * strides. Each stride is below 4 GB; the cache need not be. */
 typedef struct kh_paged_cache {
   void *k, *v;
   int64_t k_page_stride, k_slot_stride, k_head_stride;

@@ -36,12 +36,13 @@ KH_HD uint32_t kh_div(uint32_t j, const KhDiv &d) {
   return d.mul == 0 ? j : static_cast<uint32_t>((static_cast<uint64_t>(j) * d.mul) >> 32) >> d.shift;
 }
 
-// A cache and the page table over it. Element e of head h of the entry in
-// slot t of page p: k + p k_page + t k_slot + h k_head + e (v alike), strides
-// in elements and 64 bits wide: a cache may pass 2^31 elements.
+// A cache and the page table over it. Byte e of head h of the entry in slot t
+// of page p: k + p k_page + t k_slot + h k_head + e (v alike). Strides are in
+// bytes and below 2^32, so that one multiply-add per stride forms the 64-bit
+// address: a cache may pass 4 GB, a page may not.
 struct KhCache {
-  const void *k, *v;
-  int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+  const char *k, *v;
+  uint32_t k_page, k_slot, k_head, v_page, v_slot, v_head;
   int32_t pages, page_size, kv_heads, head_dim;
   KhDiv by_page;
 };
@@ -65,6 +66,12 @@ KH_HD KhSlot kh_slot(const int32_t *row, int32_t width, int32_t pages, const KhD
   s.page = i < static_cast<uint32_t>(width) ? row[i] : -1;
   if (s.page >= pages) s.page = -1;
   return s;
+}
+
+// Where the row of that entry starts, past the cache's (and head's) own start.
+KH_HD uint64_t kh_row(const KhSlot &s, uint32_t page_stride, uint32_t slot_stride) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(s.page)) * page_stride +
+         static_cast<uint64_t>(static_cast<uint32_t>(s.slot)) * slot_stride;
 }
 
 // A sequence's share of a step: entries in the cache, new tokens (the last
@@ -98,27 +105,68 @@ KH_HD KhSpan kh_seen(const KhSeq &s, int32_t i, int32_t window) {
   return r;
 }
 
-// The part of a sequence's entries that workgroups share out: all that any of
-// its new tokens sees, in chunks of `split_keys`, the last of which takes
-// whatever is left past splits * split_keys.
-struct KhSplit {
-  int32_t first, end, used;
+// How paged_attention's narrow form shares out a step. A unit is 16 rows (new
+// tokens x heads of a group) of one sequence and kv head against `blocks`
+// stretches of KH_STRETCH entries, all that any of the sequence's new tokens
+// sees; `whole` makes a unit one indivisible block. The units of all
+// sequences, those of a sequence in the order of tiles and heads, follow each
+// other in one line of blocks, of which every workgroup gets an equal share:
+// however lengths differ, all workgroups are done together.
+#define KH_STRETCH 128
+#define KH_TILE_ROWS 16
+
+struct KhUnits {
+  int32_t first;   // the first entry that any new token sees
+  int32_t blocks;  // of each unit, at least 1: rows that see nothing are written too
+  int32_t tiles;   // 0 without new tokens
 };
 
-KH_HD KhSplit kh_split(const KhSeq &s, int32_t window, int32_t splits, int32_t split_keys, int32_t split) {
-  const KhSpan all = kh_seen(s, 0, window);  // the first token's window starts earliest
-  const int32_t first = all.first;
-  const int32_t keys = s.n > first ? s.n - first : 0;
-  KhSplit r;
-  r.used = keys == 0 ? 1 : (keys - 1) / split_keys + 1;
-  if (r.used > splits) r.used = splits;
-  if (split >= r.used) {
-    r.first = r.end = s.n;
-    return r;
-  }
-  r.first = first + split * split_keys;
-  r.end = split == r.used - 1 ? s.n : r.first + split_keys;
-  return r;
+KH_HD KhUnits kh_units(const KhSeq &s, int32_t group, int32_t window, int32_t whole) {
+  KhUnits u;
+  u.first = kh_seen(s, 0, window).first;  // the first token's window starts earliest
+  const int32_t keys = s.n > u.first ? s.n - u.first : 0;
+  u.blocks = whole != 0 || keys == 0 ? 1 : (keys - 1) / KH_STRETCH + 1;
+  u.tiles = s.m == 0 ? 0 : (s.m * group - 1) / KH_TILE_ROWS + 1;
+  return u;
+}
+
+// Blocks of a sequence. The launcher sees to it that all sequences' together
+// stay below 2^30 (it makes units whole where they might not).
+KH_HD int32_t kh_work(const KhUnits &u, int32_t kv_heads) { return u.tiles * kv_heads * u.blocks; }
+
+// The share of each of at most `most` workgroups: `each` blocks, one more for the
+// first `longer` of them. Every one of them gets a block at least, so that each
+// part of a unit is one that somebody wrote.
+struct KhShares {
+  int32_t groups, each, longer;
+};
+
+// Of the two workgroups a CU can hold, one does better where each would get a
+// single block, and where shares are long (its loads alone fill the memory's
+// queues): MI355X, bf16 heads of 128, one workgroup against two, 64 x 4096
+// entries 183 us / 193, 1 x 131071 104 / 110, 8 x 1024 16.4 / 18.5; the other way
+// 128 x 512 66 / 59, 32 sequences of up to 2000 56 / 45.
+#define KH_CUS 256
+KH_HD int32_t kh_most(int32_t work, int32_t groups) {
+  return (work <= 2 * KH_CUS || work >= 32 * KH_CUS) && groups > KH_CUS ? KH_CUS : groups;
+}
+
+KH_HD KhShares kh_shares(int32_t work, int32_t most) {
+  KhShares s;
+  s.groups = work < most ? work : most;
+  s.each = s.groups > 0 ? static_cast<int32_t>(static_cast<uint32_t>(work) / static_cast<uint32_t>(s.groups)) : 0;
+  s.longer = work - s.each * s.groups;
+  return s;
+}
+
+// Where workgroup g's share starts.
+KH_HD int32_t kh_share(const KhShares &s, int32_t g) { return g * s.each + (g < s.longer ? g : s.longer); }
+
+// The workgroup whose share holds block x.
+KH_HD int32_t kh_owner(const KhShares &s, int32_t x) {
+  const int32_t long_ones = s.longer * (s.each + 1);
+  return x < long_ones ? static_cast<int32_t>(static_cast<uint32_t>(x) / static_cast<uint32_t>(s.each + 1))
+                       : s.longer + static_cast<int32_t>(static_cast<uint32_t>(x - long_ones) / static_cast<uint32_t>(s.each));
 }
 
 // qk_norm_rope.hip
@@ -145,9 +193,12 @@ struct KhAttentionParams {
   void *out;
   float *lse;  // may be null
   const int32_t *q_starts;
-  float *part_ml, *part_o;  // splits > 1: [splits][tokens q_heads][2] and [..][head_dim]
+  // Parts of units that several workgroups work on: [groups][2][rows][head_dim]
+  // and, behind them, [groups][2][rows][2] (maximum, sum). Slot 0 is of the
+  // unit in which a workgroup's share starts, slot 1 of the one it ends in.
+  float *part_o, *part_ml;
   int64_t q_stride, out_stride;
-  int32_t tokens, q_heads, group, window, splits, split_keys;
+  int32_t tokens, q_heads, group, window, groups, whole;
   KhDiv by_group;
   float scale_log2;
 };

@@ -137,7 +137,7 @@ extern "C" __global__ void __launch_bounds__(256) paged_evict_move(const KhEvict
   const int32_t *table = p.table.pages + seq * p.table.row_stride;
   const int32_t *kept_table = p.kept_pages + seq * p.kept_row_stride;
   const int32_t *chosen = p.chosen + (int64_t)blockIdx.x * p.budget;
-  const char *k = static_cast<const char *>(p.cache.k), *v = static_cast<const char *>(p.cache.v);
+  const char *k = p.cache.k + (uint64_t)head * p.cache.k_head, *v = p.cache.v + (uint64_t)head * p.cache.v_head;
   const int pieces = p.cache.head_dim * p.element / 16;
   const int64_t all = (int64_t)kept * pieces;
   for (int64_t at = (int64_t)blockIdx.y * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.y * 256) {
@@ -145,10 +145,9 @@ extern "C" __global__ void __launch_bounds__(256) paged_evict_move(const KhEvict
     const KhSlot a = kh_slot(table, p.table.width, p.cache.pages, p.cache.by_page, (uint32_t)chosen[row]);
     const KhSlot b = kh_slot(kept_table, p.kept_width, p.cache.pages, p.cache.by_page, (uint32_t)row);
     if (a.page < 0 || b.page < 0) continue;
-    const int64_t e = p.element, off = 16 * piece;
-    const float4 x = *reinterpret_cast<const float4 *>(k + (a.page * p.cache.k_page + a.slot * p.cache.k_slot + head * p.cache.k_head) * e + off);
-    const float4 y = *reinterpret_cast<const float4 *>(v + (a.page * p.cache.v_page + a.slot * p.cache.v_slot + head * p.cache.v_head) * e + off);
-    *reinterpret_cast<float4 *>(const_cast<char *>(k) + (b.page * p.cache.k_page + b.slot * p.cache.k_slot + head * p.cache.k_head) * e + off) = x;
-    *reinterpret_cast<float4 *>(const_cast<char *>(v) + (b.page * p.cache.v_page + b.slot * p.cache.v_slot + head * p.cache.v_head) * e + off) = y;
+    const float4 x = *reinterpret_cast<const float4 *>(k + kh_row(a, p.cache.k_page, p.cache.k_slot) + 16 * piece);
+    const float4 y = *reinterpret_cast<const float4 *>(v + kh_row(a, p.cache.v_page, p.cache.v_slot) + 16 * piece);
+    *reinterpret_cast<float4 *>(const_cast<char *>(k) + kh_row(b, p.cache.k_page, p.cache.k_slot) + 16 * piece) = x;
+    *reinterpret_cast<float4 *>(const_cast<char *>(v) + kh_row(b, p.cache.v_page, p.cache.v_slot) + 16 * piece) = y;
   }
 }

@@ -32,7 +32,7 @@ __device__ __forceinline__ void weights(const KhWeightsParams &p) {
   const int head = (int)(blockIdx.x % (uint32_t)p.cache.kv_heads), seq = (int)(blockIdx.x / (uint32_t)p.cache.kv_heads);
   const KhSeq s = kh_seq(p.table.lens[seq], p.q_starts[seq], p.q_starts[seq + 1], p.table.capacity, p.tokens);
   const int32_t *table = p.table.pages + seq * p.table.row_stride;
-  const elem *kbase = static_cast<const elem *>(p.cache.k) + head * p.cache.k_head;
+  const char *kbase = p.cache.k + (uint64_t)head * p.cache.k_head;
   const int64_t row = seq * p.seq_stride + head * p.head_stride;
   const int rows = s.m * p.group;
 
@@ -46,12 +46,12 @@ __device__ __forceinline__ void weights(const KhWeightsParams &p) {
       KhSlot at{-1, 0};
       if (key < s.n) at = kh_slot(table, p.table.width, p.cache.pages, p.cache.by_page, (uint32_t)key);
       there[b] = at.page >= 0;
-      const elem *kp = kbase + at.page * p.cache.k_page + at.slot * p.cache.k_slot;
+      const char *kp = kbase + kh_row(at, p.cache.k_page, p.cache.k_slot);
 #pragma unroll
       for (int c = 0; c < kSteps; ++c) {
         k[b][c] = u32x4{0, 0, 0, 0};
         if (there[b] && 64 * c + 16 * h < row_bytes)
-          k[b][c] = *reinterpret_cast<const u32x4 *>(kp + (64 * c + 16 * h) / (int)sizeof(elem));
+          k[b][c] = *reinterpret_cast<const u32x4 *>(kp + 64 * c + 16 * h);
       }
     }
     // The first token that sees any of these entries is the one whose own

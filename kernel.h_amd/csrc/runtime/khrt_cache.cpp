@@ -31,7 +31,8 @@ int guarded(const char *op, Call &&call) {
 
 constexpr int64_t kMaxPageSize = int64_t(1) << 20;
 constexpr int64_t kMaxStride = int64_t(1) << 40;   // of tables and weights
-constexpr int64_t kMaxSpan = int64_t(1) << 59;     // elements that a stride covers: three such offsets fit 64 bits in bytes
+constexpr int64_t kMaxSpan = int64_t(1) << 59;     // elements that the strides of q, k, v and out cover
+constexpr int64_t kMaxCacheStride = int64_t(1) << 32;  // bytes, exclusive (kh_paged.h)
 constexpr int64_t kMaxRows = int64_t(1) << 30;     // tokens x heads
 constexpr int64_t kMaxPairs = int64_t(1) << 20;    // sequences x kv heads
 constexpr int64_t kCapacity = (int64_t(1) << 31) - (int64_t(1) << 16);  // entries of a sequence
@@ -68,6 +69,9 @@ int check_cache(const char *op, const kh_paged_cache &c, bool written) {
   const int64_t least = written ? c.head_dim : 0;
   for (const bool is_v : {false, true}) {
     if (!aligned(is_v ? c.v : c.k)) return bad(op, "the cache must be 16-byte aligned");
+    for (const int64_t s : {is_v ? c.v_page_stride : c.k_page_stride, is_v ? c.v_slot_stride : c.k_slot_stride,
+                            is_v ? c.v_head_stride : c.k_head_stride})
+      if (s >= kMaxCacheStride / e) return bad(op, "cache strides must be below 2^32 bytes");
     if (!stride_ok(is_v ? c.v_page_stride : c.k_page_stride, c.pages, e, least) ||
         !stride_ok(is_v ? c.v_slot_stride : c.k_slot_stride, c.page_size, e, least) ||
         !stride_ok(is_v ? c.v_head_stride : c.k_head_stride, c.kv_heads, e, least))
@@ -87,8 +91,11 @@ int check_table(const char *op, const kh_page_table &t, const kh_paged_cache &c)
 }
 
 KhCache device_cache(const kh_paged_cache &c) {
-  return KhCache{c.k, c.v, c.k_page_stride, c.k_slot_stride, c.k_head_stride, c.v_page_stride, c.v_slot_stride,
-                 c.v_head_stride, static_cast<int32_t>(c.pages), static_cast<int32_t>(c.page_size),
+  const int e = element_bytes(c.dtype);
+  auto bytes = [e](int64_t stride) { return static_cast<uint32_t>(stride * e); };
+  return KhCache{static_cast<const char *>(c.k), static_cast<const char *>(c.v), bytes(c.k_page_stride),
+                 bytes(c.k_slot_stride), bytes(c.k_head_stride), bytes(c.v_page_stride), bytes(c.v_slot_stride),
+                 bytes(c.v_head_stride), static_cast<int32_t>(c.pages), static_cast<int32_t>(c.page_size),
                  static_cast<int32_t>(c.kv_heads), static_cast<int32_t>(c.head_dim),
                  kh_div_by(static_cast<uint32_t>(c.page_size))};
 }
@@ -164,27 +171,33 @@ int check_attention(const char *op, const kh_paged_attention_args &a) {
   return 0;
 }
 
-// How a launch of paged_attention spreads over the chip.
+// How a launch of paged_attention spreads over the chip (kh_paged.h, KhUnits).
 struct AttentionPlan {
-  int64_t row_tiles, splits, split_keys;
-  size_t bytes;  // of workspace that the splits take
+  int64_t groups;  // workgroups
+  bool whole;      // units are not split
+  size_t bytes;    // of workspace that their parts take
 };
 
 AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_bytes) {
   AttentionPlan p;
-  const int64_t group = a.q_heads / a.cache.kv_heads, pairs = a.table.seqs * a.cache.kv_heads;
-  p.row_tiles = std::min<int64_t>(ceil_div(ceil_div(a.tokens, a.table.seqs) * group, 16), 65535);
+  const int64_t group = a.q_heads / a.cache.kv_heads;
   int64_t len = expected_len(a.table, a.cache);
   // With a window nobody looks further back than the window and the new tokens.
   if (a.window > 0) len = std::min(len, a.window + a.tokens);
-  const int64_t rows = a.tokens * a.q_heads;
-  const size_t per_split = static_cast<size_t>(rows) * (2 + static_cast<size_t>(a.cache.head_dim)) * sizeof(float);
-  int64_t splits = std::min(ceil_div(4 * KH_GEMM_CUS, pairs * p.row_tiles), ceil_div(len, 256));
-  splits = std::min<int64_t>(splits, static_cast<int64_t>(workspace_bytes / per_split));
-  p.splits = std::max<int64_t>(splits, 1);
-  p.split_keys = std::max<int64_t>(ceil_div(ceil_div(len, p.splits), 128) * 128, 128);
-  p.splits = std::min(p.splits, ceil_div(len, p.split_keys));
-  p.bytes = p.splits > 1 ? static_cast<size_t>(p.splits) * per_split : 0;
+  // At most so many units, of at most so many blocks each.
+  const int64_t units = (a.tokens * group / KH_TILE_ROWS + std::min(a.tokens, a.table.seqs)) * a.cache.kv_heads;
+  const int64_t blocks = ceil_div(len, KH_STRETCH);
+  // As many workgroups as are on the chip at once.
+  const int64_t most = (a.cache.head_dim > 128 ? 1 : 2) * KH_GEMM_CUS;
+  const size_t per_group = size_t(2) * KH_TILE_ROWS * (2 + static_cast<size_t>(a.cache.head_dim)) * sizeof(float);
+  p.groups = std::min<int64_t>(most, std::max(ceil_div(units * blocks, 2), std::min(units, most)));
+  p.groups = std::min(p.groups, static_cast<int64_t>(workspace_bytes / per_group));
+  // The kernels count blocks in 32 bits, with what lengths beyond the expected
+  // ones may add: the whole row of the table.
+  const int64_t most_blocks = units * ceil_div(capacity_of(a.table.width, a.cache.page_size), KH_STRETCH);
+  p.whole = blocks == 1 || p.groups < KH_GEMM_CUS / 4 || most_blocks >= 1 << 30;
+  if (p.whole) p.groups = std::min(units, most);
+  p.bytes = p.whole ? 0 : static_cast<size_t>(p.groups) * per_group;
   return p;
 }
 
@@ -252,20 +265,16 @@ int kh_paged_attention(const kh_paged_attention_args *args, void *workspace, siz
     if (int rc = check_attention(op, a)) return rc;
     if (!aligned(workspace)) return bad(op, "workspace must be 16-byte aligned");
     const AttentionPlan plan = attention_plan(a, workspace != nullptr ? workspace_bytes : 0);
-    const int64_t rows = a.tokens * a.q_heads, group = a.q_heads / a.cache.kv_heads;
-    float *ml = static_cast<float *>(workspace);
-    // Joined parts are read 16 bytes at a time: they come first.
-    KhAttentionParams p{device_cache(a.cache), device_table(a.table, a.cache), a.q, a.out, a.lse, a.q_starts,
-                        ml != nullptr ? ml + plan.splits * rows * a.cache.head_dim : nullptr, ml, a.q_stride, a.out_stride,
-                        static_cast<int32_t>(a.tokens), static_cast<int32_t>(a.q_heads), static_cast<int32_t>(group),
-                        static_cast<int32_t>(a.window), static_cast<int32_t>(plan.splits),
-                        static_cast<int32_t>(plan.split_keys), kh_div_by(static_cast<uint32_t>(group)),
-                        a.scale * 1.44269504088896340736f};
-    if (int rc = launch(kAttention[width_of(a.cache.head_dim)][a.cache.dtype],
-                        a.cache.kv_heads * a.table.seqs * plan.splits, plan.row_tiles, 256, p, stream))
-      return rc;
-    if (plan.splits == 1) return 0;
-    return launch(kJoin[a.cache.dtype], ceil_div(rows, 4), 1, 256, p, stream);
+    const int64_t group = a.q_heads / a.cache.kv_heads;
+    float *part = plan.whole ? nullptr : static_cast<float *>(workspace);
+    KhAttentionParams p{device_cache(a.cache), device_table(a.table, a.cache), a.q, a.out, a.lse, a.q_starts, part,
+                        part != nullptr ? part + plan.groups * 2 * KH_TILE_ROWS * a.cache.head_dim : nullptr, a.q_stride,
+                        a.out_stride, static_cast<int32_t>(a.tokens), static_cast<int32_t>(a.q_heads),
+                        static_cast<int32_t>(group), static_cast<int32_t>(a.window), static_cast<int32_t>(plan.groups),
+                        plan.whole, kh_div_by(static_cast<uint32_t>(group)), a.scale * 1.44269504088896340736f};
+    if (int rc = launch(kAttention[width_of(a.cache.head_dim)][a.cache.dtype], plan.groups, 1, 256, p, stream)) return rc;
+    if (plan.whole) return 0;
+    return launch(kJoin[a.cache.dtype], a.tokens * a.q_heads, 1, 256, p, stream);
   });
 }
 

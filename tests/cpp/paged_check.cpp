@@ -73,33 +73,35 @@ int main() {
             expect((j >= r.first && j < r.end) == sees, "what a token sees", n, m, i);
           }
         }
-        // The splits cover all that any token sees once, in order.
-        for (int splits : {1, 2, 5})
-          for (int keys : {1, 4, 16}) {
-            int used = 0, next = -1;
-            for (int k = 0; k < splits; ++k) {
-              const KhSplit p = kh_split(s, w, splits, keys, k);
-              if (k == 0) used = p.used, next = m > 0 ? (kh_seen(s, 0, w).first < n ? kh_seen(s, 0, w).first : n) : p.first;
-              expect(p.used == used && used >= 1 && used <= splits, "how many splits are used", n, m, k);
-              if (k >= used) {
-                expect(p.first == p.end, "an unused split is empty", n, m, k);
-              } else {
-                expect(p.first == next || (n == 0 && p.first == p.end), "splits follow each other", n, m, k);
-                expect(p.first <= p.end || p.first >= n, "a split is not turned round", n, m, k);
-                next = p.end;
-              }
-            }
-            expect(next == n || next >= n, "the splits reach the end", n, m, next);
-          }
+        // The units' blocks cover all that any token sees.
+        for (int whole : {0, 1}) {
+          const KhUnits u = kh_units(s, 3, w, whole);
+          expect(u.tiles == (m * 3 + 15) / 16 && u.blocks >= 1 && (whole == 0 || u.blocks == 1), "units", n, m, w);
+          int first = n;
+          for (int i = 0; i < m; ++i) first = kh_seen(s, i, w).first < first ? kh_seen(s, i, w).first : first;
+          if (m > 0) expect(u.first <= first && (whole != 0 || u.first + u.blocks * KH_STRETCH >= n), "they cover", n, m, w);
+        }
       }
   // Near the top of the range nothing overflows (this file is built with -fsanitize=undefined).
   const int32_t big = INT32_MAX - 65536;
   const KhSeq s{big, 5, 0};
-  for (int w : {0, 1, big, INT32_MAX})
-    for (int k : {0, 1, 100, 127}) {
-      const KhSplit p = kh_split(s, w, 128, (big / 128 + 128) / 128 * 128, k);
-      expect(p.first >= 0 && p.first <= p.end && p.end <= big, "a long sequence's split", w, k, p.first);
-      expect(kh_seen(s, 4, w).end == big, "the last token's own entry");
+  for (int w : {0, 1, big, INT32_MAX}) {
+    const KhUnits u = kh_units(s, 7, w, 0);
+    expect(u.first >= 0 && u.first + int64_t(u.blocks) * KH_STRETCH >= big, "a long sequence's blocks", w, u.first);
+    expect(kh_seen(s, 4, w).end == big, "the last token's own entry");
+  }
+
+  // Shares follow each other, differ by a block at most, and know their owner.
+  for (int work : {0, 1, 2, 7, 511, 512, 513, 100000, (1 << 30) - 1})
+    for (int most : {1, 2, 3, 64, 511, 512, 4095}) {
+      const KhShares s = kh_shares(work, most);
+      expect(s.groups <= most && s.groups <= work && (work == 0 || s.groups >= 1), "workgroups with a share", work, most);
+      expect(kh_share(s, 0) == 0 && kh_share(s, s.groups) == work, "shares cover all", work, most);
+      for (int g = 0; g < s.groups; ++g) {
+        const int a = kh_share(s, g), b = kh_share(s, g + 1);
+        expect(b > a && b - a <= work / s.groups + 1, "a share", work, most, g);
+        expect(kh_owner(s, a) == g && kh_owner(s, b - 1) == g && kh_owner(s, a + (b - a) / 2) == g, "its owner", work, most, g);
+      }
     }
   std::printf("paged_check ok\n");
   return 0;

@@ -64,7 +64,8 @@ BAD_ROWS = [dict(dtype=3), dict(dtype=-1), dict(head_dim=0), dict(head_dim=60), 
 BAD_CACHE = BAD_ROWS + [
     dict(k=None), dict(v=None), dict(pages=0), dict(pages=1 << 31), dict(page_size=0), dict(page_size=(1 << 20) + 1),
     dict(k=(1 << 20) + 8), dict(v=(1 << 20) + 2), dict(k_page_stride=-64), dict(v_slot_stride=-8),
-    dict(k_head_stride=60), dict(v_page_stride=2049), dict(k_slot_stride=1 << 60), dict(k_page_stride=1 << 56)]
+    dict(k_head_stride=60), dict(v_page_stride=2049), dict(k_slot_stride=1 << 60), dict(k_page_stride=1 << 56),
+    dict(v_page_stride=1 << 31)]
 BAD_WRITTEN = [dict(k_page_stride=0), dict(v_slot_stride=56), dict(k_head_stride=8)]
 BAD_TABLE = [dict(pages=None), dict(lens=None), dict(seqs=0), dict(seqs=-1), dict(width=0), dict(width=1 << 31),
              dict(row_stride=-1), dict(seqs=1 << 20), dict(max_len=-1)]
@@ -160,12 +161,11 @@ def test_null_arguments():
 
 
 def test_workspace_of_attention():
-    """Nothing where there is enough to do without splitting; with one long
-    sequence, parts of fp32 rows and their two statistics."""
+    """Nothing where no sequence is long enough to be shared out; otherwise two
+    parts of 16 fp32 rows and their statistics for each workgroup."""
     assert kh.paged_attention_workspace(attention(table=table(seqs=4096, width=4), tokens=4096)) == 0
-    long = attention(table=table(seqs=1, width=8192), tokens=1)
-    n = kh.paged_attention_workspace(long)
-    assert n > 0 and n % (4 * (64 + 2) * 4) == 0
+    n = kh.paged_attention_workspace(attention(table=table(seqs=1, width=8192), tokens=1))
+    assert n > 0 and n % (2 * 16 * (64 + 2) * 4) == 0
     assert kh.paged_attention_workspace(attention(table=table(seqs=1, width=8192), tokens=1, window=100)) == 0
 
 
