@@ -93,6 +93,33 @@ __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 acc) {
 #endif
 }
 
+// The same over 32 bytes of 32 rows and 32 columns: lane l holds bytes
+// 16 (l / 32) .. + 15 of row, respectively column, l % 32. The result's column is
+// l % 32, its rows 8 (i / 4) + 4 (l / 32) + i % 4.
+__device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 acc) {
+#if KH_ELEM == 0
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), acc, 0, 0, 0);
+  return acc;
+#elif KH_ELEM == 1
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), acc, 0, 0, 0);
+#else
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), acc, 0, 0, 0);
+#endif
+}
+
+#if KH_ELEM != 0
+// Of 4 x 16 elements in LDS that the 16 lanes of a row point at (lane 4 r + c:
+// row r, columns 4 c ..), lane i receives column i, its four rows in order
+// (ds_read_b64_tr_b16).
+__device__ __forceinline__ u32x2 read_across(const char *p) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4 *)const_cast<char *>(p)));
+}
+#endif
+
 }  // namespace kh
 
 #define KH_PASTE2(a, b) a##_##b

@@ -169,6 +169,30 @@ KH_HD int32_t kh_owner(const KhShares &s, int32_t x) {
                        : s.longer + static_cast<int32_t>(static_cast<uint32_t>(x - long_ones) / static_cast<uint32_t>(s.each));
 }
 
+// The wide form: units of KH_WIDE_ROWS rows of a sequence of more than
+// narrow_rows rows and a kv head, each with the entries that its own rows see,
+// in up to `splits` parts of whole tiles where units are few.
+#define KH_WIDE_ROWS 128
+
+KH_HD int32_t kh_wide_tiles(const KhSeq &s, int32_t group) { return s.m == 0 ? 0 : (s.m * group - 1) / KH_WIDE_ROWS + 1; }
+
+struct KhPart {
+  int32_t first, end, used;
+};
+
+// Part `split` of entries [first, end): at least 256 entries each but for the
+// last, whole tiles of 64.
+KH_HD KhPart kh_part(int32_t first, int32_t end, int32_t splits, int32_t split) {
+  const int32_t keys = end > first ? end - first : 0;
+  KhPart r;
+  int32_t each = (keys - 1) / splits / 64 * 64 + 64;
+  if (keys == 0 || each < 256) each = 256;
+  r.used = keys == 0 ? 1 : (keys - 1) / each + 1;
+  r.first = split < r.used ? first + split * each : end;
+  r.end = split < r.used - 1 ? r.first + each : end;
+  return r;
+}
+
 // qk_norm_rope.hip
 struct KhRopeParams {
   const void *q, *k, *v;
@@ -197,8 +221,12 @@ struct KhAttentionParams {
   // and, behind them, [groups][2][rows][2] (maximum, sum). Slot 0 is of the
   // unit in which a workgroup's share starts, slot 1 of the one it ends in.
   float *part_o, *part_ml;
+  // Parts of the wide units' rows: [wide_splits][tokens q_heads][head_dim] and [..][2].
+  float *wide_o, *wide_ml;
   int64_t q_stride, out_stride;
   int32_t tokens, q_heads, group, window, groups, whole;
+  int32_t narrow_rows;  // a sequence of more rows is the wide form's
+  int32_t wide_blocks, wide_splits;
   KhDiv by_group;
   float scale_log2;
 };

@@ -34,14 +34,15 @@
 //
 // Rows of V that no row of the tile sees (past the sequence's end, in pages
 // that do not exist) count as zeros. Where some rows of the tile see an entry
-// and others do not, 0 x V must be 0 also for infinities and NaN in V: see
-// poison().
+// and others do not, infinities and NaN in V are kept out of the products and
+// added to the rows that do see them.
 #include "kh_elem.h"
 #include "kh_paged.h"
 
 namespace {
 
 using kh::elem;
+using kh::f32x16;
 using kh::f32x4;
 using kh::u32x2;
 using kh::u32x4;
@@ -74,26 +75,7 @@ struct Piece {
   uint32_t w[Form<D>::mine][Form<D>::words];
 };
 
-// Which elements of w are of a kind: ones (of the elements' type) in their places.
-// kind 0: NaN, 1: +infinity, 2: -infinity.
-__device__ __forceinline__ uint32_t marks(uint32_t w, int kind) {
-#if KH_ELEM == 0
-  const uint32_t magnitude = w & 0x7fffffffu;
-  const bool hit = kind == 0 ? magnitude > 0x7f800000u : w == (kind == 1 ? 0x7f800000u : 0xff800000u);
-  return hit ? 0x3f800000u : 0u;
-#else
-  constexpr uint32_t inf = KH_ELEM == 1 ? 0x7c00u : 0x7f80u, one = KH_ELEM == 1 ? 0x3c00u : 0x3f80u;
-  uint32_t r = 0;
-#pragma unroll
-  for (int b = 0; b < 32; b += 16) {
-    const uint32_t x = w >> b & 0xffffu;
-    const bool hit = kind == 0 ? (x & 0x7fffu) > inf : x == (kind == 1 ? inf : inf | 0x8000u);
-    r |= hit ? one << b : 0u;
-  }
-  return r;
-#endif
-}
-
+// w with zeros for infinities and NaN.
 __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
 #if KH_ELEM == 0
   return kh::not_finite(w) ? 0u : w;
@@ -103,50 +85,33 @@ __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
 #endif
 }
 
-// o += (element e of this piece of V)^T P^T, p[j] for the lane's entry j;
-// KIND >= 0: of the marks of that kind instead of the values.
+// o += (element e of this piece of V)^T P^T, p[j] for the lane's entry j.
 template <int D>
-__device__ __forceinline__ f32x4 pv(const Piece<D> &v, int e, const float (&p)[Form<D>::mine], f32x4 o, int kind = -1) {
+__device__ __forceinline__ f32x4 pv(const Piece<D> &v, int e, const float (&p)[Form<D>::mine], f32x4 o) {
 #if KH_ELEM == 0
 #pragma unroll
-  for (int j = 0; j < Form<D>::mine; ++j) {
-    const uint32_t w = kind < 0 ? v.w[j][e] : marks(v.w[j][e], kind);
-    o = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w), p[j], o, 0, 0, 0);
-  }
+  for (int j = 0; j < Form<D>::mine; ++j)
+    o = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v.w[j][e]), p[j], o, 0, 0, 0);
   return o;
 #else
   u32x4 a, b;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     a[j] = __builtin_amdgcn_perm(v.w[2 * j + 1][e / 2], v.w[2 * j][e / 2], (e & 1) != 0 ? 0x07060302u : 0x05040100u);
-    if (kind >= 0) a[j] = marks(a[j], kind);
     b[j] = kh::pack2(p[2 * j], p[2 * j + 1]);
   }
   return kh::mma16(a, b, o);
 #endif
 }
 
-// Entries with infinities or NaN in V where rows differ in what they see: adds
-// to o what those elements give the rows that do see them, and takes them out
-// of v (as zeros). Products of 0/1 marks say which rows meet a NaN, +inf or -inf
-// in which column; they are exact, and only blocks at a row's limit with such a
-// value come here.
-template <int D>
-__device__ __forceinline__ void poison(Piece<D> &v, const float (&seen)[Form<D>::mine], f32x4 (&o)[Form<D>::piece]) {
-#pragma nounroll
-  for (int kind = 0; kind < 3; ++kind) {
-    const float add = kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
+// Four elements of a row of V, zeros but for infinities and NaN.
+__device__ __forceinline__ f32x4 odd_of(const char *at) {
+  float x[4];
+  kh::load4(x, reinterpret_cast<const elem *>(at));
+  f32x4 y;
 #pragma unroll
-    for (int e = 0; e < Form<D>::piece; ++e) {
-      const f32x4 met = pv<D>(v, e, seen, f32x4{0, 0, 0, 0}, kind);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[e][i] = met[i] > 0.0f ? o[e][i] + add : o[e][i];
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < Form<D>::mine; ++j)
-#pragma unroll
-    for (int w = 0; w < Form<D>::words; ++w) v.w[j][w] = without_odd(v.w[j][w]);
+  for (int i = 0; i < 4; ++i) y[i] = (__float_as_uint(x[i]) & 0x7fffffffu) >= 0x7f800000u ? x[i] : 0.0f;
+  return y;
 }
 
 // Maximum and sum over the four lanes l % 16 + 16 h: their lanes' values swap
@@ -264,33 +229,37 @@ struct Line {
   int own, upto, all;
 };
 
-// Blocks of the lane's sequence; 0 past the last.
-__device__ __forceinline__ int work_of(const KhAttentionParams &p, int seq, KhSeq &s) {
+// Blocks of the lane's sequence, or units where `wide`; 0 past the last.
+__device__ __forceinline__ int work_of(const KhAttentionParams &p, int seq, bool wide, KhSeq &s) {
   s = KhSeq{0, 0, 0};
   if (seq < p.table.seqs) s = sequence(p, seq);
-  return kh_work(kh_units(s, p.group, p.window, p.whole), p.cache.kv_heads);
+  const bool is_wide = s.m * p.group > p.narrow_rows;
+  if (is_wide != wide) return 0;
+  return wide ? kh_wide_tiles(s, p.group) * p.cache.kv_heads
+              : kh_work(kh_units(s, p.group, p.window, p.whole), p.cache.kv_heads);
 }
 
-__device__ __forceinline__ Line line_of(const KhAttentionParams &p) {
+__device__ __forceinline__ Line line_of(const KhAttentionParams &p, bool wide) {
   const int lane = kh::lane_id();
   Line l;
-  l.own = work_of(p, lane, l.s);
+  l.own = work_of(p, lane, wide, l.s);
   l.upto = up_to(l.own);
   l.all = __builtin_amdgcn_readlane(l.upto, kh::kWave - 1);
   for (int s0 = kh::kWave; s0 < p.table.seqs; s0 += kh::kWave) {
     KhSeq s;
-    l.all += __builtin_amdgcn_readlane(up_to(work_of(p, s0 + lane, s)), kh::kWave - 1);
+    l.all += __builtin_amdgcn_readlane(up_to(work_of(p, s0 + lane, wide, s)), kh::kWave - 1);
   }
   return l;
 }
 
 // The sequence that block x (less than all) is of, and the blocks before that
-// sequence.
-__device__ __forceinline__ int sequence_at(const KhAttentionParams &p, const Line &l, int x, KhSeq &s, int &before) {
+// sequence. -1 if there is none: starts that do not ascend can make the counts
+// wrap, and every walk over the sequences ends at the last one all the same.
+__device__ __forceinline__ int sequence_at(const KhAttentionParams &p, const Line &l, int x, bool wide, KhSeq &s, int &before) {
   const int lane = kh::lane_id();
   int own = l.own, upto = l.upto;
   KhSeq mine = l.s;
-  for (int s0 = 0;; s0 += kh::kWave) {
+  for (int s0 = 0; s0 < p.table.seqs; s0 += kh::kWave) {
     const uint64_t past = __builtin_amdgcn_ballot_w64(upto > x);
     if (past != 0) {
       const int first = __builtin_ctzll(past);
@@ -301,35 +270,41 @@ __device__ __forceinline__ int sequence_at(const KhAttentionParams &p, const Lin
       return s0 + first;
     }
     const int sum = __builtin_amdgcn_readlane(upto, kh::kWave - 1);
-    own = work_of(p, s0 + kh::kWave + lane, mine);
+    own = work_of(p, s0 + kh::kWave + lane, wide, mine);
     upto = sum + up_to(own);
   }
+  return -1;
 }
 
 template <int D>
-__device__ __forceinline__ void attention(const KhAttentionParams &p, float *lds) {
+__device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, float *lds) {
   using F = Form<D>;
   const int lane = kh::lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kh::kWave);
   const int r = lane & 15, h = lane >> 4;
   const int d = p.cache.head_dim, row_bytes = d * (int)sizeof(elem);
 
-  const Line line = line_of(p);
+  const Line line = line_of(p, false);
   const KhShares shares = kh_shares(line.all, kh_most(line.all, p.groups));
-  if ((int)blockIdx.x >= shares.groups) return;
-  const int start = kh_share(shares, (int)blockIdx.x), end = kh_share(shares, (int)blockIdx.x + 1);
+  if (block >= shares.groups) return;
+  const int start = kh_share(shares, block), end = kh_share(shares, block + 1);
   // The join area: each wave's maxima and sums of its rows, what each row's
   // sum is multiplied by, and each wave's part of O.
   float *ml = lds, *inv = lds + kWaves * kRows * 2, *part = inv + kRows;
   constexpr int kPitch = D + 4;
   int before;  // blocks of the sequences before this one
   KhSeq s;
-  int seq = sequence_at(p, line, start, s, before);
+  int seq = sequence_at(p, line, start, false, s, before);
+  if (seq < 0) return;
   KhUnits units = kh_units(s, p.group, p.window, p.whole);
 
   for (int at = start; at < end;) {
     while (at >= before + kh_work(units, p.cache.kv_heads)) {
       before += kh_work(units, p.cache.kv_heads);
-      s = sequence(p, ++seq);
+      // The next sequence of few rows: wide() has the others.
+      do {
+        if (++seq >= p.table.seqs) return;
+        s = sequence(p, seq);
+      } while (s.m * p.group > p.narrow_rows);
       units = kh_units(s, p.group, p.window, p.whole);
     }
     const uint32_t unit = (uint32_t)(at - before) / (uint32_t)units.blocks;
@@ -412,22 +387,20 @@ __device__ __forceinline__ void attention(const KhAttentionParams &p, float *lds
 
         // Every row sees every entry of the block: no mask.
         const bool whole = present == (F::keys == 32 ? 0xffffffffu : 0xffffu) && key0 + F::keys <= low.end && key0 >= high.first;
-        float on[F::mine];
-        bool odd = false;
+        uint32_t odds = 0;  // bit n: entry n of the block, in this lane's columns
         if (!whole) {
 #pragma unroll
           for (int j = 0; j < F::mine; ++j) {
             const int n = 16 * (j / 4) + 4 * h + j % 4, key = key0 + n;
             const bool there = (present >> n & 1) != 0;
             const bool sees = mine && key >= seen.first && key < seen.end && there;
-            on[j] = sees ? 1.0f : 0.0f;
             y[j] = sees ? y[j] : -__builtin_inff();
 #pragma unroll
             for (int a = 0; a < F::count; ++a)
 #pragma unroll
               for (int w = 0; w < F::words; ++w) {
                 v[a].w[j][w] = there ? v[a].w[j][w] : 0u;
-                odd |= kh::not_finite(v[a].w[j][w]);
+                odds |= (uint32_t)kh::not_finite(v[a].w[j][w]) << n;
               }
           }
         }
@@ -451,10 +424,37 @@ __device__ __forceinline__ void attention(const KhAttentionParams &p, float *lds
           sum += y[j];
         }
         l += sum;
-        // After the fading: an infinity does not survive a factor of zero.
-        if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+        if (__builtin_amdgcn_ballot_w64(odds != 0) != 0) {
+          // Infinities and NaN in V where rows differ in what they see: 0 x V would
+          // reach the rows that do not. They leave the products as zeros and are
+          // added, read once more, to the rows that do see them (after the
+          // fading: an infinity does not survive a factor of zero).
+          for (int n = 0; n < F::keys; ++n) {
+            if (__builtin_amdgcn_ballot_w64((odds >> n & 1) != 0) == 0) continue;
+            const int key = key0 + n;
+            const KhSlot at = kh_slot(table, p.table.width, p.cache.pages, p.cache.by_page, (uint32_t)key);
+            const char *row = vbase + kh_row(at, p.cache.v_page, p.cache.v_slot);
+            if (mine && key >= seen.first && key < seen.end) {
 #pragma unroll
-          for (int a = 0; a < F::count; ++a) poison<D>(v[a], on, o[a]);
+              for (int a = 0; a < F::count; ++a)
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4)
+#pragma unroll
+                  for (int e = 0; e < F::piece; e += 4) {
+                    const int col = a * F::span + F::piece * (4 * h + i4) + e;
+                    if (col >= d) continue;
+                    const f32x4 x = odd_of(row + col * (int)sizeof(elem));
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) o[a][e + b][i4] += x[b];
+                  }
+            }
+          }
+#pragma unroll
+          for (int a = 0; a < F::count; ++a)
+#pragma unroll
+            for (int j = 0; j < F::mine; ++j)
+#pragma unroll
+              for (int w = 0; w < F::words; ++w) v[a].w[j][w] = without_odd(v[a].w[j][w]);
         }
 #pragma unroll
         for (int a = 0; a < F::count; ++a)
@@ -490,7 +490,7 @@ __device__ __forceinline__ void attention(const KhAttentionParams &p, float *lds
       inv[r] = alone ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f;
       if (mine && alone && p.lse != nullptr) p.lse[row_of] = lse_of(top, total);
       if (!alone) {
-        float *ml_to = p.part_ml + ((int64_t)blockIdx.x * 2 + slot) * kRows * 2 + r * 2;
+        float *ml_to = p.part_ml + ((int64_t)block * 2 + slot) * kRows * 2 + r * 2;
         ml_to[0] = top;
         ml_to[1] = total;
       }
@@ -511,7 +511,7 @@ __device__ __forceinline__ void attention(const KhAttentionParams &p, float *lds
       if (alone) {
         kh::store4(static_cast<elem *>(p.out) + (int64_t)(s.start + ii) * p.out_stride + (int64_t)hh * d + col, y);
       } else {
-        float *o_to = p.part_o + (((int64_t)blockIdx.x * 2 + slot) * kRows + row) * d + col;
+        float *o_to = p.part_o + (((int64_t)block * 2 + slot) * kRows + row) * d + col;
         *reinterpret_cast<f32x4 *>(o_to) = f32x4{y[0], y[1], y[2], y[3]};
       }
     }
@@ -519,87 +519,469 @@ __device__ __forceinline__ void attention(const KhAttentionParams &p, float *lds
   }
 }
 
-// Joins the parts of units that several workgroups worked on: a workgroup per
-// row, its waves taking the parts in turn. `lds` holds kWaves x 256 + kWaves floats.
-__device__ __forceinline__ void join(const KhAttentionParams &p, float *lds) {
-  constexpr int kMost = 256;
-  const int lane = kh::lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kh::kWave);
-  const int token = (int)(blockIdx.x / (uint32_t)p.q_heads), hq = (int)(blockIdx.x % (uint32_t)p.q_heads);
-  // The token's sequence, the blocks before it and all blocks. Tokens of no
-  // sequence have no parts.
-  int work = 0, before = -1;
-  KhSeq s{0, 0, 0};
-  for (int s0 = 0; s0 < p.table.seqs; s0 += kh::kWave) {
-    KhSeq mine;
-    const int own = work_of(p, s0 + lane, mine), upto = up_to(own);
-    const uint64_t here = __builtin_amdgcn_ballot_w64(token >= mine.start && token - mine.start < mine.m);
-    if (here != 0) {
-      const int first = __builtin_ctzll(here);
-      before = work + __builtin_amdgcn_readlane(upto - own, first);
-      s.n = __builtin_amdgcn_readlane(mine.n, first);
-      s.m = __builtin_amdgcn_readlane(mine.m, first);
-      s.start = __builtin_amdgcn_readlane(mine.start, first);
-    }
-    work += __builtin_amdgcn_readlane(upto, kh::kWave - 1);
+// ---- many rows: chunks of prompts
+//
+// A workgroup takes 128 rows, 32 to a wave, of one sequence and kv head, and
+// brings tiles of K and V through LDS for all of them, a tile ahead: the next
+// tile's loads are in flight while this one is multiplied, and the one barrier
+// of a tile orders LDS alone. Per wave
+//   S^T = K Q^T     32 x 32 tiles, A = rows of K from LDS, B = Q in registers
+//   O^T += V^T P^T  B = S^T's registers as they are, A = V read across its rows
+//                   (16 bits), or row by row (32 bits, one row to a product)
+// with the running maximum and sum of row l % 32 in lanes l and l ^ 32. Rows of
+// LDS are padded so that neither kind of read meets a bank twice.
+template <int D>
+struct Wide {
+  static constexpr int bytes = D * (int)sizeof(elem);
+  static constexpr int steps = bytes / 32;
+  static constexpr int keys = bytes > 512 ? 32 : 64;  // entries of a tile
+  static constexpr int tiles = keys / 32;
+  static constexpr int dts = D / 32;
+  static constexpr int pieces = bytes / 16;             // of 16 bytes in a row
+  static constexpr int passes = keys * pieces / 256;    // pieces that a thread brings
+  static constexpr int per_pass = 256 / pieces;         // rows of a pass
+  static constexpr int k_pitch = bytes + 16, v_pitch = bytes + (kh::kWide ? 32 : 64);
+  static constexpr int buffer = keys * (k_pitch + v_pitch) + keys;  // and a byte about each entry
+  static constexpr int lds = 2 * buffer;
+};
+constexpr int kWideRows = 32;                  // of a wave
+constexpr int kWideTile = kWaves * kWideRows;  // of a workgroup
+
+// Marks of an entry in LDS.
+constexpr uint32_t kThere = 1, kOdd = 2;
+
+template <int D>
+struct Stage {
+  KhSlot at[Wide<D>::passes];
+  u32x4 k[Wide<D>::passes], v[Wide<D>::passes];
+  uint32_t there;  // bit i: the row of pass i
+};
+
+template <int D>
+__device__ __forceinline__ void seek(Stage<D> &g, const KhAttentionParams &p, const int32_t *table, int key0, int end, int tid) {
+  using W = Wide<D>;
+#pragma unroll
+  for (int i = 0; i < W::passes; ++i) {
+    const int key = key0 + i * W::per_pass + tid / W::pieces, inside = key < end ? key : end - 1;
+    const uint32_t n = kh_div((uint32_t)inside, p.cache.by_page);
+    g.at[i].slot = inside - (int)(n * p.cache.by_page.by);
+    g.at[i].page = table[n];
   }
-  if (before < 0) return;
+}
+
+template <int D>
+__device__ __forceinline__ void fetch(Stage<D> &g, const KhAttentionParams &p, const char *kbase, const char *vbase, int key0, int end,
+                                      int row_bytes, int tid) {
+  using W = Wide<D>;
+  const int off = 16 * (tid % W::pieces);
+  g.there = 0;
+#pragma unroll
+  for (int i = 0; i < W::passes; ++i) {
+    const bool there = key0 + i * W::per_pass + tid / W::pieces < end && (uint32_t)g.at[i].page < (uint32_t)p.cache.pages;
+    if (!there) g.at[i] = KhSlot{0, 0};
+    g.there |= (uint32_t)there << i;
+    const int from = off < row_bytes ? off : 0;
+    g.k[i] = *reinterpret_cast<const u32x4 *>(kbase + kh_row(g.at[i], p.cache.k_page, p.cache.k_slot) + from);
+    g.v[i] = *reinterpret_cast<const u32x4 *>(vbase + kh_row(g.at[i], p.cache.v_page, p.cache.v_slot) + from);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void put(const Stage<D> &g, char *buffer, bool check, int row_bytes, int tid) {
+  using W = Wide<D>;
+  const int off = 16 * (tid % W::pieces);
+  char *v_at = buffer + W::keys * W::k_pitch;
+  uint8_t *marks_at = reinterpret_cast<uint8_t *>(v_at + W::keys * W::v_pitch);
+#pragma unroll
+  for (int i = 0; i < W::passes; ++i) {
+    const int row = i * W::per_pass + tid / W::pieces;
+    const bool there = (g.there >> i & 1) != 0, inside = off < row_bytes;
+    const u32x4 zero = {0, 0, 0, 0}, k = there && inside ? g.k[i] : zero;
+    u32x4 v = there && inside ? g.v[i] : zero;
+    uint32_t mark = there ? kThere : 0;
+    if (check) {
+      // Rows differ in what they see of this tile: infinities and NaN of V stay
+      // out of the products, and the lane that brought the row's first piece
+      // says that it has some.
+      const bool odd = kh::not_finite(v.x) | kh::not_finite(v.y) | kh::not_finite(v.z) | kh::not_finite(v.w);
+      const uint64_t odds = __builtin_amdgcn_ballot_w64(odd);
+      const uint64_t row_lanes = W::pieces == 64 ? ~uint64_t(0) : ((uint64_t(1) << W::pieces % 64) - 1) << (tid % kh::kWave / W::pieces * W::pieces);
+      if (odds != 0) {
+        v = u32x4{without_odd(v.x), without_odd(v.y), without_odd(v.z), without_odd(v.w)};
+        mark |= (odds & row_lanes) != 0 ? kOdd : 0;
+      }
+    }
+    *reinterpret_cast<u32x4 *>(buffer + row * W::k_pitch + off) = k;
+    *reinterpret_cast<u32x4 *>(v_at + row * W::v_pitch + off) = v;
+    if (tid % W::pieces == 0) marks_at[row] = (uint8_t)mark;
+  }
+}
+
+// A operand of V^T for columns 32 dt .. and the entries that step c of tile kt's
+// scores hold (16 bits: half a tile, 32 bits: two entries).
+template <int D>
+__device__ __forceinline__ u32x4 v_across(const char *v_at, int kt, int c, int dt, int lane) {
+  using W = Wide<D>;
+  u32x4 a = {0, 0, 0, 0};
+#if KH_ELEM == 0
+  // Four products, of registers 4 c .. + 3 of the scores.
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    a[i] = *reinterpret_cast<const uint32_t *>(v_at + (32 * kt + 8 * c + 4 * (lane >> 5) + i) * W::v_pitch + (32 * dt + (lane & 31)) * 4);
+#else
+  const char *at = v_at + (32 * kt + 16 * c + 4 * (lane >> 5) + (lane & 15) / 4) * W::v_pitch +
+                   (32 * dt + 16 * (lane >> 4 & 1) + 4 * (lane & 3)) * 2;
+  const u32x2 lo = kh::read_across(at), hi = kh::read_across(at + 8 * W::v_pitch);
+  a = u32x4{lo.x, lo.y, hi.x, hi.y};
+#endif
+  return a;
+}
+
+// B operand of P^T for that step.
+__device__ __forceinline__ u32x4 p_of(const f32x16 &s, int c) {
+#if KH_ELEM == 0
+  return u32x4{__float_as_uint(s[4 * c]), __float_as_uint(s[4 * c + 1]), __float_as_uint(s[4 * c + 2]), __float_as_uint(s[4 * c + 3])};
+#else
+  return u32x4{kh::pack2(s[8 * c], s[8 * c + 1]), kh::pack2(s[8 * c + 2], s[8 * c + 3]), kh::pack2(s[8 * c + 4], s[8 * c + 5]),
+               kh::pack2(s[8 * c + 6], s[8 * c + 7])};
+#endif
+}
+constexpr int kPvSteps = kh::kWide ? 4 : 2;  // of a 32-entry tile
+
+__device__ __forceinline__ float over_halves(float v, bool maximum) {
+  const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  const float z = __uint_as_float(b.x), w = __uint_as_float(b.y);
+  return maximum ? fmaxf(z, w) : z + w;
+}
+
+// A wide unit: its rows and all entries that any of them sees. A sequence's units
+// go from its last tile on: with causal rows the longest first.
+struct WideUnit {
+  int head, tile0, tile_end, first, end;
+};
+
+__device__ __forceinline__ WideUnit wide_unit(const KhAttentionParams &p, const KhSeq &s, int in_seq) {
+  const int rows = s.m * p.group, turn = in_seq / p.cache.kv_heads;
+  WideUnit u;
+  u.head = in_seq - turn * p.cache.kv_heads;
+  u.tile0 = (kh_wide_tiles(s, p.group) - 1 - turn) * kWideTile;
+  u.tile_end = u.tile0 + kWideTile < rows ? u.tile0 + kWideTile : rows;
+  u.first = kh_seen(s, (int)kh_div(u.tile0, p.by_group), p.window).first;
+  u.end = kh_seen(s, (int)kh_div(u.tile_end - 1, p.by_group), p.window).end;
+  return u;
+}
+
+template <int D>
+__device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char *lds) {
+  using W = Wide<D>;
+  const int tid = threadIdx.x, lane = kh::lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kh::kWave);
+  const int r = lane & 31, h = lane >> 5;
+  const int d = p.cache.head_dim, row_bytes = d * (int)sizeof(elem);
+  const int split = block % p.wide_splits, unit = block / p.wide_splits;
+  KhSeq s;
+  int before;
+  const Line line = line_of(p, true);
+  if (unit >= line.all) return;
+  const int seq = sequence_at(p, line, unit, true, s, before);
+  if (seq < 0) return;
+  const WideUnit u = wide_unit(p, s, unit - before);
+  const KhPart part = kh_part(u.first, u.end, p.wide_splits, split);
+  if (split >= part.used) return;
+
+  const int rows = u.tile_end, head = u.head;
+  const int row0 = u.tile0 + wave * kWideRows, R = row0 + r;
+  const bool mine = R < rows;
+  const int i = mine ? (int)kh_div(R, p.by_group) : 0, hq = head * p.group + (mine ? R - i * p.group : 0);
+  const int last_row = row0 + kWideRows < rows ? row0 + kWideRows - 1 : rows - 1;
+  const bool any = row0 < rows;
+  const KhSpan seen = kh_seen(s, i, p.window);
+  const KhSpan low = kh_seen(s, any ? (int)kh_div(row0, p.by_group) : 0, p.window);
+  const KhSpan high = kh_seen(s, any ? (int)kh_div(last_row, p.by_group) : 0, p.window);
+  const int32_t *table = p.table.pages + seq * p.table.row_stride;
+  const char *kbase = p.cache.k + (uint64_t)head * p.cache.k_head;
+  const char *vbase = p.cache.v + (uint64_t)head * p.cache.v_head;
+
+  u32x4 q[W::steps];
+  const char *qp = static_cast<const char *>(p.q) + ((int64_t)(s.start + i) * p.q_stride + (int64_t)hq * d) * (int)sizeof(elem);
+#pragma unroll
+  for (int c = 0; c < W::steps; ++c) {
+    q[c] = u32x4{0, 0, 0, 0};
+    if (mine && 32 * c + 16 * h < row_bytes) q[c] = *reinterpret_cast<const u32x4 *>(qp + 32 * c + 16 * h);
+  }
+  float m = kNegBig, l = 0.0f;
+  f32x16 o[W::dts];
+#pragma unroll
+  for (int a = 0; a < W::dts; ++a) o[a] = f32x16{};
+
+  // Whether rows of the unit differ in what they see of the tile at key0.
+  const int all_end = kh_seen(s, (int)kh_div(u.tile0, p.by_group), p.window).end;
+  const int all_first = kh_seen(s, (int)kh_div(u.tile_end - 1, p.by_group), p.window).first;
+  auto mixed = [&](int key0) { return key0 + W::keys > all_end || key0 < all_first; };
+  if (part.first < part.end) {
+    Stage<D> g;
+    seek<D>(g, p, table, part.first, part.end, tid);
+    fetch<D>(g, p, kbase, vbase, part.first, part.end, row_bytes, tid);
+    put<D>(g, lds, mixed(part.first), row_bytes, tid);
+    seek<D>(g, p, table, part.first + W::keys, part.end, tid);
+    fetch<D>(g, p, kbase, vbase, part.first + W::keys, part.end, row_bytes, tid);
+    seek<D>(g, p, table, part.first + 2 * W::keys, part.end, tid);
+    kh::lds_barrier();
+    int cur = 0;
+    for (int key0 = part.first; key0 < part.end; key0 += W::keys, cur ^= 1) {
+      const char *k_at = lds + cur * W::buffer, *v_at = k_at + W::keys * W::k_pitch;
+      // Nothing to do for a wave none of whose rows sees any of the tile.
+      if (any && key0 < high.end && key0 + W::keys > low.first) {
+        f32x16 x[W::tiles];
+#pragma unroll
+        for (int kt = 0; kt < W::tiles; ++kt) {
+          x[kt] = f32x16{};
+#pragma unroll
+          for (int c = 0; c < W::steps; ++c)
+            x[kt] = kh::mma32(*reinterpret_cast<const u32x4 *>(k_at + (32 * kt + r) * W::k_pitch + 32 * c + 16 * h), q[c], x[kt]);
+        }
+        const uint32_t mark = lane < W::keys ? reinterpret_cast<const uint8_t *>(v_at + W::keys * W::v_pitch)[lane] : kThere;
+        const uint64_t present = __builtin_amdgcn_ballot_w64((mark & kThere) != 0);
+        const bool whole = present == ~uint64_t(0) && key0 + W::keys <= low.end && key0 >= high.first;
+        const uint64_t odds = __builtin_amdgcn_ballot_w64((mark & kOdd) != 0);
+#pragma unroll
+        for (int kt = 0; kt < W::tiles; ++kt)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[kt][j] *= p.scale_log2;
+        if (!whole) {
+#pragma unroll
+          for (int kt = 0; kt < W::tiles; ++kt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int n = 32 * kt + 8 * (j / 4) + 4 * h + j % 4, key = key0 + n;
+              const bool sees = mine && key >= seen.first && key < seen.end && (present >> n & 1) != 0;
+              x[kt][j] = sees ? x[kt][j] : -__builtin_inff();
+            }
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int kt = 0; kt < W::tiles; ++kt)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) top = fmaxf(top, x[kt][j]);
+        top = fmaxf(m, over_halves(top, true));
+        if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+          const float fade = kh::exp2_hw(m - top);
+          m = top;
+          l *= fade;
+#pragma unroll
+          for (int a = 0; a < W::dts; ++a) o[a] *= fade;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int kt = 0; kt < W::tiles; ++kt)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            x[kt][j] = kh::exp2_hw(x[kt][j] - m);
+            sum += x[kt][j];
+          }
+        l += sum;
+        // As in narrow(): what was kept out of the products.
+        for (uint64_t left = odds; left != 0; left &= left - 1) {
+          const int key = key0 + __builtin_ctzll(left);
+          const KhSlot at = kh_slot(table, p.table.width, p.cache.pages, p.cache.by_page, (uint32_t)key);
+          const char *row = vbase + kh_row(at, p.cache.v_page, p.cache.v_slot);
+          if (mine && key >= seen.first && key < seen.end) {
+#pragma unroll
+            for (int dt = 0; dt < W::dts; ++dt)
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                const int col = 32 * dt + 2 * j + 4 * h;
+                if (col >= d) continue;
+                const f32x4 y = odd_of(row + col * (int)sizeof(elem));
+#pragma unroll
+                for (int b = 0; b < 4; ++b) o[dt][j + b] += y[b];
+              }
+          }
+        }
+#pragma unroll
+        for (int kt = 0; kt < W::tiles; ++kt)
+#pragma unroll
+          for (int c = 0; c < kPvSteps; ++c) {
+            const u32x4 b = p_of(x[kt], c);
+#pragma unroll
+            for (int dt = 0; dt < W::dts; ++dt) o[dt] = kh::mma32(v_across<D>(v_at, kt, c, dt, lane), b, o[dt]);
+          }
+      }
+      put<D>(g, lds + (cur ^ 1) * W::buffer, mixed(key0 + W::keys), row_bytes, tid);
+      fetch<D>(g, p, kbase, vbase, key0 + 2 * W::keys, part.end, row_bytes, tid);
+      seek<D>(g, p, table, key0 + 3 * W::keys, part.end, tid);
+      kh::lds_barrier();
+    }
+  }
+
+  const float total = over_halves(l, false);
+  if (!mine) return;
+  const int64_t row = (int64_t)(s.start + i) * p.q_heads + hq;
+  const bool alone = part.used == 1;
+  const int64_t at_row = (int64_t)split * p.tokens * p.q_heads + row;
+  if (h == 0) {
+    if (alone) {
+      if (p.lse != nullptr) p.lse[row] = lse_of(m, total);
+    } else {
+      p.wide_ml[at_row * 2] = m;
+      p.wide_ml[at_row * 2 + 1] = total;
+    }
+  }
+  const float inv = !alone ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+  for (int dt = 0; dt < W::dts; ++dt)
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      const int col = 32 * dt + 2 * j + 4 * h;
+      if (col >= d) continue;
+      const float y[4] = {o[dt][j] * inv, o[dt][j + 1] * inv, o[dt][j + 2] * inv, o[dt][j + 3] * inv};
+      if (alone)
+        kh::store4(static_cast<elem *>(p.out) + (int64_t)(s.start + i) * p.out_stride + (int64_t)hq * d + col, y);
+      else
+        *reinterpret_cast<f32x4 *>(p.wide_o + at_row * d + col) = f32x4{y[0], y[1], y[2], y[3]};
+    }
+}
+
+// Up to 16 rows whose parts several workgroups have: row x of part k is at
+// place base(k) + x of the parts' arrays (narrow), or base(k) + the row's own
+// place among all rows (wide).
+struct Parts {
+  const float *ml, *o;
+  int64_t first, others, step;  // base of part 0, of part 1, and from there on
+  int count;
+  int R0, rows;  // the rows of the sequence that they are
+  int head;
+  bool wide;
+};
+
+// The unit that workgroup g's share starts inside of, if it is the first to do
+// so: every unit of the narrow form in parts has one such.
+__device__ __forceinline__ bool narrow_parts(const KhAttentionParams &p, int g, KhSeq &s, Parts &parts) {
+  const Line line = line_of(p, false);
+  const KhShares shares = kh_shares(line.all, kh_most(line.all, p.groups));
+  if (g == 0 || g >= shares.groups) return false;
+  const int at = kh_share(shares, g);
+  int before;
+  if (sequence_at(p, line, at, false, s, before) < 0) return false;
   const KhUnits units = kh_units(s, p.group, p.window, p.whole);
-  const int head = hq / p.group, R = (token - s.start) * p.group + hq - head * p.group, tile = R / kRows;
-  const int begin = before + (tile * p.cache.kv_heads + head) * units.blocks, end = begin + units.blocks;
-  const KhShares shares = kh_shares(work, kh_most(work, p.groups));
-  const int g0 = kh_owner(shares, begin), g1 = kh_owner(shares, end - 1);
-  if (g0 == g1) return;  // one workgroup had the whole unit
+  const int unit = (int)((uint32_t)(at - before) / (uint32_t)units.blocks);
+  const int begin = before + unit * units.blocks, end = begin + units.blocks;
+  const int g0 = kh_owner(shares, begin);
+  if (at == begin || g0 != g - 1) return false;
+  const int tile = unit / p.cache.kv_heads, rows = s.m * p.group - tile * kRows;
   // The first part ends its workgroup's share unless that began in this unit;
   // all others begin theirs.
-  const int slot0 = kh_share(shares, g0) >= begin ? 0 : 1;
-  const int64_t row = R - tile * kRows;
-  auto place = [&](int g) { return ((int64_t)g * 2 + (g == g0 ? slot0 : 0)) * kRows + row; };
-  float top = kNegBig;
-  for (int g = g0 + lane; g <= g1; g += kh::kWave) top = fmaxf(top, p.part_ml[place(g) * 2]);
-  top = kh::wave_max(top);
-  const int d = p.cache.head_dim;
-  f32x4 o = {0, 0, 0, 0};
-  float total = 0.0f;
-  const bool live = 4 * lane < d;
-#pragma unroll 4
-  for (int g = g0 + wave; g <= g1; g += kWaves) {
-    const int64_t at = place(g);
-    const float w = kh::exp2_hw(p.part_ml[at * 2] - top);
-    total += p.part_ml[at * 2 + 1] * w;
-    if (live) o += *reinterpret_cast<const f32x4 *>(p.part_o + at * d + 4 * lane) * w;
-  }
-  if (live) *reinterpret_cast<f32x4 *>(lds + wave * kMost + 4 * lane) = o;
-  float *sums = lds + kWaves * kMost;
-  if (lane == 0) sums[wave] = total;
-  kh::lds_barrier();
-  if (wave != 0) return;
-  total = sums[0];
+  const int64_t slot0 = kh_share(shares, g0) >= begin ? 0 : 1;
+  parts = Parts{p.part_ml, p.part_o, ((int64_t)g0 * 2 + slot0) * kRows, (int64_t)g * 2 * kRows, 2 * kRows,
+                kh_owner(shares, end - 1) - g0 + 1, tile * kRows, rows < kRows ? rows : kRows,
+                unit - tile * p.cache.kv_heads, false};
+  return true;
+}
+
+__device__ __forceinline__ bool wide_parts(const KhAttentionParams &p, int unit, int row0, KhSeq &s, Parts &parts) {
+  const Line line = line_of(p, true);
+  int before;
+  if (unit >= line.all || sequence_at(p, line, unit, true, s, before) < 0) return false;
+  const WideUnit u = wide_unit(p, s, unit - before);
+  const int R0 = u.tile0 + row0, rows = u.tile_end - R0, count = kh_part(u.first, u.end, p.wide_splits, 0).used;
+  if (count == 1 || rows <= 0) return false;
+  const int64_t all = (int64_t)p.tokens * p.q_heads;
+  parts = Parts{p.wide_ml, p.wide_o, 0, all, all, count, R0, rows < kRows ? rows : kRows, u.head, true};
+  return true;
+}
+
+constexpr int kJoinParts = 32;  // statistics brought to LDS at a time
+
+// Joins the parts of 16 rows: a workgroup for every workgroup's start, then one
+// for each 16 rows of the wide units. A thread has 4 columns of a row.
+template <int D>
+__device__ __forceinline__ void join(const KhAttentionParams &p, float *lds) {
+  constexpr int kItems = kRows * (D / 4) / 256;
+  const int tid = threadIdx.x, d = p.cache.head_dim;
+  const int narrow_blocks = p.whole ? 0 : p.groups, block = (int)blockIdx.x - narrow_blocks;
+  constexpr int kPer = kWideTile / kRows;
+  KhSeq s{0, 0, 0};
+  Parts parts{};
+  if (!(block < 0 ? narrow_parts(p, (int)blockIdx.x, s, parts) : wide_parts(p, block / kPer, block % kPer * kRows, s, parts))) return;
+  auto base = [&](int k) { return k == 0 ? parts.first : parts.others + (k - 1) * parts.step; };
+  auto place_of = [&](int row) {
+    if (!parts.wide) return (int64_t)row;
+    const int R = parts.R0 + row, i = (int)kh_div(R, p.by_group);
+    return (int64_t)(s.start + i) * p.q_heads + parts.head * p.group + R - i * p.group;
+  };
+  f32x4 o[kItems];
+  float m[kItems], total[kItems];
+  int64_t place[kItems];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    total += sums[w];
-    if (live) o += *reinterpret_cast<const f32x4 *>(lds + w * kMost + 4 * lane);
+  for (int j = 0; j < kItems; ++j) {
+    const int row = (tid + 256 * j) / (D / 4);
+    o[j] = f32x4{0, 0, 0, 0}, m[j] = kNegBig, total[j] = 0.0f, place[j] = place_of(row < parts.rows ? row : 0);
   }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  if (live) {
-    const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-    kh::store4(static_cast<elem *>(p.out) + (int64_t)token * p.out_stride + (int64_t)hq * d + 4 * lane, y);
+  for (int k0 = 0; k0 < parts.count; k0 += kJoinParts) {
+    const int here = parts.count - k0 < kJoinParts ? parts.count - k0 : kJoinParts;
+    for (int x = tid; x < here * kRows; x += 256) {
+      const int k = x / kRows, row = x % kRows;
+      const float *from = parts.ml + (base(k0 + k) + place_of(row < parts.rows ? row : 0)) * 2;
+      lds[2 * x] = from[0], lds[2 * x + 1] = from[1];
+    }
+    kh::lds_barrier();
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      const int row = (tid + 256 * j) / (D / 4), col = (tid + 256 * j) % (D / 4) * 4;
+      if (row >= parts.rows || col >= d) continue;
+      float top = m[j];
+      for (int k = 0; k < here; ++k) top = fmaxf(top, lds[2 * (k * kRows + row)]);
+      const float fade = kh::exp2_hw(m[j] - top);
+      m[j] = top, total[j] *= fade, o[j] *= fade;
+#pragma unroll 8
+      for (int k = 0; k < here; ++k) {
+        const float w = kh::exp2_hw(lds[2 * (k * kRows + row)] - top);
+        total[j] += lds[2 * (k * kRows + row) + 1] * w;
+        o[j] += *reinterpret_cast<const f32x4 *>(parts.o + (base(k0 + k) + place[j]) * d + col) * w;
+      }
+    }
+    kh::lds_barrier();
   }
-  if (lane == 0 && p.lse != nullptr) p.lse[blockIdx.x] = lse_of(top, total);
+#pragma unroll
+  for (int j = 0; j < kItems; ++j) {
+    const int row = (tid + 256 * j) / (D / 4), col = (tid + 256 * j) % (D / 4) * 4;
+    if (row >= parts.rows || col >= d) continue;
+    const int R = parts.R0 + row, i = (int)kh_div(R, p.by_group), hq = parts.head * p.group + R - i * p.group;
+    const float inv = total[j] == 0.0f ? 0.0f : 1.0f / total[j];
+    const float y[4] = {o[j].x * inv, o[j].y * inv, o[j].z * inv, o[j].w * inv};
+    kh::store4(static_cast<elem *>(p.out) + (int64_t)(s.start + i) * p.out_stride + (int64_t)hq * d + col, y);
+    if (col == 0 && p.lse != nullptr) p.lse[(int64_t)(s.start + i) * p.q_heads + hq] = lse_of(m[j], total[j]);
+  }
 }
 
 }  // namespace
 
 // Two workgroups to a CU, so that one's loads are in flight while the other
 // multiplies; a wave of the widest rows needs the registers of both.
-#define KH_ATTENTION(D)                                                                                     \
-  extern "C" __global__ void __launch_bounds__(256, D > 128 ? 1 : 2) KH_TYPED(paged_attention_##D)(const KhAttentionParams p) { \
-    __shared__ float lds[kWaves * kRows * 2 + kRows + kWaves * kRows * (D + 4)];                             \
-    attention<D>(p, lds);                                                                                    \
+#define KH_ATTENTION(D, PER_CU)                                                                                  \
+  extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED(paged_attention_##D)(const KhAttentionParams p) { \
+    __shared__ float lds[kWaves * kRows * 2 + kRows + kWaves * kRows * (D + 4)];                                 \
+    narrow<D>(p, (int)blockIdx.x, lds);                                                                          \
   }
-KH_ATTENTION(64)
-KH_ATTENTION(128)
-KH_ATTENTION(256)
-extern "C" __global__ void __launch_bounds__(256) KH_TYPED(paged_attention_join)(const KhAttentionParams p) {
-  __shared__ __attribute__((aligned(16))) float lds[kWaves * 256 + kWaves];
-  join(p, lds);
-}
+KH_ATTENTION(64, 2)
+KH_ATTENTION(128, 2)
+KH_ATTENTION(256, 1)
+// Steps with sequences of many rows: their workgroups first, the longest there are.
+#define KH_ATTENTION_WIDE(D, PER_CU)                                                                              \
+  extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED(paged_attention_wide_##D)(const KhAttentionParams p) { \
+    __shared__ __attribute__((aligned(16))) char lds[Wide<D>::lds];                                               \
+    if ((int)blockIdx.x < p.wide_blocks)                                                                          \
+      wide<D>(p, (int)blockIdx.x, lds);                                                                           \
+    else                                                                                                          \
+      narrow<D>(p, (int)blockIdx.x - p.wide_blocks, reinterpret_cast<float *>(lds));                              \
+  }
+KH_ATTENTION_WIDE(64, 2)
+KH_ATTENTION_WIDE(128, kh::kWide ? 1 : 2)
+KH_ATTENTION_WIDE(256, 1)
+#define KH_ATTENTION_JOIN(D)                                                                                       \
+  extern "C" __global__ void __launch_bounds__(256) KH_TYPED(paged_attention_join_##D)(const KhAttentionParams p) { \
+    __shared__ float lds[kJoinParts * kRows * 2];                                                                   \
+    join<D>(p, lds);                                                                                                \
+  }
+KH_ATTENTION_JOIN(64)
+KH_ATTENTION_JOIN(128)
+KH_ATTENTION_JOIN(256)

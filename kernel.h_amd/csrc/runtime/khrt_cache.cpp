@@ -143,7 +143,10 @@ const Symbol kRope[3][3] = {KH_BY_TYPE(qk_norm_rope, "_8"), KH_BY_TYPE(qk_norm_r
                             KH_BY_TYPE(qk_norm_rope, "_32")};
 const Symbol kAttention[3][3] = {KH_BY_TYPE(paged_attention, "_64"), KH_BY_TYPE(paged_attention, "_128"),
                                  KH_BY_TYPE(paged_attention, "_256")};
-const Symbol kJoin[3] = KH_BY_TYPE(paged_attention, "_join");
+const Symbol kWide[3][3] = {KH_BY_TYPE(paged_attention, "_wide_64"), KH_BY_TYPE(paged_attention, "_wide_128"),
+                            KH_BY_TYPE(paged_attention, "_wide_256")};
+const Symbol kJoin[3][3] = {KH_BY_TYPE(paged_attention, "_join_64"), KH_BY_TYPE(paged_attention, "_join_128"),
+                            KH_BY_TYPE(paged_attention, "_join_256")};
 const Symbol kWeights[3][3] = {KH_BY_TYPE(paged_weights, "_64"), KH_BY_TYPE(paged_weights, "_128"),
                                KH_BY_TYPE(paged_weights, "_256")};
 const Symbol kChoose = {"paged_evict", "paged_evict_choose"};
@@ -171,25 +174,48 @@ int check_attention(const char *op, const kh_paged_attention_args &a) {
   return 0;
 }
 
-// How a launch of paged_attention spreads over the chip (kh_paged.h, KhUnits).
+// How a launch of paged_attention spreads over the chip (kh_paged.h).
 struct AttentionPlan {
-  int64_t groups;  // workgroups
-  bool whole;      // units are not split
-  size_t bytes;    // of workspace that their parts take
+  int64_t groups;              // workgroups of sequences of few rows
+  bool whole;                  // their units are not split
+  int64_t narrow_rows;         // what few rows are
+  int64_t wide_units, splits;  // of sequences of more
+  size_t part_bytes, wide_bytes;  // of workspace that their parts take
 };
 
+// A sequence of more rows than this goes to the wide form.
+constexpr int64_t kNarrowRows = 32;
+
 AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_bytes) {
-  AttentionPlan p;
-  const int64_t group = a.q_heads / a.cache.kv_heads;
+  AttentionPlan p{};
+  const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.tokens * group;
   int64_t len = expected_len(a.table, a.cache);
   // With a window nobody looks further back than the window and the new tokens.
   if (a.window > 0) len = std::min(len, a.window + a.tokens);
+  const size_t row_bytes = (2 + static_cast<size_t>(a.cache.head_dim)) * sizeof(float);
+
+  // Few rows to a sequence, by all the host can know: the narrow form has them
+  // all. One sequence: whichever suits its rows. Otherwise both.
+  const bool narrow_only = rows <= kNarrowRows * a.table.seqs, wide_only = !narrow_only && a.table.seqs == 1;
+  p.narrow_rows = narrow_only ? INT32_MAX : wide_only ? 0 : kNarrowRows;
+  if (!narrow_only) {
+    p.wide_units = (rows / KH_WIDE_ROWS + std::min(a.tokens, a.table.seqs)) * a.cache.kv_heads;
+    // Two to a CU; parts are worth it while they fill the chip no more than once.
+    p.splits = std::clamp<int64_t>(2 * KH_GEMM_CUS / p.wide_units, 1, std::max<int64_t>(1, len / 512));
+    const size_t all_rows = static_cast<size_t>(a.tokens * a.q_heads);
+    p.splits = std::max<int64_t>(1, std::min<int64_t>(p.splits, static_cast<int64_t>(workspace_bytes / (all_rows * row_bytes))));
+    p.wide_bytes = p.splits > 1 ? static_cast<size_t>(p.splits) * all_rows * row_bytes : 0;
+    workspace_bytes -= p.wide_bytes;
+  }
+  if (wide_only) return p;
+
   // At most so many units, of at most so many blocks each.
-  const int64_t units = (a.tokens * group / KH_TILE_ROWS + std::min(a.tokens, a.table.seqs)) * a.cache.kv_heads;
+  const int64_t narrow_most = narrow_only ? rows : std::min(rows, kNarrowRows * a.table.seqs);
+  const int64_t units = (narrow_most / KH_TILE_ROWS + std::min(a.tokens, a.table.seqs)) * a.cache.kv_heads;
   const int64_t blocks = ceil_div(len, KH_STRETCH);
   // As many workgroups as are on the chip at once.
   const int64_t most = (a.cache.head_dim > 128 ? 1 : 2) * KH_GEMM_CUS;
-  const size_t per_group = size_t(2) * KH_TILE_ROWS * (2 + static_cast<size_t>(a.cache.head_dim)) * sizeof(float);
+  const size_t per_group = size_t(2) * KH_TILE_ROWS * row_bytes;
   p.groups = std::min<int64_t>(most, std::max(ceil_div(units * blocks, 2), std::min(units, most)));
   p.groups = std::min(p.groups, static_cast<int64_t>(workspace_bytes / per_group));
   // The kernels count blocks in 32 bits, with what lengths beyond the expected
@@ -197,7 +223,7 @@ AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_
   const int64_t most_blocks = units * ceil_div(capacity_of(a.table.width, a.cache.page_size), KH_STRETCH);
   p.whole = blocks == 1 || p.groups < KH_GEMM_CUS / 4 || most_blocks >= 1 << 30;
   if (p.whole) p.groups = std::min(units, most);
-  p.bytes = p.whole ? 0 : static_cast<size_t>(p.groups) * per_group;
+  p.part_bytes = p.whole ? 0 : static_cast<size_t>(p.groups) * per_group;
   return p;
 }
 
@@ -252,7 +278,8 @@ int kh_paged_attention_workspace(const kh_paged_attention_args *args, size_t *by
   return guarded(op, [&] {
     if (args == nullptr || bytes == nullptr) return bad(op, "null argument");
     if (int rc = check_attention(op, *args)) return rc;
-    *bytes = attention_plan(*args, SIZE_MAX / 2).bytes;
+    const AttentionPlan p = attention_plan(*args, SIZE_MAX / 2);
+    *bytes = p.part_bytes + p.wide_bytes;
     return 0;
   });
 }
@@ -265,16 +292,28 @@ int kh_paged_attention(const kh_paged_attention_args *args, void *workspace, siz
     if (int rc = check_attention(op, a)) return rc;
     if (!aligned(workspace)) return bad(op, "workspace must be 16-byte aligned");
     const AttentionPlan plan = attention_plan(a, workspace != nullptr ? workspace_bytes : 0);
-    const int64_t group = a.q_heads / a.cache.kv_heads;
-    float *part = plan.whole ? nullptr : static_cast<float *>(workspace);
-    KhAttentionParams p{device_cache(a.cache), device_table(a.table, a.cache), a.q, a.out, a.lse, a.q_starts, part,
-                        part != nullptr ? part + plan.groups * 2 * KH_TILE_ROWS * a.cache.head_dim : nullptr, a.q_stride,
-                        a.out_stride, static_cast<int32_t>(a.tokens), static_cast<int32_t>(a.q_heads),
-                        static_cast<int32_t>(group), static_cast<int32_t>(a.window), static_cast<int32_t>(plan.groups),
-                        plan.whole, kh_div_by(static_cast<uint32_t>(group)), a.scale * 1.44269504088896340736f};
-    if (int rc = launch(kAttention[width_of(a.cache.head_dim)][a.cache.dtype], plan.groups, 1, 256, p, stream)) return rc;
-    if (plan.whole) return 0;
-    return launch(kJoin[a.cache.dtype], a.tokens * a.q_heads, 1, 256, p, stream);
+    const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.tokens * a.q_heads, d = a.cache.head_dim;
+    const bool joined = plan.part_bytes + plan.wide_bytes > 0;
+    // All rows of parts come first, 16 bytes at a time, then their statistics.
+    float *const part_o = static_cast<float *>(workspace), *wide_o = part_o, *part_ml = part_o, *wide_ml = part_o;
+    if (joined) {
+      wide_o = part_o + (plan.part_bytes > 0 ? plan.groups * 2 * KH_TILE_ROWS * d : 0);
+      part_ml = wide_o + (plan.wide_bytes > 0 ? plan.splits * rows * d : 0);
+      wide_ml = part_ml + (plan.part_bytes > 0 ? plan.groups * 2 * KH_TILE_ROWS * 2 : 0);
+    }
+    const int64_t wide_blocks = plan.wide_units * plan.splits;
+    KhAttentionParams p{device_cache(a.cache), device_table(a.table, a.cache), a.q, a.out, a.lse, a.q_starts, part_o, part_ml,
+                        wide_o, wide_ml, a.q_stride, a.out_stride, static_cast<int32_t>(a.tokens),
+                        static_cast<int32_t>(a.q_heads), static_cast<int32_t>(group), static_cast<int32_t>(a.window),
+                        static_cast<int32_t>(plan.groups), plan.whole, static_cast<int32_t>(plan.narrow_rows),
+                        static_cast<int32_t>(wide_blocks), static_cast<int32_t>(std::max<int64_t>(plan.splits, 1)),
+                        kh_div_by(static_cast<uint32_t>(group)), a.scale * 1.44269504088896340736f};
+    const auto &symbols = wide_blocks > 0 ? kWide : kAttention;
+    if (int rc = launch(symbols[width_of(d)][a.cache.dtype], wide_blocks + plan.groups, 1, 256, p, stream)) return rc;
+    if (!joined) return 0;
+    const int64_t narrow_joins = plan.part_bytes > 0 ? plan.groups : 0;
+    const int64_t wide_joins = plan.wide_bytes > 0 ? plan.wide_units * (KH_WIDE_ROWS / KH_TILE_ROWS) : 0;
+    return launch(kJoin[width_of(d)][a.cache.dtype], narrow_joins + wide_joins, 1, 256, p, stream);
   });
 }
 

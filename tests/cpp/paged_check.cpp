@@ -91,6 +91,27 @@ int main() {
     expect(kh_seen(s, 4, w).end == big, "the last token's own entry");
   }
 
+  // Parts of the wide form's units: whole tiles, in order, all of them.
+  for (int first : {0, 1, 100})
+    for (int keys : {0, 1, 63, 64, 255, 256, 257, 511, 512, 513, 5000, 100000})
+      for (int splits : {1, 2, 3, 64}) {
+        int next = first, used = 0;
+        for (int k = 0; k < splits; ++k) {
+          const KhPart p = kh_part(first, first + keys, splits, k);
+          if (k == 0) used = p.used;
+          expect(p.used == used && used >= 1 && used <= splits, "parts", keys, splits, k);
+          if (k >= used) {
+            expect(p.first >= p.end, "an unused part is empty", keys, splits, k);
+            continue;
+          }
+          expect(p.first == next && (p.end > p.first || keys == 0), "parts follow each other", keys, splits, k);
+          expect((p.first - first) % 64 == 0 && (k == used - 1 || p.end - p.first >= 256), "whole tiles", keys, splits, k);
+          next = p.end;
+        }
+        expect(next == first + keys, "parts reach the end", keys, splits, next);
+      }
+  expect(kh_part(0, big, 1, 0).end == big && kh_part(5, 3, 7, 0).used == 1, "parts at the limits");
+
   // Shares follow each other, differ by a block at most, and know their owner.
   for (int work : {0, 1, 2, 7, 511, 512, 513, 100000, (1 << 30) - 1})
     for (int most : {1, 2, 3, 64, 511, 512, 4095}) {

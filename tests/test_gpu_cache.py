@@ -68,6 +68,37 @@ def test_long_chunk(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("q_lens,lens,hq,hk,d", [([50], [4000], 4, 2, 64), ([70], [2100], 2, 1, 128), ([20], [1500], 4, 1, 256),
+                                                 ([40, 1, 0, 130, 9], [3000, 2000, 50, 700, 1300], 8, 2, 128),
+                                                 ([33, 32, 8], [900, 901, 902], 1, 1, 80)])
+@pytest.mark.parametrize("window", [0, 700])
+def test_chunks_over_long_caches(dev, dtype, q_lens, lens, hq, hk, d, window):
+    """Sequences of many rows whose entries are split over workgroups, alone
+    and beside sequences of few rows; with and without a workspace."""
+    s = Step(dtype, q_lens, lens, hq, hk, d, seed=d, window=window, page_size=24, before=1, after=2)
+    for workspace in (None, 0, 300000):
+        check_attention(s, workspace=workspace)
+
+
+def test_more_sequences_than_lanes(dev):
+    """A hundred and fifty sequences of all kinds."""
+    g = np.random.default_rng(0)
+    q_lens = [int(x) for x in g.choice([0, 1, 1, 1, 2, 30], 150)]
+    lens = [int(x) for x in g.integers(0, 300, 150)]
+    check_attention(Step("bf16", q_lens, lens, 4, 2, 64, seed=1))
+    check_attention(Step("f16", [1] * 150, lens, 4, 2, 64, seed=2))
+
+
+def test_starts_that_do_not_ascend(dev):
+    """Sequences that claim the same tokens: whatever they get, the call ends,
+    and tokens of no sequence are left alone."""
+    s = Step("bf16", [40] * 6, [100] * 6, 4, 2, 64, seed=3, before=1, after=2)
+    s.starts = [1, 200, 1, 200, 1, 200, 150]
+    out, lse = s.run_attention()
+    assert (out[[0, -1, -2]] == 7.0).all() and (lse[[0, -1, -2]] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("workspace", [0, None, 20000])
 @pytest.mark.parametrize("q", [1, 5])
 def test_long_sequences_split_and_not(dev, dtype, workspace, q):
