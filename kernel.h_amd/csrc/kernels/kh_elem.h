@@ -109,6 +109,25 @@ __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 acc) {
 #endif
 }
 
+// One wave's load straight to LDS: lane l's 16 bytes at byte voff of the resource
+// land at LDS byte address lds + 16 l. Inline assembly on purpose: the compiler
+// cannot prove the places disjoint from those it reads, and would wait for its
+// own form of this load before every later LDS read. The caller waits
+// (vm_wait) before the barrier that hands the bytes over. The resource and `lds`
+// are the same in all lanes. M0 carries the LDS address, with the one wait state
+// between writing it and such a load.
+__device__ __forceinline__ void dma16(u32x4 rsrc, uint32_t voff, uint32_t lds) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      :
+      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(rsrc)
+      : "memory", "m0");
+}
+
 #if KH_ELEM != 0
 // Of 4 x 16 elements in LDS that the 16 lanes of a row point at (lane 4 r + c:
 // row r, columns 4 c ..), lane i receives column i, its four rows in order

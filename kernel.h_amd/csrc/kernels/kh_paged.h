@@ -116,14 +116,14 @@ KH_HD KhSpan kh_seen(const KhSeq &s, int32_t i, int32_t window) {
 #define KH_TILE_ROWS 16
 
 struct KhUnits {
-  int32_t first;   // the first entry that any new token sees
+  int32_t first;   // the first entry that any new token sees, down to a multiple of 16
   int32_t blocks;  // of each unit, at least 1: rows that see nothing are written too
   int32_t tiles;   // 0 without new tokens
 };
 
 KH_HD KhUnits kh_units(const KhSeq &s, int32_t group, int32_t window, int32_t whole) {
   KhUnits u;
-  u.first = kh_seen(s, 0, window).first;  // the first token's window starts earliest
+  u.first = kh_seen(s, 0, window).first & ~15;  // the first token's window starts earliest
   const int32_t keys = s.n > u.first ? s.n - u.first : 0;
   u.blocks = whole != 0 || keys == 0 ? 1 : (keys - 1) / KH_STRETCH + 1;
   u.tiles = s.m == 0 ? 0 : (s.m * group - 1) / KH_TILE_ROWS + 1;
@@ -227,8 +227,10 @@ struct KhAttentionParams {
   int32_t tokens, q_heads, group, window, groups, whole;
   int32_t narrow_rows;  // a sequence of more rows is the wide form's
   int32_t wide_blocks, wide_splits;
+  int32_t even;  // pages hold a multiple of 16 entries, rows apart, and 16 slots' strides fit 31 bits
+  uint32_t q_sign;  // the sign bits of q's elements where the scale is negative
   KhDiv by_group;
-  float scale_log2;
+  float scale_log2;  // |scale| log2(e), above 0: maxima may be taken before it
 };
 
 // paged_weights.hip

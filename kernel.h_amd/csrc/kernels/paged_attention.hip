@@ -131,54 +131,78 @@ __device__ __forceinline__ float lse_of(float top, float total) {
   return total == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * 0.69314718055994530942f;
 }
 
+// A word of the page table by way of the scalar cache: for an address that is
+// the same in all lanes.
+__device__ __forceinline__ int scalar_load(const int32_t *p) {
+  typedef const int32_t __attribute__((address_space(4))) *constant;
+  return *(constant)(uintptr_t)p;
+}
+
+// Page and slot of entry `key`, or of one that is there in its place: nobody
+// uses what a load then brings, but every load has an address. EVEN (page_size
+// a multiple of 16): the 16 entries from a multiple of 16 on lie in one page
+// next to each other, key is such a multiple, and everything about its page is
+// the same in all lanes.
+template <bool EVEN>
+__device__ __forceinline__ KhSlot look_up(const KhAttentionParams &p, const int32_t *table, int key, int end) {
+  const int inside = key < end ? key : EVEN ? (end - 1) & ~15 : end - 1;
+  const uint32_t i = kh_div((uint32_t)inside, p.cache.by_page);  // inside < end <= capacity: i is in the row
+  return KhSlot{EVEN ? scalar_load(table + i) : table[i], inside - (int)(i * p.cache.by_page.by)};
+}
+
 // Where the rows of a block of entries lie. Loads of absent rows go to the
-// cache's first row instead of being skipped: a branch round a load would make
+// cache's first page instead of being skipped: a branch round a load would make
 // the wave wait for every load in flight where its paths join.
-template <int D>
+template <int D, bool EVEN>
 struct Block {
-  KhSlot at[Form<D>::tiles];  // of entry 16 t + l % 16
+  KhSlot at[Form<D>::tiles];  // of entry 16 t + l % 16; EVEN: of entry 16 t
   uint32_t present;           // bit k: entry k of the block has a page, and is one of this workgroup's
 };
 
-template <int D>
-__device__ __forceinline__ void find(Block<D> &b, const KhAttentionParams &p, const int32_t *table, int key0, int end, int r) {
+template <int D, bool EVEN>
+__device__ __forceinline__ void find(Block<D, EVEN> &b, const KhAttentionParams &p, const int32_t *table, int key0, int end, int r) {
 #pragma unroll
-  for (int t = 0; t < Form<D>::tiles; ++t) {
-    const int key = key0 + 16 * t + r, inside = key < end ? key : end - 1;
-    const uint32_t i = kh_div((uint32_t)inside, p.cache.by_page);
-    b.at[t].slot = inside - (int)(i * p.cache.by_page.by);
-    b.at[t].page = table[i];  // inside < end <= capacity: i is in the row
-  }
+  for (int t = 0; t < Form<D>::tiles; ++t) b.at[t] = look_up<EVEN>(p, table, key0 + 16 * t + (EVEN ? 0 : r), end);
 }
 
 // Done apart from find() so that the page numbers have time to arrive.
-template <int D>
-__device__ __forceinline__ void settle(Block<D> &b, const KhAttentionParams &p, int key0, int end, int r) {
+template <int D, bool EVEN>
+__device__ __forceinline__ void settle(Block<D, EVEN> &b, const KhAttentionParams &p, int key0, int end, int r) {
   b.present = 0;
 #pragma unroll
   for (int t = 0; t < Form<D>::tiles; ++t) {
-    const bool there = key0 + 16 * t + r < end && (uint32_t)b.at[t].page < (uint32_t)p.cache.pages;
-    b.present |= ((uint32_t)__builtin_amdgcn_ballot_w64(there) & 0xffffu) << (16 * t);
-    if (!there) b.at[t] = KhSlot{0, 0};
+    const bool paged = (uint32_t)b.at[t].page < (uint32_t)p.cache.pages;
+    if constexpr (EVEN) {
+      const int left = end - key0 - 16 * t;
+      b.present |= (!paged || left <= 0 ? 0u : left >= 16 ? 0xffffu : (1u << left) - 1) << (16 * t);
+      if (!paged) b.at[t].page = 0;
+    } else {
+      const bool there = key0 + 16 * t + r < end && paged;
+      b.present |= ((uint32_t)__builtin_amdgcn_ballot_w64(there) & 0xffffu) << (16 * t);
+      if (!there) b.at[t] = KhSlot{0, 0};
+    }
   }
 }
 
-template <int D>
-__device__ __forceinline__ void load_k(u32x4 (&k)[Form<D>::tiles][Form<D>::steps], const Block<D> &b, const KhAttentionParams &p,
-                                       const char *base, int row_bytes, int h) {
+// Byte `off` of a row, or its first where the row is shorter.
+__device__ __forceinline__ uint32_t within(int off, int row_bytes) { return (uint32_t)(off < row_bytes ? off : 0); }
+
+template <int D, bool EVEN>
+__device__ __forceinline__ void load_k(u32x4 (&k)[Form<D>::tiles][Form<D>::steps], const Block<D, EVEN> &b,
+                                       const KhAttentionParams &p, const char *base, int row_bytes, int r, int h) {
 #pragma unroll
   for (int t = 0; t < Form<D>::tiles; ++t) {
     const char *row = base + kh_row(b.at[t], p.cache.k_page, p.cache.k_slot);
 #pragma unroll
     for (int c = 0; c < Form<D>::steps; ++c) {
-      const int off = 64 * c + 16 * h;
-      k[t][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + (off < row_bytes ? off : 0)));
+      const uint32_t off = (EVEN ? (uint32_t)r * p.cache.k_slot : 0u) + within(64 * c + 16 * h, row_bytes);
+      k[t][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + off));
     }
   }
 }
 
-template <int D>
-__device__ __forceinline__ void load_v(Piece<D> (&v)[Form<D>::count], const Block<D> &b, const KhAttentionParams &p,
+template <int D, bool EVEN>
+__device__ __forceinline__ void load_v(Piece<D> (&v)[Form<D>::count], const Block<D, EVEN> &b, const KhAttentionParams &p,
                                        const char *base, int row_bytes, int r, int h) {
   using F = Form<D>;
 #pragma unroll
@@ -186,13 +210,16 @@ __device__ __forceinline__ void load_v(Piece<D> (&v)[Form<D>::count], const Bloc
     const uint64_t own = kh_row(b.at[t], p.cache.v_page, p.cache.v_slot);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      // Entry 4 h + i is the one that lane 4 h + i looked up.
-      const uint32_t lo = __shfl((uint32_t)own, 4 * h + i, kh::kWave), hi = __shfl((uint32_t)(own >> 32), 4 * h + i, kh::kWave);
-      const char *row = base + ((uint64_t)hi << 32 | lo);
+      const char *row = base + own;
+      if constexpr (!EVEN) {
+        // Entry 4 h + i is the one that lane 4 h + i looked up.
+        const uint32_t lo = __shfl((uint32_t)own, 4 * h + i, kh::kWave), hi = __shfl((uint32_t)(own >> 32), 4 * h + i, kh::kWave);
+        row = base + ((uint64_t)hi << 32 | lo);
+      }
 #pragma unroll
       for (int a = 0; a < F::count; ++a) {
-        const int off = (a * F::span + F::piece * r) * (int)sizeof(elem);
-        const char *from = row + (off < row_bytes ? off : 0);
+        const char *from = row + ((EVEN ? (uint32_t)(4 * h + i) * p.cache.v_slot : 0u) +
+                                  within((a * F::span + F::piece * r) * (int)sizeof(elem), row_bytes));
         uint32_t(&w)[F::words] = v[a].w[4 * t + i];
         if constexpr (F::words == 4) {
           const u32x4 g = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from));
@@ -204,6 +231,20 @@ __device__ __forceinline__ void load_v(Piece<D> (&v)[Form<D>::count], const Bloc
       }
     }
   }
+}
+
+// Bit n: entry key0 + n is one of those seen, n < 64.
+__device__ __forceinline__ uint64_t seen_of(const KhSpan &seen, int key0) {
+  const int from = kh_clamp(seen.first - key0, 0, 64), to = kh_clamp(seen.end - key0, 0, 64);
+  if (from >= to) return 0;
+  return (~uint64_t(0) >> (64 - to)) & (~uint64_t(0) << from);
+}
+
+// h, worked out where it is used: on a path that is hardly ever taken, what
+// follows from it is not to be kept in registers across the loop round it.
+__device__ __forceinline__ int apart(int h) {
+  asm volatile("" : "+v"(h));
+  return h;
 }
 
 __device__ __forceinline__ KhSeq sequence(const KhAttentionParams &p, int seq) {
@@ -276,7 +317,7 @@ __device__ __forceinline__ int sequence_at(const KhAttentionParams &p, const Lin
   return -1;
 }
 
-template <int D>
+template <int D, bool EVEN>
 __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, float *lds) {
   using F = Form<D>;
   const int lane = kh::lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kh::kWave);
@@ -328,15 +369,16 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
     const int i_last = (int)kh_div(row0 + kRows < rows ? row0 + kRows - 1 : rows - 1, p.by_group);
     const KhSpan seen = kh_seen(s, i, p.window);
     const KhSpan low = kh_seen(s, i_first, p.window), high = kh_seen(s, i_last, p.window);
-    const int key_first = low.first > from ? low.first : from;
+    const int key_first = (low.first > from ? low.first : from) & ~15;  // from is a multiple of 16
     const int key_end = high.end < to ? high.end : to;
 
     u32x4 q[F::steps];
-    const elem *qp = static_cast<const elem *>(p.q) + (int64_t)(s.start + i) * p.q_stride + (int64_t)hq * d;
+    const char *qp = static_cast<const char *>(p.q) + ((int64_t)(s.start + i) * p.q_stride + (int64_t)hq * d) * (int)sizeof(elem);
 #pragma unroll
     for (int c = 0; c < F::steps; ++c) {
-      q[c] = u32x4{0, 0, 0, 0};
-      if (mine && 64 * c + 16 * h < row_bytes) q[c] = *reinterpret_cast<const u32x4 *>(qp + (64 * c + 16 * h) / (int)sizeof(elem));
+      // From an address that is there in any case, as the rows of K and V.
+      const u32x4 x = *reinterpret_cast<const u32x4 *>(qp + within(64 * c + 16 * h, row_bytes)) ^ p.q_sign;
+      q[c] = mine && 64 * c + 16 * h < row_bytes ? x : u32x4{0, 0, 0, 0};
     }
 
     float m = kNegBig, l = 0.0f;  // of row l % 16; l of this lane's entries alone
@@ -354,12 +396,15 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
       constexpr int kStep = kWaves * F::keys;
       u32x4 k[F::tiles][F::steps];
       Piece<D> v[F::count];
-      Block<D> now, next;
-      find<D>(now, p, table, key0, key_end, r);
-      find<D>(next, p, table, key0 + kStep, key_end, r);
-      settle<D>(now, p, key0, key_end, r);
-      load_k<D>(k, now, p, kbase, row_bytes, h);
-      load_v<D>(v, now, p, vbase, row_bytes, r, h);
+      Block<D, EVEN> now, next;
+      find<D, EVEN>(now, p, table, key0, key_end, r);
+      find<D, EVEN>(next, p, table, key0 + kStep, key_end, r);
+      settle<D, EVEN>(now, p, key0, key_end, r);
+      load_k<D, EVEN>(k, now, p, kbase, row_bytes, r, h);
+      // K goes out before V here as in the loop: the wait for K at its top then
+      // leaves V in flight.
+      __builtin_amdgcn_sched_barrier(0);
+      load_v<D, EVEN>(v, now, p, vbase, row_bytes, r, h);
       for (; key0 < key_end; key0 += kStep) {
         const uint32_t present = now.present;
         float y[F::mine];
@@ -378,36 +423,37 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
 #pragma unroll
           for (int c = 0; c < F::steps; ++c) x = kh::mma16(k[t][c], q[c], x);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[4 * t + e] = x[e] * p.scale_log2;
+          for (int e = 0; e < 4; ++e) y[4 * t + e] = x[e];
         }
         now = next;
-        settle<D>(now, p, key0 + kStep, key_end, r);
-        load_k<D>(k, now, p, kbase, row_bytes, h);
-        find<D>(next, p, table, key0 + 2 * kStep, key_end, r);
+        settle<D, EVEN>(now, p, key0 + kStep, key_end, r);
+        load_k<D, EVEN>(k, now, p, kbase, row_bytes, r, h);
+        find<D, EVEN>(next, p, table, key0 + 2 * kStep, key_end, r);
 
         // Every row sees every entry of the block: no mask.
         const bool whole = present == (F::keys == 32 ? 0xffffffffu : 0xffffu) && key0 + F::keys <= low.end && key0 >= high.first;
         uint32_t odds = 0;  // bit n: entry n of the block, in this lane's columns
         if (!whole) {
+          // Of the lane's entries: those that its row sees, and those that are there.
+          const uint32_t sees = (mine ? (uint32_t)seen_of(seen, key0) & present : 0u) >> 4 * h, there = present >> 4 * h;
 #pragma unroll
           for (int j = 0; j < F::mine; ++j) {
-            const int n = 16 * (j / 4) + 4 * h + j % 4, key = key0 + n;
-            const bool there = (present >> n & 1) != 0;
-            const bool sees = mine && key >= seen.first && key < seen.end && there;
-            y[j] = sees ? y[j] : -__builtin_inff();
+            const uint32_t bit = 1u << (16 * (j / 4) + j % 4);
+            y[j] = (sees & bit) != 0 ? y[j] : -__builtin_inff();
 #pragma unroll
             for (int a = 0; a < F::count; ++a)
 #pragma unroll
               for (int w = 0; w < F::words; ++w) {
-                v[a].w[j][w] = there ? v[a].w[j][w] : 0u;
-                odds |= (uint32_t)kh::not_finite(v[a].w[j][w]) << n;
+                v[a].w[j][w] = (there & bit) != 0 ? v[a].w[j][w] : 0u;
+                odds |= kh::not_finite(v[a].w[j][w]) ? bit : 0u;
               }
           }
+          odds <<= 4 * h;
         }
         float top = y[0];
 #pragma unroll
         for (int j = 1; j < F::mine; ++j) top = fmaxf(top, y[j]);
-        top = fmaxf(m, over_rows(top, true));
+        top = fmaxf(m, over_rows(top, true) * p.scale_log2);
         if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
           const float fade = kh::exp2_hw(m - top);
           m = top;
@@ -420,7 +466,7 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < F::mine; ++j) {
-          y[j] = kh::exp2_hw(y[j] - m);
+          y[j] = kh::exp2_hw(fmaf(y[j], p.scale_log2, -m));
           sum += y[j];
         }
         l += sum;
@@ -435,13 +481,14 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
             const KhSlot at = kh_slot(table, p.table.width, p.cache.pages, p.cache.by_page, (uint32_t)key);
             const char *row = vbase + kh_row(at, p.cache.v_page, p.cache.v_slot);
             if (mine && key >= seen.first && key < seen.end) {
+              const int h1 = apart(h);
 #pragma unroll
               for (int a = 0; a < F::count; ++a)
 #pragma unroll
                 for (int i4 = 0; i4 < 4; ++i4)
 #pragma unroll
                   for (int e = 0; e < F::piece; e += 4) {
-                    const int col = a * F::span + F::piece * (4 * h + i4) + e;
+                    const int col = a * F::span + F::piece * (4 * h1 + i4) + e;
                     if (col >= d) continue;
                     const f32x4 x = odd_of(row + col * (int)sizeof(elem));
 #pragma unroll
@@ -460,7 +507,7 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
         for (int a = 0; a < F::count; ++a)
 #pragma unroll
           for (int e = 0; e < F::piece; ++e) o[a][e] = pv<D>(v[a], e, y, o[a][e]);
-        load_v<D>(v, now, p, vbase, row_bytes, r, h);
+        load_v<D, EVEN>(v, now, p, vbase, row_bytes, r, h);
       }
     }
 
@@ -522,116 +569,210 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
 // ---- many rows: chunks of prompts
 //
 // A workgroup takes 128 rows, 32 to a wave, of one sequence and kv head, and
-// brings tiles of K and V through LDS for all of them, a tile ahead: the next
-// tile's loads are in flight while this one is multiplied, and the one barrier
-// of a tile orders LDS alone. Per wave
+// brings tiles of K and V through LDS for all of them, a tile ahead. Per wave
 //   S^T = K Q^T     32 x 32 tiles, A = rows of K from LDS, B = Q in registers
 //   O^T += V^T P^T  B = S^T's registers as they are, A = V read across its rows
 //                   (16 bits), or row by row (32 bits, one row to a product)
-// with the running maximum and sum of row l % 32 in lanes l and l ^ 32. Rows of
-// LDS are padded so that neither kind of read meets a bank twice.
+// with the running maximum and sum of row l % 32 in lanes l and l ^ 32.
+//
+// Tiles of pages of a multiple of 16 entries go straight to LDS (a wave's load
+// brings whole rows of one page; its resource ends where the page's entries
+// do, so that absent rows and columns past the row's end arrive as zeros);
+// others through registers. A row's 16-byte pieces lie at their number
+// exclusive-or a number of the row's, so that neither kind of read meets a bank
+// twice.
 template <int D>
 struct Wide {
   static constexpr int bytes = D * (int)sizeof(elem);
   static constexpr int steps = bytes / 32;
   static constexpr int keys = bytes > 512 ? 32 : 64;  // entries of a tile
-  static constexpr int tiles = keys / 32;
+  static constexpr int tiles = keys / 32, runs = keys / 16;
   static constexpr int dts = D / 32;
-  static constexpr int pieces = bytes / 16;             // of 16 bytes in a row
-  static constexpr int passes = keys * pieces / 256;    // pieces that a thread brings
-  static constexpr int per_pass = 256 / pieces;         // rows of a pass
-  static constexpr int k_pitch = bytes + 16, v_pitch = bytes + (kh::kWide ? 32 : 64);
-  static constexpr int buffer = keys * (k_pitch + v_pitch) + keys;  // and a byte about each entry
+  static constexpr int pieces = bytes / 16;           // of 16 bytes in a row
+  static constexpr int passes = keys * pieces / 256;  // pieces that a thread brings
+  static constexpr int rows = 64 / pieces;            // that a wave brings in a pass
+  static constexpr int share = keys / kWaves;         // that it brings in all: half a run or a whole one
+  static constexpr int v_at = keys * bytes, marks_at = 2 * v_at, buffer = marks_at + keys;
   static constexpr int lds = 2 * buffer;
 };
 constexpr int kWideRows = 32;                  // of a wave
 constexpr int kWideTile = kWaves * kWideRows;  // of a workgroup
 
-// Marks of an entry in LDS.
-constexpr uint32_t kThere = 1, kOdd = 2;
-
+// What a row's piece numbers are exclusive-ored with: 16 rows of K in a column
+// fill the banks once; so do, of V, the pieces that a product's read takes of 4
+// rows (16 bits), or of a row and the one 4 below it (32 bits).
 template <int D>
+__device__ __forceinline__ int k_turn(int row) {
+  return Wide<D>::pieces == 8 ? row >> 1 & 7 : row & 15;
+}
+template <int D>
+__device__ __forceinline__ int v_turn(int row) {
+  if constexpr (kh::kWide) return (row >> 2 & 1) * 8;
+  return Wide<D>::pieces == 8 ? (row >> 1 & 1) * 4 : (row & 3) * 4;
+}
+
+// The first row that the wave brings in pass i.
+template <int D>
+__device__ __forceinline__ int first_row(int i, int wave) {
+  return wave * Wide<D>::share + i * Wide<D>::rows;
+}
+
+constexpr uint8_t kThere = 1, kOdd = 2;  // marks of a row in LDS
+
+// A tile on its way. EVEN: lane n has found run n % runs.
+template <int D, bool EVEN>
 struct Stage {
-  KhSlot at[Wide<D>::passes];
-  u32x4 k[Wide<D>::passes], v[Wide<D>::passes];
-  uint32_t there;  // bit i: the row of pass i
+  KhSlot at[EVEN ? 1 : Wide<D>::passes];
+  u32x4 k[EVEN ? 1 : Wide<D>::passes], v[EVEN ? 1 : Wide<D>::passes];
+};
+
+template <int D, bool EVEN>
+__device__ __forceinline__ void seek(Stage<D, EVEN> &g, const KhAttentionParams &p, const int32_t *table, int key0, int end, int lane, int wave) {
+  using W = Wide<D>;
+  if constexpr (EVEN) {
+    const int key = key0 + 16 * (lane % W::runs), last = (end - 1) & ~15;
+    const uint32_t inside = (uint32_t)(key < last ? key : last), i = kh_div(inside, p.cache.by_page);
+    g.at[0] = KhSlot{table[i], (int)(inside - i * p.cache.by_page.by)};
+  } else {
+#pragma unroll
+    for (int i = 0; i < W::passes; ++i)
+      g.at[i] = look_up<false>(p, table, key0 + first_row<D>(i, wave) + lane / W::pieces, end);
+  }
+}
+
+// What a lane brings of a row of K and of V in each pass: where from, past the
+// wave's first row.
+template <int D>
+struct Lanes {
+  uint32_t k[Wide<D>::passes], v[Wide<D>::passes];
 };
 
 template <int D>
-__device__ __forceinline__ void seek(Stage<D> &g, const KhAttentionParams &p, const int32_t *table, int key0, int end, int tid) {
+__device__ __forceinline__ Lanes<D> lanes_of(const KhAttentionParams &p, int row_bytes, int lane, int wave) {
   using W = Wide<D>;
+  Lanes<D> l;
 #pragma unroll
   for (int i = 0; i < W::passes; ++i) {
-    const int key = key0 + i * W::per_pass + tid / W::pieces, inside = key < end ? key : end - 1;
-    const uint32_t n = kh_div((uint32_t)inside, p.cache.by_page);
-    g.at[i].slot = inside - (int)(n * p.cache.by_page.by);
-    g.at[i].page = table[n];
+    const int own = i * W::rows + lane / W::pieces, row = wave * W::share + own;
+    const int kc = 16 * (lane % W::pieces ^ k_turn<D>(row)), vc = 16 * (lane % W::pieces ^ v_turn<D>(row));
+    l.k[i] = kc < row_bytes ? (uint32_t)own * p.cache.k_slot + (uint32_t)kc : kh::kOutside;
+    l.v[i] = vc < row_bytes ? (uint32_t)own * p.cache.v_slot + (uint32_t)vc : kh::kOutside;
+  }
+  return l;
+}
+
+// Sends a tile's rows to LDS, and says which entries are there.
+template <int D>
+__device__ __forceinline__ uint64_t send(const Stage<D, true> &g, const Lanes<D> &l, const KhAttentionParams &p, const char *kbase,
+                                         const char *vbase, int key0, int end, const char *buffer, int wave) {
+  using W = Wide<D>;
+  // Runs with a page; of a run past the end the last one's was found.
+  const uint32_t paged = (uint32_t)__builtin_amdgcn_ballot_w64((uint32_t)g.at[0].page < (uint32_t)p.cache.pages);
+  const int left = end - key0;
+  uint64_t present = W::keys == 64 ? ~uint64_t(0) : (uint64_t(1) << W::keys % 64) - 1;
+  if ((paged & ((1u << W::runs) - 1)) != (1u << W::runs) - 1 || left < W::keys) {
+    present = left <= 0 ? 0 : left < W::keys ? (uint64_t(1) << left) - 1 : present;
+#pragma unroll
+    for (int n = 0; n < W::runs; ++n)
+      if ((paged >> n & 1) == 0) present &= ~(uint64_t(0xffff) << (16 * n));
+  }
+  const int row = wave * W::share, run = row / 16;
+  KhSlot at = {__builtin_amdgcn_readlane(g.at[0].page, run), __builtin_amdgcn_readlane(g.at[0].slot, run) + (row & 15)};
+  if ((paged >> run & 1) == 0) at.page = 0;
+  const uint32_t real = (uint32_t)__builtin_popcountll(present >> row & ((uint64_t(1) << W::share) - 1));
+  const uint64_t k = (uint64_t)reinterpret_cast<uintptr_t>(kbase) + kh_row(at, p.cache.k_page, p.cache.k_slot);
+  const uint64_t v = (uint64_t)reinterpret_cast<uintptr_t>(vbase) + kh_row(at, p.cache.v_page, p.cache.v_slot);
+  // Addresses have 48 bits: the resource's stride, above them, is zero.
+  const u32x4 rk = {(uint32_t)k, (uint32_t)(k >> 32), real * p.cache.k_slot, 0x00020000u};
+  const u32x4 rv = {(uint32_t)v, (uint32_t)(v >> 32), real * p.cache.v_slot, 0x00020000u};
+  const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(buffer) + (uint32_t)(row * W::bytes);
+#pragma unroll
+  for (int i = 0; i < W::passes; ++i) kh::dma16(rk, l.k[i], lds + (uint32_t)(i * W::rows * W::bytes));
+#pragma unroll
+  for (int i = 0; i < W::passes; ++i) kh::dma16(rv, l.v[i], lds + (uint32_t)(W::v_at + i * W::rows * W::bytes));
+  return present;
+}
+
+// Starts a tile's loads into registers.
+template <int D>
+__device__ __forceinline__ void fetch(Stage<D, false> &g, const KhAttentionParams &p, const char *kbase, const char *vbase, int key0,
+                                      int end, int row_bytes, int lane, int wave) {
+  using W = Wide<D>;
+  const int own = lane / W::pieces;
+  const uint32_t off = within(16 * (lane % W::pieces), row_bytes);
+#pragma unroll
+  for (int i = 0; i < W::passes; ++i) {
+    if (key0 + first_row<D>(i, wave) + own >= end || (uint32_t)g.at[i].page >= (uint32_t)p.cache.pages) g.at[i] = KhSlot{-1, 0};
+    const KhSlot at = g.at[i].page < 0 ? KhSlot{0, 0} : g.at[i];
+    g.k[i] = *reinterpret_cast<const u32x4 *>(kbase + kh_row(at, p.cache.k_page, p.cache.k_slot) + off);
+    g.v[i] = *reinterpret_cast<const u32x4 *>(vbase + kh_row(at, p.cache.v_page, p.cache.v_slot) + off);
   }
 }
 
+// From registers to LDS, with zeros for absent rows and columns past the row's
+// end. The lane that brought a row's first piece marks the row.
 template <int D>
-__device__ __forceinline__ void fetch(Stage<D> &g, const KhAttentionParams &p, const char *kbase, const char *vbase, int key0, int end,
-                                      int row_bytes, int tid) {
+__device__ __forceinline__ void put(const Stage<D, false> &g, char *buffer, int row_bytes, int lane, int wave) {
   using W = Wide<D>;
-  const int off = 16 * (tid % W::pieces);
-  g.there = 0;
+  const int own = lane / W::pieces, piece = lane % W::pieces;
 #pragma unroll
   for (int i = 0; i < W::passes; ++i) {
-    const bool there = key0 + i * W::per_pass + tid / W::pieces < end && (uint32_t)g.at[i].page < (uint32_t)p.cache.pages;
-    if (!there) g.at[i] = KhSlot{0, 0};
-    g.there |= (uint32_t)there << i;
-    const int from = off < row_bytes ? off : 0;
-    g.k[i] = *reinterpret_cast<const u32x4 *>(kbase + kh_row(g.at[i], p.cache.k_page, p.cache.k_slot) + from);
-    g.v[i] = *reinterpret_cast<const u32x4 *>(vbase + kh_row(g.at[i], p.cache.v_page, p.cache.v_slot) + from);
+    const int row = first_row<D>(i, wave) + own;
+    const bool there = g.at[i].page >= 0, real = there && 16 * piece < row_bytes;
+    const u32x4 zero = {0, 0, 0, 0};
+    *reinterpret_cast<u32x4 *>(buffer + row * W::bytes + 16 * (piece ^ k_turn<D>(row))) = real ? g.k[i] : zero;
+    *reinterpret_cast<u32x4 *>(buffer + W::v_at + row * W::bytes + 16 * (piece ^ v_turn<D>(row))) = real ? g.v[i] : zero;
+    if (piece == 0) buffer[W::marks_at + row] = there ? kThere : 0;
   }
 }
 
+// In a tile of which rows of the unit see different entries: takes infinities
+// and NaN out of V and marks the rows that had some. Between barriers.
 template <int D>
-__device__ __forceinline__ void put(const Stage<D> &g, char *buffer, bool check, int row_bytes, int tid) {
+__device__ __forceinline__ void clean(char *buffer, int lane, int wave) {
   using W = Wide<D>;
-  const int off = 16 * (tid % W::pieces);
-  char *v_at = buffer + W::keys * W::k_pitch;
-  uint8_t *marks_at = reinterpret_cast<uint8_t *>(v_at + W::keys * W::v_pitch);
+  const int own = lane / W::pieces, piece = lane % W::pieces;
 #pragma unroll
   for (int i = 0; i < W::passes; ++i) {
-    const int row = i * W::per_pass + tid / W::pieces;
-    const bool there = (g.there >> i & 1) != 0, inside = off < row_bytes;
-    const u32x4 zero = {0, 0, 0, 0}, k = there && inside ? g.k[i] : zero;
-    u32x4 v = there && inside ? g.v[i] : zero;
-    uint32_t mark = there ? kThere : 0;
-    if (check) {
-      // Rows differ in what they see of this tile: infinities and NaN of V stay
-      // out of the products, and the lane that brought the row's first piece
-      // says that it has some.
-      const bool odd = kh::not_finite(v.x) | kh::not_finite(v.y) | kh::not_finite(v.z) | kh::not_finite(v.w);
-      const uint64_t odds = __builtin_amdgcn_ballot_w64(odd);
-      const uint64_t row_lanes = W::pieces == 64 ? ~uint64_t(0) : ((uint64_t(1) << W::pieces % 64) - 1) << (tid % kh::kWave / W::pieces * W::pieces);
-      if (odds != 0) {
-        v = u32x4{without_odd(v.x), without_odd(v.y), without_odd(v.z), without_odd(v.w)};
-        mark |= (odds & row_lanes) != 0 ? kOdd : 0;
-      }
+    const int row = first_row<D>(i, wave) + own;
+    u32x4 *at = reinterpret_cast<u32x4 *>(buffer + W::v_at + row * W::bytes + 16 * piece);
+    const u32x4 v = *at;
+    const bool odd = kh::not_finite(v.x) | kh::not_finite(v.y) | kh::not_finite(v.z) | kh::not_finite(v.w);
+    const uint64_t odds = __builtin_amdgcn_ballot_w64(odd);
+    if (odd) *at = u32x4{without_odd(v.x), without_odd(v.y), without_odd(v.z), without_odd(v.w)};
+    const uint64_t lanes = W::pieces == 64 ? ~uint64_t(0) : ((uint64_t(1) << W::pieces % 64) - 1) << (own * W::pieces);
+    if (piece == 0) {
+      uint8_t *mark = reinterpret_cast<uint8_t *>(buffer + W::marks_at + row);
+      *mark = (uint8_t)((*mark & kThere) | ((odds & lanes) != 0 ? kOdd : 0));
     }
-    *reinterpret_cast<u32x4 *>(buffer + row * W::k_pitch + off) = k;
-    *reinterpret_cast<u32x4 *>(v_at + row * W::v_pitch + off) = v;
-    if (tid % W::pieces == 0) marks_at[row] = (uint8_t)mark;
   }
+}
+
+// A operand of K for 32 bytes of the rows of tile kt.
+template <int D>
+__device__ __forceinline__ u32x4 k_rows(const char *buffer, int kt, int c, int lane) {
+  using W = Wide<D>;
+  const int r = lane & 31;
+  return *reinterpret_cast<const u32x4 *>(buffer + (32 * kt + r) * W::bytes + 16 * ((lane >> 5 ^ k_turn<D>(r)) ^ 2 * c));
 }
 
 // A operand of V^T for columns 32 dt .. and the entries that step c of tile kt's
-// scores hold (16 bits: half a tile, 32 bits: two entries).
+// scores hold (16 bits: half a tile, 32 bits: a quarter).
 template <int D>
-__device__ __forceinline__ u32x4 v_across(const char *v_at, int kt, int c, int dt, int lane) {
+__device__ __forceinline__ u32x4 v_across(const char *buffer, int kt, int c, int dt, int lane) {
   using W = Wide<D>;
   u32x4 a = {0, 0, 0, 0};
 #if KH_ELEM == 0
   // Four products, of registers 4 c .. + 3 of the scores.
+  const int h = lane >> 5, x = lane & 31;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    a[i] = *reinterpret_cast<const uint32_t *>(v_at + (32 * kt + 8 * c + 4 * (lane >> 5) + i) * W::v_pitch + (32 * dt + (lane & 31)) * 4);
+    a[i] = *reinterpret_cast<const uint32_t *>(buffer + W::v_at + (32 * kt + 8 * c + 4 * h + i) * W::bytes + 128 * (dt ^ h) + 4 * x);
 #else
-  const char *at = v_at + (32 * kt + 16 * c + 4 * (lane >> 5) + (lane & 15) / 4) * W::v_pitch +
-                   (32 * dt + 16 * (lane >> 4 & 1) + 4 * (lane & 3)) * 2;
-  const u32x2 lo = kh::read_across(at), hi = kh::read_across(at + 8 * W::v_pitch);
+  const int r = (lane & 15) / 4, turn = W::pieces == 8 ? r >> 1 : r;
+  const char *at = buffer + W::v_at + (32 * kt + 16 * c + 4 * (lane >> 5) + r) * W::bytes + 64 * (dt ^ turn) + 32 * (lane >> 4 & 1) +
+                   8 * (lane & 3);
+  const u32x2 lo = kh::read_across(at), hi = kh::read_across(at + 8 * W::bytes);
   a = u32x4{lo.x, lo.y, hi.x, hi.y};
 #endif
   return a;
@@ -666,12 +807,25 @@ __device__ __forceinline__ WideUnit wide_unit(const KhAttentionParams &p, const 
   u.head = in_seq - turn * p.cache.kv_heads;
   u.tile0 = (kh_wide_tiles(s, p.group) - 1 - turn) * kWideTile;
   u.tile_end = u.tile0 + kWideTile < rows ? u.tile0 + kWideTile : rows;
-  u.first = kh_seen(s, (int)kh_div(u.tile0, p.by_group), p.window).first;
+  u.first = kh_seen(s, (int)kh_div(u.tile0, p.by_group), p.window).first & ~15;
   u.end = kh_seen(s, (int)kh_div(u.tile_end - 1, p.by_group), p.window).end;
   return u;
 }
 
-template <int D>
+// Asks the scheduler to read `ahead` operands from LDS before the first of
+// `products` matrix instructions, and one more behind each: left to itself it
+// reads each right before its product, and the wave waits out LDS every time.
+template <int READS, int PRODUCTS, int EACH, int AHEAD>
+__device__ __forceinline__ void read_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < PRODUCTS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (AHEAD + i * EACH < READS) __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+  }
+}
+
+template <int D, bool EVEN>
 __device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char *lds) {
   using W = Wide<D>;
   const int tid = threadIdx.x, lane = kh::lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kh::kWave);
@@ -705,8 +859,8 @@ __device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char
   const char *qp = static_cast<const char *>(p.q) + ((int64_t)(s.start + i) * p.q_stride + (int64_t)hq * d) * (int)sizeof(elem);
 #pragma unroll
   for (int c = 0; c < W::steps; ++c) {
-    q[c] = u32x4{0, 0, 0, 0};
-    if (mine && 32 * c + 16 * h < row_bytes) q[c] = *reinterpret_cast<const u32x4 *>(qp + 32 * c + 16 * h);
+    const u32x4 x = *reinterpret_cast<const u32x4 *>(qp + within(32 * c + 16 * h, row_bytes)) ^ p.q_sign;
+    q[c] = mine && 32 * c + 16 * h < row_bytes ? x : u32x4{0, 0, 0, 0};
   }
   float m = kNegBig, l = 0.0f;
   f32x16 o[W::dts];
@@ -718,51 +872,78 @@ __device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char
   const int all_first = kh_seen(s, (int)kh_div(u.tile_end - 1, p.by_group), p.window).first;
   auto mixed = [&](int key0) { return key0 + W::keys > all_end || key0 < all_first; };
   if (part.first < part.end) {
-    Stage<D> g;
-    seek<D>(g, p, table, part.first, part.end, tid);
-    fetch<D>(g, p, kbase, vbase, part.first, part.end, row_bytes, tid);
-    put<D>(g, lds, mixed(part.first), row_bytes, tid);
-    seek<D>(g, p, table, part.first + W::keys, part.end, tid);
-    fetch<D>(g, p, kbase, vbase, part.first + W::keys, part.end, row_bytes, tid);
-    seek<D>(g, p, table, part.first + 2 * W::keys, part.end, tid);
-    kh::lds_barrier();
+    Stage<D, EVEN> g;
+    uint64_t here = 0, next = 0;  // entries that are there, of this tile and the next
+    seek<D, EVEN>(g, p, table, part.first, part.end, lane, wave);
+    Lanes<D> lanes;
+    if constexpr (EVEN) {
+      lanes = lanes_of<D>(p, row_bytes, lane, wave);
+      next = send<D>(g, lanes, p, kbase, vbase, part.first, part.end, lds, wave);
+      seek<D, EVEN>(g, p, table, part.first + W::keys, part.end, lane, wave);
+    } else {
+      fetch<D>(g, p, kbase, vbase, part.first, part.end, row_bytes, lane, wave);
+    }
     int cur = 0;
     for (int key0 = part.first; key0 < part.end; key0 += W::keys, cur ^= 1) {
-      const char *k_at = lds + cur * W::buffer, *v_at = k_at + W::keys * W::k_pitch;
+      char *buffer = lds + cur * W::buffer;
+      here = next;
+      // One barrier: this tile is there for everyone, and everyone is done with
+      // the tile whose place the next one takes.
+      if constexpr (EVEN) {
+        kh::vm_wait<0>();
+        kh::lds_barrier();
+        if (mixed(key0)) {
+          clean<D>(buffer, lane, wave);
+          kh::lds_barrier();
+        }
+        // The page numbers of the tile after that go out first: whoever waits for
+        // them does not wait for the tile.
+        const Stage<D, EVEN> found = g;
+        seek<D, EVEN>(g, p, table, key0 + 2 * W::keys, part.end, lane, wave);
+        next = send<D>(found, lanes, p, kbase, vbase, key0 + W::keys, part.end, lds + (cur ^ 1) * W::buffer, wave);
+      } else {
+        put<D>(g, buffer, row_bytes, lane, wave);
+        seek<D, EVEN>(g, p, table, key0 + W::keys, part.end, lane, wave);
+        fetch<D>(g, p, kbase, vbase, key0 + W::keys, part.end, row_bytes, lane, wave);
+        kh::lds_barrier();
+        if (mixed(key0)) {
+          clean<D>(buffer, lane, wave);
+          kh::lds_barrier();
+        }
+      }
       // Nothing to do for a wave none of whose rows sees any of the tile.
       if (any && key0 < high.end && key0 + W::keys > low.first) {
         f32x16 x[W::tiles];
 #pragma unroll
-        for (int kt = 0; kt < W::tiles; ++kt) {
-          x[kt] = f32x16{};
+        for (int kt = 0; kt < W::tiles; ++kt) x[kt] = f32x16{};
 #pragma unroll
-          for (int c = 0; c < W::steps; ++c)
-            x[kt] = kh::mma32(*reinterpret_cast<const u32x4 *>(k_at + (32 * kt + r) * W::k_pitch + 32 * c + 16 * h), q[c], x[kt]);
+        for (int c = 0; c < W::steps; ++c)
+#pragma unroll
+          for (int kt = 0; kt < W::tiles; ++kt) x[kt] = kh::mma32(k_rows<D>(buffer, kt, c, lane), q[c], x[kt]);
+        if constexpr (!kh::kWide) read_ahead<W::steps * W::tiles, W::steps * W::tiles, 1, 6>();
+        uint64_t present = here, odds = 0;
+        if constexpr (EVEN) present |= W::keys == 64 ? 0 : ~uint64_t(0) << W::keys % 64;
+        if (!EVEN || mixed(key0)) {
+          const uint32_t mark = lane < W::keys ? (uint8_t)buffer[W::marks_at + lane] : kThere;
+          if (!EVEN) present = __builtin_amdgcn_ballot_w64((mark & kThere) != 0);
+          if (mixed(key0)) odds = __builtin_amdgcn_ballot_w64((mark & kOdd) != 0);
         }
-        const uint32_t mark = lane < W::keys ? reinterpret_cast<const uint8_t *>(v_at + W::keys * W::v_pitch)[lane] : kThere;
-        const uint64_t present = __builtin_amdgcn_ballot_w64((mark & kThere) != 0);
         const bool whole = present == ~uint64_t(0) && key0 + W::keys <= low.end && key0 >= high.first;
-        const uint64_t odds = __builtin_amdgcn_ballot_w64((mark & kOdd) != 0);
-#pragma unroll
-        for (int kt = 0; kt < W::tiles; ++kt)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) x[kt][j] *= p.scale_log2;
         if (!whole) {
+          const uint64_t sees = mine ? seen_of(seen, key0) & present : 0;
 #pragma unroll
-          for (int kt = 0; kt < W::tiles; ++kt)
+          for (int kt = 0; kt < W::tiles; ++kt) {
+            const uint32_t own = (uint32_t)(sees >> 32 * kt) >> 4 * h;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int n = 32 * kt + 8 * (j / 4) + 4 * h + j % 4, key = key0 + n;
-              const bool sees = mine && key >= seen.first && key < seen.end && (present >> n & 1) != 0;
-              x[kt][j] = sees ? x[kt][j] : -__builtin_inff();
-            }
+            for (int j = 0; j < 16; ++j) x[kt][j] = (own >> (8 * (j / 4) + j % 4) & 1) != 0 ? x[kt][j] : -__builtin_inff();
+          }
         }
         float top = x[0][0];
 #pragma unroll
         for (int kt = 0; kt < W::tiles; ++kt)
 #pragma unroll
           for (int j = 0; j < 16; ++j) top = fmaxf(top, x[kt][j]);
-        top = fmaxf(m, over_halves(top, true));
+        top = fmaxf(m, over_halves(top, true) * p.scale_log2);
         if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
           const float fade = kh::exp2_hw(m - top);
           m = top;
@@ -775,7 +956,7 @@ __device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char
         for (int kt = 0; kt < W::tiles; ++kt)
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            x[kt][j] = kh::exp2_hw(x[kt][j] - m);
+            x[kt][j] = kh::exp2_hw(fmaf(x[kt][j], p.scale_log2, -m));
             sum += x[kt][j];
           }
         l += sum;
@@ -785,11 +966,12 @@ __device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char
           const KhSlot at = kh_slot(table, p.table.width, p.cache.pages, p.cache.by_page, (uint32_t)key);
           const char *row = vbase + kh_row(at, p.cache.v_page, p.cache.v_slot);
           if (mine && key >= seen.first && key < seen.end) {
+            const int h1 = apart(h);
 #pragma unroll
             for (int dt = 0; dt < W::dts; ++dt)
 #pragma unroll
               for (int j = 0; j < 16; j += 4) {
-                const int col = 32 * dt + 2 * j + 4 * h;
+                const int col = 32 * dt + 2 * j + 4 * h1;
                 if (col >= d) continue;
                 const f32x4 y = odd_of(row + col * (int)sizeof(elem));
 #pragma unroll
@@ -797,19 +979,23 @@ __device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char
               }
           }
         }
+        // Operands of V are read a step ahead of their products.
+        constexpr int kAll = W::tiles * kPvSteps;
+        u32x4 a[2][W::dts];
 #pragma unroll
-        for (int kt = 0; kt < W::tiles; ++kt)
+        for (int dt = 0; dt < W::dts; ++dt) a[0][dt] = v_across<D>(buffer, 0, 0, dt, lane);
 #pragma unroll
-          for (int c = 0; c < kPvSteps; ++c) {
-            const u32x4 b = p_of(x[kt], c);
+        for (int n = 0; n < kAll; ++n) {
+          if (n + 1 < kAll) {
 #pragma unroll
-            for (int dt = 0; dt < W::dts; ++dt) o[dt] = kh::mma32(v_across<D>(v_at, kt, c, dt, lane), b, o[dt]);
+            for (int dt = 0; dt < W::dts; ++dt) a[(n + 1) % 2][dt] = v_across<D>(buffer, (n + 1) / kPvSteps, (n + 1) % kPvSteps, dt, lane);
           }
+          __builtin_amdgcn_sched_barrier(0);
+          const u32x4 b = p_of(x[n / kPvSteps], n % kPvSteps);
+#pragma unroll
+          for (int dt = 0; dt < W::dts; ++dt) o[dt] = kh::mma32(a[n % 2][dt], b, o[dt]);
+        }
       }
-      put<D>(g, lds + (cur ^ 1) * W::buffer, mixed(key0 + W::keys), row_bytes, tid);
-      fetch<D>(g, p, kbase, vbase, key0 + 2 * W::keys, part.end, row_bytes, tid);
-      seek<D>(g, p, table, key0 + 3 * W::keys, part.end, tid);
-      kh::lds_barrier();
     }
   }
 
@@ -889,13 +1075,17 @@ __device__ __forceinline__ bool wide_parts(const KhAttentionParams &p, int unit,
   return true;
 }
 
-constexpr int kJoinParts = 32;  // statistics brought to LDS at a time
+constexpr int kJoinParts = 64;  // statistics brought to LDS at a time
+constexpr int kJoinAhead = 16;  // parts whose rows are in flight
 
 // Joins the parts of 16 rows: a workgroup for every workgroup's start, then one
-// for each 16 rows of the wide units. A thread has 4 columns of a row.
+// for each 16 rows of the wide units. A thread has 4 columns of a row, and where
+// that leaves threads over (few rows), only each second or fourth part of it.
+// The parts were written through other L2s, so that each round of loads takes
+// its time: bound by how many there are in a row.
 template <int D>
 __device__ __forceinline__ void join(const KhAttentionParams &p, float *lds) {
-  constexpr int kItems = kRows * (D / 4) / 256;
+  constexpr int kCols = D / 4;
   const int tid = threadIdx.x, d = p.cache.head_dim;
   const int narrow_blocks = p.whole ? 0 : p.groups, block = (int)blockIdx.x - narrow_blocks;
   constexpr int kPer = kWideTile / kRows;
@@ -908,48 +1098,70 @@ __device__ __forceinline__ void join(const KhAttentionParams &p, float *lds) {
     const int R = parts.R0 + row, i = (int)kh_div(R, p.by_group);
     return (int64_t)(s.start + i) * p.q_heads + parts.head * p.group + R - i * p.group;
   };
-  f32x4 o[kItems];
-  float m[kItems], total[kItems];
-  int64_t place[kItems];
-#pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    const int row = (tid + 256 * j) / (D / 4);
-    o[j] = f32x4{0, 0, 0, 0}, m[j] = kNegBig, total[j] = 0.0f, place[j] = place_of(row < parts.rows ? row : 0);
-  }
-  for (int k0 = 0; k0 < parts.count; k0 += kJoinParts) {
-    const int here = parts.count - k0 < kJoinParts ? parts.count - k0 : kJoinParts;
-    for (int x = tid; x < here * kRows; x += 256) {
-      const int k = x / kRows, row = x % kRows;
-      const float *from = parts.ml + (base(k0 + k) + place_of(row < parts.rows ? row : 0)) * 2;
-      lds[2 * x] = from[0], lds[2 * x + 1] = from[1];
-    }
-    kh::lds_barrier();
-#pragma unroll
-    for (int j = 0; j < kItems; ++j) {
-      const int row = (tid + 256 * j) / (D / 4), col = (tid + 256 * j) % (D / 4) * 4;
-      if (row >= parts.rows || col >= d) continue;
-      float top = m[j];
-      for (int k = 0; k < here; ++k) top = fmaxf(top, lds[2 * (k * kRows + row)]);
-      const float fade = kh::exp2_hw(m[j] - top);
-      m[j] = top, total[j] *= fade, o[j] *= fade;
-#pragma unroll 8
-      for (int k = 0; k < here; ++k) {
-        const float w = kh::exp2_hw(lds[2 * (k * kRows + row)] - top);
-        total[j] += lds[2 * (k * kRows + row) + 1] * w;
-        o[j] += *reinterpret_cast<const f32x4 *>(parts.o + (base(k0 + k) + place[j]) * d + col) * w;
+  // Rows rounded up to a power of two, times columns: items; threads that share one.
+  const int rows2 = parts.rows <= 1 ? 1 : parts.rows <= 2 ? 2 : parts.rows <= 4 ? 4 : parts.rows <= 8 ? 8 : 16;
+  const int items = rows2 * kCols, shares = items >= 256 ? 1 : 256 / items < 4 ? 256 / items : 4;
+  for (int item0 = 0; item0 < items; item0 += 256) {
+    const int share = tid / items, item = item0 + tid % items;  // item0 > 0: shares = 1
+    const int row = item / kCols, col = item % kCols * 4;
+    const bool live = row < parts.rows && col < d && share < shares;
+    const int64_t place = place_of(live ? row : 0);
+    f32x4 o = {0, 0, 0, 0};
+    float m = kNegBig, total = 0.0f;
+    for (int k0 = 0; k0 < parts.count; k0 += kJoinParts) {
+      const int here = parts.count - k0 < kJoinParts ? parts.count - k0 : kJoinParts;
+      for (int x = tid; x < here * kRows; x += 256) {
+        const int k = x / kRows, r = x % kRows;
+        const float *from = parts.ml + (base(k0 + k) + place_of(r < parts.rows ? r : 0)) * 2;
+        lds[2 * x] = from[0], lds[2 * x + 1] = from[1];
       }
-    }
-    kh::lds_barrier();
-  }
+      kh::lds_barrier();
+      if (live) {
+        float top = m;
+        for (int k = 0; k < here; ++k) top = fmaxf(top, lds[2 * (k * kRows + row)]);
+        const float fade = kh::exp2_hw(m - top);
+        m = top, total *= fade, o *= fade;
+        for (int k1 = share; k1 < here; k1 += kJoinAhead * shares) {
+          f32x4 x[kJoinAhead];
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    const int row = (tid + 256 * j) / (D / 4), col = (tid + 256 * j) % (D / 4) * 4;
-    if (row >= parts.rows || col >= d) continue;
+          for (int j = 0; j < kJoinAhead; ++j) {
+            const int k = k1 + j * shares;
+            x[j] = *reinterpret_cast<const f32x4 *>(parts.o + (base(k0 + (k < here ? k : here - 1)) + place) * d + col);
+          }
+#pragma unroll
+          for (int j = 0; j < kJoinAhead; ++j) {
+            const int k = k1 + j * shares;
+            if (k < here) {
+              const float w = kh::exp2_hw(lds[2 * (k * kRows + row)] - top);
+              total += lds[2 * (k * kRows + row) + 1] * w;
+              o += x[j] * w;
+            }
+          }
+        }
+      }
+      kh::lds_barrier();
+    }
+    // The shares' sums, in their order.
+    if (shares > 1) {
+      float *sum = lds + 5 * tid;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = o[e];
+      sum[4] = total;
+      kh::lds_barrier();
+      if (share == 0)
+        for (int k = 1; k < shares; ++k) {
+          const float *other = lds + 5 * (tid + k * items);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] += other[e];
+          total += other[4];
+        }
+    }
+    if (!live || share != 0) continue;
     const int R = parts.R0 + row, i = (int)kh_div(R, p.by_group), hq = parts.head * p.group + R - i * p.group;
-    const float inv = total[j] == 0.0f ? 0.0f : 1.0f / total[j];
-    const float y[4] = {o[j].x * inv, o[j].y * inv, o[j].z * inv, o[j].w * inv};
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     kh::store4(static_cast<elem *>(p.out) + (int64_t)(s.start + i) * p.out_stride + (int64_t)hq * d + col, y);
-    if (col == 0 && p.lse != nullptr) p.lse[(int64_t)(s.start + i) * p.q_heads + hq] = lse_of(m[j], total[j]);
+    if (col == 0 && p.lse != nullptr) p.lse[(int64_t)(s.start + i) * p.q_heads + hq] = lse_of(m, total);
   }
 }
 
@@ -960,19 +1172,29 @@ __device__ __forceinline__ void join(const KhAttentionParams &p, float *lds) {
 #define KH_ATTENTION(D, PER_CU)                                                                                  \
   extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED(paged_attention_##D)(const KhAttentionParams p) { \
     __shared__ float lds[kWaves * kRows * 2 + kRows + kWaves * kRows * (D + 4)];                                 \
-    narrow<D>(p, (int)blockIdx.x, lds);                                                                          \
+    if (p.even)                                                                                                  \
+      narrow<D, true>(p, (int)blockIdx.x, lds);                                                                  \
+    else                                                                                                         \
+      narrow<D, false>(p, (int)blockIdx.x, lds);                                                                 \
   }
 KH_ATTENTION(64, 2)
 KH_ATTENTION(128, 2)
 KH_ATTENTION(256, 1)
 // Steps with sequences of many rows: their workgroups first, the longest there are.
+template <int D, bool EVEN>
+__device__ __forceinline__ void either(const KhAttentionParams &p, char *lds) {
+  if ((int)blockIdx.x < p.wide_blocks)
+    wide<D, EVEN>(p, (int)blockIdx.x, lds);
+  else
+    narrow<D, EVEN>(p, (int)blockIdx.x - p.wide_blocks, reinterpret_cast<float *>(lds));
+}
 #define KH_ATTENTION_WIDE(D, PER_CU)                                                                              \
   extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED(paged_attention_wide_##D)(const KhAttentionParams p) { \
     __shared__ __attribute__((aligned(16))) char lds[Wide<D>::lds];                                               \
-    if ((int)blockIdx.x < p.wide_blocks)                                                                          \
-      wide<D>(p, (int)blockIdx.x, lds);                                                                           \
+    if (p.even)                                                                                                   \
+      either<D, true>(p, lds);                                                                                    \
     else                                                                                                          \
-      narrow<D>(p, (int)blockIdx.x - p.wide_blocks, reinterpret_cast<float *>(lds));                              \
+      either<D, false>(p, lds);                                                                                   \
   }
 KH_ATTENTION_WIDE(64, 2)
 KH_ATTENTION_WIDE(128, kh::kWide ? 1 : 2)

@@ -302,12 +302,19 @@ int kh_paged_attention(const kh_paged_attention_args *args, void *workspace, siz
       wide_ml = part_ml + (plan.part_bytes > 0 ? plan.groups * 2 * KH_TILE_ROWS * 2 : 0);
     }
     const int64_t wide_blocks = plan.wide_units * plan.splits;
+    const int e = element_bytes(a.cache.dtype);
+    // Rows that follow each other 16 at a time, none longer than their distance,
+    // and 16 of those distances in 31 bits.
+    const auto [near, far] = std::minmax(a.cache.k_slot_stride, a.cache.v_slot_stride);
+    const bool even = a.cache.page_size % 16 == 0 && near >= d && far * e < 1 << 27;
     KhAttentionParams p{device_cache(a.cache), device_table(a.table, a.cache), a.q, a.out, a.lse, a.q_starts, part_o, part_ml,
                         wide_o, wide_ml, a.q_stride, a.out_stride, static_cast<int32_t>(a.tokens),
                         static_cast<int32_t>(a.q_heads), static_cast<int32_t>(group), static_cast<int32_t>(a.window),
                         static_cast<int32_t>(plan.groups), plan.whole, static_cast<int32_t>(plan.narrow_rows),
                         static_cast<int32_t>(wide_blocks), static_cast<int32_t>(std::max<int64_t>(plan.splits, 1)),
-                        kh_div_by(static_cast<uint32_t>(group)), a.scale * 1.44269504088896340736f};
+                        even, a.scale < 0.0f ? (e == 4 ? 0x80000000u : 0x80008000u) : 0u,
+                        kh_div_by(static_cast<uint32_t>(group)),
+                        std::max(std::fabs(a.scale) * 1.44269504088896340736f, 1e-37f)};
     const auto &symbols = wide_blocks > 0 ? kWide : kAttention;
     if (int rc = launch(symbols[width_of(d)][a.cache.dtype], wide_blocks + plan.groups, 1, 256, p, stream)) return rc;
     if (!joined) return 0;
