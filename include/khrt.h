@@ -486,6 +486,7 @@ KHRT_API int kh_paged_attention(const kh_paged_attention_args *args, void *works
  * for j < lens[s]; behind that the row is left as it was. lse is the attention's
  * of the same tokens (-inf: adds nothing). weights_in null: zeros; it may be
  * weights itself. Both have the strides given, at least lens[s] floats a row.
+ * q_stride is below 2^24 bytes.
  * The order of the sums is fixed: a repeated call gives the same bits. */
 typedef struct kh_paged_weights_args {
   kh_paged_cache cache;

@@ -128,6 +128,27 @@ __device__ __forceinline__ void dma16(u32x4 rsrc, uint32_t voff, uint32_t lds) {
       : "memory", "m0");
 }
 
+// The same for 4 bytes a lane.
+__device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t voff, uint32_t lds) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dword %1, %2, 0 offen lds"
+      :
+      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(rsrc)
+      : "memory", "m0");
+}
+
+// For LDS that the wave alone uses: all but the last N vector-memory operations
+// are done, and what they brought is read after this.
+template <int N>
+__device__ __forceinline__ void arrived() {
+  vm_wait<N>();
+  asm volatile("" ::: "memory");
+}
+
 #if KH_ELEM != 0
 // Of 4 x 16 elements in LDS that the 16 lanes of a row point at (lane 4 r + c:
 // row r, columns 4 c ..), lane i receives column i, its four rows in order

@@ -244,6 +244,7 @@ struct KhWeightsParams {
   float *weights;
   int64_t q_stride, seq_stride, head_stride;
   int32_t tokens, q_heads, group, window;
+  int32_t chunk_keys, chunks, even;  // of a workgroup, a multiple of KH_STRETCH; that the launch has; KhAttentionParams
   KhDiv by_group;
   float scale_log2;
 };

@@ -107,6 +107,13 @@ KhTable device_table(const kh_page_table &t, const kh_paged_cache &c) {
                  static_cast<int32_t>(capacity_of(t.width, c.page_size))};
 }
 
+// Rows that follow each other 16 at a time, none longer than their distance,
+// and 16 of those distances in 31 bits: pages are walked 16 entries at a time.
+bool even_pages(const kh_paged_cache &c) {
+  const auto [near, far] = std::minmax(c.k_slot_stride, c.v_slot_stride);
+  return c.page_size % 16 == 0 && near >= c.head_dim && far * element_bytes(c.dtype) < 1 << 27;
+}
+
 // The longest sequence that a launch is sized for.
 int64_t expected_len(const kh_page_table &t, const kh_paged_cache &c) {
   const int64_t all = capacity_of(t.width, c.page_size);
@@ -303,10 +310,7 @@ int kh_paged_attention(const kh_paged_attention_args *args, void *workspace, siz
     }
     const int64_t wide_blocks = plan.wide_units * plan.splits;
     const int e = element_bytes(a.cache.dtype);
-    // Rows that follow each other 16 at a time, none longer than their distance,
-    // and 16 of those distances in 31 bits.
-    const auto [near, far] = std::minmax(a.cache.k_slot_stride, a.cache.v_slot_stride);
-    const bool even = a.cache.page_size % 16 == 0 && near >= d && far * e < 1 << 27;
+    const bool even = even_pages(a.cache);
     KhAttentionParams p{device_cache(a.cache), device_table(a.table, a.cache), a.q, a.out, a.lse, a.q_starts, part_o, part_ml,
                         wide_o, wide_ml, a.q_stride, a.out_stride, static_cast<int32_t>(a.tokens),
                         static_cast<int32_t>(a.q_heads), static_cast<int32_t>(group), static_cast<int32_t>(a.window),
@@ -337,13 +341,21 @@ int kh_paged_weights(const kh_paged_weights_args *args, void *stream) {
         a.weights_head_stride > kMaxStride || (a.cache.kv_heads > 1 && a.weights_head_stride == 0) ||
         (a.table.seqs > 1 && a.weights_seq_stride == 0))
       return bad(op, "strides of weights must be positive");
-    const int64_t group = a.q_heads / a.cache.kv_heads;
+    const int e = element_bytes(a.cache.dtype);
+    if (a.q_stride * e >= 1 << 24) return bad(op, "q_stride must be below 2^24 bytes");
+    const int64_t group = a.q_heads / a.cache.kv_heads, pairs = a.cache.kv_heads * a.table.seqs;
+    // Chunks as long as leaves every CU some eight workgroups, up to 512 entries
+    // (four blocks of a wave); one stretch where sequences may have many rows.
+    const int64_t len = expected_len(a.table, a.cache), stretches = ceil_div(len, KH_STRETCH);
+    const bool few = a.tokens * group <= 32 * a.table.seqs;
+    const int64_t each = few ? std::clamp<int64_t>(pairs * stretches / (4 * KH_GEMM_CUS), 1, 8) : 1;
+    const int64_t chunks = std::min(ceil_div(stretches, each), std::max<int64_t>(1, (int64_t(1) << 22) / pairs));
     KhWeightsParams p{device_cache(a.cache), device_table(a.table, a.cache), a.q, a.lse, a.q_starts, a.weights_in, a.weights,
                       a.q_stride, a.weights_seq_stride, a.weights_head_stride, static_cast<int32_t>(a.tokens),
                       static_cast<int32_t>(a.q_heads), static_cast<int32_t>(group), static_cast<int32_t>(a.window),
+                      static_cast<int32_t>(each * KH_STRETCH), static_cast<int32_t>(chunks), even_pages(a.cache),
                       kh_div_by(static_cast<uint32_t>(group)), a.scale * 1.44269504088896340736f};
-    const int64_t y = std::min<int64_t>(ceil_div(expected_len(a.table, a.cache), 128), 65535);
-    return launch(kWeights[width_of(a.cache.head_dim)][a.cache.dtype], a.cache.kv_heads * a.table.seqs, y, 256, p, stream);
+    return launch(kWeights[width_of(a.cache.head_dim)][a.cache.dtype], pairs * chunks, 1, 256, p, stream);
   });
 }
 

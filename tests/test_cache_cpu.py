@@ -125,7 +125,7 @@ def test_attention_refuses_a_misaligned_workspace():
 
 
 @pytest.mark.parametrize("kw", [dict(lse=None), dict(weights=None), dict(weights_seq_stride=-1), dict(weights_head_stride=0),
-                                dict(weights_seq_stride=0), dict(weights_head_stride=1 << 41)], ids=str)
+                                dict(weights_seq_stride=0), dict(weights_head_stride=1 << 41), dict(q_stride=1 << 23)], ids=str)
 def test_weights_refuse(kw):
     refused(lambda: kh.paged_weights(weights(**kw)), "paged_weights")
 
