@@ -156,6 +156,18 @@ __device__ __forceinline__ float row16_max(float v) {
   return v;
 }
 
+// Sum over the lanes up to this one: within rows of 16 lanes, then each row's
+// last lane to the rows behind it.
+__device__ __forceinline__ int up_to(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // dwordx4 loads/stores with the nontemporal hint: streamed data that is
 // touched once should not displace reusable lines in L2 / the MALL. On
 // MI355X this lifts streaming kernels from ~5.4 to ~5.9-6.1 TB/s.

@@ -245,6 +245,7 @@ struct KhWeightsParams {
   int64_t q_stride, seq_stride, head_stride;
   int32_t tokens, q_heads, group, window;
   int32_t chunk_keys, chunks, even;  // of a workgroup, a multiple of KH_STRETCH; that the launch has; KhAttentionParams
+  int32_t steady;  // 32 rows are whole tokens, and no two tokens of q share bytes
   KhDiv by_group;
   float scale_log2;
 };
@@ -260,4 +261,7 @@ struct KhEvictParams {
   int32_t *chosen;  // [seqs][kv_heads][budget]
   int64_t kept_row_stride, in_seq_stride, in_head_stride, seq_stride, head_stride;
   int32_t kept_width, budget, recent, element;
+  int32_t lanes, chunks;  // paged_evict_move: lanes to a row, workgroups to a sequence
+  int32_t heads_inner;    // the heads of an entry lie nearer than its neighbours
+  KhDiv by_heads;
 };

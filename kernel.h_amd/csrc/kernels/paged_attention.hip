@@ -139,18 +139,6 @@ __device__ __forceinline__ KhSeq sequence(const KhAttentionParams &p, int seq) {
   return kh_seq(p.table.lens[seq], p.q_starts[seq], p.q_starts[seq + 1], p.table.capacity, p.tokens);
 }
 
-// Sum over the lanes up to this one: within rows of 16 lanes, then each row's
-// last lane to the rows behind it.
-__device__ __forceinline__ int up_to(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
-  return v;
-}
-
 // The step's blocks, and of the first 64 sequences, one to a lane, what they
 // are and how many blocks they have.
 struct Line {

@@ -279,22 +279,36 @@ __device__ __forceinline__ void few(const KhWeightsParams &p, const Job &j, int 
   }
 }
 
-// Sends a tile of rows of q to LDS.
+// Where a lane's pieces of a tile of rows of q lie, past the tile's first token.
+// `steady` (the tile holds whole tokens, and no two share bytes): the same for
+// every tile, and the resource's end keeps out rows past the last; otherwise
+// they are kept out here.
 template <int D>
-__device__ __forceinline__ void send(const KhWeightsParams &p, const Job &j, int R0, const char *buffer, int lane, int wave) {
+__device__ __forceinline__ void pieces_of(const KhWeightsParams &p, const Job &j, int R0, uint32_t (&off)[Rows<D>::passes], int lane, int wave) {
   using W = Rows<D>;
-  const int row_bytes = p.cache.head_dim * (int)sizeof(elem);
-  const int i0 = (int)kh_div(R0, p.by_group);
-  const uint64_t at = (uint64_t)reinterpret_cast<uintptr_t>(p.q) +
-                      (uint64_t)((int64_t)(j.s.start + i0) * p.q_stride + (int64_t)j.head * p.group * p.cache.head_dim) * sizeof(elem);
-  const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32), kOutside, 0x00020000u};
+  const int row_bytes = p.cache.head_dim * (int)sizeof(elem), i0 = (int)kh_div(R0, p.by_group);
 #pragma unroll
   for (int i = 0; i < W::passes; ++i) {
-    const int first = wave * W::share + i * W::per_wave, row = first + lane / W::pieces, R = R0 + row;
+    const int row = wave * W::share + i * W::per_wave + lane / W::pieces, R = R0 + row;
     const int t = (int)kh_div(R, p.by_group), c = 16 * (lane % W::pieces ^ k_turn<D>(row));
-    const uint32_t off = (uint32_t)(t - i0) * (uint32_t)(p.q_stride * (int)sizeof(elem)) + (uint32_t)((R - t * p.group) * row_bytes + c);
-    dma16(rsrc, R < j.rows && c < row_bytes ? off : kOutside, (uint32_t)reinterpret_cast<uintptr_t>(buffer) + (uint32_t)(first * W::bytes));
+    off[i] = (uint32_t)(t - i0) * (uint32_t)(p.q_stride * (int)sizeof(elem)) + (uint32_t)((R - t * p.group) * row_bytes + c);
+    if (c >= row_bytes || (!p.steady && R >= j.rows)) off[i] = kOutside;
   }
+}
+
+// Sends a tile of rows of q to LDS.
+template <int D>
+__device__ __forceinline__ void send(const KhWeightsParams &p, const Job &j, int R0, const uint32_t (&off)[Rows<D>::passes],
+                                     const char *buffer, int wave) {
+  using W = Rows<D>;
+  const int i0 = (int)kh_div(R0, p.by_group), left = j.s.m > i0 ? j.s.m - i0 : 0;
+  const uint64_t at = (uint64_t)reinterpret_cast<uintptr_t>(p.q) +
+                      (uint64_t)((int64_t)(j.s.start + i0) * p.q_stride + (int64_t)j.head * p.group * p.cache.head_dim) * sizeof(elem);
+  const uint64_t bytes = (uint64_t)left * (uint64_t)p.q_stride * sizeof(elem);
+  const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32), p.steady && bytes < kOutside ? (uint32_t)bytes : kOutside, 0x00020000u};
+#pragma unroll
+  for (int i = 0; i < W::passes; ++i)
+    dma16(rsrc, off[i], (uint32_t)reinterpret_cast<uintptr_t>(buffer) + (uint32_t)((wave * W::share + i * W::per_wave) * W::bytes));
 }
 
 template <int D>
@@ -328,20 +342,24 @@ __device__ __forceinline__ void wide(const KhWeightsParams &p, const Job &j, int
   if (R_begin < R_end) {
     // The tile's lse: a thread's row, a tile ahead as the rows are.
     auto lse_at = [&](int R0) {
+      if (wave >= (W::tile + kWave - 1) / kWave) return 0.0f;
       const int R = R0 + tid % W::tile, real = R < j.rows ? R : 0, i = (int)kh_div(real, p.by_group);
-      return taken(p.lse[(int64_t)(j.s.start + i) * p.q_heads + j.head * p.group + real - i * p.group], R < j.rows);
+      return p.lse[(int64_t)(j.s.start + i) * p.q_heads + j.head * p.group + real - i * p.group];
     };
     float ahead = lse_at(R_begin);
-    send<D>(p, j, R_begin, lds, lane, wave);
+    uint32_t off[W::passes];
+    pieces_of<D>(p, j, R_begin, off, lane, wave);
+    send<D>(p, j, R_begin, off, lds, wave);
     int cur = 0;
     for (int R0 = R_begin; R0 < R_end; R0 += W::tile, cur ^= 1) {
       const char *buffer = lds + cur * kBuffer;
       float *lse = stats + cur * W::tile;
-      if (tid < W::tile) lse[tid] = ahead;
       vm_wait<0>();
+      if (tid < W::tile) lse[tid] = taken(ahead, R0 + tid < j.rows);
       lds_barrier();
       ahead = lse_at(R0 + W::tile);
-      send<D>(p, j, R0 + W::tile, lds + (cur ^ 1) * kBuffer, lane, wave);
+      if (!p.steady) pieces_of<D>(p, j, R0 + W::tile, off, lane, wave);
+      send<D>(p, j, R0 + W::tile, off, lds + (cur ^ 1) * kBuffer, wave);
 #pragma unroll
       for (int t = 0; t < W::tile / 32; ++t) {
         const int R1 = R0 + 32 * t;
@@ -373,7 +391,8 @@ __device__ __forceinline__ void wide(const KhWeightsParams &p, const Job &j, int
   if (h == 0 && key < j.s.n) p.weights[j.row + key] = kept(p, j, key, old) + (there ? sum : 0.0f);
 }
 
-template <int D, bool EVEN>
+// RING: there is LDS for few_even().
+template <int D, bool RING>
 __device__ __forceinline__ void weights(const KhWeightsParams &p, char *lds) {
   Job j;
   const int pairs = p.table.seqs * p.cache.kv_heads, chunk = (int)blockIdx.x / pairs, pair = (int)blockIdx.x - chunk * pairs;
@@ -387,7 +406,7 @@ __device__ __forceinline__ void weights(const KhWeightsParams &p, char *lds) {
   for (int64_t first = (int64_t)chunk * p.chunk_keys; first < j.s.n; first += (int64_t)p.chunks * p.chunk_keys) {
     const int end = first + p.chunk_keys < j.s.n ? (int)first + p.chunk_keys : j.s.n;
     if (j.rows <= kFewRows) {
-      if constexpr (EVEN)
+      if constexpr (RING)
         few_even<D>(p, j, (int)first, end, lds);
       else
         few<D>(p, j, (int)first, end);
@@ -402,6 +421,7 @@ __device__ __forceinline__ void weights(const KhWeightsParams &p, char *lds) {
 
 }  // namespace
 
+// Steps of single tokens, and of few: with the ring, two workgroups to a CU.
 #define KH_WEIGHTS(D)                                                                                      \
   extern "C" __global__ void __launch_bounds__(256, D > 128 ? 1 : 2) KH_TYPED(paged_weights_##D)(const KhWeightsParams p) { \
     constexpr int kWideLds = 2 * Rows<D>::tile * (Rows<D>::bytes + 4);                                      \
@@ -414,3 +434,13 @@ __device__ __forceinline__ void weights(const KhWeightsParams &p, char *lds) {
 KH_WEIGHTS(64)
 KH_WEIGHTS(128)
 KH_WEIGHTS(256)
+// Steps with chunks: without it, three (bf16, heads of 128, 2 x 1024 tokens at
+// 32 heads over 6000 entries: 109 us, or 706 TFLOP/s; with the ring's LDS 171).
+#define KH_WEIGHTS_WIDE(D)                                                                                 \
+  extern "C" __global__ void __launch_bounds__(256, D > 128 ? 1 : 3) KH_TYPED(paged_weights_wide_##D)(const KhWeightsParams p) { \
+    __shared__ __attribute__((aligned(16))) char lds[2 * Rows<D>::tile * (Rows<D>::bytes + 4)];             \
+    weights<D, false>(p, lds);                                                                              \
+  }
+KH_WEIGHTS_WIDE(64)
+KH_WEIGHTS_WIDE(128)
+KH_WEIGHTS_WIDE(256)

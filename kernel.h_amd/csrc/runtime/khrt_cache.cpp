@@ -156,6 +156,8 @@ const Symbol kJoin[3][3] = {KH_BY_TYPE(paged_attention, "_join_64"), KH_BY_TYPE(
                             KH_BY_TYPE(paged_attention, "_join_256")};
 const Symbol kWeights[3][3] = {KH_BY_TYPE(paged_weights, "_64"), KH_BY_TYPE(paged_weights, "_128"),
                                KH_BY_TYPE(paged_weights, "_256")};
+const Symbol kWeightsWide[3][3] = {KH_BY_TYPE(paged_weights, "_wide_64"), KH_BY_TYPE(paged_weights, "_wide_128"),
+                                   KH_BY_TYPE(paged_weights, "_wide_256")};
 const Symbol kChoose = {"paged_evict", "paged_evict_choose"};
 const Symbol kMove = {"paged_evict", "paged_evict_move"};
 
@@ -354,8 +356,8 @@ int kh_paged_weights(const kh_paged_weights_args *args, void *stream) {
                       a.q_stride, a.weights_seq_stride, a.weights_head_stride, static_cast<int32_t>(a.tokens),
                       static_cast<int32_t>(a.q_heads), static_cast<int32_t>(group), static_cast<int32_t>(a.window),
                       static_cast<int32_t>(each * KH_STRETCH), static_cast<int32_t>(chunks), even_pages(a.cache),
-                      kh_div_by(static_cast<uint32_t>(group)), a.scale * 1.44269504088896340736f};
-    return launch(kWeights[width_of(a.cache.head_dim)][a.cache.dtype], pairs * chunks, 1, 256, p, stream);
+                      32 % group == 0 && a.q_stride >= a.q_heads * a.cache.head_dim, kh_div_by(static_cast<uint32_t>(group)), a.scale * 1.44269504088896340736f};
+    return launch((few ? kWeights : kWeightsWide)[width_of(a.cache.head_dim)][a.cache.dtype], pairs * chunks, 1, 256, p, stream);
   });
 }
 
@@ -363,7 +365,8 @@ static int check_evict(const char *op, const kh_paged_evict_args &a) {
   if (int rc = check_cache(op, a.cache, true)) return rc;
   if (int rc = check_table(op, a.table, a.cache)) return rc;
   if (!a.kept_pages || !a.kept_lens || !a.weights_in || !a.weights) return bad(op, "null buffer");
-  if (a.budget <= 0 || a.budget > kCapacity) return bad(op, "budget must be positive");
+  if (a.budget <= 0 || a.budget > kCapacity || a.budget * a.cache.kv_heads > kMaxRows)
+    return bad(op, "budget must be positive, and at most 2^30 rows of a sequence");
   if (a.recent < 0 || a.recent > a.budget) return bad(op, "recent must be in [0, budget]");
   if (a.kept_width <= 0 || a.kept_width > INT32_MAX || a.kept_row_stride < 0 || a.kept_row_stride > kMaxStride ||
       (a.table.seqs > 1 && a.kept_row_stride < a.kept_width))
@@ -403,15 +406,18 @@ int kh_paged_evict(const kh_paged_evict_args *args, void *workspace, size_t work
     if (workspace == nullptr || workspace_bytes < evict_bytes(a))
       return bad(op, "workspace of " + std::to_string(evict_bytes(a)) + " bytes needed");
     if (!aligned(workspace)) return bad(op, "workspace must be 16-byte aligned");
+    const int64_t pairs = a.cache.kv_heads * a.table.seqs, pieces = a.cache.head_dim * element_bytes(a.cache.dtype) / 16;
+    int lanes = 1;
+    while (lanes < pieces) lanes *= 2;
+    const int64_t chunks = std::min(ceil_div(a.budget * a.cache.kv_heads, 4 * 256 / lanes),
+                                    std::max<int64_t>(1, (int64_t(1) << 22) / a.table.seqs));
     KhEvictParams p{device_cache(a.cache), device_table(a.table, a.cache), a.kept_pages, a.kept_lens, a.weights_in, a.weights,
                     static_cast<int32_t *>(workspace), a.kept_row_stride, a.in_seq_stride, a.in_head_stride, a.seq_stride,
                     a.head_stride, static_cast<int32_t>(a.kept_width), static_cast<int32_t>(a.budget),
-                    static_cast<int32_t>(a.recent), element_bytes(a.cache.dtype)};
-    const int64_t pairs = a.cache.kv_heads * a.table.seqs;
+                    static_cast<int32_t>(a.recent), element_bytes(a.cache.dtype), lanes, static_cast<int32_t>(chunks),
+                    a.cache.k_head_stride < a.cache.k_slot_stride, kh_div_by(static_cast<uint32_t>(a.cache.kv_heads))};
     if (int rc = launch(kChoose, pairs, 1, 1024, p, stream)) return rc;
-    const int64_t pieces = a.budget * (a.cache.head_dim * element_bytes(a.cache.dtype) / 16);
-    const int64_t y = std::clamp<int64_t>(ceil_div(pieces, 256 * 4), 1, std::max<int64_t>(1, 16 * KH_GEMM_CUS / pairs));
-    return launch(kMove, pairs, std::min<int64_t>(y, 65535), 256, p, stream);
+    return launch(kMove, a.table.seqs * chunks, 1, 256, p, stream);
   });
 }
 

@@ -132,6 +132,7 @@ def test_weights_refuse(kw):
 
 @pytest.mark.parametrize("kw", [
     dict(kept_pages=None), dict(kept_lens=None), dict(weights_in=None), dict(weights=None), dict(budget=0), dict(budget=-1),
+    dict(budget=1 << 30, kept_width=1 << 28, seq_stride=1 << 32, head_stride=1 << 31),
     dict(recent=-1), dict(recent=41), dict(kept_width=0), dict(kept_row_stride=2), dict(kept_row_stride=-1), dict(budget=49),
     dict(kept_pages=1 << 12), dict(kept_lens=2 << 12), dict(weights=16), dict(seq_stride=39), dict(head_stride=39),
     dict(in_seq_stride=-1), dict(in_head_stride=-1)], ids=str)

@@ -417,7 +417,8 @@ def test_eviction(dev, dtype, hk, d, page_size, budget, recent):
     run_evict(dtype, [300, 100, 101, 0, 1, 64, -3, 257], hk, d, budget, recent, page_size, seed=budget + d)
 
 
-@pytest.mark.parametrize("n,budget,recent", [(5000, 4096, 256), (1025, 1024, 1), (1024, 1023, 0), (3000, 17, 5), (2049, 2048, 2048)])
+@pytest.mark.parametrize("n,budget,recent", [(5000, 4096, 256), (1025, 1024, 1), (1024, 1023, 0), (3000, 17, 5), (2049, 2048, 2048),
+                                             (16384, 9000, 7), (16386, 16000, 100), (40000, 3333, 1111)])
 def test_eviction_of_longer_sequences(dev, n, budget, recent):
     run_evict("bf16", [n, n - 1], 2, 64, budget, recent, seed=n)
 
