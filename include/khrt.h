@@ -381,8 +381,9 @@ KHRT_API int khrt_bench_row_work(const char *kernel, const char *shape, double *
  * up the attention that each entry received (kh_paged_weights), and keep only
  * the entries that received most (kh_paged_evict). All are asynchronous on
  * `stream`, allocate nothing, take device pointers, and may be captured into a
- * graph; what a captured graph uses (workspaces included) is its own until it
- * has been replayed.
+ * graph after one eager call of the same kind and types (a first call loads its
+ * code object); what a captured graph uses (workspaces included) is its own
+ * until it has been replayed.
  *
  * Element types: fp32, fp16 and bf16; products, sums, norms and softmax
  * statistics are in 32 bits. head_dim is a multiple of 8 up to 256. Rows of
@@ -511,7 +512,8 @@ KHRT_API int kh_paged_weights(const kh_paged_weights_args *args, void *stream);
  * kept_lens[s] = min(n, budget). The caller's to see to: pages of kept_pages are
  * in it once, and no sequence of the call reads them (the source's pages may be
  * shared, and can be freed afterwards). The arrays written must not be those
- * read. workspace: kh_paged_evict_workspace bytes, 16-byte aligned. */
+ * read. budget * kv_heads is below 2^30. workspace: kh_paged_evict_workspace
+ * bytes, 16-byte aligned. */
 typedef struct kh_paged_evict_args {
   kh_paged_cache cache;
   kh_page_table table;

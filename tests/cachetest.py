@@ -241,7 +241,7 @@ class Step:
         del keep1, keep2
         return r
 
-    def run_weights(self, lse, before, in_place=False):
+    def run_weights(self, lse, before, in_place=False, stream=None):
         cache, keep1 = self.cache_on_gpu()
         table, keep2 = self.table_on_gpu()
         q, starts = values_on_gpu(self.q, self.dtype), ints_on_gpu(self.starts)
@@ -251,7 +251,9 @@ class Step:
             cache=cache, table=table, q=q.ptr, lse=dlse.ptr, q_starts=starts.ptr, q_stride=self.q_pitch,
             weights_in=din.ptr, weights=dout.ptr, weights_seq_stride=before.shape[1] * before.shape[2],
             weights_head_stride=before.shape[2], tokens=self.tokens, q_heads=self.hq, window=self.window,
-            scale=self.scale))
+            scale=self.scale), stream)
+        if stream is not None:
+            stream.synchronize()
         r = values_from_gpu(dout, before.shape, "f32")
         del keep1, keep2
         return r
