@@ -270,7 +270,7 @@ int kh_qk_norm_rope(const kh_qk_norm_rope_args *args, void *stream) {
     const int lanes = c.head_dim <= 64 ? 8 : c.head_dim <= 128 ? 16 : 32;
     // Heads of a token are shared out over waves until the chip has some
     // sixteen of them to a CU.
-    const int64_t steps = ceil_div(a.q_heads + 2 * c.kv_heads, 64 / lanes);
+    const int64_t steps = ceil_div(a.q_heads, 64 / lanes) + 2 * ceil_div(c.kv_heads, 64 / lanes);
     const int64_t parts = std::clamp<int64_t>(ceil_div(16 * KH_GEMM_CUS, a.tokens), 1, steps);
     KhRopeParams p{a.q, a.k, a.v, a.q_out, a.k_out, a.q_gamma, a.k_gamma, a.inv_freq, a.positions, a.slots, c.k, c.v,
                    a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride, c.k_page_stride, c.k_slot_stride,

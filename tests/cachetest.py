@@ -241,9 +241,9 @@ class Step:
         del keep1, keep2
         return r
 
-    def run_weights(self, lse, before, in_place=False, stream=None):
+    def run_weights(self, lse, before, in_place=False, stream=None, max_len=0):
         cache, keep1 = self.cache_on_gpu()
-        table, keep2 = self.table_on_gpu()
+        table, keep2 = self.table_on_gpu(max_len)
         q, starts = values_on_gpu(self.q, self.dtype), ints_on_gpu(self.starts)
         dlse, din = values_on_gpu(lse, "f32"), values_on_gpu(before, "f32")
         dout = din if in_place else values_on_gpu(np.full(before.shape, 7.0), "f32")

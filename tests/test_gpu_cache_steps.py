@@ -328,4 +328,20 @@ def test_weights_over_pages_of_heads(dev, dtype, q_lens):
 def test_a_length_past_the_hint(dev):
     """max_len sizes the launch; sequences longer than it are done all the same."""
     for q in (1, 40):
-        check_attention(Step("bf16", [q, 1], [1500, 900], 4, 2, 64, seed=31), max_len=20)
+        s = Step("bf16", [q, 1], [1500, 900], 4, 2, 64, seed=31)
+        _, lse = check_attention(s, max_len=20)
+        before = s.g.random((2, 2, 1500), np.float32)
+        want, bound = s.weights(lse, before)
+        got = s.run_weights(lse, before, max_len=20)
+        for i, n in enumerate(s.lens):
+            close(got[i, :, :n], want[i, :, :n], bound[i, :, :n], f"sequence {i}")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("hq", [8, 6])
+def test_tokens_that_share_their_queries(dev, dtype, hq):
+    """q_stride 0: one row of q is every token's."""
+    s = Step(dtype, [70, 1], [200, 90], hq, 2, 64, seed=32)
+    s.q, s.q_pitch = np.repeat(s.q[:1], s.tokens, 0), 0
+    check_attention(s)
+    check_weights(s)
