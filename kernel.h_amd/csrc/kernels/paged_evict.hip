@@ -11,8 +11,9 @@
 // consecutive ones to a thread, so that one sum over the workgroup places them
 // all; longer rows are read again for each step. paged_evict_move copies the
 // rows, 16 bytes to a lane: bound by memory, every kept row is read once and
-// written once. Of bf16 rows of 128, 16 sequences of 8 heads keep 4096 of 4352:
-// 14 us and 97 us (5.5 TB/s); with loads that pass the caches by, 108.
+// written once, with stores that pass the caches by. 16 sequences of 8 heads of
+// 128 (bf16), 4096 entries kept of 4200 to 4352: 14 us and 97 to 108 us (5.0 to
+// 5.5 TB/s).
 //
 // Weights are sums of exponentials, but any 32 bits are ordered: -0 counts as
 // 0, a NaN as larger than all else.
