@@ -195,6 +195,12 @@ struct AttentionPlan {
 // A sequence of more rows than this goes to the wide form.
 constexpr int64_t kNarrowRows = 32;
 
+// Units of no more blocks than this are not split: a join costs as much as some
+// blocks do. MI355X, split and whole: 1 x 300 entries (fp32, one head of 80) 16.1
+// us / 12.8, 8 x 300 (bf16, 32 heads on 8 of 128) 17.4 / 11.7, 128 x 10 to 500 51 /
+// 41; 1 x 1000 17 / 27, 8 x 1000 17 / 23.
+constexpr int64_t kWholeBlocks = 4;
+
 AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_bytes) {
   AttentionPlan p{};
   const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.tokens * group;
@@ -234,7 +240,7 @@ AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_
   // The kernels count blocks in 32 bits, with what lengths beyond the expected
   // ones may add: the whole row of the table.
   const int64_t most_blocks = units * ceil_div(capacity_of(a.table.width, a.cache.page_size), KH_STRETCH);
-  p.whole = blocks == 1 || p.groups < KH_GEMM_CUS / 4 || most_blocks >= 1 << 30;
+  p.whole = blocks <= kWholeBlocks || p.groups < std::min(units, most) || p.groups < 2 || most_blocks >= 1 << 30;
   if (p.whole) p.groups = std::min(units, most);
   p.part_bytes = p.whole ? 0 : static_cast<size_t>(p.groups) * per_group;
   return p;

@@ -345,3 +345,11 @@ def test_tokens_that_share_their_queries(dev, dtype, hq):
     s.q, s.q_pitch = np.repeat(s.q[:1], s.tokens, 0), 0
     check_attention(s)
     check_weights(s)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n", [128, 511, 512, 513, 641, 3500])
+def test_few_units_of_many_blocks(dev, dtype, n):
+    """One or two heads' rows over several workgroups, or whole in one."""
+    check_attention(Step(dtype, [1], [n], 1, 1, 80, page_size=24, seed=n))
+    check_attention(Step(dtype, [11, 3], [n, 600], 1, 1, 64, seed=n))
