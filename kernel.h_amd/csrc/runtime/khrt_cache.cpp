@@ -192,8 +192,11 @@ struct AttentionPlan {
   size_t part_bytes, wide_bytes;  // of workspace that their parts take
 };
 
-// A sequence of more rows than this goes to the wide form.
-constexpr int64_t kNarrowRows = 32;
+// A sequence of more rows than this goes to the wide form. In 32 bits its 128-row
+// tiles cost more where rows are few: MI355X, 58 sequences of 300 to 2000 entries,
+// 36 or 64 rows each, heads of 128, fp32 wide 103 / 114 us, narrow 53 / 65; bf16
+// wide 28 / 29, narrow 36 / 42.
+int64_t narrow_rows_of(int32_t dtype) { return dtype == KHRT_F32 ? 64 : 32; }
 
 // Units of no more blocks than this are not split: a join costs as much as some
 // blocks do. MI355X, split and whole: 1 x 300 entries (fp32, one head of 80) 16.1
@@ -211,8 +214,9 @@ AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_
 
   // Few rows to a sequence, by all the host can know: the narrow form has them
   // all. One sequence: whichever suits its rows. Otherwise both.
-  const bool narrow_only = rows <= kNarrowRows * a.table.seqs, wide_only = !narrow_only && a.table.seqs == 1;
-  p.narrow_rows = narrow_only ? INT32_MAX : wide_only ? 0 : kNarrowRows;
+  const int64_t few = narrow_rows_of(a.cache.dtype);
+  const bool narrow_only = rows <= few * a.table.seqs, wide_only = !narrow_only && a.table.seqs == 1;
+  p.narrow_rows = narrow_only ? INT32_MAX : wide_only ? 0 : few;
   if (!narrow_only) {
     p.wide_units = (rows / KH_WIDE_ROWS + std::min(a.tokens, a.table.seqs)) * a.cache.kv_heads;
     // Two to a CU; parts are worth it while they fill the chip no more than once,
@@ -229,7 +233,7 @@ AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_
   if (wide_only) return p;
 
   // At most so many units, of at most so many blocks each.
-  const int64_t narrow_most = narrow_only ? rows : std::min(rows, kNarrowRows * a.table.seqs);
+  const int64_t narrow_most = narrow_only ? rows : std::min(rows, few * a.table.seqs);
   const int64_t units = (narrow_most / KH_TILE_ROWS + std::min(a.tokens, a.table.seqs)) * a.cache.kv_heads;
   const int64_t blocks = ceil_div(len, KH_STRETCH);
   // As many workgroups as are on the chip at once.

@@ -353,3 +353,12 @@ def test_few_units_of_many_blocks(dev, dtype, n):
     """One or two heads' rows over several workgroups, or whole in one."""
     check_attention(Step(dtype, [1], [n], 1, 1, 80, page_size=24, seed=n))
     check_attention(Step(dtype, [11, 3], [n, 600], 1, 1, 64, seed=n))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("window", [0, 90])
+def test_row_counts_on_both_sides_of_the_forms(dev, dtype, window):
+    """Sequences of 16 to 132 rows in one batch, and one alone."""
+    check_attention(Step(dtype, [4, 8, 9, 16, 17, 33], [300, 40, 700, 1500, 64, 128], 8, 2, 64, window=window, seed=41))
+    for q in (15, 16, 17, 33):
+        check_attention(Step(dtype, [q], [900], 4, 1, 128, page_size=24, window=window, seed=q))
