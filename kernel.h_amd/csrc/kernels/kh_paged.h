@@ -105,6 +105,20 @@ KH_HD KhSpan kh_seen(const KhSeq &s, int32_t i, int32_t window) {
   return r;
 }
 
+// The token and the head of its group that row R of a sequence and kv head is.
+// A row past the last gives row 0's in its place: what is read there exists and
+// is not used. A sequence without new tokens has no row at all, its start may lie
+// behind the last token, and nothing may be read for it: token -1.
+struct KhQuery {
+  int32_t token, head;
+};
+
+KH_HD KhQuery kh_query(const KhSeq &s, int32_t group, const KhDiv &by_group, int32_t R) {
+  if (s.m == 0) return KhQuery{-1, 0};
+  const int32_t real = R < s.m * group ? R : 0, i = static_cast<int32_t>(kh_div(static_cast<uint32_t>(real), by_group));
+  return KhQuery{s.start + i, real - i * group};
+}
+
 // How paged_attention's narrow form shares out a step. A unit is 16 rows (new
 // tokens x heads of a group) of one sequence and kv head against `blocks`
 // stretches of KH_STRETCH entries, all that any of the sequence's new tokens

@@ -74,7 +74,7 @@ __device__ __forceinline__ float kept(const KhWeightsParams &p, const Job &j, in
   return __uint_as_float(old & (p.weights_in != nullptr && key < j.s.n - j.s.m ? ~0u : 0u));
 }
 
-// The rows' queries and what their scores are taken from, for up to 32 rows.
+// The rows' queries and what their scores are taken from, for 1 to 32 rows.
 template <int D>
 struct Queries {
   u32x4 q[kFewRows / 16][Form<D>::steps];
@@ -89,9 +89,9 @@ __device__ __forceinline__ Queries<D> queries(const KhWeightsParams &p, const Jo
   y.two = j.rows > 16;
 #pragma unroll
   for (int t = 0; t < kFewRows / 16; ++t) {
-    const int R = 16 * t + r < j.rows ? 16 * t + r : 0, i = (int)kh_div(R, p.by_group);
+    const KhQuery row = kh_query(j.s, p.group, p.by_group, 16 * t + r);
     const char *qp = static_cast<const char *>(p.q) +
-                     ((int64_t)(j.s.start + i) * p.q_stride + (int64_t)(j.head * p.group + R - i * p.group) * d) * (int)sizeof(elem);
+                     ((int64_t)row.token * p.q_stride + (int64_t)(j.head * p.group + row.head) * d) * (int)sizeof(elem);
 #pragma unroll
     for (int c = 0; c < Form<D>::steps; ++c) {
       const u32x4 x = *reinterpret_cast<const u32x4 *>(qp + within(64 * c + 16 * h, row_bytes));
@@ -99,8 +99,9 @@ __device__ __forceinline__ Queries<D> queries(const KhWeightsParams &p, const Jo
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int R4 = 16 * t + 4 * h + e, R5 = R4 < j.rows ? R4 : 0, i5 = (int)kh_div(R5, p.by_group);
-      y.lse[t][e] = taken(p.lse[(int64_t)(j.s.start + i5) * p.q_heads + j.head * p.group + R5 - i5 * p.group], R4 < j.rows);
+      const int R = 16 * t + 4 * h + e;
+      const KhQuery at = kh_query(j.s, p.group, p.by_group, R);
+      y.lse[t][e] = taken(p.lse[(int64_t)at.token * p.q_heads + j.head * p.group + at.head], R < j.rows);
     }
   }
   return y;
@@ -392,6 +393,12 @@ __device__ __forceinline__ void wide(const KhWeightsParams &p, const Job &j, int
   if (h == 0 && key < j.s.n) p.weights[j.row + key] = kept(p, j, key, old) + (there ? sum : 0.0f);
 }
 
+// No new tokens: what was there before, or zeros. Neither q nor lse is read.
+__device__ __forceinline__ void copy(const KhWeightsParams &p, const Job &j, int first, int end) {
+  for (int key = first + (int)threadIdx.x; key < end; key += kWaves * kWave)
+    p.weights[j.row + key] = p.weights_in != nullptr ? p.weights_in[j.row + key] : 0.0f;
+}
+
 // RING: there is LDS for few_even().
 template <int D, bool RING>
 __device__ __forceinline__ void weights(const KhWeightsParams &p, char *lds) {
@@ -406,7 +413,9 @@ __device__ __forceinline__ void weights(const KhWeightsParams &p, char *lds) {
   // Chunks past those that the launch was sized for fall to its workgroups in turn.
   for (int64_t first = (int64_t)chunk * p.chunk_keys; first < j.s.n; first += (int64_t)p.chunks * p.chunk_keys) {
     const int end = first + p.chunk_keys < j.s.n ? (int)first + p.chunk_keys : j.s.n;
-    if (j.rows <= kFewRows) {
+    if (j.rows == 0) {
+      copy(p, j, (int)first, end);
+    } else if (j.rows <= kFewRows) {
       if constexpr (RING)
         few_even<D>(p, j, (int)first, end, lds);
       else
