@@ -173,6 +173,17 @@ KH_HD KhShares kh_shares(int32_t work, int32_t most) {
   return s;
 }
 
+// Walks from unit to unit and from sequence to sequence count from the start
+// of the sequence they are in, `in` blocks: what came before may be past 32 bits
+// where starts do not ascend and many sequences claim the same tokens. Whether
+// block `in` lies behind the sequence's `work` blocks; if so, it is counted from
+// there.
+KH_HD bool kh_passed(int32_t &in, int32_t work) {
+  if (in < work) return false;
+  in -= work;
+  return true;
+}
+
 // Where workgroup g's share starts.
 KH_HD int32_t kh_share(const KhShares &s, int32_t g) { return g * s.each + (g < s.longer ? g : s.longer); }
 
@@ -181,6 +192,24 @@ KH_HD int32_t kh_owner(const KhShares &s, int32_t x) {
   const int32_t long_ones = s.longer * (s.each + 1);
   return x < long_ones ? static_cast<int32_t>(static_cast<uint32_t>(x) / static_cast<uint32_t>(s.each + 1))
                        : s.longer + static_cast<int32_t>(static_cast<uint32_t>(x - long_ones) / static_cast<uint32_t>(s.each));
+}
+
+// The workgroups that have parts of the unit of `blocks` blocks from block
+// `begin` on, of `work` in all. Where counts have passed 32 bits a unit may begin
+// before the line's first block or end behind its last: there are no parts there.
+// slot: of the first of them, 0 where its share begins in this unit, else 1;
+// all others begin theirs in it.
+struct KhOwners {
+  int32_t first, count, slot;
+};
+
+KH_HD KhOwners kh_owners(const KhShares &s, int32_t work, int32_t begin, int32_t blocks) {
+  const int64_t end = static_cast<int64_t>(begin) + blocks;
+  KhOwners o;
+  o.first = kh_owner(s, begin > 0 ? begin : 0);
+  o.count = kh_owner(s, static_cast<int32_t>(end < work ? end : work) - 1) - o.first + 1;
+  o.slot = kh_share(s, o.first) >= begin ? 0 : 1;
+  return o;
 }
 
 // The wide form: units of KH_WIDE_ROWS rows of a sequence of more than

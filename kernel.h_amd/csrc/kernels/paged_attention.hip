@@ -214,9 +214,8 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
   if (seq < 0) return;
   KhUnits units = kh_units(s, p.group, p.window, p.whole);
 
-  for (int at = start; at < end;) {
-    while (at >= before + kh_work(units, p.cache.kv_heads)) {
-      before += kh_work(units, p.cache.kv_heads);
+  for (int at = start, in = start - before; at < end;) {
+    while (kh_passed(in, kh_work(units, p.cache.kv_heads))) {
       // The next sequence of few rows: wide() has the others.
       do {
         if (++seq >= p.table.seqs) return;
@@ -224,13 +223,13 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
       } while (s.m * p.group > p.narrow_rows);
       units = kh_units(s, p.group, p.window, p.whole);
     }
-    const uint32_t unit = (uint32_t)(at - before) / (uint32_t)units.blocks;
+    const uint32_t unit = (uint32_t)in / (uint32_t)units.blocks;
     const int tile = (int)(unit / (uint32_t)p.cache.kv_heads), head = (int)(unit - (uint32_t)tile * (uint32_t)p.cache.kv_heads);
-    const int block0 = at - before - (int)unit * units.blocks;
+    const int block0 = in - (int)unit * units.blocks;
     const int block1 = end - at < units.blocks - block0 ? block0 + end - at : units.blocks;
     const bool alone = block0 == 0 && block1 == units.blocks;
     const int slot = at == start ? 0 : 1;
-    at += block1 - block0;
+    at += block1 - block0, in += block1 - block0;
     const int from = units.first + block0 * KH_STRETCH, to = block1 == units.blocks ? s.n : units.first + block1 * KH_STRETCH;
     const int rows = s.m * p.group;  // < 2^31: tokens x q_heads is
     const int row0 = tile * kRows;
@@ -889,15 +888,12 @@ __device__ __forceinline__ bool narrow_parts(const KhAttentionParams &p, int g, 
   if (sequence_at(p, line, at, false, s, before) < 0) return false;
   const KhUnits units = kh_units(s, p.group, p.window, p.whole);
   const int unit = (int)((uint32_t)(at - before) / (uint32_t)units.blocks);
-  const int begin = before + unit * units.blocks, end = begin + units.blocks;
-  const int g0 = kh_owner(shares, begin);
-  if (at == begin || g0 != g - 1) return false;
+  const int begin = before + unit * units.blocks;
+  const KhOwners owners = kh_owners(shares, line.all, begin, units.blocks);
+  if (at == begin || owners.first != g - 1) return false;
   const int tile = unit / p.cache.kv_heads, rows = s.m * p.group - tile * kRows;
-  // The first part ends its workgroup's share unless that began in this unit;
-  // all others begin theirs.
-  const int64_t slot0 = kh_share(shares, g0) >= begin ? 0 : 1;
-  parts = Parts{p.part_ml, p.part_o, ((int64_t)g0 * 2 + slot0) * kRows, (int64_t)g * 2 * kRows, 2 * kRows,
-                kh_owner(shares, end - 1) - g0 + 1, tile * kRows, rows < kRows ? rows : kRows,
+  parts = Parts{p.part_ml, p.part_o, ((int64_t)owners.first * 2 + owners.slot) * kRows, (int64_t)g * 2 * kRows, 2 * kRows,
+                owners.count, tile * kRows, rows < kRows ? rows : kRows,
                 unit - tile * p.cache.kv_heads, false};
   return true;
 }

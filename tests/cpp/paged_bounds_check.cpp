@@ -36,8 +36,62 @@ static void queries() {
     }
 }
 
+// Sequences that claim the same tokens: counts of blocks past 32 bits, as the
+// kernels add them up. The place in a sequence stays in it, and the owners of a
+// unit's parts are workgroups that there are.
+static void walks() {
+  uint32_t seed = 1;
+  auto random = [&seed](uint32_t below) {
+    seed = seed * 1664525u + 1013904223u;
+    return static_cast<int32_t>((static_cast<uint64_t>(seed) * below) >> 32);
+  };
+  int past = 0;
+  for (int run = 0; run < 3000; ++run) {
+    const int32_t blocks = 1 + random(1 << 20), seqs = 2 + random(30);
+    int32_t work[32];
+    uint32_t all = 0;
+    int64_t real = 0;
+    for (int i = 0; i < seqs; ++i) {
+      work[i] = random((1 << 30) / blocks) * blocks;
+      all += static_cast<uint32_t>(work[i]);
+      real += work[i];
+    }
+    past += real > INT32_MAX;
+    const int32_t line = static_cast<int32_t>(all);
+    const KhShares s = kh_shares(line, 512);
+    for (int32_t g = 0; g < s.groups; g += 1 + random(64)) {
+      const int32_t start = kh_share(s, g), end = kh_share(s, g + 1);
+      // The first sequence whose wrapped count passes the start.
+      uint32_t upto = 0;
+      int seq = -1;
+      int32_t in = 0;
+      for (int i = 0; i < seqs && seq < 0; ++i) {
+        const uint32_t before = upto;
+        upto += static_cast<uint32_t>(work[i]);
+        if (static_cast<int32_t>(upto) > start) {
+          seq = i;
+          in = start - static_cast<int32_t>(before);
+          const int32_t unit = in / blocks, begin = static_cast<int32_t>(before) + unit * blocks;
+          const KhOwners o = kh_owners(s, line, begin, blocks);
+          expect(o.first >= 0 && o.count >= 1 && o.first + o.count <= s.groups, "owners", run, g, o.first);
+          expect(o.first <= g && g < o.first + o.count, "the workgroup is one of them", run, g, o.first);
+        }
+      }
+      for (int32_t at = start; at < end && seq >= 0 && seq < seqs;) {
+        while (seq < seqs && kh_passed(in, work[seq])) ++seq;
+        if (seq == seqs) break;
+        expect(in >= 0 && in < work[seq], "a place in the sequence", run, g, in);
+        const int32_t left = blocks - in % blocks, step = end - at < left ? end - at : left;
+        at += step, in += step;
+      }
+    }
+  }
+  expect(past > 1000, "counts past 32 bits");
+}
+
 int main() {
   queries();
+  walks();
   std::printf("paged_bounds_check ok\n");
   return 0;
 }
