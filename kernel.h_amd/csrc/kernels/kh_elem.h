@@ -114,32 +114,35 @@ __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 acc) {
 // cannot prove the places disjoint from those it reads, and would wait for its
 // own form of this load before every later LDS read. The caller waits
 // (vm_wait) before the barrier that hands the bytes over. The resource and `lds`
-// are the same in all lanes. M0 carries the LDS address, with the one wait state
-// between writing it and such a load.
+// are the same in all lanes. M0 carries the LDS address; it is saved and restored.
+// A vector instruction's write of a scalar register (the resource's words may
+// come straight from v_readfirstlane) needs five wait states before a load reads
+// it, a write of M0 one: the compiler does not look into the assembly, so they are
+// counted here, two moves and three more.
+#define KH_DMA(load)                        \
+  uint32_t saved;                           \
+  asm volatile(                             \
+      "s_mov_b32 %0, m0\n\t"                \
+      "s_mov_b32 m0, %1\n\t"                \
+      "s_nop 2\n\t" load                    \
+      " %2, %3, 0 offen lds\n\t"            \
+      "s_mov_b32 m0, %0"                    \
+      : "=&s"(saved)                        \
+      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(rsrc) \
+      : "memory")
 __device__ __forceinline__ void dma16(u32x4 rsrc, uint32_t voff, uint32_t lds) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen lds"
-      :
-      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(rsrc)
-      : "memory", "m0");
+  KH_DMA("buffer_load_dwordx4");
 }
 
 // The same for 4 bytes a lane.
 __device__ __forceinline__ void dma4(u32x4 rsrc, uint32_t voff, uint32_t lds) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dword %1, %2, 0 offen lds"
-      :
-      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(rsrc)
-      : "memory", "m0");
+  KH_DMA("buffer_load_dword");
 }
+#undef KH_DMA
 
 // For LDS that the wave alone uses: all but the last N vector-memory operations
 // are done, and what they brought is read after this.
