@@ -7,6 +7,7 @@ Outputs under kernel.h_amd/build/:
   gen/kh_embed.S       .incbin of every product code object
   gen/kh_resources.inc resource table compiled into the runtime
   gen/kh_cli_embed.S   .incbin of the CLI-only code objects (hipref)
+  warnings.txt         what the compilers said, empty if nothing
   libkhrt.so           the C-ABI runtime (include/khrt.h)
   kernelh              the CLI (compile / bench / occupancy)
   khrt_raii_check, khrt_backend_check, co/mfma_probe.hsaco
@@ -42,6 +43,7 @@ BUILD = os.path.join(HERE, "build")
 CO = os.path.join(BUILD, "co")
 GEN = os.path.join(BUILD, "gen")
 OBJ = os.path.join(BUILD, "obj")
+WARNINGS = os.path.join(BUILD, "warnings.txt")
 
 # GEMM tune candidates: csrc/kernels/gemm_tune.hip compiled once per part of
 # its list (gemm_tune_list.h, KH_GEMM_TUNE_PARTS = 4), so the parts compile
@@ -105,7 +107,12 @@ def run(cmd, verbose=False, **kw):
     out = "\n".join(l for l in r.stdout.splitlines() if "packed-fp32-ops" not in l and l.strip())
     if r.returncode != 0:
         raise RuntimeError(f"command failed ({r.returncode}): {' '.join(cmd)}\n{out}")
-    if verbose and out:
+    if out and cmd[0] in (HIPCC, CXX):
+        # A compiler that says anything without failing warns.
+        print(out, file=sys.stderr)
+        with open(WARNINGS, "a") as f:
+            f.write(f"{' '.join(cmd)}\n{out}\n")
+    elif verbose and out:
         print(out)
     return r.stdout
 
@@ -189,6 +196,7 @@ def build(jobs: int = 8, verbose: bool = False) -> None:
         shutil.rmtree(BUILD)
     for d in (CO, GEN, OBJ):
         os.makedirs(d, exist_ok=True)
+    open(WARNINGS, "w").close()
 
     srcs = [n for n in PRODUCT if os.path.exists(os.path.join(KDIR, VARIANTS.get(n, (n,))[0] + ".hip"))]
     fixture_dir = os.path.join(TDIR, "fixtures")

@@ -447,8 +447,9 @@ KH_WEIGHTS(256)
 // Steps with chunks: without it, three. Two sequences of up to 1024 new tokens
 // and 6000 entries (bf16, 32 heads on 8 of 128): 109 us, 706 TFLOP/s. With the
 // ring's LDS, two workgroups to a CU, such a step took 171 us.
+// In 32 bits heads of 128 take 66 KB: two.
 #define KH_WEIGHTS_WIDE(D)                                                                                 \
-  extern "C" __global__ void __launch_bounds__(256, D > 128 ? 1 : 3) KH_TYPED(paged_weights_wide_##D)(const KhWeightsParams p) { \
+  extern "C" __global__ void __launch_bounds__(256, D > 128 ? 1 : kWide && D > 64 ? 2 : 3) KH_TYPED(paged_weights_wide_##D)(const KhWeightsParams p) { \
     __shared__ __attribute__((aligned(16))) char lds[2 * Rows<D>::tile * (Rows<D>::bytes + 4)];             \
     weights<D, false>(p, lds);                                                                              \
   }

@@ -174,7 +174,7 @@ int khrt_get_device_info(khrt_device_info *out) {
   if (e != hipSuccess) return fail_hip(e, "hipGetDeviceProperties");
   std::memset(out, 0, sizeof(*out));
   std::snprintf(out->name, sizeof(out->name), "%s", p.name);
-  std::snprintf(out->arch, sizeof(out->arch), "%s", p.gcnArchName);
+  std::snprintf(out->arch, sizeof(out->arch), "%.*s", static_cast<int>(sizeof(out->arch)) - 1, p.gcnArchName);
   out->lds_bytes_per_workgroup = static_cast<int64_t>(p.sharedMemPerBlock);
   out->wavefront_size = p.warpSize;
   out->max_threads_per_workgroup = p.maxThreadsPerBlock;
