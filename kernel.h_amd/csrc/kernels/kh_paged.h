@@ -119,6 +119,12 @@ KH_HD KhQuery kh_query(const KhSeq &s, int32_t group, const KhDiv &by_group, int
   return KhQuery{s.start + i, real - i * group};
 }
 
+// Of entries [first, end) of the sequence, how many are not its new tokens'.
+KH_HD int32_t kh_older(const KhSeq &s, int32_t first, int32_t end) {
+  const int32_t older = s.n - s.m < end ? s.n - s.m : end;  // may lie below 0
+  return older > first ? older - first : 0;
+}
+
 // How paged_attention's narrow form shares out a step. A unit is 16 rows (new
 // tokens x heads of a group) of one sequence and kv head against `blocks`
 // stretches of KH_STRETCH entries, all that any of the sequence's new tokens

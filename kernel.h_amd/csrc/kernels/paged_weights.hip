@@ -173,10 +173,10 @@ __device__ __forceinline__ void few_even(const KhWeightsParams &p, const Job &j,
     const int row = i * G::rows + lane / G::pieces, c = 16 * (lane % G::pieces ^ k_turn<D>(row));
     lanes[i] = c < row_bytes ? (uint32_t)row * p.cache.k_slot + (uint32_t)c : kOutside;
   }
-  // Older entries' weights; of the new tokens' own, and without weights_in, zeros.
-  const int older = p.weights_in == nullptr || j.s.n < j.s.m ? 0 : j.s.n - j.s.m;
+  // The weights of the chunk's older entries; of the new tokens' own, and without weights_in, zeros.
   const uint64_t in = (uint64_t)reinterpret_cast<uintptr_t>(p.weights_in + j.row + first);
-  const u32x4 old = {(uint32_t)in, (uint32_t)(in >> 32), older > first ? (uint32_t)(older - first) * 4u : 0u, 0x00020000u};
+  const uint32_t older = p.weights_in == nullptr ? 0u : (uint32_t)kh_older(j.s, first, end);
+  const u32x4 old = {(uint32_t)in, (uint32_t)(in >> 32), older * 4u, 0x00020000u};
   Block<D, true> b;
   uint32_t now, next;
   find<D, true>(b, p, j.table, key0, end, r);

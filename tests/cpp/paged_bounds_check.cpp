@@ -89,7 +89,22 @@ static void walks() {
   expect(past > 1000, "counts past 32 bits");
 }
 
+// A chunk's older entries, in a sequence of up to the longest there may be.
+static void older() {
+  const int32_t top = INT32_MAX - 65536;
+  for (int32_t n : {0, 1, 40, 1000, (1 << 30) + 100, top})
+    for (int32_t m : {0, 1, 7, 50, 2000})
+      for (int64_t first : {int64_t(0), int64_t(1024), int64_t(n) - m - 3, int64_t(n) - m, int64_t(n) - 5}) {
+        if (first < 0 || first >= n) continue;
+        const int64_t end = first + 1024 < n ? first + 1024 : n;
+        int64_t want = 0;
+        for (int64_t j = first; j < end; ++j) want += j < int64_t(n) - m;
+        expect(kh_older(KhSeq{n, m, 0}, static_cast<int32_t>(first), static_cast<int32_t>(end)) == want, "older entries", n, m, first);
+      }
+}
+
 int main() {
+  older();
   queries();
   walks();
   std::printf("paged_bounds_check ok\n");

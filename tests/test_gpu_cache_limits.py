@@ -58,3 +58,40 @@ def test_weights_where_starts_lie_past_the_tokens(dev, page_size):
     got = s.run_weights(lse, before)
     assert same_bits(got, want)
     assert same_bits(got[1, :, :77], before[1, :, :77]) and same_bits(got[2, :, :130], before[2, :, :130])
+
+
+# ---------------------------------------------------------------- long caches
+
+def test_weights_of_a_sequence_past_2_30_entries(dev):
+    """A table that repeats one page of 2^20 entries (heads of 8, 16 MB): what
+    entries had received before stays, at both ends, where a row of weights
+    passes 4 GB."""
+    ps, d = 1 << 20, 8
+    n = (1 << 30) + 100
+    g = np.random.default_rng(0)
+    k = values_on_gpu(np.zeros((ps, d)), "bf16")
+    table, lens = ints_on_gpu(np.zeros(1025)), ints_on_gpu([n])
+    cache = kh.PagedCache(k=k.ptr, v=k.ptr, k_page_stride=ps * d, k_slot_stride=d, k_head_stride=d, v_page_stride=ps * d,
+                          v_slot_stride=d, v_head_stride=d, pages=1, page_size=ps, kv_heads=1, head_dim=d, dtype=kh.BF16)
+    # Keys of zeros: every entry receives exp(0 - lse), a power of two as a float.
+    q, starts = values_on_gpu(g.standard_normal((1, d)), "bf16"), ints_on_gpu([0, 1])
+    lse = values_on_gpu([math.log(4.0)], "f32")
+    w, out = kh.Buffer(n * 4), kh.Buffer(n * 4)
+    parts = [(0, 4096), ((1 << 29) - 5, 4096), (n - 4096, 4096)]
+    old = [g.random(m, np.float32) for _, m in parts]
+    for (at, m), x in zip(parts, old):
+        kh.check(kh.lib.khrt_memcpy_h2d(w.ptr + at * 4, x.ctypes.data, x.nbytes))
+    say("weights of 2^30 + 100 entries")
+    kh.paged_weights(kh.PagedWeights(
+        cache=cache, table=kh.PageTable(pages=table.ptr, lens=lens.ptr, row_stride=1025, seqs=1, width=1025, max_len=n),
+        q=q.ptr, lse=lse.ptr, q_starts=starts.ptr, q_stride=d, weights_in=w.ptr, weights=out.ptr, weights_seq_stride=n,
+        weights_head_stride=n, tokens=1, q_heads=1, window=0, scale=1.0))
+    kh.synchronize()
+    for (at, m), x in zip(parts, old):
+        got = np.empty(m, np.float32)
+        kh.check(kh.lib.khrt_memcpy_d2h(got.ctypes.data, out.ptr + at * 4, got.nbytes))
+        want = x.astype(np.float64) + 0.25
+        if at + m == n:
+            want[-1] = 0.25  # the new token's own
+        # lse and its exponent round once each, 2^x and the sum once more.
+        close(got, want, np.abs(want) * 8 * 2.0 ** -24, f"entries from {at}")
