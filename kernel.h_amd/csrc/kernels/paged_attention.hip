@@ -49,7 +49,8 @@ using kh::u32x4;
 
 constexpr int kRows = KH_TILE_ROWS;
 constexpr int kWaves = 4;          // waves of a workgroup; they take blocks of entries in turn
-constexpr float kNegBig = -1e30f;  // seed of the running maximum: finite, so that max - max is never NaN
+constexpr float kSeed = -3.402823466e38f;  // of the running maximum: no finite score lies below it, and max - max is never NaN
+constexpr float kFine = 4194304.0f;        // 2^22, see coarse()
 
 // The lane's rows of V, one piece of columns.
 template <int D>
@@ -133,6 +134,23 @@ __device__ __forceinline__ void load_v(Piece<D> (&v)[Form<D>::count], const Bloc
 __device__ __forceinline__ int apart(int h) {
   asm volatile("" : "+v"(h));
   return h;
+}
+
+// 2^x takes scores times a factor less the row's maximum m (in powers of two):
+// one multiply-add, exact but for its last rounding, while m itself was rounded.
+// The largest score is so off by half a step of m: 2^-2 at kFine, whole powers of
+// two further up. Where the wave has such maxima (coarse), the products are
+// rounded as m was before it is taken from them (less), and nothing else is done.
+__device__ __forceinline__ bool coarse(float m) { return __builtin_amdgcn_ballot_w64(__builtin_fabsf(m) > kFine) != 0; }
+
+template <int N, class X>
+__device__ __forceinline__ void less(X &x, float factor, float m) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    float y = x[j] * factor;
+    asm volatile("" : "+v"(y));  // not fused with the subtraction
+    x[j] = y - m;
+  }
 }
 
 __device__ __forceinline__ KhSeq sequence(const KhAttentionParams &p, int seq) {
@@ -256,7 +274,9 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
       q[c] = mine && 64 * c + 16 * h < row_bytes ? x : u32x4{0, 0, 0, 0};
     }
 
-    float m = kNegBig, l = 0.0f;  // of row l % 16; l of this lane's entries alone
+    // Of row l % 16; l of this lane's entries alone. A row that there is none of has
+    // no scores, and no maximum to look after either.
+    float m = mine ? kSeed : 0.0f, l = 0.0f;
     f32x4 o[F::count][F::piece];
 #pragma unroll
     for (int a = 0; a < F::count; ++a)
@@ -338,10 +358,13 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
 #pragma unroll
             for (int e = 0; e < F::piece; ++e) o[a][e] *= fade;
         }
+        const bool far = coarse(m);
+        const float factor = far ? 1.0f : p.scale_log2, shift = far ? 0.0f : -m;
+        if (far) less<F::mine>(y, p.scale_log2, m);
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < F::mine; ++j) {
-          y[j] = kh::exp2_hw(fmaf(y[j], p.scale_log2, -m));
+          y[j] = kh::exp2_hw(fmaf(y[j], factor, shift));
           sum += y[j];
         }
         l += sum;
@@ -393,7 +416,7 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
       ml[(wave * kRows + r) * 2 + 1] = l;
     }
     kh::lds_barrier();
-    float top = kNegBig;
+    float top = kSeed;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml[(w * kRows + r) * 2]);
     float total = 0.0f;
@@ -699,7 +722,7 @@ __device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char
     const u32x4 x = *reinterpret_cast<const u32x4 *>(qp + within(32 * c + 16 * h, row_bytes)) ^ p.q_sign;
     q[c] = mine && 32 * c + 16 * h < row_bytes ? x : u32x4{0, 0, 0, 0};
   }
-  float m = kNegBig, l = 0.0f;
+  float m = mine ? kSeed : 0.0f, l = 0.0f;
   f32x16 o[W::dts];
 #pragma unroll
   for (int a = 0; a < W::dts; ++a) o[a] = f32x16{};
@@ -788,12 +811,18 @@ __device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char
 #pragma unroll
           for (int a = 0; a < W::dts; ++a) o[a] *= fade;
         }
+        const bool far = coarse(m);
+        const float factor = far ? 1.0f : p.scale_log2, shift = far ? 0.0f : -m;
+        if (far) {
+#pragma unroll
+          for (int kt = 0; kt < W::tiles; ++kt) less<16>(x[kt], p.scale_log2, m);
+        }
         float sum = 0.0f;
 #pragma unroll
         for (int kt = 0; kt < W::tiles; ++kt)
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            x[kt][j] = kh::exp2_hw(fmaf(x[kt][j], p.scale_log2, -m));
+            x[kt][j] = kh::exp2_hw(fmaf(x[kt][j], factor, shift));
             sum += x[kt][j];
           }
         l += sum;
@@ -942,7 +971,7 @@ __device__ __forceinline__ void join(const KhAttentionParams &p, float *lds) {
     const bool live = row < parts.rows && col < d && share < shares;
     const int64_t place = place_of(live ? row : 0);
     f32x4 o = {0, 0, 0, 0};
-    float m = kNegBig, total = 0.0f;
+    float m = kSeed, total = 0.0f;
     for (int k0 = 0; k0 < parts.count; k0 += kJoinParts) {
       const int here = parts.count - k0 < kJoinParts ? parts.count - k0 : kJoinParts;
       for (int x = tid; x < here * kRows; x += 256) {

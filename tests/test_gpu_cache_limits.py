@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import kernelh as kh
-from cachetest import DTYPES, Step, ints_on_gpu, same_bits, values_from_gpu, values_on_gpu
+from cachetest import DTYPES, Step, half_step, ints_on_gpu, rounded, same_bits, values_from_gpu, values_on_gpu
 from khtest import say
 from test_gpu_cache import check_attention, check_weights, close
 
@@ -95,3 +95,47 @@ def test_weights_of_a_sequence_past_2_30_entries(dev):
             want[-1] = 0.25  # the new token's own
         # lse and its exponent round once each, 2^x and the sum once more.
         close(got, want, np.abs(want) * 8 * 2.0 ** -24, f"entries from {at}")
+
+
+# ---------------------------------------------------------------- scores of any size
+
+def row_of_scores(dtype, m, n, spread, window=0, hq=2, hk=1, d=64):
+    """A step of m tokens of n entries whose scores are a * c_j in every row, a
+    product of one column: c_j from `spread` in turn. Values of V are small whole
+    numbers. The Step, and c."""
+    s = Step(dtype, [m], [n], hq, hk, d, seed=n, window=window)
+    c = np.array([spread[j % len(spread)] for j in range(n)], np.float64)
+    page, slot = s.table[0][np.arange(n) // 16], np.arange(n) % 16
+    s.k[page, slot] = 0.0
+    s.q[:] = 0.0
+    s.v[page, slot] = s.g.integers(-8, 9, (n, hk, d)).astype(np.float32)
+    return s, c, page, slot
+
+
+@pytest.mark.parametrize("dtype,q,k", [("f32", 2.0 ** 60, -2.0 ** 55), ("bf16", 2.0 ** 60, -2.0 ** 55), ("f32", 2.0 ** 60, 2.0 ** 55),
+                                       ("f32", 1.1e18, -1.3e17), ("bf16", -1.3125e19, 1.0625e17), ("f16", 60000.0, -20000.0),
+                                       ("f16", 60000.0, 21024.0), ("bf16", 23040.0, -52480.0), ("f32", 60001.0, -20011.0)])
+@pytest.mark.parametrize("m,n", [(1, 50), (1, 3000), (9, 700), (100, 1500)])
+def test_scores_far_from_zero(dev, dtype, q, k, m, n):
+    """Scores of 10^8 to 10^35 of either sign, few values apart by more than
+    the exponential can tell: a row's largest, each counted once, and nothing
+    else. Single tokens, chunks, whole and in parts."""
+    spread = [3.0, 2.0, 1.0, 1.0, 2.0]
+    s, c, page, slot = row_of_scores(dtype, m, n, spread)
+    s.q.reshape(s.tokens, s.hq, s.d)[:, :, 7] = q = rounded(np.full(1, q), dtype)[0]
+    s.k[page, slot, 0, 7] = k = rounded(c * k, dtype)
+    for workspace in (None, 0):
+        say(f"far scores {dtype} {q} {k} m={m} n={n} ws={workspace}")
+        out, lse = s.run_attention(workspace=workspace)
+        x = k.astype(np.float64) * float(q) * s.scale
+        for i in range(m):
+            here = x[:n - m + i + 1]
+            top = here == here.max()
+            want = s.v[page, slot, 0][:n - m + i + 1][top].astype(np.float64).mean(0)
+            # Weights of ones: their sums are exact, the quotient rounds twice
+            # (reciprocal and product), the result once.
+            bound = np.abs(want) * (2.0 ** -21 + half_step(dtype)) + (2.0 ** -25 if dtype == "f16" else 1e-30)
+            for h in range(s.hq):
+                close(out[i, h], want, bound, f"token {i}")
+                # The product and the factor round, and what the sum adds is less than a step of it.
+                close(lse[i, h], here.max(), abs(here.max()) * 2.0 ** -21, "lse")
