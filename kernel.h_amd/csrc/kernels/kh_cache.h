@@ -38,10 +38,10 @@ __device__ __forceinline__ float over_rows(float v, bool maximum) {
   return maximum ? fmaxf(z, w) : z + w;
 }
 
-// Natural log of a sum of exponentials held as its binary maximum and the
-// sum relative to it.
-__device__ __forceinline__ float lse_of(float top, float total) {
-  return total == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * 0.69314718055994530942f;
+// Natural log of a sum of exponentials held as its binary maximum and 2^lift
+// times the sum relative to it.
+__device__ __forceinline__ float lse_of(float top, float total, float lift) {
+  return total == 0.0f ? -__builtin_inff() : (top + (__builtin_amdgcn_logf(total) - lift)) * 0.69314718055994530942f;
 }
 
 __device__ __forceinline__ float over_halves(float v, bool maximum) {

@@ -26,7 +26,9 @@
 //                 nothing goes through LDS but the waves' join at the end.
 // Products accumulate in 32 bits. P is rounded to the elements' type for the
 // second product, the sum of P is not: the rounding is off by half a step of
-// that type at most, as the output's is.
+// that type at most, as the output's is. fp16 ends soon below one, so there P and
+// its sums are 2^15 times their value (kLift): entries a 2^25th of the largest, of
+// which a long cache may hold many, would be in the sum alone.
 //
 // Bound by reading K and V: each wave holds a block of both and has the next
 // ones in flight (nontemporal: nobody else reads them), 64 KB to a CU. One
@@ -50,6 +52,7 @@ using kh::u32x4;
 constexpr int kRows = KH_TILE_ROWS;
 constexpr int kWaves = 4;          // waves of a workgroup; they take blocks of entries in turn
 constexpr float kSeed = -3.402823466e38f;  // of the running maximum: no finite score lies below it, and max - max is never NaN
+constexpr float kLift = KH_ELEM == 1 ? 15.0f : 0.0f;  // fp16 holds 2^kLift times what the largest score can be off by (2^0.25)
 constexpr float kFine = 4194304.0f;        // 2^22, see coarse()
 
 // The lane's rows of V, one piece of columns.
@@ -136,7 +139,8 @@ __device__ __forceinline__ int apart(int h) {
   return h;
 }
 
-// 2^x takes scores times a factor less the row's maximum m (in powers of two):
+// 2^x takes scores times a factor less the row's maximum m (in powers of two) and
+// more kLift:
 // one multiply-add, exact but for its last rounding, while m itself was rounded.
 // The largest score is so off by half a step of m: 2^-2 at kFine, whole powers of
 // two further up. Where the wave has such maxima (coarse), the products are
@@ -359,7 +363,7 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
             for (int e = 0; e < F::piece; ++e) o[a][e] *= fade;
         }
         const bool far = coarse(m);
-        const float factor = far ? 1.0f : p.scale_log2, shift = far ? 0.0f : -m;
+        const float factor = far ? 1.0f : p.scale_log2, shift = far ? kLift : kLift - m;
         if (far) less<F::mine>(y, p.scale_log2, m);
         float sum = 0.0f;
 #pragma unroll
@@ -433,7 +437,7 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
     const int64_t row_of = (int64_t)(s.start + i) * p.q_heads + hq;  // this lane's row
     if (wave == 0 && h == 0) {
       inv[r] = alone ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f;
-      if (mine && alone && p.lse != nullptr) p.lse[row_of] = lse_of(top, total);
+      if (mine && alone && p.lse != nullptr) p.lse[row_of] = lse_of(top, total, kLift);
       if (!alone) {
         float *ml_to = p.part_ml + ((int64_t)block * 2 + slot) * kRows * 2 + r * 2;
         ml_to[0] = top;
@@ -812,7 +816,7 @@ __device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char
           for (int a = 0; a < W::dts; ++a) o[a] *= fade;
         }
         const bool far = coarse(m);
-        const float factor = far ? 1.0f : p.scale_log2, shift = far ? 0.0f : -m;
+        const float factor = far ? 1.0f : p.scale_log2, shift = far ? kLift : kLift - m;
         if (far) {
 #pragma unroll
           for (int kt = 0; kt < W::tiles; ++kt) less<16>(x[kt], p.scale_log2, m);
@@ -873,7 +877,7 @@ __device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char
   const int64_t at_row = (int64_t)split * p.tokens * p.q_heads + row;
   if (h == 0) {
     if (alone) {
-      if (p.lse != nullptr) p.lse[row] = lse_of(m, total);
+      if (p.lse != nullptr) p.lse[row] = lse_of(m, total, kLift);
     } else {
       p.wide_ml[at_row * 2] = m;
       p.wide_ml[at_row * 2 + 1] = total;
@@ -1025,7 +1029,7 @@ __device__ __forceinline__ void join(const KhAttentionParams &p, float *lds) {
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     kh::store4(static_cast<elem *>(p.out) + (int64_t)(s.start + i) * p.out_stride + (int64_t)hq * d + col, y);
-    if (col == 0 && p.lse != nullptr) p.lse[(int64_t)(s.start + i) * p.q_heads + hq] = lse_of(m, total);
+    if (col == 0 && p.lse != nullptr) p.lse[(int64_t)(s.start + i) * p.q_heads + hq] = lse_of(m, total, kLift);
   }
 }
 

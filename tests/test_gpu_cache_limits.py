@@ -139,3 +139,29 @@ def test_scores_far_from_zero(dev, dtype, q, k, m, n):
                 close(out[i, h], want, bound, f"token {i}")
                 # The product and the factor round, and what the sum adds is less than a step of it.
                 close(lse[i, h], here.max(), abs(here.max()) * 2.0 ** -21, "lse")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m,n", [(1, 4000), (1, 60000), (5, 4000), (100, 4000)])
+def test_many_small_weights_beside_a_large_one(dev, dtype, m, n):
+    """An entry whose value is 0 takes all but e^-18 of the others' weight, each
+    a little below 2^-25 of its own: what the others add is the result."""
+    s, _, page, slot = row_of_scores(dtype, m, n, [0.0])
+    s.q.reshape(s.tokens, s.hq, s.d)[:, :, 7] = 1.0
+    s.k[page[0], slot[0], 0, 7] = 18.0 / s.scale
+    s.v[page, slot] = 64.0
+    s.v[page[0], slot[0]] = 0.0
+    for workspace in (None, 0):
+        say(f"small weights {dtype} m={m} n={n} ws={workspace}")
+        out, lse = s.run_attention(workspace=workspace)
+        rest = (n - m + np.arange(m)) * math.exp(-18.0)
+        want = (64.0 * rest / (1.0 + rest))[:, None, None]
+        # A small weight rounds once to the type, all of them alike, and so does
+        # the result; the exponent is off by a few steps of 26 in 32 bits, and n
+        # terms are added in that many.
+        u = half_step(dtype)
+        rel = 8 * 26 * 2.0 ** -24 + 2 * (n + 64) * 2.0 ** -24
+        bound = want * ((2 * u if dtype != "f32" else u) + rel) + (2.0 ** -25 if dtype == "f16" else 0.0)
+        close(out, np.broadcast_to(want, out.shape), np.broadcast_to(bound, out.shape), "out")
+        y = (18.0 + np.log1p(rest))[:, None]
+        close(lse, np.broadcast_to(y, lse.shape), np.broadcast_to(rel + 2.0 ** -22 * y, lse.shape), "lse")
