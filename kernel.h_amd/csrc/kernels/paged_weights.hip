@@ -49,11 +49,14 @@ __device__ __forceinline__ uint32_t rows_of(const Seers &s, int R0) {
   return from >= to ? 0u : (~0u >> (32 - to)) & (~0u << from);
 }
 
-// lse as it is subtracted from scores in powers of two; a row that saw nothing
-// (or is none) gives 2^-inf.
+// lse as it is subtracted from scores in powers of two; of a row that saw nothing
+// (or is none) infinity. Such a row adds nothing whatever its scores are: those of
+// infinities and NaN would not become 2^-inf, so it is masked like one that
+// does not see the entry.
 __device__ __forceinline__ float taken(float lse, bool real) {
   return real && lse != -__builtin_inff() ? lse * kLog2e : __builtin_inff();
 }
+__device__ __forceinline__ bool adds(float taken) { return taken != __builtin_inff(); }
 
 struct Job {
   KhSeq s;
@@ -79,7 +82,8 @@ template <int D>
 struct Queries {
   u32x4 q[kFewRows / 16][Form<D>::steps];
   float lse[kFewRows / 16][4];
-  bool two;  // more than 16 rows
+  uint32_t some;  // bit 16 t + e: the lane's row e of tile t is one that saw something
+  bool two;       // more than 16 rows
 };
 
 template <int D>
@@ -87,6 +91,7 @@ __device__ __forceinline__ Queries<D> queries(const KhWeightsParams &p, const Jo
   const int d = p.cache.head_dim, row_bytes = d * (int)sizeof(elem);
   Queries<D> y;
   y.two = j.rows > 16;
+  y.some = 0;
 #pragma unroll
   for (int t = 0; t < kFewRows / 16; ++t) {
     const KhQuery row = kh_query(j.s, p.group, p.by_group, 16 * t + r);
@@ -102,6 +107,7 @@ __device__ __forceinline__ Queries<D> queries(const KhWeightsParams &p, const Jo
       const int R = 16 * t + 4 * h + e;
       const KhQuery at = kh_query(j.s, p.group, p.by_group, R);
       y.lse[t][e] = taken(p.lse[(int64_t)at.token * p.q_heads + j.head * p.group + at.head], R < j.rows);
+      y.some |= adds(y.lse[t][e]) ? 1u << (16 * t + e) : 0u;
     }
   }
   return y;
@@ -111,7 +117,7 @@ __device__ __forceinline__ Queries<D> queries(const KhWeightsParams &p, const Jo
 template <int D>
 __device__ __forceinline__ float received(const KhWeightsParams &p, const Job &j, const Queries<D> &y, const f32x4 (&x)[kFewRows / 16],
                                           int key, bool there, int h) {
-  const uint32_t sees = there ? rows_of(seers_of(j.s, key, p.group, p.window), 0) >> 4 * h : 0;
+  const uint32_t sees = there ? rows_of(seers_of(j.s, key, p.group, p.window), 0) >> 4 * h & y.some : 0;
   float sum = 0.0f;
 #pragma unroll
   for (int t = 0; t < kFewRows / 16; ++t)
@@ -313,11 +319,16 @@ __device__ __forceinline__ void send(const KhWeightsParams &p, const Job &j, int
     dma16(rsrc, off[i], (uint32_t)reinterpret_cast<uintptr_t>(buffer) + (uint32_t)((wave * W::share + i * W::per_wave) * W::bytes));
 }
 
+// Two tiles of rows, what is taken of each row's scores, and which rows add something.
+template <int D>
+constexpr int kWideLdsOf = 2 * (Rows<D>::tile * (Rows<D>::bytes + 4) + 8);
+
 template <int D>
 __device__ __forceinline__ void wide(const KhWeightsParams &p, const Job &j, int key0, char *lds) {
   using W = Rows<D>;
   constexpr int kSteps = W::bytes / 32, kBuffer = W::tile * W::bytes;
   float *stats = reinterpret_cast<float *>(lds + 2 * kBuffer);  // [2][tile]
+  uint32_t *some = reinterpret_cast<uint32_t *>(stats + 2 * W::tile);  // [2][2], bit n: row n of 32 adds something
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int r = lane & 31, h = lane >> 5;
   const int row_bytes = p.cache.head_dim * (int)sizeof(elem);
@@ -357,8 +368,16 @@ __device__ __forceinline__ void wide(const KhWeightsParams &p, const Job &j, int
       const char *buffer = lds + cur * kBuffer;
       float *lse = stats + cur * W::tile;
       vm_wait<0>();
-      if (tid < W::tile) lse[tid] = taken(ahead, R0 + tid < j.rows);
+      if (wave == 0) {  // a tile has no more rows than a wave lanes
+        const float y = taken(ahead, R0 + tid < j.rows);
+        const uint64_t all = __builtin_amdgcn_ballot_w64(adds(y));
+        if (tid < W::tile) lse[tid] = y;
+        if (tid < 2) some[2 * cur + tid] = (uint32_t)(all >> 32 * tid);
+      }
       lds_barrier();
+      uint32_t added[2];
+#pragma unroll
+      for (int t = 0; t < W::tile / 32; ++t) added[t] = __builtin_amdgcn_readfirstlane(some[2 * cur + t]);
       ahead = lse_at(R0 + W::tile);
       if (!p.steady) pieces_of<D>(p, j, R0 + W::tile, off, lane, wave);
       send<D>(p, j, R0 + W::tile, off, lds + (cur ^ 1) * kBuffer, wave);
@@ -369,8 +388,8 @@ __device__ __forceinline__ void wide(const KhWeightsParams &p, const Job &j, int
         f32x16 x = {};
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) x = mma32(k_rows<D>(buffer, t, c, lane), k[c], x);
-        const bool whole = R1 >= wave_last.first && R1 + 32 <= wave_first.end;
-        const uint32_t sees = whole ? ~0u : rows_of(own, R1) >> 4 * h;
+        const bool whole = R1 >= wave_last.first && R1 + 32 <= wave_first.end && added[t] == ~0u;
+        const uint32_t sees = whole ? ~0u : (rows_of(own, R1) & added[t]) >> 4 * h;
         float part = 0.0f;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -434,7 +453,7 @@ __device__ __forceinline__ void weights(const KhWeightsParams &p, char *lds) {
 // Steps of single tokens, and of few: with the ring, two workgroups to a CU.
 #define KH_WEIGHTS(D)                                                                                      \
   extern "C" __global__ void __launch_bounds__(256, D > 128 ? 1 : 2) KH_TYPED(paged_weights_##D)(const KhWeightsParams p) { \
-    constexpr int kWideLds = 2 * Rows<D>::tile * (Rows<D>::bytes + 4);                                      \
+    constexpr int kWideLds = kWideLdsOf<D>;                                                                 \
     __shared__ __attribute__((aligned(16))) char lds[kWideLds > Ring<D>::lds ? kWideLds : Ring<D>::lds];    \
     if (p.even)                                                                                             \
       weights<D, true>(p, lds);                                                                             \
@@ -450,7 +469,7 @@ KH_WEIGHTS(256)
 // In 32 bits heads of 128 take 66 KB: two.
 #define KH_WEIGHTS_WIDE(D)                                                                                 \
   extern "C" __global__ void __launch_bounds__(256, D > 128 ? 1 : kWide && D > 64 ? 2 : 3) KH_TYPED(paged_weights_wide_##D)(const KhWeightsParams p) { \
-    __shared__ __attribute__((aligned(16))) char lds[2 * Rows<D>::tile * (Rows<D>::bytes + 4)];             \
+    __shared__ __attribute__((aligned(16))) char lds[kWideLdsOf<D>];                                        \
     weights<D, false>(p, lds);                                                                              \
   }
 KH_WEIGHTS_WIDE(64)

@@ -165,3 +165,30 @@ def test_many_small_weights_beside_a_large_one(dev, dtype, m, n):
         close(out, np.broadcast_to(want, out.shape), np.broadcast_to(bound, out.shape), "out")
         y = (18.0 + np.log1p(rest))[:, None]
         close(lse, np.broadcast_to(y, lse.shape), np.broadcast_to(rel + 2.0 ** -22 * y, lse.shape), "lse")
+
+
+# ---------------------------------------------------------------- rows that add nothing
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("page_size", [16, 24])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("m", [3, 70])
+def test_weights_skip_rows_of_minus_infinity_whatever_they_hold(dev, dtype, page_size, value, m):
+    """lse = -inf says that a row saw nothing: what stands in its queries, or in
+    a key that only such rows see, reaches no weight."""
+    s = Step(dtype, [m, 1], [m + 130, 40], 4, 2, 64, page_size=page_size, seed=m)
+    y = s.attention()[2].astype(np.float32)
+    rows = [1, 2] if m == 3 else [1, 30, 31, 47, 69]
+    y[rows] = -math.inf
+    want_from = Step(dtype, [m, 1], [m + 130, 40], 4, 2, 64, page_size=page_size, seed=m)
+    s.q[rows] = value
+    # The last token's own entry, which no other token sees.
+    at = m + 129
+    s.k[s.table[0, at // page_size], at % page_size, 0, 5] = value
+    cap = m + 135
+    before = want_from.g.random((2, 2, cap), np.float32)
+    say(f"weights {dtype} page={page_size} m={m} value={value} in rows of lse -inf")
+    got = s.run_weights(y, before)
+    want, bound = want_from.weights(y, before)
+    for i, n in enumerate((m + 130, 40)):
+        close(got[i, :, :n], want[i, :, :n], bound[i, :, :n], f"sequence {i}")
