@@ -286,13 +286,24 @@ int kh_qk_norm_rope(const kh_qk_norm_rope_args *args, void *stream) {
     // sixteen of them to a CU.
     const int64_t steps = ceil_div(a.q_heads, 64 / lanes) + 2 * ceil_div(c.kv_heads, 64 / lanes);
     const int64_t parts = std::clamp<int64_t>(ceil_div(16 * KH_GEMM_CUS, a.tokens), 1, steps);
-    KhRopeParams p{a.q, a.k, a.v, a.q_out, a.k_out, a.q_gamma, a.k_gamma, a.inv_freq, a.positions, a.slots, c.k, c.v,
-                   a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride, c.k_page_stride, c.k_slot_stride,
-                   c.k_head_stride, c.v_page_stride, c.v_slot_stride, c.v_head_stride, cached ? c.pages * c.page_size : 0,
-                   static_cast<int32_t>(c.page_size), static_cast<int32_t>(a.tokens), static_cast<int32_t>(a.q_heads),
-                   static_cast<int32_t>(c.kv_heads), static_cast<int32_t>(c.head_dim), static_cast<int32_t>(a.rotary_dim),
-                   a.interleaved != 0, a.norm != 0, static_cast<int32_t>(parts), a.eps};
-    return launch(kRope[lanes / 16][c.dtype], ceil_div(a.tokens * parts, 4), 1, 256, p, stream);
+    // A launch has fewer than 2^32 threads: more tokens than this take several.
+    constexpr int64_t kMost = int64_t(1) << 25;
+    const auto row = [](const void *at, int64_t elements, int size) {
+      return at != nullptr ? const_cast<char *>(static_cast<const char *>(at)) + elements * size : nullptr;
+    };
+    for (int64_t t = 0; t < a.tokens; t += kMost) {
+      const int64_t tokens = std::min(kMost, a.tokens - t);
+      KhRopeParams p{row(a.q, t * a.q_stride, e), row(a.k, t * a.k_stride, e), cached ? row(a.v, t * a.v_stride, e) : nullptr,
+                     row(a.q_out, t * a.q_out_stride, e), row(a.k_out, t * a.k_out_stride, e), a.q_gamma, a.k_gamma, a.inv_freq,
+                     a.positions != nullptr ? a.positions + t : nullptr, a.slots != nullptr ? a.slots + t : nullptr, c.k, c.v,
+                     a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride, c.k_page_stride, c.k_slot_stride,
+                     c.k_head_stride, c.v_page_stride, c.v_slot_stride, c.v_head_stride, cached ? c.pages * c.page_size : 0,
+                     static_cast<int32_t>(c.page_size), static_cast<int32_t>(tokens), static_cast<int32_t>(a.q_heads),
+                     static_cast<int32_t>(c.kv_heads), static_cast<int32_t>(c.head_dim), static_cast<int32_t>(a.rotary_dim),
+                     a.interleaved != 0, a.norm != 0, static_cast<int32_t>(parts), a.eps};
+      if (int rc = launch(kRope[lanes / 16][c.dtype], ceil_div(tokens * parts, 4), 1, 256, p, stream)) return rc;
+    }
+    return 0;
   });
 }
 

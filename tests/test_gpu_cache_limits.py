@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import kernelh as kh
-from cachetest import DTYPES, Step, half_step, ints_on_gpu, rounded, same_bits, values_from_gpu, values_on_gpu
+from cachetest import DTYPES, Step, decode, half_step, ints_on_gpu, rope_reference, rounded, same_bits, values_from_gpu, values_on_gpu
 from khtest import say
 from test_gpu_cache import check_attention, check_weights, close
 
@@ -192,3 +192,31 @@ def test_weights_skip_rows_of_minus_infinity_whatever_they_hold(dev, dtype, page
     want, bound = want_from.weights(y, before)
     for i, n in enumerate((m + 130, 40)):
         close(got[i, :, :n], want[i, :, :n], bound[i, :, :n], f"sequence {i}")
+
+
+# ---------------------------------------------------------------- many tokens
+
+def test_rotation_of_more_tokens_than_a_launch_has_threads_for(dev):
+    """2^26 and some tokens of one short head, one row shared by all as a stride
+    of 0 says: each turned by its own position."""
+    t, d = (1 << 26) + 1003, 8
+    g = np.random.default_rng(2)
+    x = [rounded(g.standard_normal((1, 1, d), np.float32), "bf16") for _ in "qk"]
+    dx = [values_on_gpu(v, "bf16") for v in x]
+    freq = np.array([1.0, 0.37, 0.01, 1e-4], np.float32)
+    df, pos = values_on_gpu(freq, "f32"), np.arange(t, dtype=np.int64)
+    dp = ints_on_gpu(pos, np.int64)
+    out = [kh.Buffer(t * d * 2) for _ in "qk"]
+    say(f"rope of {t} tokens")
+    kh.qk_norm_rope(kh.QkNormRope(q=dx[0].ptr, k=dx[1].ptr, q_out=out[0].ptr, k_out=out[1].ptr, inv_freq=df.ptr, positions=dp.ptr,
+                                  q_stride=0, k_stride=0, q_out_stride=d, k_out_stride=d,
+                                  cache=kh.PagedCache(kv_heads=1, head_dim=d, dtype=kh.BF16), tokens=t, q_heads=1, rotary_dim=d,
+                                  interleaved=0, norm=1, eps=1e-6))
+    kh.synchronize()
+    for at in (0, (1 << 25) - 500, (1 << 26) - 500, t - 1000):
+        mine = pos[at:at + 1000]
+        for i, name in enumerate("qk"):
+            bits = np.empty((1000, 1, d), np.int16)
+            kh.check(kh.lib.khrt_memcpy_d2h(bits.ctypes.data, out[i].ptr + at * d * 2, bits.nbytes))
+            want, bound = rope_reference(np.broadcast_to(x[i], (1000, 1, d)), None, mine, freq, d, 0, 1e-6, 1, "bf16")
+            close(decode(bits, "bf16"), want, bound, f"{name} from token {at}")
