@@ -277,7 +277,7 @@ struct KhAttentionParams {
   int32_t narrow_rows;  // a sequence of more rows is the wide form's
   int32_t wide_blocks, wide_splits;
   int32_t even;  // pages hold a multiple of 16 entries, rows apart, and 16 slots' strides fit 31 bits
-  uint32_t q_sign;  // the sign bits of q's elements where the scale is negative
+  uint32_t q_keep, q_sign;  // q's bits that count (none with a scale of 0); the sign bits where the scale is negative
   KhDiv by_group;
   float scale_log2;  // |scale| log2(e), above 0: maxima may be taken before it
 };

@@ -274,7 +274,7 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
 #pragma unroll
     for (int c = 0; c < F::steps; ++c) {
       // From an address that is there in any case, as the rows of K and V.
-      const u32x4 x = *reinterpret_cast<const u32x4 *>(qp + within(64 * c + 16 * h, row_bytes)) ^ p.q_sign;
+      const u32x4 x = *reinterpret_cast<const u32x4 *>(qp + within(64 * c + 16 * h, row_bytes)) & p.q_keep ^ p.q_sign;
       q[c] = mine && 64 * c + 16 * h < row_bytes ? x : u32x4{0, 0, 0, 0};
     }
 
@@ -723,7 +723,7 @@ __device__ __forceinline__ void wide(const KhAttentionParams &p, int block, char
   const char *qp = static_cast<const char *>(p.q) + ((int64_t)(s.start + i) * p.q_stride + (int64_t)hq * d) * (int)sizeof(elem);
 #pragma unroll
   for (int c = 0; c < W::steps; ++c) {
-    const u32x4 x = *reinterpret_cast<const u32x4 *>(qp + within(32 * c + 16 * h, row_bytes)) ^ p.q_sign;
+    const u32x4 x = *reinterpret_cast<const u32x4 *>(qp + within(32 * c + 16 * h, row_bytes)) & p.q_keep ^ p.q_sign;
     q[c] = mine && 32 * c + 16 * h < row_bytes ? x : u32x4{0, 0, 0, 0};
   }
   float m = mine ? kSeed : 0.0f, l = 0.0f;

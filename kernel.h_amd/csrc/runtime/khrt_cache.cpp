@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cmath>
 #include <exception>
+#include <limits>
 #include <string>
 
 namespace {
@@ -183,6 +184,12 @@ int check_attention(const char *op, const kh_paged_attention_args &a) {
   return 0;
 }
 
+// log2(e) times the scale, finite as that is: a score of 0 stays one.
+float in_powers_of_two(float scale) {
+  constexpr float most = std::numeric_limits<float>::max();
+  return std::clamp(scale * 1.44269504088896340736f, -most, most);
+}
+
 // How a launch of paged_attention spreads over the chip (kh_paged.h).
 struct AttentionPlan {
   int64_t groups;              // workgroups of sequences of few rows
@@ -338,14 +345,16 @@ int kh_paged_attention(const kh_paged_attention_args *args, void *workspace, siz
     const int64_t wide_blocks = plan.wide_units * plan.splits;
     const int e = element_bytes(a.cache.dtype);
     const bool even = even_pages(a.cache);
+    // Scores are masked before the factor: it is above 0, which a scale of 0 makes up
+    // for with queries of 0.
+    const float factor = a.scale == 0.0f ? 1.0f : std::fabs(in_powers_of_two(a.scale));
     KhAttentionParams p{device_cache(a.cache), device_table(a.table, a.cache), a.q, a.out, a.lse, a.q_starts, part_o, part_ml,
                         wide_o, wide_ml, a.q_stride, a.out_stride, static_cast<int32_t>(a.tokens),
                         static_cast<int32_t>(a.q_heads), static_cast<int32_t>(group), static_cast<int32_t>(a.window),
                         static_cast<int32_t>(plan.groups), plan.whole, static_cast<int32_t>(plan.narrow_rows),
                         static_cast<int32_t>(wide_blocks), static_cast<int32_t>(std::max<int64_t>(plan.splits, 1)),
-                        even, a.scale < 0.0f ? (e == 4 ? 0x80000000u : 0x80008000u) : 0u,
-                        kh_div_by(static_cast<uint32_t>(group)),
-                        std::max(std::fabs(a.scale) * 1.44269504088896340736f, 1e-37f)};
+                        even, a.scale == 0.0f ? 0u : 0xffffffffu, a.scale < 0.0f ? (e == 4 ? 0x80000000u : 0x80008000u) : 0u,
+                        kh_div_by(static_cast<uint32_t>(group)), factor};
     const auto &symbols = wide_blocks > 0 ? kWide : kAttention;
     if (int rc = launch(symbols[width_of(d)][a.cache.dtype], wide_blocks + plan.groups, 1, 256, p, stream)) return rc;
     if (!joined) return 0;
@@ -381,7 +390,7 @@ int kh_paged_weights(const kh_paged_weights_args *args, void *stream) {
                       a.q_stride, a.weights_seq_stride, a.weights_head_stride, static_cast<int32_t>(a.tokens),
                       static_cast<int32_t>(a.q_heads), static_cast<int32_t>(group), static_cast<int32_t>(a.window),
                       static_cast<int32_t>(each * KH_STRETCH), static_cast<int32_t>(chunks), even_pages(a.cache),
-                      32 % group == 0 && a.q_stride >= a.q_heads * a.cache.head_dim, kh_div_by(static_cast<uint32_t>(group)), a.scale * 1.44269504088896340736f};
+                      32 % group == 0 && a.q_stride >= a.q_heads * a.cache.head_dim, kh_div_by(static_cast<uint32_t>(group)), in_powers_of_two(a.scale)};
     return launch((few ? kWeights : kWeightsWide)[width_of(a.cache.head_dim)][a.cache.dtype], pairs * chunks, 1, 256, p, stream);
   });
 }

@@ -167,6 +167,56 @@ def test_many_small_weights_beside_a_large_one(dev, dtype, m, n):
         close(lse, np.broadcast_to(y, lse.shape), np.broadcast_to(rel + 2.0 ** -22 * y, lse.shape), "lse")
 
 
+@pytest.mark.parametrize("dtype,size", [("f32", 2.0 ** 62), ("bf16", 2.0 ** 62), ("f16", 2.0 ** 14)])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 2.0 ** -149, -2.0 ** -140, 2.0 ** -120, 3.4e38])
+@pytest.mark.parametrize("m,n", [(1, 300), (100, 300)])
+def test_scales_at_their_ends(dev, dtype, size, scale, m, n):
+    """Scores of q . k = 0 or +-size^2 under scales of 0, of denormal numbers and
+    of the largest: the softmax of the scaled ones."""
+    s, _, page, slot = row_of_scores(dtype, m, n, [0.0])
+    s.scale = scale
+    signs = s.g.integers(-1, 2, n)
+    signs[0] = 1
+    if scale > 1:
+        signs[:] = 0  # the largest scale has only scores of 0 left that are numbers
+    s.q.reshape(s.tokens, s.hq, s.d)[:, :, 7] = size
+    s.k[page, slot, 0, 7] = signs * size
+    say(f"scale {scale} {dtype} m={m}")
+    out, lse = s.run_attention()
+    # The scale as it is taken: a float of the call.
+    x = signs.astype(np.float64) * size * size * float(np.float32(scale))
+    for i in range(m):
+        here = x[:n - m + i + 1]
+        top = here.max()
+        p = np.exp(here - top)
+        v = s.v[page, slot, 0][:len(here)].astype(np.float64)
+        want, room = p @ v / p.sum(), p @ np.abs(v) / p.sum()
+        # The factor of a denormal scale is one too, off by half the smallest of
+        # them (2^-150) or less: of 2^124 at the most. The exponent rounds, and n terms.
+        off = 2.0 ** -150 * size * size + 2.0 ** -22 * np.abs(here).max() + 2 * (n + 64) * 2.0 ** -24
+        u = half_step(dtype)
+        bound = room * (off + u) + np.abs(want) * u + (2.0 ** -25 if dtype == "f16" else 1e-30)
+        for h in range(s.hq):
+            close(out[i, h], want, bound, f"token {i}")
+            y = top + math.log(p.sum())
+            close(lse[i, h], y, off + 2.0 ** -22 * (abs(y) + 1), "lse")
+
+
+@pytest.mark.parametrize("scale", [3.4e38, -3.4e38, 0.0])
+@pytest.mark.parametrize("m", [1, 100])
+def test_weights_of_scores_of_zero(dev, scale, m):
+    """Keys of zeros under the largest scales: every entry receives exp(-lse)."""
+    s, _, page, slot = row_of_scores("bf16", m, 200, [0.0])
+    s.scale = scale
+    s.q[:] = 1.0
+    y = np.full((s.tokens, s.hq), math.log(4.0), np.float32)
+    before = s.g.random((1, 1, 205), np.float32)
+    say(f"weights, scale {scale} m={m}")
+    got = s.run_weights(y, before)
+    want, bound = s.weights(y, before)
+    close(got[0, :, :200], want[0, :, :200], bound[0, :, :200], "weights")
+
+
 # ---------------------------------------------------------------- rows that add nothing
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
