@@ -462,10 +462,12 @@ KHRT_API int kh_qk_norm_rope(const kh_qk_norm_rope_args *args, void *stream);
  * do not reach it. out must not be q.
  *
  * workspace (16-byte aligned, may be null): with it a long sequence is split
- * over several workgroups. More than
- * kh_paged_attention_workspace reports is not used, less means fewer splits.
- * Its contents need no preparation; calls that overlap in time need one
- * each. */
+ * over several workgroups. What kh_paged_attention_workspace reports suffices for
+ * this step and every smaller one: of at most its tokens, sequences, expected
+ * lengths and window (0 is the largest), the rest as it is. A program that asks
+ * once for its largest step may use it for all. Less means fewer splits, and that
+ * a long sequence takes longer. Its contents need no preparation; calls that
+ * overlap in time need one each. */
 typedef struct kh_paged_attention_args {
   kh_paged_cache cache;
   kh_page_table table;

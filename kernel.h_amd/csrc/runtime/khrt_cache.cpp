@@ -211,13 +211,24 @@ int64_t narrow_rows_of(int32_t dtype) { return dtype == KHRT_F32 ? 64 : 32; }
 // 41; 1 x 1000 17 / 27, 8 x 1000 17 / 23.
 constexpr int64_t kWholeBlocks = 4;
 
+// Entries of a sequence that any of its new tokens sees: with a window nobody
+// looks further back than the window and the new tokens.
+int64_t seen_len(const kh_paged_attention_args &a) {
+  const int64_t len = expected_len(a.table, a.cache);
+  return a.window > 0 ? std::min(len, a.window + a.tokens) : len;
+}
+
+// A row of a part: fp32, with its maximum and sum.
+size_t part_row_bytes(const kh_paged_attention_args &a) { return (2 + static_cast<size_t>(a.cache.head_dim)) * sizeof(float); }
+
+// Workgroups of the narrow form that are on the chip at once.
+int64_t most_groups(const kh_paged_attention_args &a) { return (a.cache.head_dim > 128 ? 1 : 2) * KH_GEMM_CUS; }
+
 AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_bytes) {
   AttentionPlan p{};
   const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.tokens * group;
-  int64_t len = expected_len(a.table, a.cache);
-  // With a window nobody looks further back than the window and the new tokens.
-  if (a.window > 0) len = std::min(len, a.window + a.tokens);
-  const size_t row_bytes = (2 + static_cast<size_t>(a.cache.head_dim)) * sizeof(float);
+  const int64_t len = seen_len(a);
+  const size_t row_bytes = part_row_bytes(a);
 
   // Few rows to a sequence, by all the host can know: the narrow form has them
   // all. One sequence: whichever suits its rows. Otherwise both.
@@ -243,8 +254,7 @@ AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_
   const int64_t narrow_most = narrow_only ? rows : std::min(rows, few * a.table.seqs);
   const int64_t units = (narrow_most / KH_TILE_ROWS + std::min(a.tokens, a.table.seqs)) * a.cache.kv_heads;
   const int64_t blocks = ceil_div(len, KH_STRETCH);
-  // As many workgroups as are on the chip at once.
-  const int64_t most = (a.cache.head_dim > 128 ? 1 : 2) * KH_GEMM_CUS;
+  const int64_t most = most_groups(a);
   const size_t per_group = size_t(2) * KH_TILE_ROWS * row_bytes;
   p.groups = std::min<int64_t>(most, std::max(ceil_div(units * blocks, 2), std::min(units, most)));
   p.groups = std::min(p.groups, static_cast<int64_t>(workspace_bytes / per_group));
@@ -255,6 +265,25 @@ AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_
   if (p.whole) p.groups = std::min(units, most);
   p.part_bytes = p.whole ? 0 : static_cast<size_t>(p.groups) * per_group;
   return p;
+}
+
+// What the plan of no step of at most these tokens, sequences, lengths and window
+// takes more than. A single step's own need does not grow with the step: a long
+// chunk fills the chip without parts, a short one and single tokens do not. Each
+// of the plan's two terms is bounded by one that does grow.
+size_t attention_workspace(const kh_paged_attention_args &a) {
+  const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.tokens * group, len = seen_len(a);
+  const size_t row_bytes = part_row_bytes(a);
+  // Narrow: two parts of 16 rows for each workgroup.
+  const int64_t blocks = ceil_div(len, KH_STRETCH), most = most_groups(a);
+  const int64_t units = (rows / KH_TILE_ROWS + std::min(a.tokens, a.table.seqs)) * a.cache.kv_heads;
+  const int64_t groups = blocks <= kWholeBlocks ? 0 : std::min(most, units * blocks);
+  // Wide: its splits times its units are at most two to a CU, and its rows fewer
+  // than its units times theirs.
+  const int64_t splits = len / 256;
+  const int64_t wide_rows = splits < 2 || rows <= narrow_rows_of(a.cache.dtype)
+                                ? 0 : std::min<int64_t>(2 * KH_GEMM_CUS * KH_WIDE_ROWS, splits * a.tokens * a.q_heads);
+  return (static_cast<size_t>(groups < 2 ? 0 : groups) * 2 * KH_TILE_ROWS + static_cast<size_t>(wide_rows)) * row_bytes;
 }
 
 }  // namespace
@@ -319,8 +348,7 @@ int kh_paged_attention_workspace(const kh_paged_attention_args *args, size_t *by
   return guarded(op, [&] {
     if (args == nullptr || bytes == nullptr) return bad(op, "null argument");
     if (int rc = check_attention(op, *args)) return rc;
-    const AttentionPlan p = attention_plan(*args, SIZE_MAX / 2);
-    *bytes = p.part_bytes + p.wide_bytes;
+    *bytes = attention_workspace(*args);
     return 0;
   });
 }

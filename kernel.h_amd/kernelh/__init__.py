@@ -697,7 +697,7 @@ def qk_norm_rope(args: QkNormRope, stream=None) -> None:
 
 
 def paged_attention_workspace(args: PagedAttention) -> int:
-    """Bytes with which paged_attention splits these sequences as far as it pays."""
+    """Bytes with which paged_attention splits the sequences of this step, and of every smaller one, as far as it pays."""
     n = ctypes.c_size_t()
     check(lib.kh_paged_attention_workspace(args, ctypes.byref(n)))
     return n.value

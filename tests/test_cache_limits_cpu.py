@@ -1,7 +1,13 @@
 """The sequence-cache operators at their limits, without a GPU: that no address
 leaves its array whatever device memory holds."""
+import itertools
 import os
 import subprocess
+
+import pytest
+
+import kernelh as kh
+from test_cache_cpu import attention, cache, table
 
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -15,3 +21,28 @@ def test_addresses_stay_inside(tmp_path):
     assert r.returncode == 0, r.stdout
     r = subprocess.run([str(exe)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.strip().endswith("paged_bounds_check ok"), r.stdout
+
+
+@pytest.mark.parametrize("dtype", [kh.F32, kh.BF16])
+@pytest.mark.parametrize("hq,hk,d", [(32, 8, 128), (16, 16, 64), (8, 1, 256), (7, 1, 80)])
+def test_a_workspace_suffices_for_every_smaller_step(dtype, hq, hk, d):
+    """What the largest step reports, no smaller one asks more than: of fewer
+    tokens, fewer sequences, shorter ones, under a window."""
+    st = dict(k_page_stride=16 * hk * d, k_slot_stride=hk * d, k_head_stride=d, v_page_stride=16 * hk * d, v_slot_stride=hk * d,
+              v_head_stride=d)
+    tokens, seqs, lens, windows = (1, 4, 33, 127, 512, 2048, 8192), (1, 4, 64), (300, 1024, 8192, 131072), (0, 4096, 100)
+
+    def size(t, s, n, w):
+        return kh.paged_attention_workspace(attention(
+            cache=cache(kv_heads=hk, head_dim=d, dtype=dtype, **st), table=table(seqs=s, width=8192, row_stride=8192, max_len=n),
+            q_heads=hq, q_stride=hq * d, out_stride=hq * d, tokens=t, window=w))
+
+    all_of = {x: size(*x) for x in itertools.product(tokens, seqs, lens, windows)}
+    for t, s, n, w in all_of:
+        for x, need in all_of.items():
+            if x[0] <= t and x[1] <= s and x[2] <= n and (w == 0 or 0 < x[3] <= w):
+                assert need <= all_of[t, s, n, w], (x, (t, s, n, w))
+    # A single token of a long sequence is split, whatever else the step may have had.
+    assert all_of[1, 1, 131072, 0] >= 100 * (d + 2) * 4
+    # Two workgroups to a CU, of two parts of 16 rows or one of 128.
+    assert max(all_of.values()) <= 512 * (32 + 128) * (d + 2) * 4

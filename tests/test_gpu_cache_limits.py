@@ -270,3 +270,25 @@ def test_rotation_of_more_tokens_than_a_launch_has_threads_for(dev):
             kh.check(kh.lib.khrt_memcpy_d2h(bits.ctypes.data, out[i].ptr + at * d * 2, bits.nbytes))
             want, bound = rope_reference(np.broadcast_to(x[i], (1000, 1, d)), None, mine, freq, d, 0, 1e-6, 1, "bf16")
             close(decode(bits, "bf16"), want, bound, f"{name} from token {at}")
+
+
+# ---------------------------------------------------------------- workspaces
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_the_largest_steps_workspace_splits_smaller_ones_as_far_as_pays(dev, dtype):
+    """With what the largest step reports, every smaller one comes out bit for
+    bit as with any amount."""
+    hq, hk, d = 8, 2, 64
+    most = Step(dtype, [2048, 1, 1, 1], [4000, 3000, 2000, 100], hq, hk, d)
+    cache, keep1 = most.cache_on_gpu()
+    table, keep2 = most.table_on_gpu(4000)
+    size = kh.paged_attention_workspace(kh.PagedAttention(
+        cache=cache, table=table, q=cache.k, out=cache.v, lse=None, q_starts=table.lens, q_stride=hq * d, out_stride=hq * d,
+        tokens=most.tokens, q_heads=hq, window=0, scale=0.125))
+    del keep1, keep2
+    for q_lens, lens in (([1], [4000]), ([1, 1, 1, 1], [4000, 3000, 2000, 100]), ([40], [4000]), ([300], [3999]),
+                         ([128, 1], [2000, 4000]), ([700, 5, 9], [1000, 4000, 3000]), ([2048], [4000])):
+        s = Step(dtype, q_lens, lens, hq, hk, d, seed=len(lens))
+        a = check_attention(s, workspace=size, max_len=max(lens))
+        b = s.run_attention(workspace=1 << 28, max_len=max(lens))
+        assert all(same_bits(x, y) for x, y in zip(a, b))
