@@ -461,6 +461,11 @@ KHRT_API int kh_qk_norm_rope(const kh_qk_norm_rope_args *args, void *stream);
  * left as they were. Infinities and NaN in entries that a token does not see
  * do not reach it. out must not be q.
  *
+ * max_new: the most new tokens that the caller expects of one sequence, 0 if
+ * unknown (every sequence is then taken to have one at least). As max_len it
+ * shapes the launch and changes no result but its rounding: with it a batch of
+ * a few tokens each need not be prepared for a long chunk among them.
+ *
  * workspace (16-byte aligned, may be null): with it a long sequence is split
  * over several workgroups. What kh_paged_attention_workspace reports suffices for
  * this step and every smaller one: of at most its tokens, sequences, expected
@@ -477,6 +482,7 @@ typedef struct kh_paged_attention_args {
   const int32_t *q_starts; /* [seqs + 1] */
   int64_t q_stride, out_stride;
   int64_t tokens, q_heads, window;
+  int64_t max_new;
   float scale;
 } kh_paged_attention_args;
 KHRT_API int kh_paged_attention_workspace(const kh_paged_attention_args *args, size_t *bytes);

@@ -218,6 +218,23 @@ KH_HD KhOwners kh_owners(const KhShares &s, int32_t work, int32_t begin, int32_t
   return o;
 }
 
+// Whether a step goes to the narrow form alone, by what the host can know: `few`
+// rows to a sequence on the whole, and `most` at the most in one of them. new: the
+// most new tokens of a sequence as the caller expects, 0 if it does not say; then
+// every sequence is taken to have one at least. A long chunk among single tokens
+// would read its entries once for every 16 rows; one that is not there costs the
+// launch's idle wide workgroups. MI355X, bf16, 32 heads on 8 of 128, 2000 entries
+// each, narrow alone against both: 127 single tokens and a chunk of 33 186 us / 202,
+// 64 198 / 200, 128 218 / 202, 512 344 / 203, 896 443 / 212; 64 sequences of 5
+// tokens 179 / 184. fp32: a chunk of 128 397 / 414, 256 475 / 408, 896 816 / 568.
+// One sequence: whichever form suits its rows.
+KH_HD bool kh_narrow_only(int64_t tokens, int64_t seqs, int64_t group, int64_t max_new, int64_t few, int64_t most) {
+  if (tokens * group > few * seqs) return false;
+  const int64_t left = tokens > seqs ? tokens - seqs + 1 : 1;
+  const int64_t longest = max_new > 0 && max_new < tokens ? max_new : max_new > 0 ? tokens : left;
+  return longest * group <= (seqs == 1 ? few : most);
+}
+
 // The wide form: units of KH_WIDE_ROWS rows of a sequence of more than
 // narrow_rows rows and a kv head, each with the entries that its own rows see,
 // in up to `splits` parts of whole tiles where units are few.

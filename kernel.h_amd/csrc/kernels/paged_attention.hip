@@ -215,6 +215,12 @@ __device__ __forceinline__ int sequence_at(const KhAttentionParams &p, const Lin
   return -1;
 }
 
+// Behind a launch's wide workgroups one to a CU cannot be had: where the idle ones
+// of them leave first, two of the others come to lie on one CU beside empty ones.
+__device__ __forceinline__ KhShares shares_of(const KhAttentionParams &p, const Line &line) {
+  return kh_shares(line.all, p.wide_blocks > 0 ? p.groups : kh_most(line.all, p.groups));
+}
+
 template <int D, bool EVEN>
 __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, float *lds) {
   using F = Form<D>;
@@ -223,7 +229,7 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
   const int d = p.cache.head_dim, row_bytes = d * (int)sizeof(elem);
 
   const Line line = line_of(p, false);
-  const KhShares shares = kh_shares(line.all, kh_most(line.all, p.groups));
+  const KhShares shares = shares_of(p, line);
   if (block >= shares.groups) return;
   const int start = kh_share(shares, block), end = kh_share(shares, block + 1);
   // The join area: each wave's maxima and sums of its rows, what each row's
@@ -914,7 +920,7 @@ struct Parts {
 // so: every unit of the narrow form in parts has one such.
 __device__ __forceinline__ bool narrow_parts(const KhAttentionParams &p, int g, KhSeq &s, Parts &parts) {
   const Line line = line_of(p, false);
-  const KhShares shares = kh_shares(line.all, kh_most(line.all, p.groups));
+  const KhShares shares = shares_of(p, line);
   if (g == 0 || g >= shares.groups) return false;
   const int at = kh_share(shares, g);
   int before;

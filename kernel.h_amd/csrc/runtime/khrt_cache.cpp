@@ -181,6 +181,7 @@ int check_attention(const char *op, const kh_paged_attention_args &a) {
   if (!stride_ok(a.out_stride, a.tokens, element_bytes(a.cache.dtype), a.q_heads * a.cache.head_dim))
     return bad(op, "out_stride must be a multiple of 16 bytes and hold a token");
   if (a.out == a.q) return bad(op, "out must not be q");
+  if (a.max_new < 0) return bad(op, "max_new must not be negative");
   return 0;
 }
 
@@ -232,8 +233,9 @@ AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_
 
   // Few rows to a sequence, by all the host can know: the narrow form has them
   // all. One sequence: whichever suits its rows. Otherwise both.
-  const int64_t few = narrow_rows_of(a.cache.dtype);
-  const bool narrow_only = rows <= few * a.table.seqs, wide_only = !narrow_only && a.table.seqs == 1;
+  const int64_t few = narrow_rows_of(a.cache.dtype), most_rows = a.cache.dtype == KHRT_F32 ? 1024 : 256;
+  const bool narrow_only = kh_narrow_only(a.tokens, a.table.seqs, group, a.max_new, few, most_rows);
+  const bool wide_only = !narrow_only && a.table.seqs == 1;
   p.narrow_rows = narrow_only ? INT32_MAX : wide_only ? 0 : few;
   if (!narrow_only) {
     p.wide_units = (rows / KH_WIDE_ROWS + std::min(a.tokens, a.table.seqs)) * a.cache.kv_heads;

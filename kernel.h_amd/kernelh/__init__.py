@@ -136,7 +136,7 @@ class PagedAttention(ctypes.Structure):
     _fields_ = [("cache", PagedCache), ("table", PageTable), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
                 ("lse", ctypes.c_void_p), ("q_starts", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
                 ("out_stride", ctypes.c_int64), ("tokens", ctypes.c_int64), ("q_heads", ctypes.c_int64),
-                ("window", ctypes.c_int64), ("scale", ctypes.c_float)]
+                ("window", ctypes.c_int64), ("max_new", ctypes.c_int64), ("scale", ctypes.c_float)]
 
 
 class PagedWeights(ctypes.Structure):

@@ -103,7 +103,22 @@ static void older() {
       }
 }
 
+// Which steps the narrow form has alone: single tokens and few each, not a batch
+// that may have a long chunk among them.
+static void forms() {
+  expect(kh_narrow_only(64, 64, 4, 0, 32, 256), "single tokens");
+  expect(kh_narrow_only(1, 1, 32, 0, 32, 256) && !kh_narrow_only(9, 1, 4, 0, 32, 256), "one sequence by its rows");
+  expect(kh_narrow_only(64, 8, 4, 0, 32, 256), "a few tokens each");
+  expect(!kh_narrow_only(127 + 128, 128, 4, 0, 32, 256) && !kh_narrow_only(127 + 896, 128, 4, 0, 32, 256), "a chunk among single tokens");
+  expect(kh_narrow_only(127 + 33, 128, 4, 0, 32, 256), "a short one");
+  expect(!kh_narrow_only(320, 64, 4, 0, 32, 256) && kh_narrow_only(320, 64, 4, 5, 32, 256), "five tokens each, said and not");
+  expect(!kh_narrow_only(320, 64, 4, 100, 32, 256) && !kh_narrow_only(320, 64, 4, INT64_MAX, 32, 256), "more than that said");
+  expect(!kh_narrow_only(1000, 10, 4, 1, 32, 256), "said too few: the average tells");
+  expect(kh_narrow_only(3, 100, 4, 0, 32, 256), "fewer tokens than sequences");
+}
+
 int main() {
+  forms();
   older();
   queries();
   walks();

@@ -7,7 +7,7 @@ import subprocess
 import pytest
 
 import kernelh as kh
-from test_cache_cpu import attention, cache, table
+from test_cache_cpu import attention, cache, refused, table
 
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -46,3 +46,7 @@ def test_a_workspace_suffices_for_every_smaller_step(dtype, hq, hk, d):
     assert all_of[1, 1, 131072, 0] >= 100 * (d + 2) * 4
     # Two workgroups to a CU, of two parts of 16 rows or one of 128.
     assert max(all_of.values()) <= 512 * (32 + 128) * (d + 2) * 4
+
+
+def test_attention_refuses_a_negative_max_new():
+    refused(lambda: kh.paged_attention(attention(max_new=-1)), "paged_attention")

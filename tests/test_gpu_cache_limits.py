@@ -292,3 +292,35 @@ def test_the_largest_steps_workspace_splits_smaller_ones_as_far_as_pays(dev, dty
         a = check_attention(s, workspace=size, max_len=max(lens))
         b = s.run_attention(workspace=1 << 28, max_len=max(lens))
         assert all(same_bits(x, y) for x, y in zip(a, b))
+
+
+# ---------------------------------------------------------------- a chunk among single tokens
+
+class Hinted(Step):
+    """A step whose attention says max_new."""
+    max_new = 0
+
+    def run_attention(self, *args, **kw):
+        made = kh.PagedAttention
+        kh.PagedAttention = lambda **f: made(max_new=self.max_new, **f)
+        try:
+            return super().run_attention(*args, **kw)
+        finally:
+            kh.PagedAttention = made
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("chunk", [60, 150, 400])
+def test_a_chunk_among_single_tokens(dev, dtype, chunk):
+    """Forty single tokens with a chunk first, between and last; the longest
+    said, not said, said too short and too long; with and without a workspace."""
+    g = np.random.default_rng(chunk)
+    lens = [int(x) for x in g.integers(1, 900, 41)]
+    for at in (0, 17, 40):
+        q_lens = [1] * 41
+        q_lens[at], lens[at] = chunk, chunk + int(g.integers(0, 500))
+        s = Hinted(dtype, q_lens, lens, 4, 1, 64, seed=chunk + at)
+        for s.max_new in (0, chunk, 1, 1 << 40):
+            for workspace in (None, 0):
+                say(f"max_new={s.max_new} workspace={workspace}")
+                check_attention(s, workspace=workspace)
