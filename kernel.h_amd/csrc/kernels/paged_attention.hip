@@ -404,6 +404,9 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
                   }
             }
           }
+          // Its loads end here: one that the compiler took for still on its way would
+          // have the common path wait for all, the next block among them.
+          kh::vm_wait<0>();
 #pragma unroll
           for (int a = 0; a < F::count; ++a)
 #pragma unroll
