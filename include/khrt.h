@@ -394,7 +394,12 @@ KHRT_API int khrt_bench_row_work(const char *kernel, const char *shape, double *
  * What lies in device memory is brought into range by the kernels: a length is
  * clamped to what its table row can hold, a start to [0, tokens], and an entry
  * whose page number is not in [0, pages) is one that nobody sees and nobody
- * writes. */
+ * writes.
+ *
+ * Rows that a call writes lie apart, and what it writes overlaps nothing that it
+ * reads but where it may be the same (q_out and q, k_out and k, weights and
+ * weights_in): where strides or equal pointers show that it is not so, the call
+ * is refused; the rest is the caller's to see to. */
 #define KHRT_F32 0
 #define KHRT_F16 1
 #define KHRT_BF16 2

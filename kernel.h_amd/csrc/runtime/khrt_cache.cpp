@@ -9,6 +9,7 @@
 #include <exception>
 #include <limits>
 #include <string>
+#include <utility>
 
 namespace {
 
@@ -51,6 +52,31 @@ bool stride_ok(int64_t stride, int64_t extent, int element, int64_t least) {
   return stride >= least && stride <= kMaxSpan / extent && stride % (16 / element) == 0;
 }
 
+// Whether rows of `row` elements at i a.stride + j b.stride, i < a.extent,
+// j < b.extent, lie apart. One of the extents is below 2^10 wherever this is asked
+// of strides that do not nest (pairs of sequence and kv head).
+struct Steps {
+  int64_t stride, extent;
+};
+
+bool nest(Steps inner, Steps outer, int64_t row) {
+  if (inner.extent <= 1) return outer.extent <= 1 || outer.stride >= row;
+  return inner.stride >= row && (outer.extent <= 1 || outer.stride >= (inner.extent - 1) * inner.stride + row);
+}
+
+bool rows_apart(Steps a, Steps b, int64_t row) {
+  if (nest(a, b, row) || nest(b, a, row)) return true;
+  if (a.extent > b.extent) std::swap(a, b);
+  if (a.extent <= 1 || b.stride < row || a.stride < row) return false;
+  // Two rows differ by i steps of a and, in the other direction, j of b.
+  for (int64_t i = 1; i < a.extent; ++i) {
+    const int64_t off = i * a.stride, j = off / b.stride;
+    if (j < b.extent && off - j * b.stride < row) return false;
+    if (j + 1 < b.extent && (j + 1) * b.stride - off < row) return false;
+  }
+  return true;
+}
+
 // The fields that describe rows, of a cache that may have none.
 int check_rows(const char *op, const kh_paged_cache &c) {
   if (c.dtype != KHRT_F32 && c.dtype != KHRT_F16 && c.dtype != KHRT_BF16)
@@ -78,6 +104,17 @@ int check_cache(const char *op, const kh_paged_cache &c, bool written) {
         !stride_ok(is_v ? c.v_head_stride : c.k_head_stride, c.kv_heads, e, least))
       return bad(op, written ? "cache strides must be multiples of 16 bytes and hold a row"
                              : "cache strides must be multiples of 16 bytes, not negative");
+    if (!written) continue;
+    // Rows that are written lie apart: whatever the order of pages, slots and heads, each holds the ones inside.
+    Steps s[] = {{is_v ? c.v_page_stride : c.k_page_stride, c.pages}, {is_v ? c.v_slot_stride : c.k_slot_stride, c.page_size},
+                 {is_v ? c.v_head_stride : c.k_head_stride, c.kv_heads}};
+    std::sort(s, s + 3, [](const Steps &a, const Steps &b) { return (a.extent > 1 ? a.stride : 0) < (b.extent > 1 ? b.stride : 0); });
+    int64_t inside = c.head_dim;
+    for (const Steps &x : s) {
+      if (x.extent <= 1) continue;
+      if (x.stride < inside) return bad(op, "rows of a cache that is written must not overlap");
+      inside += (x.extent - 1) * x.stride;
+    }
   }
   return 0;
 }
@@ -309,6 +346,7 @@ int kh_qk_norm_rope(const kh_qk_norm_rope_args *args, void *stream) {
     for (const void *p : {a.q, a.k, cached ? a.v : nullptr, static_cast<const void *>(a.q_out),
                           static_cast<const void *>(a.k_out), a.q_gamma, a.k_gamma})
       if (!aligned(p)) return bad(op, "buffers must be 16-byte aligned");
+    if (cached && c.k == c.v) return bad(op, "k and v of the cache must not be the same");
     const int e = element_bytes(c.dtype);
     const int64_t q_row = a.q_heads * c.head_dim, k_row = c.kv_heads * c.head_dim;
     if (!stride_ok(a.q_stride, a.tokens, e, 0) || !stride_ok(a.k_stride, a.tokens, e, 0) ||
@@ -407,6 +445,8 @@ int kh_paged_weights(const kh_paged_weights_args *args, void *stream) {
         a.weights_head_stride > kMaxStride || (a.cache.kv_heads > 1 && a.weights_head_stride == 0) ||
         (a.table.seqs > 1 && a.weights_seq_stride == 0))
       return bad(op, "strides of weights must be positive");
+    if (!rows_apart({a.weights_seq_stride, a.table.seqs}, {a.weights_head_stride, a.cache.kv_heads}, 1))
+      return bad(op, "rows of weights must not be the same");
     const int e = element_bytes(a.cache.dtype);
     if (a.q_stride * e >= 1 << 24) return bad(op, "q_stride must be below 2^24 bytes");
     const int64_t group = a.q_heads / a.cache.kv_heads, pairs = a.cache.kv_heads * a.table.seqs;
@@ -444,6 +484,8 @@ static int check_evict(const char *op, const kh_paged_evict_args &a) {
     if (s[0] < 0 || s[0] > kMaxStride) return bad(op, "strides of weights must not be negative");
   if ((a.table.seqs > 1 && a.seq_stride < a.budget) || (a.cache.kv_heads > 1 && a.head_stride < a.budget))
     return bad(op, "rows of weights must hold budget entries");
+  if (!rows_apart({a.seq_stride, a.table.seqs}, {a.head_stride, a.cache.kv_heads}, a.budget))
+    return bad(op, "rows of weights must not overlap");
   return 0;
 }
 

@@ -7,7 +7,7 @@ import subprocess
 import pytest
 
 import kernelh as kh
-from test_cache_cpu import attention, cache, refused, table
+from test_cache_cpu import attention, cache, evict, refused, rope, table, weights
 
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -50,3 +50,35 @@ def test_a_workspace_suffices_for_every_smaller_step(dtype, hq, hk, d):
 
 def test_attention_refuses_a_negative_max_new():
     refused(lambda: kh.paged_attention(attention(max_new=-1)), "paged_attention")
+
+
+# ---------------------------------------------------------------- rows that are written lie apart
+
+def test_rows_of_weights_lie_apart():
+    """Three sequences of two heads. The page table and the pointers are not
+    touched: what is accepted here would go on to the device."""
+    for kw in (dict(seq_stride=48, head_stride=48), dict(seq_stride=60, head_stride=40), dict(seq_stride=100, head_stride=200),
+               dict(seq_stride=50, head_stride=139)):
+        refused(lambda: kh.paged_evict_workspace(evict(**kw)), "paged_evict_workspace")
+    for kw in (dict(seq_stride=80, head_stride=40), dict(seq_stride=40, head_stride=120), dict(seq_stride=100, head_stride=50),
+               dict(seq_stride=100, head_stride=140), dict(seq_stride=50, head_stride=140)):
+        assert kh.paged_evict_workspace(evict(**kw)) > 0, kw
+    for kw in (dict(weights_seq_stride=64, weights_head_stride=64), dict(weights_seq_stride=64, weights_head_stride=128)):
+        refused(lambda: kh.paged_weights(weights(**kw)), "paged_weights")
+
+
+def test_rows_of_a_cache_that_is_written_lie_apart():
+    """Ten pages of sixteen slots of two heads of 64."""
+    page, slot, head = 16 * 2 * 64, 2 * 64, 64
+    for x in "kv":
+        def strides(p, t, h):
+            return cache(**{f"{x}_page_stride": p, f"{x}_slot_stride": t, f"{x}_head_stride": h})
+
+        for bad in ((page, head, head), (page, slot, slot), (page - 64, slot, head), (page, slot - 64, head), (head, slot, head),
+                    (page, 64, 15 * 64)):
+            refused(lambda: kh.paged_evict_workspace(evict(cache=strides(*bad))), "paged_evict_workspace")
+            refused(lambda: kh.qk_norm_rope(rope(cache=strides(*bad))), "qk_norm_rope")
+        for good in ((page, slot, head), (page, 64, 16 * 64), (2 * page, 2 * slot, head), (slot, 10 * slot, head), (64, 10 * 64, 160 * 64)):
+            assert kh.paged_evict_workspace(evict(cache=strides(*good))) > 0, good
+    refused(lambda: kh.qk_norm_rope(rope(cache=cache(v=1 << 20))), "qk_norm_rope")
+    assert kh.paged_evict_workspace(evict(cache=cache(v=1 << 20))) > 0  # one row that is both: copied twice, the same
