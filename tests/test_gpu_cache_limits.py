@@ -7,7 +7,8 @@ import numpy as np
 import pytest
 
 import kernelh as kh
-from cachetest import DTYPES, Step, decode, half_step, ints_on_gpu, rope_reference, rounded, same_bits, values_from_gpu, values_on_gpu
+from cachetest import (DTYPES, Step, decode, encode, evict_reference, half_step, ints_on_gpu, rope_reference, rounded, same_bits,
+                       values_from_gpu, values_on_gpu)
 from khtest import say
 from test_gpu_cache import check_attention, check_weights, close
 
@@ -324,3 +325,91 @@ def test_a_chunk_among_single_tokens(dev, dtype, chunk):
             for workspace in (None, 0):
                 say(f"max_new={s.max_new} workspace={workspace}")
                 check_attention(s, workspace=workspace)
+
+
+# ---------------------------------------------------------------- caches past 4 GB
+
+class Far:
+    """A cache whose pages lie 2^28 elements of 16 bits apart, past 2^31 elements
+    and 2^32 bytes: of each page only the slots are ever written or read."""
+
+    def __init__(self, page_size, d=64, pages=20, seed=1):
+        self.ps, self.d, self.pages, self.stride = page_size, d, pages, 1 << 28
+        self.buf = kh.Buffer(pages * self.stride * 2)
+        self.v_at = page_size * d * 2  # V behind K in each page
+        self.g = np.random.default_rng(seed)
+        self.k, self.v = (rounded(self.g.standard_normal((pages, page_size, 1, d), np.float32), "bf16") for _ in "kv")
+        for p in range(pages):
+            for at, x in ((0, self.k), (self.v_at, self.v)):
+                a = encode(x[p], "bf16")
+                kh.check(kh.lib.khrt_memcpy_h2d(self.buf.ptr + p * self.stride * 2 + at, a.ctypes.data, a.nbytes))
+        self.cache = kh.PagedCache(k=self.buf.ptr, v=self.buf.ptr + self.v_at, k_page_stride=self.stride, k_slot_stride=d,
+                                   k_head_stride=0, v_page_stride=self.stride, v_slot_stride=d, v_head_stride=0, pages=pages,
+                                   page_size=page_size, kv_heads=1, head_dim=d, dtype=kh.BF16)
+
+    def read(self):
+        kh.synchronize()
+        out = []
+        for at in (0, self.v_at):
+            x = np.empty((self.pages, self.ps, 1, self.d), np.int16)
+            for p in range(self.pages):
+                page = np.empty((self.ps, 1, self.d), np.int16)
+                kh.check(kh.lib.khrt_memcpy_d2h(page.ctypes.data, self.buf.ptr + p * self.stride * 2 + at, page.nbytes))
+                x[p] = page
+            out.append(decode(x, "bf16"))
+        return out
+
+    def step(self, m, n):
+        s = Step("bf16", [m], [n], 4, 1, self.d, page_size=self.ps, seed=m)
+        s.pages, s.k, s.v = self.pages, self.k, self.v
+        s.table = self.g.permutation(self.pages)[:-(-n // self.ps)].astype(np.int32).reshape(1, -1)
+        s.cache_on_gpu = lambda: (self.cache, self.buf)
+        return s
+
+
+@pytest.mark.parametrize("page_size", [16, 24])
+def test_attention_and_weights_past_4_gb(dev, page_size):
+    far = Far(page_size)
+    for m in (1, 5, 100):
+        s = far.step(m, 20 * page_size - 3)
+        say(f"far pages of {page_size}, {m} tokens")
+        check_attention(s)
+        check_weights(s)
+
+
+@pytest.mark.parametrize("page_size", [16, 24])
+def test_rotation_and_eviction_past_4_gb(dev, page_size):
+    """New keys and values into every page, then eviction from the last pages
+    to the first and the other way."""
+    far = Far(page_size)
+    d, t, pages = far.d, 20 * page_size, far.pages
+    x = rounded(far.g.standard_normal((t, 6, d), np.float32), "bf16")
+    slots = far.g.permutation(t).astype(np.int64)
+    dx, ds, dq = values_on_gpu(x, "bf16"), ints_on_gpu(slots, np.int64), values_on_gpu(np.zeros((t, 4, d)), "bf16")
+    say(f"far pages of {page_size}, rope")
+    kh.qk_norm_rope(kh.QkNormRope(q=dx.ptr, k=dx.ptr + 4 * d * 2, v=dx.ptr + 5 * d * 2, q_out=dq.ptr, k_out=None, slots=ds.ptr,
+                                  q_stride=6 * d, k_stride=6 * d, v_stride=6 * d, q_out_stride=4 * d, k_out_stride=d, cache=far.cache,
+                                  tokens=t, q_heads=4, rotary_dim=0, interleaved=0, norm=0, eps=0.0))
+    for got, want, i in zip(far.read(), (far.k, far.v), (4, 5)):
+        want.reshape(t, d)[slots] = x[:, i]
+        assert same_bits(got, want)
+    for source, kept in ((np.arange(pages - 10, pages), np.arange(5)), (np.arange(8), np.arange(pages - 5, pages))):
+        n, budget, recent = len(source) * page_size, 5 * page_size - 1, 7
+        w = far.g.random((1, 1, n), np.float32)
+        table, lens, dw, kt = ints_on_gpu(source), ints_on_gpu([n]), values_on_gpu(w, "f32"), ints_on_gpu(kept)
+        out, klens = values_on_gpu(np.full((1, 1, budget), 7.0), "f32"), ints_on_gpu([-7])
+        a = kh.PagedEvict(cache=far.cache, table=kh.PageTable(pages=table.ptr, lens=lens.ptr, row_stride=len(source), seqs=1,
+                                                              width=len(source), max_len=0),
+                          kept_pages=kt.ptr, kept_row_stride=5, kept_width=5, kept_lens=klens.ptr, weights_in=dw.ptr, in_seq_stride=n,
+                          in_head_stride=n, weights=out.ptr, seq_stride=budget, head_stride=budget, budget=budget, recent=recent)
+        size = kh.paged_evict_workspace(a)
+        ws = kh.Buffer(size)
+        say(f"far pages of {page_size}, eviction")
+        kh.paged_evict(a, ws, size)
+        ids = np.array(evict_reference(w[0, 0], n, budget, recent))
+        to = np.arange(len(ids))
+        for y in (far.k, far.v):
+            y[kept[to // page_size], to % page_size] = y[source[ids // page_size], ids % page_size]
+        for got, want in zip(far.read(), (far.k, far.v)):
+            assert same_bits(got, want)
+        assert same_bits(values_from_gpu(out, (budget,), "f32"), w[0, 0, ids]) and klens.to_host(np.int32)[0] == budget
