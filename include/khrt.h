@@ -385,8 +385,10 @@ KHRT_API int khrt_bench_row_work(const char *kernel, const char *shape, double *
  * code object); what a captured graph uses (workspaces included) is its own
  * until it has been replayed.
  *
- * Element types: fp32, fp16 and bf16; products, sums, norms and softmax
- * statistics are in 32 bits. head_dim is a multiple of 8 up to 256. Rows of
+ * Element types: fp32, fp16 and bf16. Products, sums, norms and softmax
+ * statistics are in 32 bits; the attention's weights are rounded to the element
+ * type (fp16: 2^15 times their value) where V is multiplied by them, and outputs
+ * are rounded to it once. head_dim is a multiple of 8 up to 256. Rows of
  * head_dim elements are contiguous; pointers to them are 16-byte aligned and
  * strides (in elements) multiples of 16 bytes. Anything else the host can see
  * is refused with KHRT_E_INVALID before any device work.
@@ -462,7 +464,7 @@ KHRT_API int kh_qk_norm_rope(const kh_qk_norm_rope_args *args, void *stream);
  * `window` of them. Head h reads kv head h / (q_heads / kv_heads). lse[t, h]
  * (fp32, may be null) is the natural log of the sum of exponentials. A token
  * that sees nothing (an empty cache, a sequence with fewer entries than new
- * tokens, absent pages) gives zeros and -inf; tokens outside every sequence are
+ * tokens, absent pages), or only scores of -inf, gives zeros and -inf; tokens outside every sequence are
  * left as they were. Infinities and NaN in entries that a token does not see
  * do not reach it. out must not be q.
  *

@@ -32,7 +32,7 @@
 //
 // Bound by reading K and V: each wave holds a block of both and has the next
 // ones in flight (nontemporal: nobody else reads them), 64 KB to a CU. One
-// sequence of 131071 entries takes 104 us, 5.2 TB/s.
+// sequence of 131071 entries takes 103 us, 5.2 TB/s.
 //
 // Rows of V that no row of the tile sees (past the sequence's end, in pages
 // that do not exist) count as zeros. Where some rows of the tile see an entry
@@ -493,10 +493,11 @@ __device__ __forceinline__ void narrow(const KhAttentionParams &p, int block, fl
 // exclusive-or a number of the row's, so that neither kind of read meets a bank
 // twice (measured: no conflicts).
 //
-// Bound by the matrix units and what stands between their two products, which
-// a wave does one after the other: 2048 new tokens of 8192 entries (bf16, 32
-// heads on 8 of 128) take 269 us, 901 TFLOP/s; a large library product reaches
-// 1228.
+// A wave does a tile's two products and the softmax between them one after the
+// other, with two waves to a SIMD to fill each other's gaps: the matrix units are
+// busy for 96 us of the 277 to 281 (271 to 308 from one card to another) that 2048
+// new tokens of 8192 entries take (bf16, 32 heads on 8 of 128), 865 TFLOP/s. A large
+// library product reaches 1228.
 template <int D>
 struct Wide {
   static constexpr int bytes = D * (int)sizeof(elem);

@@ -15,10 +15,13 @@
 //
 // Sequences of few rows: bound by reading K. A wave has all the rows' queries in
 // registers and goes through blocks of 32 entries, the next block in flight: 32
-// sequences of 1025 to 8192 entries (bf16, 32 heads on 8 of 128) 68 us, 4.7 TB/s.
+// sequences of 1025 to 8192 entries (bf16, 32 heads on 8 of 128) 67 to 72 us, 4.4 to
+// 4.7 TB/s.
 // Sequences of many: a wave has 32 entries in registers and the workgroup brings
-// tiles of 64 rows through LDS, one ahead. Bound by the exponentials (16 cycles
-// to 64 of them, against 32 cycles of products for 32 x 32 scores).
+// tiles of 64 rows through LDS, one ahead. 32 x 32 scores of heads of 128 are eight
+// product instructions of 32 cycles and 16 exponentials of 16 cycles for 64
+// values: 256 cycles each, which a wave spends one after the other, with the masks
+// and sums behind them.
 #include "kh_cache.h"
 
 namespace {
@@ -464,8 +467,8 @@ KH_WEIGHTS(64)
 KH_WEIGHTS(128)
 KH_WEIGHTS(256)
 // Steps with chunks: without it, three. Two sequences of up to 1024 new tokens
-// and 6000 entries (bf16, 32 heads on 8 of 128): 109 us, 706 TFLOP/s. With the
-// ring's LDS, two workgroups to a CU, such a step took 171 us.
+// and 6000 entries (bf16, 32 heads on 8 of 128): 116 to 120 us, 645 to 665 TFLOP/s.
+// With the ring's LDS, two workgroups to a CU, such a step took half as long again.
 // In 32 bits heads of 128 take 66 KB: two.
 #define KH_WEIGHTS_WIDE(D)                                                                                 \
   extern "C" __global__ void __launch_bounds__(256, D > 128 ? 1 : kWide && D > 64 ? 2 : 3) KH_TYPED(paged_weights_wide_##D)(const KhWeightsParams p) { \

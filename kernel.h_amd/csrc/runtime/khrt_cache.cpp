@@ -450,8 +450,8 @@ int kh_paged_weights(const kh_paged_weights_args *args, void *stream) {
     const int e = element_bytes(a.cache.dtype);
     if (a.q_stride * e >= 1 << 24) return bad(op, "q_stride must be below 2^24 bytes");
     const int64_t group = a.q_heads / a.cache.kv_heads, pairs = a.cache.kv_heads * a.table.seqs;
-    // Chunks as long as leaves every CU some eight workgroups, up to 512 entries
-    // (four blocks of a wave); one stretch where sequences may have many rows.
+    // Chunks as long as leaves every CU some four workgroups, up to 1024 entries
+    // (eight blocks of a wave); one stretch where sequences may have many rows.
     const int64_t len = expected_len(a.table, a.cache), stretches = ceil_div(len, KH_STRETCH);
     const bool few = a.tokens * group <= 32 * a.table.seqs;
     const int64_t each = few ? std::clamp<int64_t>(pairs * stretches / (4 * KH_GEMM_CUS), 1, 8) : 1;
