@@ -2,6 +2,7 @@
 by build.py beside the code objects): rules that the compiler cannot keep for
 inline assembly."""
 import glob
+import json
 import os
 import re
 
@@ -75,3 +76,16 @@ def test_loads_to_lds_bring_their_own_wait_states_and_keep_m0(path):
         assert save[0] == set_m0[0] == restore[0] == "s_mov_b32" and nop[0] == "s_nop", code[i - 3:i + 2]
         assert save[1][1] == "m0" and set_m0[1][0] == "m0" and restore[1] == ["m0", save[1][0]], code[i - 3:i + 2]
         assert int(nop[1][0]) + 3 >= 5, code[i - 3:i + 2]
+
+
+# Symbols that spill, and how much at the most: registers and bytes of scratch of a lane.
+SPILLS = {"paged_attention_wide_256_f32": (34, 140), "paged_attention_wide_256_f16": (8, 36), "paged_attention_wide_256_bf16": (8, 36)}
+
+
+@pytest.mark.parametrize("path", [f[:-len("isa")] + "notes.json" for f in FILES if os.path.basename(f).startswith(("paged_", "qk_"))],
+                         ids=os.path.basename)
+def test_what_the_sequence_cache_kernels_spill(path):
+    with open(path) as f:
+        for k in json.load(f):
+            registers, scratch = SPILLS.get(k["name"], (0, 0))
+            assert k["vgpr_spill_count"] <= registers and k["private_segment_bytes"] <= scratch, k["name"]
