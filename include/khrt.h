@@ -27,6 +27,7 @@
  *      argument lists of lib/dsl/kernels/<name>.cpp).
  *   8. Sequence caches: the operators of a decoder's serving step over a
  *      paged cache of keys and values. No counterpart in the reference.
+ *   9. Sequence caches in 8 bits. No counterpart in the reference.
  */
 #ifndef KHRT_H
 #define KHRT_H
@@ -543,6 +544,106 @@ typedef struct kh_paged_evict_args {
 } kh_paged_evict_args;
 KHRT_API int kh_paged_evict_workspace(const kh_paged_evict_args *args, size_t *bytes);
 KHRT_API int kh_paged_evict(const kh_paged_evict_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- 9. Sequence caches in 8 bits ---------------------------------------- */
+/* The same step over a cache of half the size: the new tokens' keys and values
+ * are rounded as they are written (kh_qk_norm_rope8), rows can be read back
+ * (kh_paged_read8), and attention is over what the cache holds
+ * (kh_paged_attention8). All that group 8 says of streams, graphs, types,
+ * alignment, device memory and overlaps holds here; head_dim is a multiple of 16
+ * up to 256, and q, k, v and outputs have the type that `dtype` names.
+ *
+ * A row (one entry's key or value of one head) is head_dim e4m3 numbers (8-bit
+ * floats of 4 exponent and 3 mantissa bits, largest 448, a NaN and no infinity)
+ * and a byte b: element i stands for its number times 2^(b - 127), exactly. As
+ * written, b - 127 is the least integer from -117 to 119 with which 448 times the
+ * power is no less than the row's largest magnitude, each number is rounded to
+ * nearest even, and infinities and NaN are NaN (they do not count for b). So a
+ * row that is read back and written again keeps its values. A byte below 10
+ * counts as 10, one past 246 as 246.
+ *
+ * Strides of k and v are bytes, an element each, and multiples of 16. The byte of
+ * slot t of page p and head h is k_scale[p scale_page_stride + h scale_head_stride +
+ * t], and v_scale alike: [pages, kv_heads, page_size], say. Scales that are 4-byte
+ * aligned, with strides that are, are read faster. */
+typedef struct kh_paged_cache8 {
+  void *k, *v;
+  uint8_t *k_scale, *v_scale;
+  int64_t k_page_stride, k_slot_stride, k_head_stride;
+  int64_t v_page_stride, v_slot_stride, v_head_stride;
+  int64_t scale_page_stride, scale_head_stride;
+  int64_t pages, page_size, kv_heads, head_dim;
+} kh_paged_cache8;
+
+/* kh_qk_norm_rope over a cache in 8 bits, and with positions of several axes
+ * (time, height and width of images and video): pair i of token t is rotated by
+ * positions[pair_axis[i] axis_stride + t] inv_freq[i]. pair_axis null: axis 0 for
+ * all; a number outside [0, axes) counts as the nearest in it. k is rounded once,
+ * from 32 bits; k_out (may be null) is k in the rows' type. A token whose slot is
+ * not in the cache writes nothing there. */
+typedef struct kh_qk_norm_rope8_args {
+  const void *q, *k, *v;
+  void *q_out, *k_out;
+  const void *q_gamma, *k_gamma; /* [head_dim], of the rows' type */
+  const float *inv_freq;         /* [rotary_dim / 2] */
+  const int64_t *positions;      /* [axes, tokens] */
+  const int32_t *pair_axis;      /* [rotary_dim / 2] */
+  const int64_t *slots;          /* [tokens] */
+  int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride, axis_stride;
+  kh_paged_cache8 cache;
+  int64_t tokens, q_heads, rotary_dim, axes;
+  int32_t interleaved, norm, dtype;
+  float eps;
+} kh_qk_norm_rope8_args;
+KHRT_API int kh_qk_norm_rope8(const kh_qk_norm_rope8_args *args, void *stream);
+
+/* k_out[t, h] and v_out[t, h] (rows of head_dim elements, a token's heads next to
+ * each other, tokens k_out_stride and v_out_stride elements apart) become what the
+ * rows in slot slots[t] = page * page_size + slot stand for, exactly in fp32 and
+ * bf16, rounded in fp16. A token whose slot is not in the cache (-1 for padding) is
+ * left as it was. One of k_out and v_out may be null. */
+typedef struct kh_paged_read8_args {
+  kh_paged_cache8 cache;
+  const int64_t *slots; /* [tokens] */
+  void *k_out, *v_out;
+  int64_t k_out_stride, v_out_stride;
+  int64_t tokens;
+  int32_t dtype;
+} kh_paged_read8_args;
+KHRT_API int kh_paged_read8(const kh_paged_read8_args *args, void *stream);
+
+/* kh_paged_attention over a cache in 8 bits, with two additions.
+ *
+ * cap > 0: the scores are cap tanh(scale q . k / cap).
+ *
+ * shared > 0: the first `shared` entries of the sequences, as far as each is that
+ * long, are the same entries (every sequence's row of the table names pages that
+ * hold them, the same pages or copies). They may then be read once for all, from
+ * sequence 0's pages and as far as it reaches; as max_len and max_new this changes
+ * no result but its rounding.
+ *
+ * Products are of bf16 numbers, exactly what the cache holds; queries count in
+ * full, the softmax's weights to 8 bits (bf16), 16 (fp16) or 24 (fp32). A NaN
+ * in an entry that a token does not see does not reach it.
+ *
+ * workspace: as kh_paged_attention's; it also holds what shared entries give each
+ * row. A smaller step is one of fewer shared entries too. */
+typedef struct kh_paged_attention8_args {
+  kh_paged_cache8 cache;
+  kh_page_table table;
+  const void *q;
+  void *out;
+  float *lse;
+  const int32_t *q_starts; /* [seqs + 1] */
+  int64_t q_stride, out_stride;
+  int64_t tokens, q_heads, window;
+  int64_t max_new, shared;
+  float scale, cap;
+  int32_t dtype;
+} kh_paged_attention8_args;
+KHRT_API int kh_paged_attention8_workspace(const kh_paged_attention8_args *args, size_t *bytes);
+KHRT_API int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, size_t workspace_bytes,
+                                 void *stream);
 
 #ifdef __cplusplus
 }

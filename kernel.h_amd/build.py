@@ -56,6 +56,11 @@ VARIANTS = {f"gemm_tune{p}": ("gemm_tune", [f"-DKH_GEMM_TUNE_PART={p}"]) for p i
 ELEMENTS = {"f32": 0, "f16": 1, "bf16": 2}
 TYPED = ["qk_norm_rope", "paged_attention", "paged_weights"]
 VARIANTS |= {f"{b}_{t}": (b, [f"-DKH_ELEM={e}"]) for b in TYPED for t, e in ELEMENTS.items()}
+# Over a cache in 8 bits: rows of each type; attention8 multiplies bf16 numbers
+# whatever the rows are.
+VARIANTS |= {f"rope8_{t}": ("qk_norm_rope", [f"-DKH_ELEM={e}", "-DKH_CACHE8"]) for t, e in ELEMENTS.items()}
+VARIANTS |= {f"read8_{t}": ("read8", [f"-DKH_ELEM={e}"]) for t, e in ELEMENTS.items()}
+VARIANTS |= {f"attention8_{t}": ("attention8", ["-DKH_ELEM=2", f"-DKH_ROWS={e}"]) for t, e in ELEMENTS.items()}
 # Product code objects embedded in libkhrt.so (order = kh_embed.S order).
 PRODUCT = ["vecadd", "fused_gelu", "softmax", "layernorm", "scan", "gemm", "attention", "util", "roofline",
            "paged_evict", *VARIANTS]

@@ -275,6 +275,14 @@ struct KhRopeParams {
   float eps;
 };
 
+// qk_norm_rope.hip with a cache in 8 bits: its strides above are bytes.
+struct KhRope8Params : KhRopeParams {
+  uint8_t *k_scale, *v_scale;
+  const int32_t *pair_axis;  // may be null: axis 0
+  int64_t axis_stride, scale_page, scale_head;
+  int32_t axes;
+};
+
 // paged_attention.hip
 struct KhAttentionParams {
   KhCache cache;
@@ -297,6 +305,72 @@ struct KhAttentionParams {
   uint32_t q_keep, q_sign;  // q's bits that count (none with a scale of 0); the sign bits where the scale is negative
   KhDiv by_group;
   float scale_log2;  // |scale| log2(e), above 0: maxima may be taken before it
+};
+
+KH_HD KhUnits kh_units_of(const KhAttentionParams &p, const KhSeq &s) { return kh_units(s, p.group, p.window, p.whole); }
+KH_HD KhSpan kh_span_of(const KhAttentionParams &p, const KhSeq &s, int32_t i) { return kh_seen(s, i, p.window); }
+
+// Rows of a cache in 8 bits: e4m3 numbers times 2^(byte - 127) of the row's own
+// byte. Written bytes lie between these two: nothing a number stands for is then
+// past fp32's normal range. What lies outside counts as the nearer of them.
+#define KH_SCALE_LEAST 10
+#define KH_SCALE_MOST 246
+
+// attention8.hip. The cache's strides are bytes as above, one to an element.
+struct KhAttention8Params : KhAttentionParams {
+  const uint8_t *k_scale, *v_scale;  // of slot t of page p and head h: p scale_page + h scale_head + t
+  uint32_t scale_page, scale_head;
+  int32_t shared;  // entries that all sequences share, worked on once for all rows; 0: none
+  // Its parts: workgroups, how many parts of each 128 rows, entries of a part.
+  int32_t shared_blocks, shared_splits, shared_each;
+  // [shared_splits + 1][tokens q_heads][head_dim], and [..][2]: the last is the sequences' own entries'.
+  float *shared_o, *shared_ml;
+  float cap_in, cap_out;  // scores y become cap_out tanh(y cap_in / (2 log2 e)); cap_in 0: they do not
+};
+
+// Entries that sequences share lie before those that are each one's own.
+KH_HD KhSpan kh_span_of(const KhAttention8Params &p, const KhSeq &s, int32_t i) {
+  KhSpan r = kh_seen(s, i, p.window);
+  if (r.first < p.shared) r.first = p.shared;
+  return r;
+}
+
+KH_HD KhUnits kh_units_of(const KhAttention8Params &p, const KhSeq &s) {
+  KhUnits u = kh_units(s, p.group, p.window, p.whole);
+  if (u.first < (p.shared & ~15)) {
+    u.first = p.shared & ~15;
+    const int32_t keys = s.n > u.first ? s.n - u.first : 0;
+    u.blocks = p.whole != 0 || keys == 0 ? 1 : (keys - 1) / KH_STRETCH + 1;
+  }
+  return u;
+}
+
+// The sequence that has `token`: the last one that starts at or before it, if
+// starts ascend. Ends for any starts.
+template <class Starts>
+KH_HD int32_t kh_sequence_of(const Starts &starts, int32_t seqs, int32_t token) {
+  int32_t lo = 0, hi = seqs - 1;
+  while (lo < hi) {
+    const int32_t mid = lo + (hi - lo + 1) / 2;
+    if (starts[mid] <= token)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// read8.hip
+struct KhRead8Params {
+  const uint8_t *k, *v, *k_scale, *v_scale;
+  const int64_t *slots;
+  void *k_out, *v_out;
+  int64_t k_out_stride, v_out_stride;
+  int64_t rows;  // slots of the cache
+  uint32_t k_page, k_slot, k_head, v_page, v_slot, v_head, scale_page, scale_head;
+  int32_t page_size, kv_heads, head_dim;
+  int32_t tokens, each;  // of a workgroup
+  KhDiv by_token, by_row;  // 16-byte pieces of the rows of a token, and of one row
 };
 
 // paged_weights.hip

@@ -21,6 +21,13 @@
 // up to 0.06 rad. Its part past whole quarter turns, below pi/4, goes through
 // the Taylor series of sine and cosine in 32 bits (first terms left out
 // 2e-9 and 2e-10).
+//
+// Built with KH_CACHE8 the cache is one in 8 bits (rope8_*): pair i is rotated by
+// the position of its own axis, and a row of k or v becomes e4m3 numbers times the
+// least power of two 2^e, e >= -117, with which the row's largest is at most 448:
+// the type's relative step is the same under any scale, so that a power of two loses
+// nothing by it, and what is read back is exact. k is rounded once, from 32 bits.
+// Infinities and NaN become NaN; a row's power is that of its finite elements.
 #include "kh_elem.h"
 #include "kh_paged.h"
 
@@ -87,8 +94,61 @@ __device__ __forceinline__ void store_past(kh::elem *p, const float (&x)[4]) {
 #endif
 }
 
+#ifdef KH_CACHE8
+using Params = KhRope8Params;
+
+// The largest over the L lanes of a row.
 template <int L>
-__device__ __forceinline__ void rope(const KhRopeParams &p) {
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, moved<0xb1>(v));  // as row_sum
+  v = fmaxf(v, moved<0x4e>(v));
+  v = fmaxf(v, moved<0x141>(v));
+  if constexpr (L >= 16) v = fmaxf(v, moved<0x140>(v));
+  if constexpr (L >= 32) v = fmaxf(v, __shfl_xor(v, 16, kh::kWave));
+  return v;
+}
+
+__device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u; }
+
+// The byte of the least power of two 2^e with 448 2^e = 1.75 2^(e + 8) >= top.
+__device__ __forceinline__ uint32_t scale_of(float top) {
+  const uint32_t w = __float_as_uint(top);
+  const int byte = (int)(w >> 23) - 8 + ((w & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return (uint32_t)(byte < KH_SCALE_LEAST ? KH_SCALE_LEAST : byte < KH_SCALE_MOST ? byte : KH_SCALE_MOST);
+}
+
+// Four numbers times a power of two as e4m3, rounded to nearest even; past 448,
+// as only the largest scale leaves some, they are 448.
+__device__ __forceinline__ uint32_t narrowed(const float (&x)[4], float power) {
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = is_finite(x[i]) ? fminf(fmaxf(x[i] * power, -448.0f), 448.0f) : __builtin_nanf("");
+  const uint32_t low = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], (int)low, true);
+}
+
+// A lane's eight elements of a row to the cache, the row's scale by its first lane.
+template <int L>
+__device__ __forceinline__ void store8(const float (&x)[2][4], bool live, bool on, uint8_t *row, int a0, int a1, uint8_t *scale, int u) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = x[i / 4][i % 4];
+    top = fmaxf(top, is_finite(y) ? fabsf(y) : 0.0f);
+  }
+  const uint32_t byte = scale_of(row_max<L>(live ? top : 0.0f));
+  if (!on) return;
+  const float power = __uint_as_float((254 - byte) << 23);  // 2^(127 - byte), byte in [10, 246]
+  __builtin_nontemporal_store(narrowed(x[0], power), reinterpret_cast<uint32_t *>(row + a0));
+  __builtin_nontemporal_store(narrowed(x[1], power), reinterpret_cast<uint32_t *>(row + a1));
+  if (u == 0) *scale = (uint8_t)byte;
+}
+#else
+using Params = KhRopeParams;
+#endif
+
+template <int L>
+__device__ __forceinline__ void rope(const Params &p) {
   using kh::elem;
   const int lane = kh::lane_id();
   // A job is one part of one token's heads; a wave takes one.
@@ -138,9 +198,17 @@ __device__ __forceinline__ void rope(const KhRopeParams &p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) c[i] = 1.0f, s[i] = 0.0f;
   if (turned) {
+#ifdef KH_CACHE8
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int axis = p.pair_axis != nullptr ? kh_clamp(p.pair_axis[4 * u + i], 0, p.axes - 1) : 0;
+      turn(static_cast<double>(p.positions[axis * p.axis_stride + t]) * static_cast<double>(p.inv_freq[4 * u + i]), c[i], s[i]);
+    }
+#else
     const double pos = static_cast<double>(p.positions[t]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) turn(pos * static_cast<double>(p.inv_freq[4 * u + i]), c[i], s[i]);
+#endif
   }
   for (int step = part; step < steps; step += parts) {
     const bool is_q = step < of_q, is_v = step >= of_q + of_k;
@@ -151,11 +219,20 @@ __device__ __forceinline__ void rope(const KhRopeParams &p) {
     const int n = is_q ? q_heads : kv_heads, h = (step - (is_q ? 0 : is_v ? of_q + of_k : of_q)) * kRows + lane / L;
     const bool on = live && h < n;
     if (is_v) {
+#ifdef KH_CACHE8
+      float y[2][4];
+      unpack(y[0], raw[0]);
+      unpack(y[1], raw[1]);
+      const int64_t at = page * p.v_page + in_page * p.v_slot + h * p.v_head;
+      store8<L>(y, live, on, static_cast<uint8_t *>(p.v_cache) + at, a0, a1,
+                p.v_scale + (page * p.scale_page + h * p.scale_head + in_page), u);
+#else
       if (on) {
         elem *dst = static_cast<elem *>(p.v_cache) + page * p.v_page + in_page * p.v_slot + h * p.v_head;
         __builtin_nontemporal_store(raw[0], reinterpret_cast<Four *>(dst + a0));
         __builtin_nontemporal_store(raw[1], reinterpret_cast<Four *>(dst + a1));
       }
+#endif
       continue;
     }
     float x[2][4];
@@ -197,16 +274,29 @@ __device__ __forceinline__ void rope(const KhRopeParams &p) {
       store_past(dst + a0, x[0]);
       store_past(dst + a1, x[1]);
     }
+#ifdef KH_CACHE8
+    if (!is_q && cached) {
+      const int64_t at = page * p.k_page + in_page * p.k_slot + h * p.k_head;
+      store8<L>(x, live, on, static_cast<uint8_t *>(p.k_cache) + at, a0, a1,
+                p.k_scale + (page * p.scale_page + h * p.scale_head + in_page), u);
+    }
+#else
     if (on && !is_q && cached) {
       elem *dst = static_cast<elem *>(p.k_cache) + page * p.k_page + in_page * p.k_slot + h * p.k_head;
       store_past(dst + a0, x[0]);
       store_past(dst + a1, x[1]);
     }
+#endif
   }
 }
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(256) KH_TYPED(qk_norm_rope_8)(const KhRopeParams p) { rope<8>(p); }
-extern "C" __global__ void __launch_bounds__(256) KH_TYPED(qk_norm_rope_16)(const KhRopeParams p) { rope<16>(p); }
-extern "C" __global__ void __launch_bounds__(256) KH_TYPED(qk_norm_rope_32)(const KhRopeParams p) { rope<32>(p); }
+#ifdef KH_CACHE8
+#define KH_ROPE(name) KH_TYPED(rope8_##name)
+#else
+#define KH_ROPE(name) KH_TYPED(qk_norm_rope_##name)
+#endif
+extern "C" __global__ void __launch_bounds__(256) KH_ROPE(8)(const Params p) { rope<8>(p); }
+extern "C" __global__ void __launch_bounds__(256) KH_ROPE(16)(const Params p) { rope<16>(p); }
+extern "C" __global__ void __launch_bounds__(256) KH_ROPE(32)(const Params p) { rope<32>(p); }

@@ -48,6 +48,9 @@ KH_DECLARE_CO(gemm_tune3)
 KH_DECLARE_TYPED(qk_norm_rope)
 KH_DECLARE_TYPED(paged_attention)
 KH_DECLARE_TYPED(paged_weights)
+KH_DECLARE_TYPED(rope8)
+KH_DECLARE_TYPED(read8)
+KH_DECLARE_TYPED(attention8)
 KH_DECLARE_CO(paged_evict)
 static_assert(KH_GEMM_TUNE_PARTS == 4, "one code object per part of the tune list");
 
@@ -72,6 +75,7 @@ const CodeObject kCodeObjects[] = {
 #define KH_CO(name) {#name, kh_co_##name, kh_co_##name##_end}
 #define KH_TYPED_CO(name) KH_CO(name##_f32), KH_CO(name##_f16), KH_CO(name##_bf16)
     KH_TYPED_CO(qk_norm_rope), KH_TYPED_CO(paged_attention), KH_TYPED_CO(paged_weights), KH_CO(paged_evict),
+    KH_TYPED_CO(rope8),        KH_TYPED_CO(read8),           KH_TYPED_CO(attention8),
 };
 
 struct KernelResources {

@@ -157,6 +157,45 @@ class PagedEvict(ctypes.Structure):
                 ("budget", ctypes.c_int64), ("recent", ctypes.c_int64)]
 
 
+class PagedCache8(ctypes.Structure):
+    """kh_paged_cache8: keys and values in 8 bits in pages. Pointers are integers; strides are in bytes."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("k_page_stride", ctypes.c_int64), ("k_slot_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+                ("v_page_stride", ctypes.c_int64), ("v_slot_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+                ("scale_page_stride", ctypes.c_int64), ("scale_head_stride", ctypes.c_int64),
+                ("pages", ctypes.c_int64), ("page_size", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("head_dim", ctypes.c_int64)]
+
+
+class QkNormRope8(ctypes.Structure):
+    """Arguments of qk_norm_rope8 (kh_qk_norm_rope8_args)."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+                ("q_gamma", ctypes.c_void_p), ("k_gamma", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+                ("positions", ctypes.c_void_p), ("pair_axis", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
+                ("q_out_stride", ctypes.c_int64), ("k_out_stride", ctypes.c_int64), ("axis_stride", ctypes.c_int64),
+                ("cache", PagedCache8), ("tokens", ctypes.c_int64), ("q_heads", ctypes.c_int64),
+                ("rotary_dim", ctypes.c_int64), ("axes", ctypes.c_int64), ("interleaved", ctypes.c_int32),
+                ("norm", ctypes.c_int32), ("dtype", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+class PagedRead8(ctypes.Structure):
+    """Arguments of paged_read8 (kh_paged_read8_args)."""
+    _fields_ = [("cache", PagedCache8), ("slots", ctypes.c_void_p), ("k_out", ctypes.c_void_p), ("v_out", ctypes.c_void_p),
+                ("k_out_stride", ctypes.c_int64), ("v_out_stride", ctypes.c_int64), ("tokens", ctypes.c_int64),
+                ("dtype", ctypes.c_int32)]
+
+
+class PagedAttention8(ctypes.Structure):
+    """Arguments of paged_attention8 (kh_paged_attention8_args)."""
+    _fields_ = [("cache", PagedCache8), ("table", PageTable), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("lse", ctypes.c_void_p), ("q_starts", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
+                ("out_stride", ctypes.c_int64), ("tokens", ctypes.c_int64), ("q_heads", ctypes.c_int64),
+                ("window", ctypes.c_int64), ("max_new", ctypes.c_int64), ("shared", ctypes.c_int64),
+                ("scale", ctypes.c_float), ("cap", ctypes.c_float), ("dtype", ctypes.c_int32)]
+
+
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
@@ -236,6 +275,10 @@ SIGNATURES = {
     "kh_paged_weights": (_i, [ctypes.POINTER(PagedWeights), _vp]),
     "kh_paged_evict_workspace": (_i, [ctypes.POINTER(PagedEvict), ctypes.POINTER(_sz)]),
     "kh_paged_evict": (_i, [ctypes.POINTER(PagedEvict), _vp, _sz, _vp]),
+    "kh_qk_norm_rope8": (_i, [ctypes.POINTER(QkNormRope8), _vp]),
+    "kh_paged_read8": (_i, [ctypes.POINTER(PagedRead8), _vp]),
+    "kh_paged_attention8_workspace": (_i, [ctypes.POINTER(PagedAttention8), ctypes.POINTER(_sz)]),
+    "kh_paged_attention8": (_i, [ctypes.POINTER(PagedAttention8), _vp, _sz, _vp]),
     "khrt_bench_metric": (_i, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double), _i, ctypes.POINTER(ctypes.c_double)]),
     "khrt_bench_row_work": (_i, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),
                                  ctypes.POINTER(_i)]),
@@ -720,6 +763,27 @@ def paged_evict_workspace(args: PagedEvict) -> int:
 
 def paged_evict(args: PagedEvict, workspace, workspace_bytes: int, stream=None) -> None:
     check(lib.kh_paged_evict(args, _ptr(workspace), workspace_bytes, _ptr(stream)))
+
+
+# The same over a cache in 8 bits (khrt.h, group 9).
+
+def qk_norm_rope8(args: QkNormRope8, stream=None) -> None:
+    check(lib.kh_qk_norm_rope8(args, _ptr(stream)))
+
+
+def paged_read8(args: PagedRead8, stream=None) -> None:
+    check(lib.kh_paged_read8(args, _ptr(stream)))
+
+
+def paged_attention8_workspace(args: PagedAttention8) -> int:
+    """Bytes with which paged_attention8 splits this step and reads its shared entries once, and every smaller one's, as far as it pays."""
+    n = ctypes.c_size_t()
+    check(lib.kh_paged_attention8_workspace(args, ctypes.byref(n)))
+    return n.value
+
+
+def paged_attention8(args: PagedAttention8, workspace=None, workspace_bytes: int = 0, stream=None) -> None:
+    check(lib.kh_paged_attention8(args, _ptr(workspace), workspace_bytes, _ptr(stream)))
 
 
 def roofline_triad(a, b, c, n: int, stream=None) -> None:
