@@ -252,7 +252,13 @@ inline size_t part_row_bytes(const kh_paged_attention_args &a) { return (2 + sta
 // Workgroups of the narrow form that are on the chip at once.
 inline int64_t most_groups(const kh_paged_attention_args &a) { return (a.cache.head_dim > 128 ? 1 : 2) * KH_GEMM_CUS; }
 
-inline AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_bytes) {
+// How sequences of few rows are worked on: workgroups on the chip at once, kv heads
+// that each takes.
+struct NarrowForm {
+  int64_t most, together = 1;
+};
+
+inline AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_bytes, const NarrowForm &form) {
   AttentionPlan p{};
   const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.tokens * group;
   const int64_t len = seen_len(a);
@@ -281,10 +287,9 @@ inline AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t wor
 
   // At most so many units, of at most so many blocks each.
   const int64_t narrow_most = narrow_only ? rows : std::min(rows, few * a.table.seqs);
-  const int64_t units = (narrow_most / KH_TILE_ROWS + std::min(a.tokens, a.table.seqs)) * a.cache.kv_heads;
-  const int64_t blocks = ceil_div(len, KH_STRETCH);
-  const int64_t most = most_groups(a);
-  const size_t per_group = size_t(2) * KH_TILE_ROWS * row_bytes;
+  const int64_t units = (narrow_most / KH_TILE_ROWS + std::min(a.tokens, a.table.seqs)) * ceil_div(a.cache.kv_heads, form.together);
+  const int64_t blocks = ceil_div(len, KH_STRETCH), most = form.most;
+  const size_t per_group = static_cast<size_t>(2 * KH_TILE_ROWS * form.together) * row_bytes;
   p.groups = std::min<int64_t>(most, std::max(ceil_div(units * blocks, 2), std::min(units, most)));
   p.groups = std::min(p.groups, static_cast<int64_t>(workspace_bytes / per_group));
   // The kernels count blocks in 32 bits, with what lengths beyond the expected
@@ -299,20 +304,20 @@ inline AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t wor
 // What the plan of no step of at most these tokens, sequences, lengths and window
 // takes more than. A single step's own need does not grow with the step: a long
 // chunk fills the chip without parts, a short one and single tokens do not. Each
-// of the plan's two terms is bounded by one that does grow.
-inline size_t attention_workspace(const kh_paged_attention_args &a) {
+// of the plan's two terms is bounded by one that does grow. form: of the most heads.
+inline size_t attention_workspace(const kh_paged_attention_args &a, const NarrowForm &form) {
   const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.tokens * group, len = seen_len(a);
   const size_t row_bytes = part_row_bytes(a);
-  // Narrow: two parts of 16 rows for each workgroup.
-  const int64_t blocks = ceil_div(len, KH_STRETCH), most = most_groups(a);
-  const int64_t units = (rows / KH_TILE_ROWS + std::min(a.tokens, a.table.seqs)) * a.cache.kv_heads;
-  const int64_t groups = blocks <= kWholeBlocks ? 0 : std::min(most, units * blocks);
+  // Narrow: two parts of 16 rows of its heads for each workgroup.
+  const int64_t blocks = ceil_div(len, KH_STRETCH);
+  const int64_t units = (rows / KH_TILE_ROWS + std::min(a.tokens, a.table.seqs)) * (a.cache.kv_heads + form.together - 1);
+  const int64_t groups = blocks <= kWholeBlocks ? 0 : std::min(form.most * form.together, units * blocks);
   // Wide: its splits times its units are at most two to a CU, and its rows fewer
   // than its units times theirs.
   const int64_t splits = len / 256;
   const int64_t wide_rows = splits < 2 || rows <= narrow_rows_of(a.cache.dtype)
                                 ? 0 : std::min<int64_t>(2 * KH_GEMM_CUS * KH_WIDE_ROWS, splits * a.tokens * a.q_heads);
-  return (static_cast<size_t>(groups < 2 ? 0 : groups) * 2 * KH_TILE_ROWS + static_cast<size_t>(wide_rows)) * row_bytes;
+  return (static_cast<size_t>((groups < 2 ? 0 : groups) * 2 * KH_TILE_ROWS) + static_cast<size_t>(wide_rows)) * row_bytes;
 }
 
 }  // namespace khrt::cache

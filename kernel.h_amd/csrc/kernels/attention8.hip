@@ -158,33 +158,44 @@ struct Few {
   static constexpr int piece = D / 16, words = D / 64;  // columns of V of a lane
 };
 
+// Where a block's rows lie. EVEN: the 16 entries from a multiple of 16 on lie next
+// to each other in one page; lane n finds 16 entries' page, n % tiles, so that all
+// of the block's are one load, on its way with the rows.
 template <int D, bool EVEN>
 struct Stretch {
-  KhSlot at[Few<D>::tiles];  // of entry 16 t + l % 16; EVEN: of entry 16 t
+  KhSlot found[EVEN ? 1 : Few<D>::tiles], at[Few<D>::tiles];  // of entry 16 t + l % 16; EVEN: at is of entry 16 t
   uint64_t present;
 };
 
 template <int D, bool EVEN>
-__device__ __forceinline__ void find(Stretch<D, EVEN> &b, const KhAttention8Params &p, const int32_t *table, int key0, int end, int r) {
+__device__ __forceinline__ void find(Stretch<D, EVEN> &b, const KhAttention8Params &p, const int32_t *table, int key0, int end, int lane) {
+  if constexpr (EVEN) {
+    const int key = key0 + 16 * (lane % Few<D>::tiles), last = (end - 1) & ~15;
+    const uint32_t inside = (uint32_t)(key < last ? key : last);  // < capacity: the page's number is in the row
+    const uint32_t i = __umulhi(inside, p.cache.by_page.mul) >> p.cache.by_page.shift;  // kh_div: pages hold 16 entries at least
+    b.found[0] = KhSlot{table[i], (int)(inside - i * p.cache.by_page.by)};
+  } else {
 #pragma unroll
-  for (int t = 0; t < Few<D>::tiles; ++t) b.at[t] = look_up<EVEN>(p, table, key0 + 16 * t + (EVEN ? 0 : r), end);
+    for (int t = 0; t < Few<D>::tiles; ++t) b.found[t] = look_up<false>(p, table, key0 + 16 * t + lane % 16, end);
+  }
 }
 
 // Absent rows are read from the cache's first page: kh_cache.h, Block.
 template <int D, bool EVEN>
-__device__ __forceinline__ void settle(Stretch<D, EVEN> &b, const KhAttention8Params &p, int key0, int end, int r) {
+__device__ __forceinline__ void settle(Stretch<D, EVEN> &b, const KhAttention8Params &p, int key0, int end, int lane) {
   b.present = 0;
 #pragma unroll
   for (int t = 0; t < Few<D>::tiles; ++t) {
-    const bool paged = (uint32_t)b.at[t].page < (uint32_t)p.cache.pages;
     if constexpr (EVEN) {
+      b.at[t] = KhSlot{__builtin_amdgcn_readlane(b.found[0].page, t), __builtin_amdgcn_readlane(b.found[0].slot, t)};
+      const bool paged = (uint32_t)b.at[t].page < (uint32_t)p.cache.pages;
       const int left = end - key0 - 16 * t;
       b.present |= (uint64_t)(!paged || left <= 0 ? 0u : left >= 16 ? 0xffffu : (1u << left) - 1) << (16 * t);
       if (!paged) b.at[t].page = 0;
     } else {
-      const bool there = key0 + 16 * t + r < end && paged;
+      const bool there = key0 + 16 * t + lane % 16 < end && (uint32_t)b.found[t].page < (uint32_t)p.cache.pages;
       b.present |= (__builtin_amdgcn_ballot_w64(there) & 0xffffu) << (16 * t);
-      if (!there) b.at[t] = KhSlot{0, 0};
+      b.at[t] = there ? b.found[t] : KhSlot{0, 0};
     }
   }
 }
@@ -287,6 +298,35 @@ __device__ __forceinline__ void finish(const KhAttention8Params &p, int token, i
   if (col == 0 && p.lse != nullptr) p.lse[row] = lse_of(m, total, 0.0f);
 }
 
+// Writes down what workgroup `block` is the second to work on: the unit, of the
+// sequence s with `before` blocks before it, that its share starts inside of.
+__device__ __forceinline__ void tell(const KhAttention8Params &p, const Line &line, const KhShares &shares, int block, int start,
+                                     int seq, const KhSeq &s, int before) {
+  if (p.whole != 0 || threadIdx.x != 0) return;
+  KhJoin j{};
+  if (block > 0 && block < shares.groups && seq >= 0) {
+    const KhUnits units = kh_units_of(p, s);
+    const int unit = (int)((uint32_t)(start - before) / (uint32_t)units.blocks), begin = before + unit * units.blocks;
+    const KhOwners owners = kh_owners(shares, line.all, begin, units.blocks);
+    if (start != begin && owners.first == block - 1) {
+      const int tile = unit / p.head_groups, rows = s.m * p.group - tile * kRows;
+      j = KhJoin{owners.count, owners.first, owners.slot, s.start, tile * kRows, rows < kRows ? rows : kRows,
+                 (unit - tile * p.head_groups) * p.together, 0};
+    }
+  }
+  p.joins[block] = j;
+}
+
+__device__ __forceinline__ bool told_parts(const KhAttention8Params &p, int block, KhSeq &s, Parts &parts) {
+  const int g = block / p.together, nth = block - g * p.together;
+  const KhJoin j = p.joins[g];
+  if (j.count == 0 || j.head0 + nth >= p.cache.kv_heads) return false;
+  s.start = j.start;
+  parts = Parts{p.part_ml, p.part_o, (((int64_t)j.first * 2 + j.slot) * p.together + nth) * kRows,
+                ((int64_t)g * 2 * p.together + nth) * kRows, 2 * p.together * kRows, j.count, j.row0, j.rows, j.head0 + nth, false};
+  return true;
+}
+
 template <int D, bool EVEN>
 __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, float *lds) {
   using F = Few<D>;
@@ -296,16 +336,16 @@ __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, f
 
   const Line line = line_of(p, false);
   const KhShares shares = shares_of(p, line);
-  if (block >= shares.groups) return;
+  KhSeq s{0, 0, 0};
+  int seq = -1, before = 0;  // blocks of the sequences before this one
   const int start = kh_share(shares, block), end = kh_share(shares, block + 1);
+  if (block < shares.groups) seq = sequence_at(p, line, start, false, s, before);
+  tell(p, line, shares, block, start, seq, s, before);
+  if (seq < 0) return;
   // The join area: each wave's maxima and sums of its rows, the rows' own of the
   // workgroup, and each wave's part of O.
   float *ml = lds, *both = lds + kWaves * kRows * 2, *part = both + kRows * 2;
   constexpr int kPitch = D + 4;
-  int before;  // blocks of the sequences before this one
-  KhSeq s;
-  int seq = sequence_at(p, line, start, false, s, before);
-  if (seq < 0) return;
   KhUnits units = kh_units_of(p, s);
   const float factor0 = p.cap_in != 0.0f ? 1.0f : p.scale_log2;
 
@@ -369,9 +409,9 @@ __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, f
       RowsOfK<D> k;
       RowsOfV<D> v;
       Stretch<D, EVEN> now, next;
-      find<D, EVEN>(now, p, table, key0, key_end, r);
-      find<D, EVEN>(next, p, table, key0 + kStep, key_end, r);
-      settle<D, EVEN>(now, p, key0, key_end, r);
+      find<D, EVEN>(now, p, table, key0, key_end, lane);
+      find<D, EVEN>(next, p, table, key0 + kStep, key_end, lane);
+      settle<D, EVEN>(now, p, key0, key_end, lane);
       load_k<D, EVEN>(k, now, p, kbase, kscales, d, r, h);
       // K goes out before V here as in the loop: the wait for K at its top then
       // leaves V in flight.
@@ -404,9 +444,9 @@ __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, f
           for (int e = 0; e < 4; ++e) y[4 * t + e] = x[e];
         }
         now = next;
-        settle<D, EVEN>(now, p, key0 + kStep, key_end, r);
+        settle<D, EVEN>(now, p, key0 + kStep, key_end, lane);
         load_k<D, EVEN>(k, now, p, kbase, kscales, d, r, h);
-        find<D, EVEN>(next, p, table, key0 + 2 * kStep, key_end, r);
+        find<D, EVEN>(next, p, table, key0 + 2 * kStep, key_end, lane);
 
         if (p.cap_in != 0.0f) {
 #pragma unroll
@@ -555,6 +595,438 @@ __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, f
         *reinterpret_cast<f32x4 *>(p.part_o + (((int64_t)block * 2 + slot) * kRows + row) * d + col) = y;
     }
     lds_barrier();  // before the next unit writes the join area
+  }
+}
+
+// ---- few rows, pages of whole sixteens
+//
+// The same products with K and V straight to LDS, whole rows at a time (a load of
+// 64 bytes of each row, as the matrix operand lies, takes the memory 17% longer),
+// two blocks ahead of their use. A wave has its own LDS, and nobody waits for
+// others: two buffers of a block's rows of K, and of V, their scales' bytes, the
+// powers of two these stand for, and the page numbers of the next blocks, 64
+// tiles' at a time.
+//   S^T   A = 16 bytes of a row of K, two steps' operands.
+//   O^T   A = eight entries of a column of V, read across its rows; V's powers
+//         of two are multiplied into P, and lane l ends with columns
+//         16 c + 4 (l / 16) + i of row l % 16.
+// A row's 16-byte pieces lie at their number exclusive-or a number of the row's, so
+// that 16 rows of K in a column, and the rows of V that two groups of 16 lanes read
+// across, fill the banks once.
+template <int D, int TILES>
+struct Ring {
+  static constexpr int tiles = TILES, keys = 16 * TILES, mine = 4 * TILES;  // entries of a block, and of a lane
+  static constexpr int pieces = D / 16, rows = 64 / pieces;  // rows that a load brings
+  static constexpr int loads = 16 / rows;                    // of a tile
+  static constexpr int ops = tiles * loads + 1;              // of a block's rows of K, or V, and their scales
+  static constexpr int block = keys * D;
+  static constexpr int k_at = 0, v_at = 2 * block, scales_at = 4 * block;  // scales: [K, V][2 buffers][256]
+  static constexpr int powers_at = scales_at + 4 * 256, pages_at = powers_at + 2 * 256;  // powers: [K, V][64] floats
+  static constexpr int places_at = pages_at + 256, there_at = places_at + 64 * 32;  // of 64 tiles
+  static constexpr int lds = there_at + 64 * 2;   // of a wave
+  static constexpr int ahead = 64 / tiles;        // blocks whose pages are found at a time
+};
+
+template <int D>
+__device__ __forceinline__ int k_swap(int row) {
+  return D == 64 ? row >> 2 & 3 : D == 128 ? row >> 1 & 7 : row & 15;
+}
+template <int D>
+__device__ __forceinline__ int v_swap(int row) {
+  return D == 64 ? (row >> 2 & 1) | (row >> 3 & 2) : D == 128 ? (row >> 1 & 3) | (row >> 2 & 4) : (row & 7) | (row >> 1 & 8);
+}
+
+// Of 8 x 16 bytes in LDS that the 16 lanes of a row point at (lane 2 r + c: row r,
+// columns 8 c ..), lane i receives column i, its eight rows in order.
+__device__ __forceinline__ u32x2 read_across8(const char *p) {
+  typedef int Two __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                       (__attribute__((address_space(3))) Two *)const_cast<char *>(p)));
+}
+
+// What was read from LDS has arrived: what it was read from may be written.
+__device__ __forceinline__ void read_out() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t lds_of(const char *p) { return (uint32_t)reinterpret_cast<uintptr_t>(p); }
+
+// Asks for the page numbers of 64 tiles, those of `ahead` blocks of the wave's, the
+// first at key0 and `step` entries apart: lane n the n-th's.
+template <class F>
+__device__ __forceinline__ void ask(const KhAttention8Params &p, const int32_t *table, int key0, int step, int end, char *own, int lane) {
+  // In 64 bits: blocks that are asked for may lie past 2^31.
+  const int64_t key = (int64_t)key0 + (int64_t)(lane / F::tiles) * step + 16 * (lane % F::tiles);
+  const int last = (end - 1) & ~15;
+  const uint32_t inside = (uint32_t)(key < last ? key : last);
+  const uint32_t i = __umulhi(inside, p.cache.by_page.mul) >> p.cache.by_page.shift;  // kh_div: pages hold 16 entries at least
+  const uint64_t at = reinterpret_cast<uintptr_t>(table);
+  dma4(u32x4{(uint32_t)at, (uint32_t)(at >> 32), (uint32_t)p.table.width * 4u, 0x00020000u}, 4 * i, lds_of(own + F::pages_at));
+}
+
+// From page numbers to where the tiles' rows lie, a lane each: two resources' words
+// but the last, the scales' place, and which entries are there. A resource ends
+// where the tile's entries do: absent rows arrive as zeros.
+template <class F>
+__device__ __forceinline__ void place(const KhAttention8Params &p, const char *kbase, const char *vbase, int key0, int step, int end,
+                                      char *own, int lane) {
+  const int64_t far = (int64_t)key0 + (int64_t)(lane / F::tiles) * step + 16 * (lane % F::tiles);
+  const int key = (int)(far < end ? far : 0), left = far < end ? (end - key < 16 ? end - key : 16) : 0;
+  const int page = reinterpret_cast<const int32_t *>(own + F::pages_at)[lane];
+  const bool there = left > 0 && (uint32_t)page < (uint32_t)p.cache.pages;
+  const uint32_t i = __umulhi((uint32_t)key, p.cache.by_page.mul) >> p.cache.by_page.shift;
+  const KhSlot at = there ? KhSlot{page, key - (int)(i * p.cache.by_page.by)} : KhSlot{0, 0};
+  const uint32_t rows = there ? (uint32_t)left : 0;
+  // Addresses have 48 bits: the resource's stride, above them, is zero.
+  const uint64_t k = reinterpret_cast<uintptr_t>(kbase) + kh_row(at, p.cache.k_page, p.cache.k_slot);
+  const uint64_t v = reinterpret_cast<uintptr_t>(vbase) + kh_row(at, p.cache.v_page, p.cache.v_slot);
+  u32x4 *to = reinterpret_cast<u32x4 *>(own + F::places_at) + 2 * lane;
+  to[0] = u32x4{(uint32_t)k, (uint32_t)(k >> 32), rows * p.cache.k_slot, (uint32_t)at.page * p.scale_page + (uint32_t)at.slot};
+  to[1] = u32x4{(uint32_t)v, (uint32_t)(v >> 32), rows * p.cache.v_slot, 0u};
+  reinterpret_cast<uint16_t *>(own + F::there_at)[lane] = (uint16_t)((1u << rows) - 1);
+}
+
+// The loads of a tile: dma16 (kh_elem.h) 1, 2 or 4 times, 1 KB further in LDS each.
+#define KH_DMA_NEXT(n) "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %" #n ", %3, 0 offen nt lds\n\t"
+#define KH_DMA_TILE(more, ...)                                     \
+  asm volatile(                                                    \
+      "s_mov_b32 %0, m0\n\t"                                       \
+      "s_mov_b32 m0, %1\n\t"                                       \
+      "s_nop 2\n\t"                                                \
+      "buffer_load_dwordx4 %2, %3, 0 offen nt lds\n\t" more           \
+      "s_mov_b32 m0, %0"                                           \
+      : "=&s"(saved)                                               \
+      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff[0]), "s"(rsrc) __VA_ARGS__ \
+      : "memory", "scc")
+template <int LOADS>
+__device__ __forceinline__ void dma_tile(u32x4 rsrc, const uint32_t (&voff)[LOADS], uint32_t lds) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
+  uint32_t saved;
+  if constexpr (LOADS == 1)
+    KH_DMA_TILE("");
+  else if constexpr (LOADS == 2)
+    KH_DMA_TILE(KH_DMA_NEXT(4), , "v"(voff[1]));
+  else
+    KH_DMA_TILE(KH_DMA_NEXT(4) KH_DMA_NEXT(5) KH_DMA_NEXT(6), , "v"(voff[1]), "v"(voff[2]), "v"(voff[3]));
+}
+#undef KH_DMA_TILE
+#undef KH_DMA_NEXT
+
+// Sends a block's rows of K, or of V (which: 0 or 1), and their scales to LDS; n: its
+// number among those placed, `ahead` for one that there is none of. voff: what a
+// lane brings of a tile's rows in each load, tiles of even and odd number.
+template <class F>
+__device__ __forceinline__ void send(const KhAttention8Params &p, const char *own, int n, int which, const uint32_t (&voff)[2][F::loads],
+                                     const uint8_t *scales, const char *to, const char *scales_to, int lane) {
+  const u32x4 *places = reinterpret_cast<const u32x4 *>(own + F::places_at) + 2 * F::tiles * (n % F::ahead);
+  const uint32_t scale = places[2 * (lane / 4 % F::tiles)].w + 4u * (uint32_t)(lane % 4);
+#pragma unroll
+  for (int t = 0; t < F::tiles; ++t) {
+    u32x4 r = places[2 * t + which];
+    r.z = n < F::ahead ? r.z : 0u;
+    r.w = 0x00020000u;
+    dma_tile<F::loads>(r, voff[t % 2], lds_of(to) + (uint32_t)(t * F::loads * 1024));
+  }
+  const uint64_t at = reinterpret_cast<uintptr_t>(scales);
+  const uint32_t size = (uint32_t)(p.cache.pages - 1) * p.scale_page + (uint32_t)p.cache.page_size;
+  dma4(u32x4{(uint32_t)at, (uint32_t)(at >> 32), size, 0x00020000u}, scale, lds_of(scales_to));
+}
+
+// Which entries of a placed block are there.
+template <class F>
+__device__ __forceinline__ uint64_t there_of(const char *own, int n) {
+  const uint16_t *at = reinterpret_cast<const uint16_t *>(own + F::there_at) + F::tiles * (n % F::ahead);
+  uint64_t there = 0;
+  if constexpr (F::tiles == 4) {
+    const u32x2 w = *reinterpret_cast<const u32x2 *>(at);
+    there = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(w.y) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane(w.x);
+  } else {
+    there = (uint32_t)__builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(at));
+  }
+  return n < F::ahead ? there : 0;
+}
+
+template <int D, int TILES, int WAVES>
+__device__ __forceinline__ void narrow_even(const KhAttention8Params &p, int block, char *lds) {
+  using F = Ring<D, TILES>;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane & 15, h = lane >> 4;
+  const int d = p.cache.head_dim;
+
+  const Line line = line_of(p, false);
+  const KhShares shares = shares_of(p, line);
+  KhSeq s{0, 0, 0};
+  int seq = -1, before = 0;  // blocks of the sequences before this one
+  const int start = kh_share(shares, block), end = kh_share(shares, block + 1);
+  if (block < shares.groups) seq = sequence_at(p, line, start, false, s, before);
+  tell(p, line, shares, block, start, seq, s, before);
+  if (seq < 0) return;
+  // The join area, behind which nobody's loads are on their way any more: each
+  // wave's maxima and sums of its rows, the rows' own of the workgroup, and each
+  // wave's part of O.
+  float *ml = reinterpret_cast<float *>(lds), *both = ml + WAVES * kRows * 2, *part = both + WAVES * kRows * 2;
+  constexpr int kPitch = D + 4;
+  char *own = lds + wave * F::lds;
+  float *powers = reinterpret_cast<float *>(own + F::powers_at);
+  KhUnits units = kh_units_of(p, s);
+  const float factor0 = p.cap_in != 0.0f ? 1.0f : p.scale_log2;
+
+  uint32_t k_off[2][F::loads], v_off[2][F::loads];
+#pragma unroll
+  for (int i = 0; i < F::loads; ++i)
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      const int row = i * F::rows + lane / F::pieces, piece = lane % F::pieces;
+      const int kc = 16 * (piece ^ k_swap<D>(row)), vc = 16 * (piece ^ v_swap<D>(row + 16 * odd));
+      k_off[odd][i] = kc < d ? (uint32_t)row * p.cache.k_slot + (uint32_t)kc : kOutside;
+      v_off[odd][i] = vc < d ? (uint32_t)row * p.cache.v_slot + (uint32_t)vc : kOutside;
+    }
+
+  // Of two workgroups on a CU the older one's waves go first, and the other one would
+  // end alone, some 15% later. So the second goes first for half of its share, the
+  // older one after that (64 sequences of 513 to 8192 entries: PRIOTXT).
+  const int second = block >= shares.groups / 2 && shares.groups > KH_CUS;
+  int first_half = second ? (end - start) * (KH_STRETCH / 2) : 0;  // entries until then
+  if (second) __builtin_amdgcn_s_setprio(1);
+  for (int at = start, in = start - before; at < end;) {
+    while (kh_passed(in, kh_work(units, p.head_groups))) {
+      // The next sequence of few rows: wide() has the others.
+      do {
+        if (++seq >= p.table.seqs) return;
+        s = sequence(p, seq);
+      } while (s.m * p.group > p.narrow_rows);
+      units = kh_units_of(p, s);
+    }
+    const uint32_t unit = (uint32_t)in / (uint32_t)units.blocks;
+    const int tile = (int)(unit / (uint32_t)p.head_groups), head0 = (int)(unit - (uint32_t)tile * (uint32_t)p.head_groups) * p.together;
+    // The waves share the unit's heads out, and a head's share the entries.
+    const int heads = p.cache.kv_heads - head0 < p.together ? p.cache.kv_heads - head0 : p.together;
+    const int per_head = heads == 1 ? WAVES : heads == 2 ? WAVES / 2 : 1;
+    const int nth = wave / per_head, head = head0 + (nth < heads ? nth : 0);
+    const int block0 = in - (int)unit * units.blocks;
+    const int block1 = end - at < units.blocks - block0 ? block0 + end - at : units.blocks;
+    const bool alone = block0 == 0 && block1 == units.blocks;
+    const int slot = at == start ? 0 : 1;
+    at += block1 - block0, in += block1 - block0;
+    const int from = units.first + block0 * KH_STRETCH, to = block1 == units.blocks ? s.n : units.first + block1 * KH_STRETCH;
+    const int rows = s.m * p.group;  // < 2^31: tokens x q_heads is
+    const int row0 = tile * kRows;
+    const int32_t *table = p.table.pages + seq * p.table.row_stride;
+    const char *kbase = p.cache.k + (uint64_t)head * p.cache.k_head;
+    const char *vbase = p.cache.v + (uint64_t)head * p.cache.v_head;
+    const uint8_t *kscales = p.k_scale + (uint64_t)head * p.scale_head, *vscales = p.v_scale + (uint64_t)head * p.scale_head;
+
+    const int R = row0 + r;
+    const bool mine = R < rows;
+    const int i = mine ? (int)kh_div(R, p.by_group) : 0, hq = head * p.group + (mine ? R - i * p.group : 0);
+    const int i_first = (int)kh_div(row0, p.by_group);
+    const int i_last = (int)kh_div(row0 + kRows < rows ? row0 + kRows - 1 : rows - 1, p.by_group);
+    const KhSpan seen = kh_span_of(p, s, i);
+    const KhSpan low = kh_span_of(p, s, i_first), high = kh_span_of(p, s, i_last);
+    const int key_first = (low.first > from ? low.first : from) & ~15;  // from is a multiple of 16
+    const int key_end = high.end < to ? high.end : to;
+
+    // Of row l % 16; l of this lane's entries alone. A row that there is none of has
+    // no scores, and no maximum to look after either.
+    float m = mine ? kSeed : 0.0f, l = 0.0f;
+    f32x4 o[F::pieces];
+#pragma unroll
+    for (int c = 0; c < F::pieces; ++c) o[c] = f32x4{0, 0, 0, 0};
+
+    int key0 = nth < heads ? key_first + wave % per_head * F::keys : key_end;
+    if (key0 < key_end) {
+      const int kStep = per_head * F::keys;
+      uint64_t present[2];
+      ask<F>(p, table, key0, kStep, key_end, own, lane);
+      // q's columns as K's bytes lie: of each 64, 16 of a lane, in two steps.
+      u32x4 q[D / 32][kParts];
+      const row_t *qp = static_cast<const row_t *>(p.q) + ((int64_t)(s.start + i) * p.q_stride + (int64_t)hq * d);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const int col = 64 * (c / 2) + 16 * h + 8 * (c % 2);
+        // From an address that is there in any case.
+        load_q(q[c], qp + within(col, d), mine && col < d, p);
+      }
+      arrived<0>();
+      place<F>(p, kbase, vbase, key0, kStep, key_end, own, lane);
+      int placed = 0;  // blocks from the first of those placed to this one
+      read_out();
+      if (key_end - key0 > F::ahead * kStep) ask<F>(p, table, key0 + F::ahead * kStep, kStep, key_end, own, lane);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        present[n] = there_of<F>(own, n);
+        send<F>(p, own, n, 0, k_off, kscales, own + F::k_at + n * F::block, own + F::scales_at + n * 256, lane);
+        send<F>(p, own, n, 1, v_off, vscales, own + F::v_at + n * F::block, own + F::scales_at + 512 + n * 256, lane);
+      }
+      for (int n = 0; key0 < key_end; ++n, key0 += kStep) {
+        const int b = n & 1;
+        first_half -= kStep;
+        if (first_half < 0) __builtin_amdgcn_s_setprio(0);
+        const uint64_t here = present[0];
+        // Of K, V of this block, K, V of the next: all but the first may be on their way.
+        arrived<3 * F::ops>();
+        const char *kb = own + F::k_at + b * F::block;
+        powers[lane] = power_of((uint8_t)own[F::scales_at + b * 256 + lane % F::keys]);
+        float y[F::mine];
+#pragma unroll
+        for (int t = 0; t < F::tiles; ++t) {
+          f32x4 x = {0, 0, 0, 0};
+          const float power = powers[16 * t + r];
+          const char *row = kb + (16 * t + r) * D;
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(row + 16 * ((4 * c + h) ^ k_swap<D>(r)));
+            const u32x4 a0 = {widen<false>(w.x, power), widen<true>(w.x, power), widen<false>(w.y, power), widen<true>(w.y, power)};
+            const u32x4 a1 = {widen<false>(w.z, power), widen<true>(w.z, power), widen<false>(w.w, power), widen<true>(w.w, power)};
+#pragma unroll
+            for (int n1 = 0; n1 < kParts; ++n1) x = mma16(a0, q[2 * c][n1], x);
+#pragma unroll
+            for (int n1 = 0; n1 < kParts; ++n1) x = mma16(a1, q[2 * c + 1][n1], x);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[4 * t + e] = x[e];
+        }
+        // The block after the next takes this one's place. The page numbers of the
+        // next `ahead` blocks were asked for as many ago.
+        if (placed + 2 == F::ahead && key_end - key0 > 2 * kStep) [[unlikely]] {
+          place<F>(p, kbase, vbase, key0 + 2 * kStep, kStep, key_end, own, lane);
+          placed = -2;
+          read_out();
+          if (key_end - key0 > (2 + F::ahead) * kStep) ask<F>(p, table, key0 + (2 + F::ahead) * kStep, kStep, key_end, own, lane);
+        }
+        const int then = key_end - key0 > 2 * kStep ? placed + 2 : F::ahead;
+        ++placed;
+        present[0] = present[1], present[1] = there_of<F>(own, then);
+        read_out();
+        send<F>(p, own, then, 0, k_off, kscales, kb, own + F::scales_at + b * 256, lane);
+
+        if (p.cap_in != 0.0f) [[unlikely]] {
+#pragma unroll
+          for (int j = 0; j < F::mine; ++j) y[j] = capped(y[j], p);
+        }
+        // Every row sees every entry of the block: no mask.
+        const bool whole = here == ~uint64_t(0) >> (64 - F::keys) && key0 + F::keys <= low.end && key0 >= high.first;
+        if (!whole) [[unlikely]] {
+          const uint64_t sees = (mine ? seen_of(seen, key0) & here : 0) >> 4 * h;
+#pragma unroll
+          for (int j = 0; j < F::mine; ++j) y[j] = (sees >> (16 * (j / 4) + j % 4) & 1) != 0 ? y[j] : -__builtin_inff();
+        }
+        float top = y[0];
+#pragma unroll
+        for (int j = 1; j < F::mine; ++j) top = fmaxf(top, y[j]);
+        top = fmaxf(m, over_rows(top, true) * factor0);
+        if (__builtin_amdgcn_ballot_w64(top > m) != 0) [[unlikely]] {
+          const float fade = exp2_hw(m - top);
+          m = top;
+          l *= fade;
+#pragma unroll
+          for (int c = 0; c < F::pieces; ++c) o[c] *= fade;
+        }
+        const bool far = coarse(m);
+        const float factor = far ? 1.0f : factor0, shift = far ? 0.0f : -m;
+        if (far) [[unlikely]] less<F::mine>(y, factor0, m);
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < F::mine; ++j) {
+          y[j] = exp2_hw(fmaf(y[j], factor, shift));
+          sum += y[j];
+        }
+        l += sum;
+
+        // Of V of this block, K, V of the next, K of the one after it.
+        arrived<3 * F::ops>();
+        char *vb = own + F::v_at + b * F::block;
+        powers[64 + lane] = power_of((uint8_t)own[F::scales_at + 512 + b * 256 + lane % F::keys]);
+        if (!whole) [[unlikely]] {
+          // NaN in V where rows differ in what they see: 0 x V would reach the rows
+          // that do not. They are added to the rows that do see them, and leave the
+          // products as zeros.
+#pragma unroll 1
+          for (int at16 = 0; at16 < F::block; at16 += 1024) {
+            u32x4 *mine16 = reinterpret_cast<u32x4 *>(vb + at16 + 16 * lane);
+            const u32x4 w = *mine16;
+            const bool odd = (nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w)) != 0;
+            uint64_t odds = __builtin_amdgcn_ballot_w64(odd);
+            if (odds == 0) continue;
+            while (odds != 0) {
+              const int in1024 = __builtin_ctzll(odds) / F::pieces;
+              odds &= ~((F::pieces == 64 ? ~uint64_t(0) : (uint64_t(1) << F::pieces) - 1) << (in1024 * F::pieces));
+              const int row = at16 / D + in1024, key = key0 + row;
+              if (!(mine && key >= seen.first && key < seen.end)) continue;
+#pragma unroll
+              for (int c = 0; c < F::pieces; ++c) {
+                const uint32_t n4 = nan_bytes(*reinterpret_cast<const uint32_t *>(vb + row * D + 16 * (c ^ v_swap<D>(row)) + 4 * h));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if ((n4 >> 8 * e & 0x80u) != 0) o[c][e] = __builtin_nanf("");
+              }
+            }
+            *mine16 = u32x4{without_nan(w.x), without_nan(w.y), without_nan(w.z), without_nan(w.w)};
+          }
+        }
+        // The row that lane 2 x + c of 16 points at, of 32 entries: x % 4 of the
+        // lane's four of each 16.
+        const int across = 16 * (r / 8) + 4 * h + r / 2 % 4;
+#pragma unroll
+        for (int g = 0; g < F::tiles / 2; ++g) {
+          u32x4 bp[kParts];
+          const f32x4 p0 = *reinterpret_cast<const f32x4 *>(powers + 64 + 32 * g + 4 * h);
+          const f32x4 p1 = *reinterpret_cast<const f32x4 *>(powers + 64 + 32 * g + 16 + 4 * h);
+          float eight[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) eight[j] = y[8 * g + j] * p0[j], eight[4 + j] = y[8 * g + 4 + j] * p1[j];
+          in_parts(bp, eight, false);
+          const char *row = vb + (32 * g + across) * D + 8 * (r % 2);
+#pragma unroll
+          for (int c = 0; c < F::pieces; ++c) {
+            const u32x2 w = read_across8(row + 16 * (c ^ v_swap<D>(across)));
+            const u32x4 a = {widen<false>(w.x, 1.0f), widen<true>(w.x, 1.0f), widen<false>(w.y, 1.0f), widen<true>(w.y, 1.0f)};
+#pragma unroll
+            for (int n1 = 0; n1 < kParts; ++n1) o[c] = mma16(a, bp[n1], o[c]);
+          }
+        }
+        read_out();
+        send<F>(p, own, then, 1, v_off, vscales, vb, own + F::scales_at + 512 + b * 256, lane);
+      }
+    }
+
+    // Join the waves: rescale to the rows' common maximum, add in wave order.
+    l = over_rows(l, false);
+    vm_wait<0>();
+    lds_barrier();  // everyone's last loads have come to LDS
+    if (h == 0) {
+      ml[(wave * kRows + r) * 2] = m;
+      ml[(wave * kRows + r) * 2 + 1] = l;
+    }
+    lds_barrier();
+    const int wave0 = nth * per_head;  // the head's first wave
+    float top = kSeed;
+    for (int w = 0; w < per_head; ++w) top = fmaxf(top, ml[((wave0 + w) * kRows + r) * 2]);
+    float total = 0.0f;
+    for (int w = 0; w < per_head; ++w) total += ml[((wave0 + w) * kRows + r) * 2 + 1] * exp2_hw(ml[((wave0 + w) * kRows + r) * 2] - top);
+    const float fade = exp2_hw(m - top);
+#pragma unroll
+    for (int c = 0; c < F::pieces; ++c) *reinterpret_cast<f32x4 *>(part + (wave * kRows + r) * kPitch + 16 * c + 4 * h) = o[c] * fade;
+    if (wave == wave0 && nth < heads && h == 0) {
+      both[2 * (nth * kRows + r)] = top, both[2 * (nth * kRows + r) + 1] = total;
+      if (!alone) {
+        float *ml_to = p.part_ml + ((((int64_t)block * 2 + slot) * p.together + nth) * kRows + r) * 2;
+        ml_to[0] = top;
+        ml_to[1] = total;
+      }
+    }
+    lds_barrier();
+    for (int x = threadIdx.x; x < heads * kRows * (D / 4); x += WAVES * kWave) {
+      const int of = x / (kRows * (D / 4)), row = x / (D / 4) % kRows, col = x % (D / 4) * 4, RR = row0 + row;
+      if (RR >= rows || col >= d) continue;
+      const int ii = (int)kh_div(RR, p.by_group), hh = (head0 + of) * p.group + RR - ii * p.group;
+      f32x4 y = {0, 0, 0, 0};
+      for (int w = 0; w < per_head; ++w) y += *reinterpret_cast<const f32x4 *>(part + ((of * per_head + w) * kRows + row) * kPitch + col);
+      if (alone)
+        finish(p, s.start + ii, hh, col, y, both[2 * (of * kRows + row)], both[2 * (of * kRows + row) + 1]);
+      else
+        *reinterpret_cast<f32x4 *>(p.part_o + ((((int64_t)block * 2 + slot) * p.together + of) * kRows + row) * d + col) = y;
+    }
+    lds_barrier();  // before the next unit's loads come to the join area
   }
 }
 
@@ -971,17 +1443,25 @@ __device__ __forceinline__ void settle_shared(KhAttention8Params &p) {
 #define KH_TYPED8(name) KH_PASTE(name, bf16)
 #endif
 
-#define KH_ATTENTION8(D, PER_CU)                                                                               \
-  extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED8(attention8_##D)(KhAttention8Params p) { \
-    __shared__ __attribute__((aligned(16))) float lds[kWaves * kRows * 2 + kRows * 2 + kWaves * kRows * (D + 4)]; \
-    if (p.even)                                                                                               \
-      narrow<D, true>(p, (int)blockIdx.x, lds);                                                               \
-    else                                                                                                      \
-      narrow<D, false>(p, (int)blockIdx.x, lds);                                                              \
+#define KH_ATTENTION8(D, TILES, WAVES, PER_CU)                                                                          \
+  extern "C" __global__ void __launch_bounds__(64 * WAVES, PER_CU) KH_TYPED8(attention8_##D)(KhAttention8Params p) { \
+    __shared__ __attribute__((aligned(16))) char lds[WAVES * Ring<D, TILES>::lds];                                   \
+    narrow_even<D, TILES, WAVES>(p, (int)blockIdx.x, lds);                                                           \
   }
-KH_ATTENTION8(64, 2)
-KH_ATTENTION8(128, 2)
-KH_ATTENTION8(256, 1)
+#ifndef V64
+#define V64 2
+#endif
+KH_ATTENTION8(64, V64, 4, 2)
+KH_ATTENTION8(128, 2, 4, 2)
+KH_ATTENTION8(256, 2, 2, 1)
+#define KH_ATTENTION8_ODD(D, PER_CU)                                                                               \
+  extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED8(attention8_odd_##D)(KhAttention8Params p) { \
+    __shared__ __attribute__((aligned(16))) float lds[kWaves * kRows * 2 + kRows * 2 + kWaves * kRows * (D + 4)]; \
+    narrow<D, false>(p, (int)blockIdx.x, lds);                                                                    \
+  }
+KH_ATTENTION8_ODD(64, 2)
+KH_ATTENTION8_ODD(128, 2)
+KH_ATTENTION8_ODD(256, 1)
 // Steps with sequences of many rows or shared entries: their workgroups first.
 #define KH_ATTENTION8_WIDE(D, PER_CU)                                                                               \
   extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED8(attention8_wide_##D)(KhAttention8Params p) { \
@@ -1002,7 +1482,7 @@ KH_ATTENTION8_WIDE(256, 1)
   extern "C" __global__ void __launch_bounds__(256) KH_TYPED8(attention8_join_##D)(KhAttention8Params p) {      \
     __shared__ float lds[kJoinParts * kRows * 2];                                                               \
     settle_shared(p);                                                                                           \
-    join<D>(p, lds, [&](int token, int hq, int col, f32x4 o, float m, float total) {                            \
+    join<D, true, 8>(p, lds, [&](int g, KhSeq &s, Parts &parts) { return told_parts(p, g, s, parts); }, [&](int token, int hq, int col, f32x4 o, float m, float total) {                            \
       finish(p, token, hq, col, o, m, total);                                                                   \
     });                                                                                                         \
   }                                                                                                             \

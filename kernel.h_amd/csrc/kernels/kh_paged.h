@@ -308,6 +308,10 @@ struct KhAttentionParams {
 };
 
 KH_HD KhUnits kh_units_of(const KhAttentionParams &p, const KhSeq &s) { return kh_units(s, p.group, p.window, p.whole); }
+// kv heads that a unit of few rows takes together, and how many such groups there are.
+KH_HD int32_t kh_together(const KhAttentionParams &) { return 1; }
+KH_HD int32_t kh_groups_of(const KhAttentionParams &p) { return p.cache.kv_heads; }
+KH_HD int32_t kh_most_of(const KhAttentionParams &p, int32_t work) { return p.wide_blocks > 0 ? p.groups : kh_most(work, p.groups); }
 KH_HD KhSpan kh_span_of(const KhAttentionParams &p, const KhSeq &s, int32_t i) { return kh_seen(s, i, p.window); }
 
 // Rows of a cache in 8 bits: e4m3 numbers times 2^(byte - 127) of the row's own
@@ -315,6 +319,15 @@ KH_HD KhSpan kh_span_of(const KhAttentionParams &p, const KhSeq &s, int32_t i) {
 // past fp32's normal range. What lies outside counts as the nearer of them.
 #define KH_SCALE_LEAST 10
 #define KH_SCALE_MOST 246
+
+// A unit of few rows that several workgroups worked on, as the second of them writes
+// it down; count 0: that workgroup is not the second of any. Otherwise whoever joins
+// the parts would have to walk the sequences again.
+struct KhJoin {
+  int32_t count, first, slot;  // KhOwners
+  int32_t start, row0, rows;   // the sequence's first token, the unit's rows
+  int32_t head0, spare;
+};
 
 // attention8.hip. The cache's strides are bytes as above, one to an element.
 struct KhAttention8Params : KhAttentionParams {
@@ -325,8 +338,14 @@ struct KhAttention8Params : KhAttentionParams {
   int32_t shared_blocks, shared_splits, shared_each;
   // [shared_splits + 1][tokens q_heads][head_dim], and [..][2]: the last is the sequences' own entries'.
   float *shared_o, *shared_ml;
+  KhJoin *joins;  // [groups]
+  int32_t together, head_groups;  // kv heads that a unit of few rows takes together (the last fewer), and their groups
   float cap_in, cap_out;  // scores y become cap_out tanh(y cap_in / (2 log2 e)); cap_in 0: they do not
 };
+
+KH_HD int32_t kh_together(const KhAttention8Params &p) { return p.together; }
+KH_HD int32_t kh_groups_of(const KhAttention8Params &p) { return p.head_groups; }
+KH_HD int32_t kh_most_of(const KhAttention8Params &p, int32_t) { return p.groups; }
 
 // Entries that sequences share lie before those that are each one's own.
 KH_HD KhSpan kh_span_of(const KhAttention8Params &p, const KhSeq &s, int32_t i) {

@@ -89,7 +89,7 @@ int kh_paged_attention_workspace(const kh_paged_attention_args *args, size_t *by
   return guarded(op, [&] {
     if (args == nullptr || bytes == nullptr) return bad(op, "null argument");
     if (int rc = check_attention(op, *args)) return rc;
-    *bytes = attention_workspace(*args);
+    *bytes = attention_workspace(*args, {most_groups(*args)});
     return 0;
   });
 }
@@ -101,7 +101,7 @@ int kh_paged_attention(const kh_paged_attention_args *args, void *workspace, siz
     const kh_paged_attention_args &a = *args;
     if (int rc = check_attention(op, a)) return rc;
     if (!aligned(workspace)) return bad(op, "workspace must be 16-byte aligned");
-    const AttentionPlan plan = attention_plan(a, workspace != nullptr ? workspace_bytes : 0);
+    const AttentionPlan plan = attention_plan(a, workspace != nullptr ? workspace_bytes : 0, {most_groups(a)});
     const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.tokens * a.q_heads, d = a.cache.head_dim;
     const bool joined = plan.part_bytes + plan.wide_bytes > 0;
     // All rows of parts come first, 16 bytes at a time, then their statistics.

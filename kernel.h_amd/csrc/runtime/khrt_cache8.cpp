@@ -12,6 +12,9 @@ namespace {
 const Symbol kRope[3][3] = {KH_BY_TYPE(rope8, "_8"), KH_BY_TYPE(rope8, "_16"), KH_BY_TYPE(rope8, "_32")};
 const Symbol kRead[3] = KH_BY_TYPE(read8, "");
 const Symbol kAttention[3][3] = {KH_BY_TYPE(attention8, "_64"), KH_BY_TYPE(attention8, "_128"), KH_BY_TYPE(attention8, "_256")};
+constexpr size_t kJoinBytes = sizeof(KhJoin) * 2 * KH_GEMM_CUS;
+constexpr unsigned kWaves[3] = {4, 4, 2};  // of a workgroup of kAttention's
+const Symbol kOdd[3][3] = {KH_BY_TYPE(attention8, "_odd_64"), KH_BY_TYPE(attention8, "_odd_128"), KH_BY_TYPE(attention8, "_odd_256")};
 const Symbol kWide[3][3] = {KH_BY_TYPE(attention8, "_wide_64"), KH_BY_TYPE(attention8, "_wide_128"),
                             KH_BY_TYPE(attention8, "_wide_256")};
 const Symbol kJoin[3][3] = {KH_BY_TYPE(attention8, "_join_64"), KH_BY_TYPE(attention8, "_join_128"),
@@ -81,6 +84,38 @@ kh_paged_attention_args as_plain(const kh_paged_attention8_args &a, int64_t behi
   p.tokens = a.tokens, p.q_heads = a.q_heads, p.window = a.window, p.max_new = a.max_new;
   p.table.max_len = std::max<int64_t>(1, expected_len(a.table, p.cache) - behind);
   return p;
+}
+
+// As even_pages; four scales from a multiple of four slots on are a word; and
+// places of scales and page numbers, past a head's first and a row's, fit 32 bits.
+bool even_pages8(const kh_paged_attention8_args &a) {
+  const kh_paged_cache8 &c = a.cache;
+  const auto [near, far] = std::minmax(c.k_slot_stride, c.v_slot_stride);
+  const uintptr_t words = reinterpret_cast<uintptr_t>(c.k_scale) | reinterpret_cast<uintptr_t>(c.v_scale) |
+                          static_cast<uintptr_t>(c.scale_page_stride) | static_cast<uintptr_t>(c.scale_head_stride);
+  return c.page_size % 16 == 0 && near >= c.head_dim && far < 1 << 27 && words % 4 == 0 &&
+         c.pages * c.scale_page_stride + c.page_size < int64_t(1) << 32 && a.table.width < 1 << 29;
+}
+
+// kv heads that a workgroup reads together at the most: where those of an entry lie
+// next to each other, as many as make 256 bytes. Memory is slower by as much as a
+// quarter where neighbours of 128 bytes are read at different times: MI355X, 64
+// sequences of 513 to 8192 entries, 8 kv heads of 128, one at a time 131 us, two
+// 115, four 112 (and longer where parts are joined).
+int64_t most_together(const kh_paged_attention8_args &a) {
+  const kh_paged_cache8 &c = a.cache;
+  if (c.kv_heads == 1 || c.k_head_stride > 256 || c.v_head_stride > 256) return 1;
+  return std::min<int64_t>(c.kv_heads, c.head_dim <= 64 ? 4 : c.head_dim <= 128 ? 2 : 1);
+}
+
+// Fewer where there would not be a block of entries for every workgroup.
+int64_t heads_together(const kh_paged_attention8_args &a) {
+  const kh_paged_cache8 &c = a.cache;
+  const int64_t units = std::min(a.tokens, a.table.seqs) + a.tokens * (a.q_heads / c.kv_heads) / KH_TILE_ROWS;
+  const int64_t blocks = ceil_div(seen_len(as_plain(a, 0)), KH_STRETCH);
+  int64_t n = most_together(a);
+  while (n > 1 && units * ceil_div(c.kv_heads, n) * blocks < 2 * KH_GEMM_CUS) n = (n + 1) / 2;
+  return n;
 }
 
 // How the entries that sequences share are worked on: not at all (splits 0), or by
@@ -235,7 +270,7 @@ int kh_paged_attention8_workspace(const kh_paged_attention8_args *args, size_t *
   return guarded(op, [&] {
     if (args == nullptr || bytes == nullptr) return bad(op, "null argument");
     if (int rc = check_attention8(op, *args)) return rc;
-    *bytes = attention_workspace(as_plain(*args, 0)) + shared_workspace(*args);
+    *bytes = attention_workspace(as_plain(*args, 0), {2 * KH_GEMM_CUS, most_together(*args)}) + shared_workspace(*args) + kJoinBytes;
     return 0;
   });
 }
@@ -252,27 +287,30 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
     const SharedPlan shared = shared_plan(a, workspace_bytes);
     const bool common = shared.splits > 0;
     const kh_paged_attention_args plain = as_plain(a, common ? a.shared : 0);
-    const AttentionPlan plan = attention_plan(plain, workspace_bytes - shared.bytes);
     const int64_t group = a.q_heads / c.kv_heads, rows = a.tokens * a.q_heads, d = c.head_dim;
+    const bool even = even_pages8(a);
+    // Straight to LDS, two workgroups fill a CU's.
+    const bool alone = even && !common && kh_narrow_only(a.tokens, a.table.seqs, group, a.max_new, narrow_rows_of(KHRT_BF16), 256);
+    const int64_t together = alone ? heads_together(a) : 1;
+    // What tells who joins which parts comes last.
+    size_t left = workspace_bytes - shared.bytes;
+    left -= std::min(left, kJoinBytes);
+    const AttentionPlan plan = attention_plan(plain, left, {alone ? 2 * KH_GEMM_CUS : most_groups(plain), together});
     const bool joined = plan.part_bytes + plan.wide_bytes > 0;
     // All rows of parts come first, 16 bytes at a time, then their statistics.
     float *at = static_cast<float *>(workspace);
     const auto take = [&at](int64_t floats) { return std::exchange(at, floats > 0 ? at + floats : at); };
-    const int64_t narrow_parts = plan.part_bytes > 0 ? plan.groups * 2 * KH_TILE_ROWS : 0, wide_parts = plan.wide_bytes > 0 ? plan.splits * rows : 0;
+    const int64_t narrow_parts = plan.part_bytes > 0 ? plan.groups * 2 * KH_TILE_ROWS * together : 0, wide_parts = plan.wide_bytes > 0 ? plan.splits * rows : 0;
     const int64_t common_parts = common ? (shared.splits + 1) * rows : 0;
     float *const part_o = take(narrow_parts * d), *const wide_o = take(wide_parts * d), *const shared_o = take(common_parts * d);
     float *const part_ml = take(narrow_parts * 2), *const wide_ml = take(wide_parts * 2), *const shared_ml = take(common_parts * 2);
+    KhJoin *const joins = reinterpret_cast<KhJoin *>(at);
     const int64_t wide_blocks = plan.wide_units * plan.splits, shared_blocks = shared.units * shared.splits;
     const auto u32 = [](int64_t x) { return static_cast<uint32_t>(x); };
     const KhCache cache{static_cast<const char *>(c.k), static_cast<const char *>(c.v), u32(c.k_page_stride), u32(c.k_slot_stride),
                         u32(c.k_head_stride), u32(c.v_page_stride), u32(c.v_slot_stride), u32(c.v_head_stride),
                         static_cast<int32_t>(c.pages), static_cast<int32_t>(c.page_size), static_cast<int32_t>(c.kv_heads),
                         static_cast<int32_t>(d), kh_div_by(u32(c.page_size))};
-    // As even_pages, and four scales from a multiple of four slots on are a word.
-    const auto [near, far] = std::minmax(c.k_slot_stride, c.v_slot_stride);
-    const uintptr_t words = reinterpret_cast<uintptr_t>(c.k_scale) | reinterpret_cast<uintptr_t>(c.v_scale) |
-                            static_cast<uintptr_t>(c.scale_page_stride) | static_cast<uintptr_t>(c.scale_head_stride);
-    const bool even = c.page_size % 16 == 0 && near >= d && far < 1 << 27 && words % 4 == 0;
     // Scores are masked before the factor: it is above 0, which a scale of 0 makes up
     // for with queries of 0. tanh(x / cap) takes its argument in powers of two, twice.
     constexpr float most = std::numeric_limits<float>::max();
@@ -287,15 +325,21 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
                           a.scale < 0.0f ? (two_bytes ? 0x80008000u : 0x80000000u) : 0u, kh_div_by(u32(group)), factor},
                          c.k_scale, c.v_scale, u32(c.scale_page_stride), u32(c.scale_head_stride),
                          common ? static_cast<int32_t>(std::min(a.shared, kCapacity)) : 0, static_cast<int32_t>(shared_blocks),
-                         static_cast<int32_t>(std::max<int64_t>(shared.splits, 1)), static_cast<int32_t>(shared.each), shared_o, shared_ml,
-                         cap_in, std::min(a.cap * 1.44269504088896340736f, most)};
+                         static_cast<int32_t>(std::max<int64_t>(shared.splits, 1)), static_cast<int32_t>(shared.each), shared_o, shared_ml, joins,
+                         static_cast<int32_t>(together), static_cast<int32_t>(ceil_div(c.kv_heads, together)), cap_in, std::min(a.cap * 1.44269504088896340736f, most)};
     const int width = width_of(d);
-    const auto &symbols = wide_blocks + shared_blocks > 0 ? kWide : kAttention;
-    if (int rc = launch(symbols[width][a.dtype], shared_blocks + wide_blocks + plan.groups, 1, 256, p, stream)) return rc;
+    const auto &symbols = wide_blocks + shared_blocks > 0 ? kWide : alone ? kAttention : kOdd;
+    const unsigned threads = alone ? 64u * kWaves[width] : 256u;
+    if (int rc = launch(symbols[width][a.dtype], shared_blocks + wide_blocks + plan.groups, 1, threads, p, stream)) return rc;
     if (joined) {
-      const int64_t narrow_joins = plan.part_bytes > 0 ? plan.groups : 0;
+      const int64_t narrow_joins = plan.part_bytes > 0 ? plan.groups * together : 0;
       const int64_t wide_joins = plan.wide_bytes > 0 ? plan.wide_units * (KH_WIDE_ROWS / KH_TILE_ROWS) : 0;
-      if (int rc = launch(kJoin[width][a.dtype], narrow_joins + wide_joins, 1, 256, p, stream)) return rc;
+      // Few units of many parts: a workgroup to 32 columns. MI355X, one sequence of
+      // 131071 entries (128 parts) 69 us against 82, 64 of 513 to 8192 (two or three)
+      // 112 against 109.
+      const int64_t units = std::min(a.tokens, a.table.seqs) * c.kv_heads;
+      const int64_t columns = plan.groups * together >= 32 * units ? (width == 0 ? 2 : width == 1 ? 4 : 8) : 1;
+      if (int rc = launch(kJoin[width][a.dtype], narrow_joins + wide_joins, columns, 256, p, stream)) return rc;
     }
     if (!common) return 0;
     const int64_t each = 256 / (width == 0 ? 16 : width == 1 ? 32 : 64);
