@@ -253,9 +253,9 @@ inline size_t part_row_bytes(const kh_paged_attention_args &a) { return (2 + sta
 inline int64_t most_groups(const kh_paged_attention_args &a) { return (a.cache.head_dim > 128 ? 1 : 2) * KH_GEMM_CUS; }
 
 // How sequences of few rows are worked on: workgroups on the chip at once, kv heads
-// that each takes.
+// that each takes, blocks of units that are not split.
 struct NarrowForm {
-  int64_t most, together = 1;
+  int64_t most, together = 1, whole = kWholeBlocks;
 };
 
 inline AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t workspace_bytes, const NarrowForm &form) {
@@ -295,7 +295,7 @@ inline AttentionPlan attention_plan(const kh_paged_attention_args &a, size_t wor
   // The kernels count blocks in 32 bits, with what lengths beyond the expected
   // ones may add: the whole row of the table.
   const int64_t most_blocks = units * ceil_div(capacity_of(a.table.width, a.cache.page_size), KH_STRETCH);
-  p.whole = blocks <= kWholeBlocks || p.groups < std::min(units, most) || p.groups < 2 || most_blocks >= 1 << 30;
+  p.whole = blocks <= form.whole || p.groups < std::min(units, most) || p.groups < 2 || most_blocks >= 1 << 30;
   if (p.whole) p.groups = std::min(units, most);
   p.part_bytes = p.whole ? 0 : static_cast<size_t>(p.groups) * per_group;
   return p;

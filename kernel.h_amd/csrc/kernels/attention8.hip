@@ -133,18 +133,25 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) {
   return w & ~((n >> 7) * 0xffu);
 }
 
-// Scores in powers of two, capped: cap_out tanh(y cap_in / (2 log2 e)), by way of
-// t = 2^(y cap_in) as 1 - 2 / (t + 1), off by some 2^-23 of the cap, and up to a
-// quarter of the cap, where that is much, by way of the power series (first term
-// left out 2e-9 of the score).
-__device__ __forceinline__ float capped(float y, const KhAttention8Params &p) {
-  const float x = y * p.cap_in;
-  const float t = exp2_hw(x);
-  float r = fmaf(-2.0f, __builtin_amdgcn_rcpf(t + 1.0f), 1.0f);
-  const float a = x * 0.34657359027997265471f, z = a * a;  // log(2) / 2
-  const float series = a + a * z * (-1.0f / 3 + z * (2.0f / 15 + z * (-17.0f / 315 + z * (62.0f / 2835 + z * (-1382.0f / 155925)))));
-  r = z < 0.0625f ? series : r;
-  return r * p.cap_out;
+// Scores over the cap, capped: tanh(y cap_in / (2 log2 e)), which cap_out takes back to
+// scores in powers of two. By way of t = 2^(y cap_in) it is 1 - 2 / (t + 1), off by
+// some 2^-23 of the cap: of 16-bit rows' weights that is nothing up to a cap of 256
+// (2^-15 of a weight). Past that, and for fp32 rows (near), what lies below a quarter
+// of the cap comes from the power series (first term left out 2e-9 of the score): 16
+// instructions a score instead of 5, of which chunks feel every one.
+template <int N, class X>
+__device__ __forceinline__ void cap(X &y, const KhAttention8Params &p) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float x = y[j] * p.cap_in;
+    float r = fmaf(-2.0f, __builtin_amdgcn_rcpf(exp2_hw(x) + 1.0f), 1.0f);
+    if (p.cap_near) {
+      const float a = x * 0.34657359027997265471f, z = a * a;  // log(2) / 2
+      const float series = a + a * z * (-1.0f / 3 + z * (2.0f / 15 + z * (-17.0f / 315 + z * (62.0f / 2835 + z * (-1382.0f / 155925)))));
+      r = z < 0.0625f ? series : r;
+    }
+    y[j] = r;
+  }
 }
 
 // ---- few rows
@@ -158,45 +165,28 @@ struct Few {
   static constexpr int piece = D / 16, words = D / 64;  // columns of V of a lane
 };
 
-// Where a block's rows lie. EVEN: the 16 entries from a multiple of 16 on lie next
-// to each other in one page; lane n finds 16 entries' page, n % tiles, so that all
-// of the block's are one load, on its way with the rows.
-template <int D, bool EVEN>
+// Where a block's rows lie.
+template <int D>
 struct Stretch {
-  KhSlot found[EVEN ? 1 : Few<D>::tiles], at[Few<D>::tiles];  // of entry 16 t + l % 16; EVEN: at is of entry 16 t
+  KhSlot at[Few<D>::tiles];  // of entry 16 t + l % 16
   uint64_t present;
 };
 
-template <int D, bool EVEN>
-__device__ __forceinline__ void find(Stretch<D, EVEN> &b, const KhAttention8Params &p, const int32_t *table, int key0, int end, int lane) {
-  if constexpr (EVEN) {
-    const int key = key0 + 16 * (lane % Few<D>::tiles), last = (end - 1) & ~15;
-    const uint32_t inside = (uint32_t)(key < last ? key : last);  // < capacity: the page's number is in the row
-    const uint32_t i = __umulhi(inside, p.cache.by_page.mul) >> p.cache.by_page.shift;  // kh_div: pages hold 16 entries at least
-    b.found[0] = KhSlot{table[i], (int)(inside - i * p.cache.by_page.by)};
-  } else {
+template <int D>
+__device__ __forceinline__ void find(Stretch<D> &b, const KhAttention8Params &p, const int32_t *table, int key0, int end, int lane) {
 #pragma unroll
-    for (int t = 0; t < Few<D>::tiles; ++t) b.found[t] = look_up<false>(p, table, key0 + 16 * t + lane % 16, end);
-  }
+  for (int t = 0; t < Few<D>::tiles; ++t) b.at[t] = look_up<false>(p, table, key0 + 16 * t + lane % 16, end);
 }
 
 // Absent rows are read from the cache's first page: kh_cache.h, Block.
-template <int D, bool EVEN>
-__device__ __forceinline__ void settle(Stretch<D, EVEN> &b, const KhAttention8Params &p, int key0, int end, int lane) {
+template <int D>
+__device__ __forceinline__ void settle(Stretch<D> &b, const KhAttention8Params &p, int key0, int end, int lane) {
   b.present = 0;
 #pragma unroll
   for (int t = 0; t < Few<D>::tiles; ++t) {
-    if constexpr (EVEN) {
-      b.at[t] = KhSlot{__builtin_amdgcn_readlane(b.found[0].page, t), __builtin_amdgcn_readlane(b.found[0].slot, t)};
-      const bool paged = (uint32_t)b.at[t].page < (uint32_t)p.cache.pages;
-      const int left = end - key0 - 16 * t;
-      b.present |= (uint64_t)(!paged || left <= 0 ? 0u : left >= 16 ? 0xffffu : (1u << left) - 1) << (16 * t);
-      if (!paged) b.at[t].page = 0;
-    } else {
-      const bool there = key0 + 16 * t + lane % 16 < end && (uint32_t)b.found[t].page < (uint32_t)p.cache.pages;
-      b.present |= (__builtin_amdgcn_ballot_w64(there) & 0xffffu) << (16 * t);
-      b.at[t] = there ? b.found[t] : KhSlot{0, 0};
-    }
+    const bool there = key0 + 16 * t + lane % 16 < end && (uint32_t)b.at[t].page < (uint32_t)p.cache.pages;
+    b.present |= (__builtin_amdgcn_ballot_w64(there) & 0xffffu) << (16 * t);
+    if (!there) b.at[t] = KhSlot{0, 0};
   }
 }
 
@@ -208,32 +198,29 @@ struct RowsOfK {
   uint32_t scale[Few<D>::tiles];
 };
 
-// Of V: D / 16 columns of the lane's entries. Scales: EVEN: of the lane's four
-// entries of each 16, a byte each; else of entry l % 16.
+// Of V: D / 16 columns of the lane's entries, and the scale of entry l % 16.
 template <int D>
 struct RowsOfV {
   uint32_t w[Few<D>::mine][Few<D>::words];
   uint32_t scale[Few<D>::tiles];
 };
 
-template <int D, bool EVEN>
-__device__ __forceinline__ void load_k(RowsOfK<D> &k, const Stretch<D, EVEN> &b, const KhAttention8Params &p, const char *base,
-                                       const uint8_t *scales, int row_bytes, int r, int h) {
+template <int D>
+__device__ __forceinline__ void load_k(RowsOfK<D> &k, const Stretch<D> &b, const KhAttention8Params &p, const char *base,
+                                       const uint8_t *scales, int row_bytes, int h) {
   using F = Few<D>;
 #pragma unroll
   for (int t = 0; t < F::tiles; ++t) {
     const char *row = base + kh_row(b.at[t], p.cache.k_page, p.cache.k_slot);
 #pragma unroll
-    for (int c = 0; c < F::steps; ++c) {
-      const uint32_t off = (EVEN ? (uint32_t)r * p.cache.k_slot : 0u) + within(64 * c + 16 * h, row_bytes);
-      k.w[t][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + off));
-    }
-    k.scale[t] = scales[(uint64_t)(uint32_t)b.at[t].page * p.scale_page + (uint32_t)(b.at[t].slot + (EVEN ? r : 0))];
+    for (int c = 0; c < F::steps; ++c)
+      k.w[t][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + within(64 * c + 16 * h, row_bytes)));
+    k.scale[t] = scales[(uint64_t)(uint32_t)b.at[t].page * p.scale_page + (uint32_t)b.at[t].slot];
   }
 }
 
-template <int D, bool EVEN>
-__device__ __forceinline__ void load_v(RowsOfV<D> &v, const Stretch<D, EVEN> &b, const KhAttention8Params &p, const char *base,
+template <int D>
+__device__ __forceinline__ void load_v(RowsOfV<D> &v, const Stretch<D> &b, const KhAttention8Params &p, const char *base,
                                        const uint8_t *scales, int row_bytes, int r, int h) {
   using F = Few<D>;
 #pragma unroll
@@ -241,13 +228,9 @@ __device__ __forceinline__ void load_v(RowsOfV<D> &v, const Stretch<D, EVEN> &b,
     const uint64_t own = kh_row(b.at[t], p.cache.v_page, p.cache.v_slot);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const char *row = base + own;
-      if constexpr (!EVEN) {
-        // Entry 4 h + i is the one that lane 4 h + i looked up.
-        const uint32_t lo = __shfl((uint32_t)own, 4 * h + i, kWave), hi = __shfl((uint32_t)(own >> 32), 4 * h + i, kWave);
-        row = base + ((uint64_t)hi << 32 | lo);
-      }
-      const char *from = row + ((EVEN ? (uint32_t)(4 * h + i) * p.cache.v_slot : 0u) + within(F::piece * r, row_bytes));
+      // Entry 4 h + i is the one that lane 4 h + i looked up.
+      const uint32_t lo = __shfl((uint32_t)own, 4 * h + i, kWave), hi = __shfl((uint32_t)(own >> 32), 4 * h + i, kWave);
+      const char *from = base + ((uint64_t)hi << 32 | lo) + within(F::piece * r, row_bytes);
       uint32_t(&w)[F::words] = v.w[4 * t + i];
       if constexpr (F::words == 4) {
         const u32x4 g = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from));
@@ -259,26 +242,15 @@ __device__ __forceinline__ void load_v(RowsOfV<D> &v, const Stretch<D, EVEN> &b,
         w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(from));
       }
     }
-    const uint8_t *at = scales + ((uint64_t)(uint32_t)b.at[t].page * p.scale_page + (uint32_t)b.at[t].slot);
-    // Four entries from a multiple of 4 on, of scales that are 4-byte aligned.
-    if constexpr (EVEN)
-      v.scale[t] = *reinterpret_cast<const uint32_t *>(at + 4 * h);
-    else
-      v.scale[t] = *at;
+    v.scale[t] = scales[(uint64_t)(uint32_t)b.at[t].page * p.scale_page + (uint32_t)b.at[t].slot];
   }
 }
 
 // The scales' powers of the lane's entries of 32, half `g` of the block.
-template <int D, bool EVEN>
+template <int D>
 __device__ __forceinline__ void powers_of(float (&power)[8], const RowsOfV<D> &v, int g, int h) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t word = v.scale[2 * g + j / 4];
-    if constexpr (EVEN)
-      power[j] = power_of(word >> 8 * (j % 4) & 0xffu);
-    else
-      power[j] = power_of(__shfl(word, 4 * h + j % 4, kWave));
-  }
+  for (int j = 0; j < 8; ++j) power[j] = power_of(__shfl(v.scale[2 * g + j / 4], 4 * h + j % 4, kWave));
 }
 
 // Writes of results: to out, or where sequences share entries to the parts that
@@ -327,7 +299,7 @@ __device__ __forceinline__ bool told_parts(const KhAttention8Params &p, int bloc
   return true;
 }
 
-template <int D, bool EVEN>
+template <int D>
 __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, float *lds) {
   using F = Few<D>;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -347,7 +319,7 @@ __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, f
   float *ml = lds, *both = lds + kWaves * kRows * 2, *part = both + kRows * 2;
   constexpr int kPitch = D + 4;
   KhUnits units = kh_units_of(p, s);
-  const float factor0 = p.cap_in != 0.0f ? 1.0f : p.scale_log2;
+  const float factor0 = p.cap_in != 0.0f ? p.cap_out : p.scale_log2;
 
   for (int at = start, in = start - before; at < end;) {
     while (kh_passed(in, kh_work(units, p.cache.kv_heads))) {
@@ -408,15 +380,15 @@ __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, f
       constexpr int kStep = kWaves * F::keys;
       RowsOfK<D> k;
       RowsOfV<D> v;
-      Stretch<D, EVEN> now, next;
-      find<D, EVEN>(now, p, table, key0, key_end, lane);
-      find<D, EVEN>(next, p, table, key0 + kStep, key_end, lane);
-      settle<D, EVEN>(now, p, key0, key_end, lane);
-      load_k<D, EVEN>(k, now, p, kbase, kscales, d, r, h);
+      Stretch<D> now, next;
+      find<D>(now, p, table, key0, key_end, lane);
+      find<D>(next, p, table, key0 + kStep, key_end, lane);
+      settle<D>(now, p, key0, key_end, lane);
+      load_k<D>(k, now, p, kbase, kscales, d, h);
       // K goes out before V here as in the loop: the wait for K at its top then
       // leaves V in flight.
       __builtin_amdgcn_sched_barrier(0);
-      load_v<D, EVEN>(v, now, p, vbase, vscales, d, r, h);
+      load_v<D>(v, now, p, vbase, vscales, d, r, h);
       for (; key0 < key_end; key0 += kStep) {
         const uint64_t present = now.present;
         float y[F::mine];
@@ -444,13 +416,12 @@ __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, f
           for (int e = 0; e < 4; ++e) y[4 * t + e] = x[e];
         }
         now = next;
-        settle<D, EVEN>(now, p, key0 + kStep, key_end, lane);
-        load_k<D, EVEN>(k, now, p, kbase, kscales, d, r, h);
-        find<D, EVEN>(next, p, table, key0 + 2 * kStep, key_end, lane);
+        settle<D>(now, p, key0 + kStep, key_end, lane);
+        load_k<D>(k, now, p, kbase, kscales, d, h);
+        find<D>(next, p, table, key0 + 2 * kStep, key_end, lane);
 
         if (p.cap_in != 0.0f) {
-#pragma unroll
-          for (int j = 0; j < F::mine; ++j) y[j] = capped(y[j], p);
+          cap<F::mine>(y, p);
         }
         // Every row sees every entry of the block: no mask.
         const bool whole = present == ~uint64_t(0) >> (64 - F::keys) && key0 + F::keys <= low.end && key0 >= high.first;
@@ -529,7 +500,7 @@ __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, f
           const float eight[8] = {y[8 * g], y[8 * g + 1], y[8 * g + 2], y[8 * g + 3], y[8 * g + 4], y[8 * g + 5], y[8 * g + 6], y[8 * g + 7]};
           in_parts(b, eight, false);
           float power[8];
-          powers_of<D, EVEN>(power, v, g, h);
+          powers_of<D>(power, v, g, h);
 #pragma unroll
           for (int e = 0; e < F::piece; e += 2) {
             uint32_t x[8];  // columns e and e + 1 of the eight entries
@@ -551,7 +522,7 @@ __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, f
             }
           }
         }
-        load_v<D, EVEN>(v, now, p, vbase, vscales, d, r, h);
+        load_v<D>(v, now, p, vbase, vscales, d, r, h);
       }
     }
 
@@ -768,7 +739,7 @@ __device__ __forceinline__ void narrow_even(const KhAttention8Params &p, int blo
   char *own = lds + wave * F::lds;
   float *powers = reinterpret_cast<float *>(own + F::powers_at);
   KhUnits units = kh_units_of(p, s);
-  const float factor0 = p.cap_in != 0.0f ? 1.0f : p.scale_log2;
+  const float factor0 = p.cap_in != 0.0f ? p.cap_out : p.scale_log2;
 
   uint32_t k_off[2][F::loads], v_off[2][F::loads];
 #pragma unroll
@@ -900,8 +871,7 @@ __device__ __forceinline__ void narrow_even(const KhAttention8Params &p, int blo
         send<F>(p, own, then, 0, k_off, kscales, kb, own + F::scales_at + b * 256, lane);
 
         if (p.cap_in != 0.0f) [[unlikely]] {
-#pragma unroll
-          for (int j = 0; j < F::mine; ++j) y[j] = capped(y[j], p);
+          cap<F::mine>(y, p);
         }
         // Every row sees every entry of the block: no mask.
         const bool whole = here == ~uint64_t(0) >> (64 - F::keys) && key0 + F::keys <= low.end && key0 >= high.first;
@@ -1104,7 +1074,7 @@ __device__ __forceinline__ void put(const Tile<D> &g, char *buffer, int d, bool 
     const u32x4 k = real ? g.k[i] : zero;
     u32x4 v = real ? g.v[i] : zero;
     uint8_t mark = there ? kThere : 0;
-    if (mixed) {
+    if (mixed) [[unlikely]] {
       const bool odd = (nan_bytes(v.x) | nan_bytes(v.y) | nan_bytes(v.z) | nan_bytes(v.w)) != 0;
       const uint64_t odds = __builtin_amdgcn_ballot_w64(odd);
       if (odds != 0) {
@@ -1228,7 +1198,7 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
 
   const int32_t *table = p.table.pages + seq * p.table.row_stride;
   const char *vbase = p.cache.v + (uint64_t)head * p.cache.v_head;
-  const float factor0 = p.cap_in != 0.0f ? 1.0f : p.scale_log2;
+  const float factor0 = p.cap_in != 0.0f ? p.cap_out : p.scale_log2;
 
   u32x4 q[W::steps][kParts];
   const row_t *qp = static_cast<const row_t *>(p.q) + ((int64_t)token * p.q_stride + (int64_t)hq * d);
@@ -1264,6 +1234,7 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
         f32x16 x[W::tiles];
 #pragma unroll
         for (int kt = 0; kt < W::tiles; ++kt) x[kt] = f32x16{};
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int c = 0; c < W::steps; ++c)
 #pragma unroll
@@ -1273,17 +1244,16 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
             for (int n = 0; n < kParts; ++n) x[kt] = mma32(a, q[c][n], x[kt]);
           }
         if constexpr (kParts == 1) read_ahead<W::steps * W::tiles, W::steps * W::tiles, 1, 6>();
+        __builtin_amdgcn_s_setprio(0);
         const uint32_t mark = (uint8_t)buffer[W::marks_at + lane];
         const uint64_t present = __builtin_amdgcn_ballot_w64((mark & kThere) != 0);
         const uint64_t odds = mixed(key0) ? __builtin_amdgcn_ballot_w64((mark & kOdd) != 0) : 0;
-        if (p.cap_in != 0.0f) {
+        if (p.cap_in != 0.0f) [[unlikely]] {
 #pragma unroll
-          for (int kt = 0; kt < W::tiles; ++kt)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[kt][j] = capped(x[kt][j], p);
+          for (int kt = 0; kt < W::tiles; ++kt) cap<16>(x[kt], p);
         }
         const bool whole = present == ~uint64_t(0) && key0 + W::keys <= low.end && key0 >= high.first;
-        if (!whole) {
+        if (!whole) [[unlikely]] {
           const uint64_t sees = mine ? seen_of(seen, key0) & present : 0;
 #pragma unroll
           for (int kt = 0; kt < W::tiles; ++kt) {
@@ -1298,7 +1268,7 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
 #pragma unroll
           for (int j = 0; j < 16; ++j) top = fmaxf(top, x[kt][j]);
         top = fmaxf(m, over_halves(top, true) * factor0);
-        if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+        if (__builtin_amdgcn_ballot_w64(top > m) != 0) [[unlikely]] {
           const float fade = exp2_hw(m - top);
           m = top;
           l *= fade;
@@ -1307,7 +1277,7 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
         }
         const bool far = coarse(m);
         const float factor = far ? 1.0f : factor0, shift = far ? 0.0f : -m;
-        if (far) {
+        if (far) [[unlikely]] {
 #pragma unroll
           for (int kt = 0; kt < W::tiles; ++kt) less<16>(x[kt], factor0, m);
         }
@@ -1321,6 +1291,7 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
           }
         l += sum;
         // As in narrow(): what was kept out of the products.
+        if (odds != 0) [[unlikely]]
         for (uint64_t left = odds; left != 0; left &= left - 1) {
           const int key = key0 + __builtin_ctzll(left);
           const KhSlot at = kh_slot(table, p.table.width, p.cache.pages, p.cache.by_page, (uint32_t)key);
@@ -1340,6 +1311,7 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
               }
           }
         }
+        __builtin_amdgcn_s_setprio(1);
         // Operands of V are read a step ahead of their products.
         constexpr int kAll = W::tiles * 2;
         u32x4 a[2][W::dts];
@@ -1362,6 +1334,7 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
 #pragma unroll
             for (int i = 0; i < kParts; ++i) o[dt] = mma32(a[n % 2][dt], b[i], o[dt]);
         }
+        __builtin_amdgcn_s_setprio(0);
       }
     }
   }
@@ -1387,38 +1360,46 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
     }
 }
 
-// Joins what the shared entries' parts and the sequences' own entries gave each row.
+// Joins what the shared entries' parts and the sequences' own entries gave each row:
+// D / 4 lanes to a row, four columns each. Its statistics come a part to a lane, and
+// with them the first rows.
 template <int D>
 __device__ __forceinline__ void combine(const KhAttention8Params &p) {
-  constexpr int kLanes = D / 4;
-  const int d = p.cache.head_dim, col = threadIdx.x % kLanes * 4, count = p.shared_splits + 1;
+  constexpr int kLanes = D / 4, kAhead = 16;
+  const int d = p.cache.head_dim, lane = threadIdx.x % kLanes, col = lane * 4, count = p.shared_splits + 1;
   const int64_t rows = (int64_t)p.tokens * p.q_heads;
-  const int64_t row = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  if (row >= rows || col >= d) return;
-  const float *ml = p.shared_ml + 2 * row;
-  if (p.shared == 0 || ml[1] < 0.0f) return;  // everything is done; no sequence's
-  float top = kSeed;
-  for (int k = 0; k < count; ++k) top = fmaxf(top, ml[2 * (int64_t)k * rows]);
-  float total = 0.0f;
+  const int64_t at = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const int64_t row = at < rows ? at : rows - 1;
+  const float *ml = p.shared_ml + 2 * row, *from = p.shared_o + row * d + (col < d ? col : 0);
+  f32x4 x[kAhead];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) x[j] = *reinterpret_cast<const f32x4 *>(from + (int64_t)(k0 + j < count ? k0 + j : count - 1) * rows * d);
+  };
+  fetch(0);
+  const bool nobodys = ml[1] < 0.0f;
+  float top = kSeed, total = 0.0f;
+  for (int k = lane; k < count; k += kLanes) top = fmaxf(top, ml[2 * (int64_t)k * rows]);
+#pragma unroll
+  for (int n = 1; n < kLanes; n *= 2) top = fmaxf(top, __shfl_xor(top, n, kWave));
   f32x4 o = {0, 0, 0, 0};
-  constexpr int kAhead = 8;
-  for (int k0 = 0; k0 < count; k0 += kAhead) {
-    f32x4 x[kAhead];
-    float w[kAhead], l[kAhead];
+  for (int k0 = 0; k0 < count; k0 += kLanes) {
+    const int mine = k0 + lane < count ? k0 + lane : count - 1;
+    const float w = k0 + lane < count ? exp2_hw(ml[2 * (int64_t)mine * rows] - top) : 0.0f;
+    total += ml[2 * (int64_t)mine * rows + 1] * w;
+    for (int k1 = k0; k1 < count && k1 < k0 + kLanes; k1 += kAhead) {
+      if (k1 != 0) fetch(k1);
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int64_t at = (int64_t)(k0 + j < count ? k0 + j : count - 1) * rows;
-      x[j] = *reinterpret_cast<const f32x4 *>(p.shared_o + (at + row) * d + col);
-      w[j] = ml[2 * at], l[j] = ml[2 * at + 1];
-    }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (k0 + j < count) {
-        const float f = exp2_hw(w[j] - top);
-        total += l[j] * f;
-        o += x[j] * f;
+      for (int j = 0; j < kAhead; ++j) {
+        const float f = __shfl(w, (int)(threadIdx.x % kWave / kLanes * kLanes) + (k1 - k0 + j) % kLanes, kWave);
+        if (k1 + j < count) o += x[j] * f;
       }
+    }
   }
+#pragma unroll
+  for (int n = 1; n < kLanes; n *= 2) total += __shfl_xor(total, n, kWave);
+  // Every lane takes part in the exchanges above.
+  if (p.shared == 0 || at >= rows || nobodys || col >= d) return;
   const int token = (int)(row / p.q_heads), hq = (int)(row - (int64_t)token * p.q_heads);
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
@@ -1448,36 +1429,34 @@ __device__ __forceinline__ void settle_shared(KhAttention8Params &p) {
     __shared__ __attribute__((aligned(16))) char lds[WAVES * Ring<D, TILES>::lds];                                   \
     narrow_even<D, TILES, WAVES>(p, (int)blockIdx.x, lds);                                                           \
   }
-#ifndef V64
-#define V64 2
-#endif
-KH_ATTENTION8(64, V64, 4, 2)
+KH_ATTENTION8(64, 2, 4, 2)
 KH_ATTENTION8(128, 2, 4, 2)
 KH_ATTENTION8(256, 2, 2, 1)
 #define KH_ATTENTION8_ODD(D, PER_CU)                                                                               \
   extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED8(attention8_odd_##D)(KhAttention8Params p) { \
     __shared__ __attribute__((aligned(16))) float lds[kWaves * kRows * 2 + kRows * 2 + kWaves * kRows * (D + 4)]; \
-    narrow<D, false>(p, (int)blockIdx.x, lds);                                                                    \
+    narrow<D>(p, (int)blockIdx.x, lds);                                                                    \
   }
 KH_ATTENTION8_ODD(64, 2)
 KH_ATTENTION8_ODD(128, 2)
 KH_ATTENTION8_ODD(256, 1)
 // Steps with sequences of many rows or shared entries: their workgroups first.
-#define KH_ATTENTION8_WIDE(D, PER_CU)                                                                               \
+#define KH_ATTENTION8_WIDE(D, TILES, PER_CU)                                                                       \
   extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED8(attention8_wide_##D)(KhAttention8Params p) { \
-    __shared__ __attribute__((aligned(16))) char lds[Many<D>::lds];                                                \
+    constexpr int kFew = kWaves * Ring<D, TILES>::lds;                                                             \
+    __shared__ __attribute__((aligned(16))) char lds[Many<D>::lds > kFew ? Many<D>::lds : kFew];                   \
     settle_shared(p);                                                                                              \
     const int block = (int)blockIdx.x, wide_end = p.shared_blocks + p.wide_blocks;                                 \
     if (block < wide_end)                                                                                          \
       wide<D>(p, block < p.shared_blocks ? block : block - p.shared_blocks, block < p.shared_blocks, lds);         \
     else if (p.even)                                                                                               \
-      narrow<D, true>(p, block - wide_end, reinterpret_cast<float *>(lds));                                        \
+      narrow_even<D, TILES, kWaves>(p, block - wide_end, lds);                                                     \
     else                                                                                                           \
-      narrow<D, false>(p, block - wide_end, reinterpret_cast<float *>(lds));                                       \
+      narrow<D>(p, block - wide_end, reinterpret_cast<float *>(lds));                                              \
   }
-KH_ATTENTION8_WIDE(64, 2)
-KH_ATTENTION8_WIDE(128, 2)
-KH_ATTENTION8_WIDE(256, 1)
+KH_ATTENTION8_WIDE(64, 2, 2)
+KH_ATTENTION8_WIDE(128, 2, 2)
+KH_ATTENTION8_WIDE(256, 2, 1)
 #define KH_ATTENTION8_JOIN(D)                                                                                   \
   extern "C" __global__ void __launch_bounds__(256) KH_TYPED8(attention8_join_##D)(KhAttention8Params p) {      \
     __shared__ float lds[kJoinParts * kRows * 2];                                                               \

@@ -108,11 +108,15 @@ int64_t most_together(const kh_paged_attention8_args &a) {
   return std::min<int64_t>(c.kv_heads, c.head_dim <= 64 ? 4 : c.head_dim <= 128 ? 2 : 1);
 }
 
+// Beside entries that sequences share, whose units take some 25 us, units of up to
+// this many blocks are not split: a join is another launch.
+constexpr int64_t kWholeShared = 8;
+
 // Fewer where there would not be a block of entries for every workgroup.
-int64_t heads_together(const kh_paged_attention8_args &a) {
+int64_t heads_together(const kh_paged_attention8_args &a, int64_t behind) {
   const kh_paged_cache8 &c = a.cache;
   const int64_t units = std::min(a.tokens, a.table.seqs) + a.tokens * (a.q_heads / c.kv_heads) / KH_TILE_ROWS;
-  const int64_t blocks = ceil_div(seen_len(as_plain(a, 0)), KH_STRETCH);
+  const int64_t blocks = ceil_div(seen_len(as_plain(a, behind)), KH_STRETCH);
   int64_t n = most_together(a);
   while (n > 1 && units * ceil_div(c.kv_heads, n) * blocks < 2 * KH_GEMM_CUS) n = (n + 1) / 2;
   return n;
@@ -289,13 +293,15 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
     const kh_paged_attention_args plain = as_plain(a, common ? a.shared : 0);
     const int64_t group = a.q_heads / c.kv_heads, rows = a.tokens * a.q_heads, d = c.head_dim;
     const bool even = even_pages8(a);
-    // Straight to LDS, two workgroups fill a CU's.
-    const bool alone = even && !common && kh_narrow_only(a.tokens, a.table.seqs, group, a.max_new, narrow_rows_of(KHRT_BF16), 256);
-    const int64_t together = alone ? heads_together(a) : 1;
     // What tells who joins which parts comes last.
     size_t left = workspace_bytes - shared.bytes;
     left -= std::min(left, kJoinBytes);
-    const AttentionPlan plan = attention_plan(plain, left, {alone ? 2 * KH_GEMM_CUS : most_groups(plain), together});
+    // Straight to LDS, two workgroups fill a CU's (rows past 128 elements beside wide
+    // ones: one).
+    const bool narrow_only = kh_narrow_only(a.tokens, a.table.seqs, group, a.max_new, narrow_rows_of(KHRT_BF16), 256);
+    const bool alone = even && !common && narrow_only;
+    const int64_t together = even ? heads_together(a, common ? a.shared : 0) : 1;
+    const AttentionPlan plan = attention_plan(plain, left, {alone ? 2 * KH_GEMM_CUS : most_groups(plain), together, common ? kWholeShared : kWholeBlocks});
     const bool joined = plan.part_bytes + plan.wide_bytes > 0;
     // All rows of parts come first, 16 bytes at a time, then their statistics.
     float *at = static_cast<float *>(workspace);
@@ -326,7 +332,7 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
                          c.k_scale, c.v_scale, u32(c.scale_page_stride), u32(c.scale_head_stride),
                          common ? static_cast<int32_t>(std::min(a.shared, kCapacity)) : 0, static_cast<int32_t>(shared_blocks),
                          static_cast<int32_t>(std::max<int64_t>(shared.splits, 1)), static_cast<int32_t>(shared.each), shared_o, shared_ml, joins,
-                         static_cast<int32_t>(together), static_cast<int32_t>(ceil_div(c.kv_heads, together)), cap_in, std::min(a.cap * 1.44269504088896340736f, most)};
+                         static_cast<int32_t>(together), static_cast<int32_t>(ceil_div(c.kv_heads, together)), cap_in, std::min(a.cap * 1.44269504088896340736f, most), a.dtype == KHRT_F32 || a.cap > 256.0f};
     const int width = width_of(d);
     const auto &symbols = wide_blocks + shared_blocks > 0 ? kWide : alone ? kAttention : kOdd;
     const unsigned threads = alone ? 64u * kWaves[width] : 256u;
