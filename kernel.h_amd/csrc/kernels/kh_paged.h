@@ -281,6 +281,7 @@ struct KhRope8Params : KhRopeParams {
   const int32_t *pair_axis;  // may be null: axis 0
   int64_t axis_stride, scale_page, scale_head;
   int32_t axes;
+  KhDiv by_parts, by_page;
 };
 
 // paged_attention.hip
