@@ -12,17 +12,23 @@
 // of the matrix units, and 8 bits times 8 bits would need K and V's other operand
 // in e4m3, 4 bits of it.
 //
-// Few rows to a sequence (narrow), per wave: 16 rows against blocks of 64 entries
-// (rows past 128 elements: 32), in shares of the step as in paged_attention.hip.
-//   S^T = K Q^T   A = 16 bytes of a row of K, two steps' operands; the result's
-//                 lane l holds row l % 16 and entries 4 (l / 16) + i of each 16.
-//   O^T += V^T P^T  B = those; lane l's entries are the ones whose rows of V it
-//                 loads, D / 16 columns at (l % 16) D / 16.
-// Bound by reading K and V.
+// Few rows to a sequence: 16 rows of a wave against blocks of 64 entries (rows past
+// 128 elements: 32), in shares of the step as in paged_attention.hip.
+//   S^T = K Q^T     the result's lane l holds row l % 16 and entries 4 (l / 16) + i
+//                   of each 16: a row's softmax crosses lanes twice.
+//   O^T += V^T P^T  P as the lanes hold it, in bf16.
+// In two forms: narrow_even() for pages of whole sixteens (K and V straight to LDS),
+// narrow() for others (K and V in registers). Bound by reading K and V: MI355X, bf16,
+// 8 kv heads of 128, 64 sequences of 513 to 8192 entries 110 us, 5.2 TB/s, with
+// pages of 24 slots 138; one of 131071 69 us, 3.9 TB/s with the launch of the join
+// and both kernels' ends; four of 1024, 16 heads of 64 in fp32, 14 us, of which the
+// two launches are ten.
 //
 // Many rows (wide): 128 rows of a workgroup against tiles of 64 entries, which go
-// to LDS as bf16: each byte is converted once for 128 rows. Bound by the matrix
-// units and the vector units' softmax in turn.
+// to LDS as bf16: each byte is converted once for 128 rows. Bound by what the waves
+// issue, the softmax's and the conversions' instructions (54% of the time) and the
+// matrix units' (32%) in turn: a chunk of 2048 at 8192 entries, 32 heads on 8 of
+// 128, bf16, 295 us, 820 TFLOP/s.
 //
 // Entries that all sequences share are worked on by wide units whose rows are all
 // tokens of the step; their parts and the sequences' own are joined row by row.
@@ -754,7 +760,8 @@ __device__ __forceinline__ void narrow_even(const KhAttention8Params &p, int blo
 
   // Of two workgroups on a CU the older one's waves go first, and the other one would
   // end alone, some 15% later. So the second goes first for half of its share, the
-  // older one after that (64 sequences of 513 to 8192 entries: PRIOTXT).
+  // older one after that (64 sequences of 513 to 8192 entries, 122 us without, 114
+  // with).
   const int second = block >= shares.groups / 2 && shares.groups > KH_CUS;
   int first_half = second ? (end - start) * (KH_STRETCH / 2) : 0;  // entries until then
   if (second) __builtin_amdgcn_s_setprio(1);
@@ -1440,7 +1447,9 @@ KH_ATTENTION8(256, 2, 2, 1)
 KH_ATTENTION8_ODD(64, 2)
 KH_ATTENTION8_ODD(128, 2)
 KH_ATTENTION8_ODD(256, 1)
-// Steps with sequences of many rows or shared entries: their workgroups first.
+// Steps with sequences of many rows or shared entries: their workgroups first. fp32
+// rows of 128, three parts of each, leave registers for one workgroup to a CU: two
+// chunks of 1024 at 4096 entries, 16 heads on 4, 224 us; for two, which spill, 247.
 #define KH_ATTENTION8_WIDE(D, TILES, PER_CU)                                                                       \
   extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED8(attention8_wide_##D)(KhAttention8Params p) { \
     constexpr int kFew = kWaves * Ring<D, TILES>::lds;                                                             \
@@ -1455,7 +1464,7 @@ KH_ATTENTION8_ODD(256, 1)
       narrow<D>(p, block - wide_end, reinterpret_cast<float *>(lds));                                              \
   }
 KH_ATTENTION8_WIDE(64, 2, 2)
-KH_ATTENTION8_WIDE(128, 2, 2)
+KH_ATTENTION8_WIDE(128, 2, kParts == 3 ? 1 : 2)
 KH_ATTENTION8_WIDE(256, 2, 1)
 #define KH_ATTENTION8_JOIN(D)                                                                                   \
   extern "C" __global__ void __launch_bounds__(256) KH_TYPED8(attention8_join_##D)(KhAttention8Params p) {      \
