@@ -108,6 +108,14 @@ int64_t most_together(const kh_paged_attention8_args &a) {
   return std::min<int64_t>(c.kv_heads, c.head_dim <= 64 ? 4 : c.head_dim <= 128 ? 2 : 1);
 }
 
+// Units of up to this many blocks are not split by workgroups of four waves that have
+// pages of whole sixteens: shares that end anywhere change units, and a join is
+// another launch. MI355X, bf16, 32 heads on 8 of 128, split and whole: 16 x 700
+// entries 20.2 us / 15.6, 128 x 10 to 880 45 / 35, 32 x 100 to 880 24.7 / 25.4; of one
+// more block, 8 x 1024, 16.5 / 18.0. Workgroups of two waves: 8 x 850, 8 heads of 256,
+// 27 / 37.
+constexpr int64_t kWholeEven = 7;
+
 // Beside entries that sequences share, whose units take some 25 us, units of up to
 // this many blocks are not split: a join is another launch.
 constexpr int64_t kWholeShared = 8;
@@ -302,7 +310,7 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
     const bool narrow_only = kh_narrow_only(a.tokens, a.table.seqs, group, a.max_new, narrow_rows_of(KHRT_BF16), 256);
     const bool alone = even && !common && narrow_only;
     const int64_t together = even ? heads_together(a, common ? a.shared : 0) : 1;
-    const AttentionPlan plan = attention_plan(plain, left, {alone ? 2 * KH_GEMM_CUS : most_groups(plain), together, common ? kWholeShared : kWholeBlocks});
+    const AttentionPlan plan = attention_plan(plain, left, {alone ? 2 * KH_GEMM_CUS : most_groups(plain), together, common ? kWholeShared : alone && d <= 128 ? kWholeEven : kWholeBlocks});
     const bool joined = plan.part_bytes + plan.wide_bytes > 0;
     // All rows of parts come first, 16 bytes at a time, then their statistics.
     float *at = static_cast<float *>(workspace);
