@@ -282,6 +282,72 @@ def test_infinite_scores_and_queries(dev, dtype, q):
     assert np.isfinite(out).all() and np.isfinite(lse).all()
 
 
+def laid_out(s, k_strides, v_strides, offsets):
+    """The step's cache with rows at these (page, slot, head) strides, K's and V's in
+    one buffer from these offsets on, and NaN between them."""
+    size = max(o + (s.pages - 1) * st[0] + (s.page_size - 1) * st[1] + (s.hk - 1) * st[2] + s.d
+               for o, st in zip(offsets, (k_strides, v_strides)))
+    both = np.full(-(-size // 16) * 16, 0x7F, np.uint8)
+    for o, st, codes in zip(offsets, (k_strides, v_strides), (s.k_codes, s.v_codes)):
+        at = np.add.outer(np.add.outer(np.arange(s.pages) * st[0], np.arange(s.page_size) * st[1]), np.arange(s.hk) * st[2])
+        both[o + at[..., None] + np.arange(s.d)] = codes
+    data = kh.Buffer.from_array(both)
+    scales = [kh.Buffer.from_array(np.ascontiguousarray(x.transpose(0, 2, 1))) for x in (s.k_scales, s.v_scales)]
+    s.cache8_on_gpu = lambda: (kh.PagedCache8(
+        k=data.ptr + offsets[0], v=data.ptr + offsets[1], k_scale=scales[0].ptr, v_scale=scales[1].ptr, k_page_stride=k_strides[0],
+        k_slot_stride=k_strides[1], k_head_stride=k_strides[2], v_page_stride=v_strides[0], v_slot_stride=v_strides[1],
+        v_head_stride=v_strides[2], scale_page_stride=s.hk * s.page_size, scale_head_stride=s.page_size, pages=s.pages,
+        page_size=s.page_size, kv_heads=s.hk, head_dim=s.d), (data, scales))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("layout", ["k and v in turn", "short heads first", "padded heads", "one head for all", "k by heads, v by slots"])
+@pytest.mark.parametrize("q", [1, 40])
+def test_heads_at_other_distances(dev, dtype, layout, q):
+    """Heads of an entry that lie near each other, but not end to end."""
+    hk, d = {"k and v in turn": (4, 64), "short heads first": (4, 16), "padded heads": (3, 64), "one head for all": (4, 64),
+             "k by heads, v by slots": (2, 16)}[layout]
+    s = Step8(dtype, [q] * 40, [500 + 11 * i for i in range(40)], 2 * hk, hk, d, page_size=16, seed=d + hk)
+    ps = 16
+    slots = (hk * ps * d, hk * d, d)
+    k, v, offsets = slots, slots, (0, -(-s.pages * hk * ps * d // 16) * 16)
+    if layout == "k and v in turn":
+        k = v = (2 * hk * ps * d, 2 * hk * d, 2 * d)
+        offsets = (0, d)
+    elif layout == "short heads first":
+        k = v = (hk * ps * d, d, ps * d)
+    elif layout == "padded heads":
+        k = v = (hk * ps * (d + 16), hk * (d + 16), d + 16)
+        offsets = (0, s.pages * k[0])
+    elif layout == "one head for all":
+        k = v = (ps * d, d, 0)
+        for name in "kv":
+            codes, scales = getattr(s, name + "_codes"), getattr(s, name + "_scales")
+            codes[:] = codes[:, :, :1]
+            s.put(name, codes, scales)
+        offsets = (0, s.pages * ps * d)
+    else:
+        k = (hk * ps * d, d, ps * d)
+    laid_out(s, k, v, offsets)
+    check_attention(s)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("q,page_size", [(1, 16), (1, 7), (40, 16)])
+def test_rows_of_v_of_any_size(dev, dtype, q, page_size):
+    """Sequences whose rows of V are near the largest or the smallest that a row can be,
+    each within a factor of 2^6."""
+    lens = [900, 300, 70, 33]
+    s = Step8(dtype, [q if q == 1 else min(q, n) for n in lens], lens, 4, 2, 64, page_size=page_size, seed=q + page_size)
+    codes, scales = s.v_codes, s.v_scales
+    codes[(codes & 0x7F) == 0x7F] = 0
+    for i, byte in enumerate((230, 127, 40, 24)):
+        pages = s.table[i][:-(-lens[i] // page_size)]
+        scales[pages] = byte + s.g.integers(0, 6, scales[pages].shape)
+    s.put("v", codes, scales)
+    check_attention(s)
+
+
 # ---------------------------------------------------------------- caches past 4 GB
 
 FAR = 1 << 27  # from page to page
