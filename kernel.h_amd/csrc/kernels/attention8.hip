@@ -28,7 +28,7 @@
 // to LDS as bf16: each byte is converted once for 128 rows. Bound by what the waves
 // issue, the softmax's and the conversions' instructions (54% of the time) and the
 // matrix units' (32%) in turn: a chunk of 2048 at 8192 entries, 32 heads on 8 of
-// 128, bf16, 295 us, 820 TFLOP/s.
+// 128, bf16, 288 us, 840 TFLOP/s.
 //
 // Entries that all sequences share are worked on by wide units whose rows are all
 // tokens of the step; their parts and the sequences' own are joined row by row.
@@ -1019,6 +1019,11 @@ struct Many {
   static constexpr int rows = 256 / pieces, passes = keys / rows;  // rows that the workgroup brings at a time
   static constexpr int v_at = keys * bytes, marks_at = 2 * v_at, buffer = marks_at + keys;
   static constexpr int lds = 2 * buffer;
+  // The columns of piece n of eight of a row in LDS. A thread brings sixteen: the first
+  // eight of all threads come before the second ones, so that neighbours write to
+  // neighbouring banks (a chunk of 2048 at 8192 entries 288 us, in the columns' own
+  // order 295).
+  static __device__ constexpr int column(int n) { return n < pieces ? 16 * n : 16 * (n - pieces) + 8; }
 };
 static_assert(Rows<64>::tile == 64 && Rows<128>::tile == 64 && Rows<256>::tile == 64);
 
@@ -1066,21 +1071,21 @@ __device__ __forceinline__ void widen16(u32x4 &a, u32x4 &b, u32x4 w, float power
   b = u32x4{widen<false>(w.z, power), widen<true>(w.z, power), widen<false>(w.w, power), widen<true>(w.w, power)};
 }
 
-// From registers to LDS as bf16, zeros for absent rows and columns past the row's
-// end. Where rows of the unit see different entries of the tile (mixed), NaN in V
-// become zeros and their row is marked.
+// From registers to LDS as bf16. Columns past the row's end are copies of its first:
+// q has zeros there, and nobody takes them from O. Absent rows of K have no score; of V
+// they are zeros. Where rows of the unit see different entries of the tile (mixed), NaN
+// in V become zeros and their row is marked.
 template <int D>
-__device__ __forceinline__ void put(const Tile<D> &g, char *buffer, int d, bool mixed, int tid) {
+__device__ __forceinline__ void put(const Tile<D> &g, char *buffer, bool mixed, int tid) {
   using W = Many<D>;
   const int own = tid / W::pieces, piece = tid % W::pieces, lane = lane_id();
 #pragma unroll
   for (int i = 0; i < W::passes; ++i) {
     const int row = i * W::rows + own;
-    const bool there = g.at[i].page >= 0, real = there && 16 * piece < d;
-    const u32x4 zero = {0, 0, 0, 0};
-    const u32x4 k = real ? g.k[i] : zero;
-    u32x4 v = real ? g.v[i] : zero;
+    const bool there = g.at[i].page >= 0;
+    u32x4 v = g.v[i];
     uint8_t mark = there ? kThere : 0;
+    if (__builtin_amdgcn_ballot_w64(!there) != 0) [[unlikely]] v = there ? v : u32x4{0, 0, 0, 0};
     if (mixed) [[unlikely]] {
       const bool odd = (nan_bytes(v.x) | nan_bytes(v.y) | nan_bytes(v.z) | nan_bytes(v.w)) != 0;
       const uint64_t odds = __builtin_amdgcn_ballot_w64(odd);
@@ -1090,14 +1095,14 @@ __device__ __forceinline__ void put(const Tile<D> &g, char *buffer, int d, bool 
       }
     }
     u32x4 a, b;
-    widen16(a, b, k, power_of(g.k_scale[i]));
+    widen16(a, b, g.k[i], power_of(g.k_scale[i]));
     char *to = buffer + row * W::bytes;
-    *reinterpret_cast<u32x4 *>(to + 16 * (2 * piece ^ k_turn<D>(row))) = a;
-    *reinterpret_cast<u32x4 *>(to + 16 * (2 * piece + 1 ^ k_turn<D>(row))) = b;
+    *reinterpret_cast<u32x4 *>(to + 16 * (piece ^ k_turn<D>(row))) = a;
+    *reinterpret_cast<u32x4 *>(to + 16 * (W::pieces + piece ^ k_turn<D>(row))) = b;
     widen16(a, b, v, power_of(g.v_scale[i]));
     to += W::v_at;
-    *reinterpret_cast<u32x4 *>(to + 16 * (2 * piece ^ v_turn<D>(row))) = a;
-    *reinterpret_cast<u32x4 *>(to + 16 * (2 * piece + 1 ^ v_turn<D>(row))) = b;
+    *reinterpret_cast<u32x4 *>(to + 16 * (piece ^ v_turn<D>(row))) = a;
+    *reinterpret_cast<u32x4 *>(to + 16 * (W::pieces + piece ^ v_turn<D>(row))) = b;
     if (piece == 0) buffer[W::marks_at + row] = (char)mark;
   }
 }
@@ -1211,7 +1216,7 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
   const row_t *qp = static_cast<const row_t *>(p.q) + ((int64_t)token * p.q_stride + (int64_t)hq * d);
 #pragma unroll
   for (int c = 0; c < W::steps; ++c) {
-    const int col = 16 * c + 8 * h;
+    const int col = W::column(2 * c) + 16 * h;
     load_q(q[c], qp + within(col, d), mine && col < d, p);
   }
   float m = mine ? kSeed : 0.0f, l = 0.0f;
@@ -1229,7 +1234,7 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
     int cur = 0;
     for (int key0 = part.first; key0 < part.end; key0 += W::keys, cur ^= 1) {
       char *buffer = lds + cur * W::buffer;
-      put<D>(g, buffer, d, mixed(key0), tid);
+      put<D>(g, buffer, mixed(key0), tid);
       // The page numbers of the tile after the next go out behind its loads.
       fetch<D>(g, p, head, key0 + W::keys, part.end, tid);
       seek<D>(g, p, table, key0 + 2 * W::keys, part.end, tid);
@@ -1309,7 +1314,7 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
             for (int dt = 0; dt < W::dts; ++dt)
 #pragma unroll
               for (int j = 0; j < 16; j += 4) {
-                const int col = 32 * dt + 2 * j + 4 * h1;
+                const int col = W::column(4 * dt + j / 4) + 4 * h1;
                 if (col >= d) continue;
                 const uint32_t odd = nan_bytes(*reinterpret_cast<const uint32_t *>(row + col));
 #pragma unroll
@@ -1357,7 +1362,7 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
   for (int dt = 0; dt < W::dts; ++dt)
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
-      const int col = 32 * dt + 2 * j + 4 * h;
+      const int col = W::column(4 * dt + j / 4) + 4 * h;
       if (col >= d) continue;
       const f32x4 y = {o[dt][j], o[dt][j + 1], o[dt][j + 2], o[dt][j + 3]};
       if (alone)
