@@ -20,7 +20,7 @@
 // In two forms: narrow_even() for pages of whole sixteens (K and V straight to LDS),
 // narrow() for others (K and V in registers). Bound by reading K and V: MI355X, bf16,
 // 8 kv heads of 128, 64 sequences of 513 to 8192 entries 110 us, 5.2 TB/s, with
-// pages of 24 slots 138; one of 131071 69 us, 3.9 TB/s with the launch of the join
+// pages of 24 slots 138; one of 131071 60-67 us, 4.0-4.5 TB/s with the launch of the join
 // and both kernels' ends; four of 1024, 16 heads of 64 in fp32, 14 us, of which the
 // two launches are ten.
 //
@@ -1419,6 +1419,128 @@ __device__ __forceinline__ void combine(const KhAttention8Params &p) {
   if (col == 0 && p.lse != nullptr) p.lse[row] = lse_of(top, total, 0.0f);
 }
 
+constexpr int kJoinMost = 128;
+
+struct JoinLds {
+  float weights[kJoinMost * kRows];  // of a part's row against the row's maximum so far
+  float tops[kWaves * kRows], fades[kRows], totals[kWaves * kRows];
+  float sums[256 * 4];
+};
+
+// Joins the parts of 16 rows. They were written through other L2s, so that each round
+// of loads takes its time: the statistics of AT parts and AHEAD of its rows come to a
+// thread in one. Statistics lie a part's row to a lane, which works out what the row
+// counts for once for all columns. A thread has 4 columns of a row, and where that
+// leaves threads over (few rows), only each second to eighth part of it.
+template <int D, int AT, int AHEAD>
+__device__ __forceinline__ void join_rows(const KhAttention8Params &p, JoinLds &lds, const KhSeq &s, const Parts &parts) {
+  constexpr int kMine = AT * kRows / 256;
+  const int shift = __builtin_ctz(D / 4) - __builtin_ctz(gridDim.y), cols = 1 << shift;
+  const int tid = threadIdx.x, lane = lane_id(), wave = tid / kWave, d = p.cache.head_dim;
+  auto base = [&](int k) { return k == 0 ? parts.first : parts.others + (k - 1) * parts.step; };
+  auto place_of = [&](int row) {
+    if (!parts.wide) return (int64_t)row;
+    const int R = parts.R0 + row, i = (int)kh_div(R, p.by_group);
+    return (int64_t)(s.start + i) * p.q_heads + parts.head * p.group + R - i * p.group;
+  };
+  // Rows rounded up to a power of two, times columns: items; threads that share one.
+  const int rows2 = parts.rows <= 1 ? 1 : parts.rows <= 2 ? 2 : parts.rows <= 4 ? 4 : parts.rows <= 8 ? 8 : 16;
+  const int items = rows2 * cols, shares = items >= 256 ? 1 : 256 / items < 8 ? 256 / items : 8;
+  const int own = tid % kRows;  // whose statistics the thread has, of parts tid / 16, ..
+  const float *ml = parts.ml + 2 * place_of(own < parts.rows ? own : 0);
+  for (int item0 = 0; item0 < items; item0 += 256) {
+    const int share = tid / items, item = item0 + tid % items;  // item0 > 0: shares = 1
+    const int row = item >> shift, col = (item & (cols - 1)) * 4 + (int)blockIdx.y * 4 * cols;
+    const bool live = row < parts.rows && col < d && share < shares;
+    const float *from = parts.o + place_of(live ? row : 0) * d + (live ? col : 0);
+    f32x4 o = {0, 0, 0, 0};
+    float m = kSeed, total = 0.0f;  // of row `own`
+    for (int k0 = 0; k0 < parts.count; k0 += AT) {
+      const int here = parts.count - k0 < AT ? parts.count - k0 : AT;
+      f32x4 x[AHEAD];
+      auto fetch = [&](int k1) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+          const int k = k1 + j * shares;
+          x[j] = *reinterpret_cast<const f32x4 *>(from + base(k0 + (k < here ? k : here - 1)) * d);
+        }
+      };
+      // The first rows come with the statistics.
+      if (live) fetch(share);
+      f32x2 mine[kMine];
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int k = tid / kRows + 256 / kRows * i;
+        mine[i] = *reinterpret_cast<const f32x2 *>(ml + 2 * base(k0 + (k < here ? k : here - 1)));
+        if (k >= here) mine[i] = f32x2{kSeed, 0.0f};
+      }
+      float top = mine[0].x;
+#pragma unroll
+      for (int i = 1; i < kMine; ++i) top = fmaxf(top, mine[i].x);
+#pragma unroll
+      for (int n = kRows; n < kWave; n *= 2) top = fmaxf(top, __shfl_xor(top, n, kWave));
+      if (lane < kRows) lds.tops[wave * kRows + lane] = top;
+      lds_barrier();
+      top = m;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, lds.tops[w * kRows + own]);
+      const float fade = exp2_hw(m - top);
+      m = top, total *= fade;
+      if (tid < kRows) lds.fades[tid] = fade;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const float weight = exp2_hw(mine[i].x - top);
+        total += mine[i].y * weight;
+        lds.weights[256 * i + tid] = weight;
+      }
+      lds_barrier();
+      if (live) {
+        o *= lds.fades[row];
+        for (int k1 = share; k1 < here; k1 += AHEAD * shares) {
+          if (k1 != share) fetch(k1);
+#pragma unroll
+          for (int j = 0; j < AHEAD; ++j) {
+            const int k = k1 + j * shares;
+            if (k < here) o += x[j] * lds.weights[k * kRows + row];
+          }
+        }
+      }
+      lds_barrier();
+    }
+#pragma unroll
+    for (int n = kRows; n < kWave; n *= 2) total += __shfl_xor(total, n, kWave);
+    if (lane < kRows) lds.totals[wave * kRows + lane] = total, lds.tops[wave * kRows + lane] = m;
+    if (shares > 1) *reinterpret_cast<f32x4 *>(lds.sums + 4 * tid) = o;
+    lds_barrier();
+    if (live && share == 0) {
+      // The shares' sums, in their order.
+      for (int k = 1; k < shares; ++k) o += *reinterpret_cast<const f32x4 *>(lds.sums + 4 * (tid + k * items));
+      float all = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) all += lds.totals[w * kRows + row];
+      const int R = parts.R0 + row, i = (int)kh_div(R, p.by_group);
+      finish(p, s.start + i, parts.head * p.group + R - i * p.group, col, o, lds.tops[row], all);
+    }
+    lds_barrier();
+  }
+}
+
+// A workgroup for every workgroup's start and head, as that one told it, then one for
+// each 16 rows of the wide units; a grid's y shares out the columns. Parts of up to
+// 16 take fewer loads: four sequences of 2000 entries 16.6 us, by the other form 18.3
+template <int D>
+__device__ __forceinline__ void join_told(const KhAttention8Params &p, JoinLds &lds) {
+  constexpr int kPer = kWideTile / kRows;
+  const int narrow_blocks = p.whole ? 0 : p.groups * p.together, block = (int)blockIdx.x - narrow_blocks;
+  KhSeq s{0, 0, 0};
+  Parts parts{};
+  if (!(block < 0 ? told_parts(p, (int)blockIdx.x, s, parts) : wide_parts(p, block / kPer, block % kPer * kRows, s, parts))) return;
+  if (parts.count <= 16)
+    join_rows<D, 16, 4>(p, lds, s, parts);
+  else
+    join_rows<D, kJoinMost, 16>(p, lds, s, parts);
+}
+
 // As far as sequence 0 reaches: its row of the table is the one that is read.
 __device__ __forceinline__ void settle_shared(KhAttention8Params &p) {
   if (p.shared == 0) return;
@@ -1473,11 +1595,9 @@ KH_ATTENTION8_WIDE(128, 2, kParts == 3 ? 1 : 2)
 KH_ATTENTION8_WIDE(256, 2, 1)
 #define KH_ATTENTION8_JOIN(D)                                                                                   \
   extern "C" __global__ void __launch_bounds__(256) KH_TYPED8(attention8_join_##D)(KhAttention8Params p) {      \
-    __shared__ float lds[kJoinParts * kRows * 2];                                                               \
+    __shared__ JoinLds lds;                                                                                     \
     settle_shared(p);                                                                                           \
-    join<D, true, 8>(p, lds, [&](int g, KhSeq &s, Parts &parts) { return told_parts(p, g, s, parts); }, [&](int token, int hq, int col, f32x4 o, float m, float total) {                            \
-      finish(p, token, hq, col, o, m, total);                                                                   \
-    });                                                                                                         \
+    join_told<D>(p, lds);                                                                                       \
   }                                                                                                             \
   extern "C" __global__ void __launch_bounds__(256) KH_TYPED8(attention8_combine_##D)(KhAttention8Params p) { \
     settle_shared(p);                                                                                           \

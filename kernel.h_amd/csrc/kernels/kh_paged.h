@@ -310,7 +310,6 @@ struct KhAttentionParams {
 
 KH_HD KhUnits kh_units_of(const KhAttentionParams &p, const KhSeq &s) { return kh_units(s, p.group, p.window, p.whole); }
 // kv heads that a unit of few rows takes together, and how many such groups there are.
-KH_HD int32_t kh_together(const KhAttentionParams &) { return 1; }
 KH_HD int32_t kh_groups_of(const KhAttentionParams &p) { return p.cache.kv_heads; }
 KH_HD int32_t kh_most_of(const KhAttentionParams &p, int32_t work) { return p.wide_blocks > 0 ? p.groups : kh_most(work, p.groups); }
 KH_HD KhSpan kh_span_of(const KhAttentionParams &p, const KhSeq &s, int32_t i) { return kh_seen(s, i, p.window); }
@@ -345,7 +344,6 @@ struct KhAttention8Params : KhAttentionParams {
   int32_t cap_near;       // what is small against the cap counts too
 };
 
-KH_HD int32_t kh_together(const KhAttention8Params &p) { return p.together; }
 KH_HD int32_t kh_groups_of(const KhAttention8Params &p) { return p.head_groups; }
 KH_HD int32_t kh_most_of(const KhAttention8Params &p, int32_t) { return p.groups; }
 

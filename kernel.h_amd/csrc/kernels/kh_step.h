@@ -142,7 +142,7 @@ struct Parts {
 
 // The unit that workgroup g's share starts inside of, if it is the first to do
 // so: every unit of the narrow form in parts has one such.
-__device__ __forceinline__ bool narrow_parts_of(const KhAttentionParams &p, int g, KhSeq &s, Parts &parts) {
+__device__ __forceinline__ bool narrow_parts(const KhAttentionParams &p, int g, KhSeq &s, Parts &parts) {
   const Line line = line_of(p, false);
   const KhShares shares = shares_of(p, line);
   if (g == 0 || g >= shares.groups) return false;
@@ -175,24 +175,22 @@ __device__ __forceinline__ bool wide_parts(const P &p, int unit, int row0, KhSeq
 }
 
 constexpr int kJoinParts = 64;  // statistics brought to LDS at a time
+constexpr int kJoinAhead = 16;  // parts whose rows are in flight
 
 // Joins the parts of 16 rows: a workgroup for every workgroup's start, then one
 // for each 16 rows of the wide units. A thread has 4 columns of a row, and where
 // that leaves threads over (few rows), only each second or fourth part of it.
 // The parts were written through other L2s, so that each round of loads takes
-// its time: bound by how many there are in a row. With SPLIT a grid's y shares out
-// the columns: with fewer of them, more threads share a row's parts. AHEAD: parts
-// whose rows a thread has in flight. narrow_parts: of block b, as narrow_parts_of.
-template <int D, bool SPLIT, int AHEAD, class P, class Find, class Done>
-__device__ __forceinline__ void join(const P &p, float *lds, Find &&narrow_parts, Done &&done) {
-  constexpr int kShares = SPLIT ? 8 : 4;
-  const int shift = __builtin_ctz(D / 4) - (SPLIT ? __builtin_ctz(gridDim.y) : 0), kCols = 1 << shift;
+// its time: bound by how many there are in a row.
+template <int D, class Done>
+__device__ __forceinline__ void join(const KhAttentionParams &p, float *lds, Done &&done) {
+  constexpr int kCols = D / 4;
   const int tid = threadIdx.x, d = p.cache.head_dim;
-  const int narrow_blocks = p.whole ? 0 : p.groups * kh_together(p), block = (int)blockIdx.x - narrow_blocks;
+  const int narrow_blocks = p.whole ? 0 : p.groups, block = (int)blockIdx.x - narrow_blocks;
   constexpr int kPer = kWideTile / kRows;
   KhSeq s{0, 0, 0};
   Parts parts{};
-  if (!(block < 0 ? narrow_parts((int)blockIdx.x, s, parts) : wide_parts(p, block / kPer, block % kPer * kRows, s, parts))) return;
+  if (!(block < 0 ? narrow_parts(p, (int)blockIdx.x, s, parts) : wide_parts(p, block / kPer, block % kPer * kRows, s, parts))) return;
   auto base = [&](int k) { return k == 0 ? parts.first : parts.others + (k - 1) * parts.step; };
   auto place_of = [&](int row) {
     if (!parts.wide) return (int64_t)row;
@@ -201,30 +199,20 @@ __device__ __forceinline__ void join(const P &p, float *lds, Find &&narrow_parts
   };
   // Rows rounded up to a power of two, times columns: items; threads that share one.
   const int rows2 = parts.rows <= 1 ? 1 : parts.rows <= 2 ? 2 : parts.rows <= 4 ? 4 : parts.rows <= 8 ? 8 : 16;
-  const int items = rows2 * kCols, shares = items >= 256 ? 1 : 256 / items < kShares ? 256 / items : kShares;
+  const int items = rows2 * kCols, shares = items >= 256 ? 1 : 256 / items < 4 ? 256 / items : 4;
   for (int item0 = 0; item0 < items; item0 += 256) {
     const int share = tid / items, item = item0 + tid % items;  // item0 > 0: shares = 1
-    const int row = item >> shift, col = (item & (kCols - 1)) * 4 + (SPLIT ? (int)blockIdx.y * 4 * kCols : 0);
+    const int row = item / kCols, col = item % kCols * 4;
     const bool live = row < parts.rows && col < d && share < shares;
     const int64_t place = place_of(live ? row : 0);
     f32x4 o = {0, 0, 0, 0};
     float m = kSeed, total = 0.0f;
     for (int k0 = 0; k0 < parts.count; k0 += kJoinParts) {
       const int here = parts.count - k0 < kJoinParts ? parts.count - k0 : kJoinParts;
-      f32x4 x[AHEAD];
-      auto fetch = [&](int k1) {
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-          const int k = k1 + j * shares;
-          x[j] = *reinterpret_cast<const f32x4 *>(parts.o + (base(k0 + (k < here ? k : here - 1)) + place) * d + col);
-        }
-      };
-      // The first rows come with the statistics.
-      if (live) fetch(share);
-      for (int n = tid; n < here * kRows; n += 256) {
-        const int k = n / kRows, r = n % kRows;
+      for (int x = tid; x < here * kRows; x += 256) {
+        const int k = x / kRows, r = x % kRows;
         const float *from = parts.ml + (base(k0 + k) + place_of(r < parts.rows ? r : 0)) * 2;
-        lds[2 * n] = from[0], lds[2 * n + 1] = from[1];
+        lds[2 * x] = from[0], lds[2 * x + 1] = from[1];
       }
       lds_barrier();
       if (live) {
@@ -232,10 +220,15 @@ __device__ __forceinline__ void join(const P &p, float *lds, Find &&narrow_parts
         for (int k = 0; k < here; ++k) top = fmaxf(top, lds[2 * (k * kRows + row)]);
         const float fade = exp2_hw(m - top);
         m = top, total *= fade, o *= fade;
-        for (int k1 = share; k1 < here; k1 += AHEAD * shares) {
-          if (k1 != share) fetch(k1);
+        for (int k1 = share; k1 < here; k1 += kJoinAhead * shares) {
+          f32x4 x[kJoinAhead];
 #pragma unroll
-          for (int j = 0; j < AHEAD; ++j) {
+          for (int j = 0; j < kJoinAhead; ++j) {
+            const int k = k1 + j * shares;
+            x[j] = *reinterpret_cast<const f32x4 *>(parts.o + (base(k0 + (k < here ? k : here - 1)) + place) * d + col);
+          }
+#pragma unroll
+          for (int j = 0; j < kJoinAhead; ++j) {
             const int k = k1 + j * shares;
             if (k < here) {
               const float w = exp2_hw(lds[2 * (k * kRows + row)] - top);

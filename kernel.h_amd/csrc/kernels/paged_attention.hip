@@ -835,7 +835,7 @@ KH_ATTENTION_WIDE(256, 1)
 #define KH_ATTENTION_JOIN(D)                                                                                       \
   extern "C" __global__ void __launch_bounds__(256) KH_TYPED(paged_attention_join_##D)(const KhAttentionParams p) { \
     __shared__ float lds[kJoinParts * kRows * 2];                                                                   \
-    join<D, false, 16>(p, lds, [&](int g, KhSeq &s, Parts &parts) { return narrow_parts_of(p, g, s, parts); }, [&](int token, int hq, int col, f32x4 o, float m, float total) {                                \
+    join<D>(p, lds, [&](int token, int hq, int col, f32x4 o, float m, float total) {                                \
       const float inv = total == 0.0f ? 0.0f : 1.0f / total;                                                        \
       const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};                                              \
       kh::store4(static_cast<elem *>(p.out) + (int64_t)token * p.out_stride + (int64_t)hq * p.cache.head_dim + col, y); \

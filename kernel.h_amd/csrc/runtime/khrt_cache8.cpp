@@ -350,8 +350,8 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
       const int64_t narrow_joins = plan.part_bytes > 0 ? plan.groups * together : 0;
       const int64_t wide_joins = plan.wide_bytes > 0 ? plan.wide_units * (KH_WIDE_ROWS / KH_TILE_ROWS) : 0;
       // Few units of many parts: a workgroup to 32 columns. MI355X, one sequence of
-      // 131071 entries (128 parts) 69 us against 82, 64 of 513 to 8192 (two or three)
-      // 112 against 109.
+      // 131071 entries (128 parts) 67 us against 72, 64 of 513 to 8192 (two or three)
+      // 117 against 109.
       const int64_t units = std::min(a.tokens, a.table.seqs) * c.kv_heads;
       const int64_t columns = plan.groups * together >= 32 * units ? (width == 0 ? 2 : width == 1 ? 4 : 8) : 1;
       if (int rc = launch(kJoin[width][a.dtype], narrow_joins + wide_joins, columns, 256, p, stream)) return rc;
