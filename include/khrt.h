@@ -579,7 +579,7 @@ typedef struct kh_paged_cache8 {
  * (time, height and width of images and video): pair i of token t is rotated by
  * positions[pair_axis[i] axis_stride + t] inv_freq[i]. pair_axis null: axis 0 for
  * all; a number outside [0, axes) counts as the nearest in it. k is rounded once,
- * from 32 bits; k_out (may be null) is k in the rows' type. A token whose slot is
+ * from 64 bits; k_out (may be null) is k in the rows' type. A token whose slot is
  * not in the cache writes nothing there. Two tokens with the same slot: either's
  * numbers, in part, and either's byte, so that the row may stand for neither's. */
 typedef struct kh_qk_norm_rope8_args {

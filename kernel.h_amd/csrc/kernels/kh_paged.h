@@ -282,6 +282,7 @@ struct KhRope8Params : KhRopeParams {
   int64_t axis_stride, scale_page, scale_head;
   int32_t axes;
   KhDiv by_parts, by_page;
+  double inverse_d;  // 1 / head_dim
 };
 
 // paged_attention.hip

@@ -26,17 +26,35 @@
 // the position of its own axis, and a row of k or v becomes e4m3 numbers times the
 // least power of two 2^e, e >= -117, with which the row's largest is at most 448:
 // the type's relative step is the same under any scale, so that a power of two loses
-// nothing by it, and what is read back is exact. k is rounded once, from 32 bits.
-// Infinities and NaN become NaN; a row's power is that of its finite elements. The
-// 8192 tokens take 44 us, 4.2 TB/s: fewer bytes, but as many rows to work through,
-// each with a maximum across its lanes. 5 fp32 tokens of 16 heads of 64 5.9 us, a
-// launch and one row's way through (7.2 with four angles to a lane and divisions in
-// 64 bits).
+// nothing by it, and what is read back is exact. Rows of k are worked out in 64 bits,
+// the angles' series too, and rounded once: between two numbers of four bits there are
+// ties, which 32 bits take either way (some 20 of 8 million numbers). Infinities and NaN
+// become NaN; a row's power is that of its finite elements. A wave's token, part and
+// page are the same in all lanes, and are kept so. The 8192 tokens take 41-44 us, 4.2-4.5
+// TB/s: fewer bytes, but as many rows to work through, each with a maximum across its
+// lanes (in 32 bits 42). 5 fp32 tokens of 16 heads of 64 7 us, a launch and one row's way
+// through (6.3 in 32 bits).
 #include "kh_elem.h"
 #include "kh_paged.h"
 
 namespace {
 
+#ifdef KH_CACHE8
+// The series in 64 bits too (first terms left out 7e-12 and 4e-13).
+__device__ __forceinline__ void turn(double angle, double &c, double &s) {
+  const double quarters = angle * 0.63661977236758134308;  // 2 / pi
+  const double whole = __builtin_rint(quarters);
+  const double x = (quarters - whole) * 1.57079632679489661923;
+  const int q = static_cast<int>(static_cast<int64_t>(whole)) & 3;
+  const double z = x * x;
+  const double si = x + x * z * (-1.0 / 6 + z * (1.0 / 120 + z * (-1.0 / 5040 + z * (1.0 / 362880 + z * (-1.0 / 39916800)))));
+  const double co =
+      1.0 + z * (-0.5 + z * (1.0 / 24 + z * (-1.0 / 720 + z * (1.0 / 40320 + z * (-1.0 / 3628800 + z * (1.0 / 479001600))))));
+  const double a = (q & 1) != 0 ? si : co, b = (q & 1) != 0 ? co : si;
+  c = q == 1 || q == 2 ? -a : a;
+  s = q >= 2 ? -b : b;
+}
+#else
 __device__ __forceinline__ void turn(double angle, float &c, float &s) {
   const double quarters = angle * 0.63661977236758134308;  // 2 / pi
   const double whole = __builtin_rint(quarters);
@@ -49,6 +67,7 @@ __device__ __forceinline__ void turn(double angle, float &c, float &s) {
   c = q == 1 || q == 2 ? -a : a;
   s = q >= 2 ? -b : b;
 }
+#endif
 
 template <int CONTROL>
 __device__ __forceinline__ float moved(float v) {
@@ -65,6 +84,41 @@ __device__ __forceinline__ float row_sum(float v) {
   if constexpr (L >= 32) v += __shfl_xor(v, 16, kh::kWave);
   return v;
 }
+
+#ifdef KH_CACHE8
+template <int CONTROL>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, v);
+  const uint32_t low = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)w, CONTROL, 0xf, 0xf, false);
+  const uint32_t high = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(w >> 32), CONTROL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)high << 32 | low);
+}
+
+template <int L>
+__device__ __forceinline__ double row_sum(double v) {
+  v += moved<0xb1>(v);
+  v += moved<0x4e>(v);
+  v += moved<0x141>(v);
+  if constexpr (L >= 16) v += moved<0x140>(v);
+  if constexpr (L >= 32) v += __shfl_xor(v, 16, kh::kWave);
+  return v;
+}
+
+// In 64 bits: the instruction's 2^-25 or so, and a Newton step.
+__device__ __forceinline__ double inverse_root(double x) {
+  const double y = __builtin_amdgcn_rsq(x);
+  const double z = y * (1.5 - 0.5 * x * y * y);
+  return x > 0.0 && x < __builtin_inf() ? z : y;
+}
+
+// y in 21 bits, the last of them set where that is not all of it: rounded further to
+// nearest, it becomes what y does.
+__device__ __forceinline__ float leading(double y) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, y);
+  const uint32_t high = (uint32_t)(w >> 32) | ((uint32_t)w != 0 ? 1u : 0u);
+  return static_cast<float>(__builtin_bit_cast(double, (uint64_t)high << 32));
+}
+#endif
 
 // 1 / sqrt(x), x >= 0, to a unit in the last place: v_rsq_f32, which takes no
 // denormal numbers (and gives what the formula gives for 0, infinities, NaN).
@@ -100,6 +154,10 @@ __device__ __forceinline__ void store_past(kh::elem *p, const float (&x)[4]) {
 
 #ifdef KH_CACHE8
 using Params = KhRope8Params;
+
+struct Turn {
+  double c, s;
+};
 
 // The largest over the L lanes of a row.
 template <int L>
@@ -158,7 +216,7 @@ __device__ __forceinline__ void rope(const Params &p) {
   // A job is one part of one token's heads; a wave takes one.
 #ifdef KH_CACHE8
   // Fewer than 2^31 jobs: the launcher sees to it.
-  const uint32_t job = blockIdx.x * (256 / kh::kWave) + threadIdx.x / kh::kWave;
+  const uint32_t job = blockIdx.x * (256 / kh::kWave) + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x / kh::kWave);
   const int64_t t = kh_div(job, p.by_parts);
   const int part = (int)(job - (uint32_t)t * p.by_parts.by);
 #else
@@ -185,6 +243,12 @@ __device__ __forceinline__ void rope(const Params &p) {
     const bool is_q = step < of_q, is_v = step >= of_q + of_k;
     const elem *src = is_q ? of_t[0] : is_v ? of_t[2] : of_t[1];
     const int n = is_q ? q_heads : kv_heads, h = (step - (is_q ? 0 : is_v ? of_q + of_k : of_q)) * kRows + lane / L;
+#ifdef KH_CACHE8
+    const uint32_t row = (uint32_t)(h < n ? h : n - 1) * (uint32_t)d;  // below 2^24
+    ahead[0] = *reinterpret_cast<const Four *>(src + (row + (uint32_t)l0));
+    ahead[1] = *reinterpret_cast<const Four *>(src + (row + (uint32_t)l1));
+    return;
+#endif
     src += (int64_t)(h < n ? h : n - 1) * d;
     ahead[0] = *reinterpret_cast<const Four *>(src + l0);
     ahead[1] = *reinterpret_cast<const Four *>(src + l1);
@@ -215,14 +279,19 @@ __device__ __forceinline__ void rope(const Params &p) {
   float c[4], s[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) c[i] = 1.0f, s[i] = 0.0f;
+#ifdef KH_CACHE8
+  __shared__ Turn of_waves[256 / kh::kWave][4][L];
+  Turn(*const turns)[L] = of_waves[threadIdx.x / kh::kWave];
+#endif
   if (turned) {
 #ifdef KH_CACHE8
-    // A lane works out kOwn of its row's four angles, and gets the others from the
-    // lanes with the same elements of the other rows of the wave.
+    // A lane works out kOwn of its row's four angles, and gets the others by way of LDS
+    // from the lanes with the same elements of the other rows of the wave.
     constexpr int kOwn = L == 32 ? 2 : 1;
     const int own = 4 * u + (lane / L * kOwn) % 4;
     int axis[kOwn];
-    float freq[kOwn], co[kOwn], si[kOwn];
+    float freq[kOwn];
+    double co[kOwn], si[kOwn];
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       axis[i] = p.pair_axis != nullptr ? p.pair_axis[own + i] : 0;
@@ -231,10 +300,14 @@ __device__ __forceinline__ void rope(const Params &p) {
 #pragma unroll
     for (int i = 0; i < kOwn; ++i)
       turn(static_cast<double>(p.positions[kh_clamp(axis[i], 0, p.axes - 1) * p.axis_stride + t]) * static_cast<double>(freq[i]), co[i], si[i]);
+    // The wave's own part of LDS: nobody else waits for it.
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) turns[(lane / L * kOwn + i) % 4][u] = Turn{co[i], si[i]};
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      c[i] = __shfl(co[i % kOwn], u + L * (i / kOwn), kh::kWave);
-      s[i] = __shfl(si[i % kOwn], u + L * (i / kOwn), kh::kWave);
+      const Turn at = turns[i][u];
+      c[i] = static_cast<float>(at.c), s[i] = static_cast<float>(at.s);
     }
 #else
     const double pos = static_cast<double>(p.positions[t]);
@@ -270,6 +343,59 @@ __device__ __forceinline__ void rope(const Params &p) {
     float x[2][4];
     unpack(x[0], raw[0]);
     unpack(x[1], raw[1]);
+#ifdef KH_CACHE8
+    if (!is_q) {
+      // In 64 bits: a row is rounded once, to four bits a number. In 32, ties between
+      // two of them go either way: of 8192 tokens' 8 heads of 128 some 20 numbers.
+      double scale = 1.0;
+      if (p.norm) {
+        double sq = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sq += static_cast<double>(x[i / 4][i % 4]) * static_cast<double>(x[i / 4][i % 4]);
+        scale = inverse_root(row_sum<L>(live ? sq : 0.0) * p.inverse_d + static_cast<double>(p.eps));
+      }
+      float g[2][4];
+      unpack(g[0], gamma[1][0]);
+      unpack(g[1], gamma[1][1]);
+      auto weighted = [&](int half, int i) {
+        if (!k_gamma) return static_cast<double>(x[half][i]);
+        // Exact in 16 bits' types.
+        return KH_ELEM == 0 ? static_cast<double>(x[half][i]) * static_cast<double>(g[half][i]) : static_cast<double>(x[half][i] * g[half][i]);
+      };
+      elem *const k_out = static_cast<elem *>(p.k_out) + t * p.k_out_stride;
+      float exact[2][4];  // fp32's own rounding, for k_out
+      auto pair = [&](int ha, int ia, int hb, int ib, int i) {
+        double y = weighted(ha, ia), z = weighted(hb, ib);
+        if (turned) {
+          const Turn at = turns[i][u];
+          const double first = y * at.c - z * at.s;
+          z = z * at.c + y * at.s;
+          y = first;
+        }
+        y *= scale, z *= scale;
+        if (KH_ELEM == 0) exact[ha][ia] = static_cast<float>(y), exact[hb][ib] = static_cast<float>(z);
+        x[ha][ia] = leading(y), x[hb][ib] = leading(z);
+      };
+      if (p.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pair(i / 2, 2 * (i % 2), i / 2, 2 * (i % 2) + 1, i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pair(0, i, 1, i, i);
+      }
+      if (on && p.k_out != nullptr) {
+        const uint32_t row = (uint32_t)h * (uint32_t)d;
+        store_past(k_out + (row + (uint32_t)a0), KH_ELEM == 0 ? exact[0] : x[0]);
+        store_past(k_out + (row + (uint32_t)a1), KH_ELEM == 0 ? exact[1] : x[1]);
+      }
+      if (cached) {
+        const int64_t at = page * p.k_page + in_page * p.k_slot + h * p.k_head;
+        store8<L>(x, live, on, static_cast<uint8_t *>(p.k_cache) + at, a0, a1,
+                  p.k_scale + (page * p.scale_page + h * p.scale_head + in_page), u);
+      }
+      continue;
+    }
+#endif
     if (p.norm) {
       float sq = 0.0f;
 #pragma unroll
@@ -300,19 +426,20 @@ __device__ __forceinline__ void rope(const Params &p) {
         a = y;
       }
     }
+#ifdef KH_CACHE8
+    if (on) {
+      elem *const dst = static_cast<elem *>(p.q_out) + t * p.q_out_stride;
+      const uint32_t row = (uint32_t)h * (uint32_t)d;
+      store_past(dst + (row + (uint32_t)a0), x[0]);
+      store_past(dst + (row + (uint32_t)a1), x[1]);
+    }
+#else
     if (on && (is_q || p.k_out != nullptr)) {
       elem *dst = is_q ? static_cast<elem *>(p.q_out) + t * p.q_out_stride : static_cast<elem *>(p.k_out) + t * p.k_out_stride;
       dst += (int64_t)h * d;
       store_past(dst + a0, x[0]);
       store_past(dst + a1, x[1]);
     }
-#ifdef KH_CACHE8
-    if (!is_q && cached) {
-      const int64_t at = page * p.k_page + in_page * p.k_slot + h * p.k_head;
-      store8<L>(x, live, on, static_cast<uint8_t *>(p.k_cache) + at, a0, a1,
-                p.k_scale + (page * p.scale_page + h * p.scale_head + in_page), u);
-    }
-#else
     if (on && !is_q && cached) {
       elem *dst = static_cast<elem *>(p.k_cache) + page * p.k_page + in_page * p.k_slot + h * p.k_head;
       store_past(dst + a0, x[0]);
@@ -325,10 +452,12 @@ __device__ __forceinline__ void rope(const Params &p) {
 }  // namespace
 
 #ifdef KH_CACHE8
-#define KH_ROPE(name) KH_TYPED(rope8_##name)
+// Six waves to a SIMD where the elements leave registers for it: 1999 fp16 tokens of 24
+// heads of 96 17.4 us, 18.8 with five; fp32 would spill 37 and has four.
+#define KH_ROPE(name) __launch_bounds__(256, KH_ELEM == 0 ? 1 : 6) KH_TYPED(rope8_##name)
 #else
-#define KH_ROPE(name) KH_TYPED(qk_norm_rope_##name)
+#define KH_ROPE(name) __launch_bounds__(256) KH_TYPED(qk_norm_rope_##name)
 #endif
-extern "C" __global__ void __launch_bounds__(256) KH_ROPE(8)(const Params p) { rope<8>(p); }
-extern "C" __global__ void __launch_bounds__(256) KH_ROPE(16)(const Params p) { rope<16>(p); }
-extern "C" __global__ void __launch_bounds__(256) KH_ROPE(32)(const Params p) { rope<32>(p); }
+extern "C" __global__ void KH_ROPE(8)(const Params p) { rope<8>(p); }
+extern "C" __global__ void KH_ROPE(16)(const Params p) { rope<16>(p); }
+extern "C" __global__ void KH_ROPE(32)(const Params p) { rope<32>(p); }

@@ -227,7 +227,7 @@ int kh_qk_norm_rope8(const kh_qk_norm_rope8_args *args, void *stream) {
                        static_cast<int32_t>(parts), a.eps},
                       c.k_scale, c.v_scale, a.pair_axis, a.axis_stride, c.scale_page_stride, c.scale_head_stride,
                       static_cast<int32_t>(std::max<int64_t>(a.axes, 1)), kh_div_by(static_cast<uint32_t>(parts)),
-                      kh_div_by(static_cast<uint32_t>(c.page_size))};
+                      kh_div_by(static_cast<uint32_t>(c.page_size)), 1.0 / static_cast<double>(c.head_dim)};
       if (int rc = launch(kRope[lanes / 16][a.dtype], ceil_div(tokens * parts, 4), 1, 256, p, stream)) return rc;
     }
     return 0;

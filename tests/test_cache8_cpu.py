@@ -199,7 +199,8 @@ int main() {
 
 # Symbols that spill, and how much at the most: registers and bytes of scratch of a lane.
 SPILLS = {"attention8_odd_128_f32": (24, 100), "attention8_odd_128_f16": (6, 28), "attention8_wide_256_f32": (106, 416),
-          "attention8_wide_128_f16": (20, 48), "attention8_wide_256_f16": (42, 160)}
+          "attention8_wide_128_f16": (20, 48), "attention8_wide_256_f16": (42, 160),
+          "rope8_8_f16": (2, 12), "rope8_16_f16": (2, 12), "rope8_32_f16": (4, 20), "rope8_32_bf16": (1, 8)}
 
 
 def test_what_the_kernels_spill():

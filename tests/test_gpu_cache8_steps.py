@@ -7,11 +7,11 @@ import numpy as np
 import pytest
 
 import kernelh as kh
-from cachetest import DTYPES, ints_on_gpu, rounded, same_bits, values_from_gpu, values_on_gpu
+from cachetest import DTYPES, half_step, ints_on_gpu, rounded, same_bits, values_from_gpu, values_on_gpu
 from cache8test import Step8, held, stand_for
 from khtest import say
 from test_gpu_cache import check_attention, close
-from test_gpu_cache8 import rotated
+from test_gpu_cache8 import rotated, run_write
 from test_gpu_cache_steps import Graph
 
 pytestmark = pytest.mark.gpu
@@ -346,6 +346,33 @@ def test_rows_of_v_of_any_size(dev, dtype, q, page_size):
         scales[pages] = byte + s.g.integers(0, 6, scales[pages].shape)
     s.put("v", codes, scales)
     check_attention(s)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("hk,d,rotary,interleaved", [(8, 128, 128, False), (8, 96, 48, True), (4, 256, 256, False), (8, 64, 64, True)])
+def test_keys_are_rounded_once(dev, dtype, hk, d, rotary, interleaved):
+    """Worked out in 64 bits: of more than a million numbers none goes to the other side of
+    a tie, as some do in 32 bits."""
+    say(f"keys {dtype} {hk} d={d} rotary={rotary}")
+    g = np.random.default_rng(d)
+    t, page_size = 1 << 20 >> int(math.log2(hk * d)), 16
+    pages = t // page_size + 1
+    q, k = (rounded(3 * g.standard_normal((t, h, d), np.float32), dtype) for h in (1, hk))
+    gamma = rounded(1 + 0.2 * g.standard_normal(d).astype(np.float32), dtype)
+    freq = (10000.0 ** (-np.arange(0, rotary, 2) / rotary)).astype(np.float32)
+    pos, pair_axis = g.integers(0, 1000000, (3, t)), g.integers(0, 3, rotary // 2)
+    slots = g.permutation(pages * page_size)[:t]
+    out = run_write(dtype, np.repeat(q, hk, 1), k, k, (gamma, gamma), freq, pos, pair_axis, slots, pages, page_size, rotary, interleaved,
+                    eps=0.0, k_out=True)
+    want, _ = rotated(k, gamma, pos, freq, pair_axis, rotary, interleaved, 0.0, True, dtype)
+    codes, scales = held(want)
+    at = slots // page_size, slots % page_size
+    assert np.array_equal(out[4][at[0], :, at[1]], scales)
+    assert np.array_equal(out[2][at], codes)
+    # k_out: half a step of its type, and what is left of 64 bits. An angle of up to 2^20
+    # is 2^20 quarters, rounded to 2^-53 of them: 2^-32 rad; the series' rest is less.
+    size = 2 * np.abs(want).max(-1, keepdims=True)
+    close(out[1], want, np.abs(want) * half_step(dtype) + size * 2.0 ** -31 + (2.0 ** -25 if dtype == "f16" else 0.0), "k_out")
 
 
 # ---------------------------------------------------------------- caches past 4 GB
