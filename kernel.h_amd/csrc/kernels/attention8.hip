@@ -141,17 +141,19 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) {
 
 // Scores over the cap, capped: tanh(y cap_in / (2 log2 e)), which cap_out takes back to
 // scores in powers of two. By way of t = 2^(y cap_in) it is 1 - 2 / (t + 1), off by
-// some 2^-23 of the cap: of 16-bit rows' weights that is nothing up to a cap of 256
-// (2^-15 of a weight). Past that, and for fp32 rows (near), what lies below a quarter
-// of the cap comes from the power series (first term left out 2e-9 of the score): 16
-// instructions a score instead of 5, of which chunks feel every one.
+// some 2^-23 of the cap. near: what lies below a quarter of the cap comes from the
+// power series (first term left out 2e-9 of the score), 16 instructions a score instead
+// of 5. Few rows have the time for it (64 sequences of 513 to 8192 entries
+// 112 us with either); chunks feel every instruction. Of a chunk's 16-bit rows' weights 2^-23 of a cap up to
+// 256 is nothing (2^-15 of a weight), nor is it of their lse over many entries; rows of
+// fp32, of larger caps or of short sequences take the series there too.
 template <int N, class X>
-__device__ __forceinline__ void cap(X &y, const KhAttention8Params &p) {
+__device__ __forceinline__ void cap(X &y, const KhAttention8Params &p, bool near) {
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const float x = y[j] * p.cap_in;
     float r = fmaf(-2.0f, __builtin_amdgcn_rcpf(exp2_hw(x) + 1.0f), 1.0f);
-    if (p.cap_near) {
+    if (near) {
       const float a = x * 0.34657359027997265471f, z = a * a;  // log(2) / 2
       const float series = a + a * z * (-1.0f / 3 + z * (2.0f / 15 + z * (-17.0f / 315 + z * (62.0f / 2835 + z * (-1382.0f / 155925)))));
       r = z < 0.0625f ? series : r;
@@ -427,7 +429,7 @@ __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, f
         find<D>(next, p, table, key0 + 2 * kStep, key_end, lane);
 
         if (p.cap_in != 0.0f) {
-          cap<F::mine>(y, p);
+          cap<F::mine>(y, p, true);
         }
         // Every row sees every entry of the block: no mask.
         const bool whole = present == ~uint64_t(0) >> (64 - F::keys) && key0 + F::keys <= low.end && key0 >= high.first;
@@ -878,7 +880,7 @@ __device__ __forceinline__ void narrow_even(const KhAttention8Params &p, int blo
         send<F>(p, own, then, 0, k_off, kscales, kb, own + F::scales_at + b * 256, lane);
 
         if (p.cap_in != 0.0f) [[unlikely]] {
-          cap<F::mine>(y, p);
+          cap<F::mine>(y, p, true);
         }
         // Every row sees every entry of the block: no mask.
         const bool whole = here == ~uint64_t(0) >> (64 - F::keys) && key0 + F::keys <= low.end && key0 >= high.first;
@@ -1262,7 +1264,12 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
         const uint64_t odds = mixed(key0) ? __builtin_amdgcn_ballot_w64((mark & kOdd) != 0) : 0;
         if (p.cap_in != 0.0f) [[unlikely]] {
 #pragma unroll
-          for (int kt = 0; kt < W::tiles; ++kt) cap<16>(x[kt], p);
+          for (int kt = 0; kt < W::tiles; ++kt) {
+            if (p.cap_near)
+              cap<16>(x[kt], p, true);
+            else
+              cap<16>(x[kt], p, false);
+          }
         }
         const bool whole = present == ~uint64_t(0) && key0 + W::keys <= low.end && key0 >= high.first;
         if (!whole) [[unlikely]] {

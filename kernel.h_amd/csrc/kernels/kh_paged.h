@@ -342,7 +342,7 @@ struct KhAttention8Params : KhAttentionParams {
   KhJoin *joins;  // [groups]
   int32_t together, head_groups;  // kv heads that a unit of few rows takes together (the last fewer), and their groups
   float cap_in, cap_out;  // scores y become cap_out tanh(y cap_in / (2 log2 e)); cap_in 0: they do not
-  int32_t cap_near;       // what is small against the cap counts too
+  int32_t cap_near;       // what is small against the cap counts for units of many rows too
 };
 
 KH_HD int32_t kh_groups_of(const KhAttention8Params &p) { return p.head_groups; }

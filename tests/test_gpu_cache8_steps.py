@@ -8,7 +8,7 @@ import pytest
 
 import kernelh as kh
 from cachetest import DTYPES, half_step, ints_on_gpu, rounded, same_bits, values_from_gpu, values_on_gpu
-from cache8test import Step8, held, stand_for
+from cache8test import Step8, codes_of, held, stand_for
 from khtest import say
 from test_gpu_cache import check_attention, close
 from test_gpu_cache8 import rotated, run_write
@@ -373,6 +373,26 @@ def test_keys_are_rounded_once(dev, dtype, hk, d, rotary, interleaved):
     # is 2^20 quarters, rounded to 2^-53 of them: 2^-32 rad; the series' rest is less.
     size = 2 * np.abs(want).max(-1, keepdims=True)
     close(out[1], want, np.abs(want) * half_step(dtype) + size * 2.0 ** -31 + (2.0 ** -25 if dtype == "f16" else 0.0), "k_out")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("q", [1, 40])
+@pytest.mark.parametrize("cap", [20.0, 200.0])
+def test_small_scores_under_a_cap(dev, dtype, q, cap):
+    """A row that sees one entry has its score for lse: exact before the cap (small whole
+    numbers), and off by some 8 roundings of the series behind it, or where the
+    other form takes over, at a quarter of the cap, by 2^-23 of the cap: 2^-20 of it."""
+    s = Step8(dtype, [q] * 30, [q] * 30, 4, 2, 64, cap=cap, seed=q)
+    whole = s.g.integers(-2, 3, s.k_codes.shape).astype(float)
+    s.put("k", codes_of(whole), np.full(s.k_scales.shape, 127, np.uint8))
+    s.q = s.g.integers(-2, 3, s.q.shape).astype(np.float32)
+    s.scale = 0.125
+    _, lse = s.run_attention()
+    first = np.arange(30) * q  # these tokens see one entry
+    k = whole[s.table[:, 0], 0]
+    x = s.scale * (s.q.reshape(-1, 4, 64)[first] * np.repeat(k, 2, 1)).sum(-1)
+    y = cap * np.tanh(x / cap)
+    close(lse[first], y, np.abs(y) * 2.0 ** -20, "lse")
 
 
 # ---------------------------------------------------------------- caches past 4 GB
