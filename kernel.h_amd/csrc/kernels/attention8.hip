@@ -28,7 +28,7 @@
 // to LDS as bf16: each byte is converted once for 128 rows. Bound by what the waves
 // issue, the softmax's and the conversions' instructions (54% of the time) and the
 // matrix units' (32%) in turn: a chunk of 2048 at 8192 entries, 32 heads on 8 of
-// 128, bf16, 288 us, 840 TFLOP/s.
+// 128, bf16, 287 to 302 us, 800 to 845 TFLOP/s.
 //
 // Entries that all sequences share are worked on by wide units whose rows are all
 // tokens of the step; their parts and the sequences' own are joined row by row.
