@@ -270,6 +270,20 @@ def test_page_numbers_are_found_again_and_again(dev, n):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n,hq,d", [(40000, 1, 64), (70001, 16, 128), (140000, 3, 64), (36000, 2, 256)])
+def test_more_parts_than_a_join_takes_at_a_time(dev, dtype, n, hq, d):
+    """One kv head, so that every workgroup has a part of the one unit: up to 512 of them."""
+    check_attention(Step8(dtype, [1], [n], hq, 1, d, seed=hq))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_parts_with_and_without_scores(dev, dtype):
+    """Windows that end inside parts: some of a unit's rows have nothing in its first ones."""
+    check_attention(Step8(dtype, [5, 3], [30000, 9000], 6, 2, 64, window=4000, seed=44))
+    check_attention(Step8(dtype, [4], [60000], 8, 1, 128, window=50001, seed=45))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("q", [1, 40])
 def test_infinite_scores_and_queries(dev, dtype, q):
     """Scores that overflow, and a cap that takes them back."""
