@@ -122,7 +122,7 @@ constexpr int64_t kWholeShared = 8;
 
 // Up to this many entries to a sequence, capped scores of chunks come from the series
 // near zero too: where a row sees few, its lse is as far off as they are. MI355X, 16
-// chunks of up to 301 of 4001 fp16 tokens, 87 us without, 98 with.
+// chunks of up to 301 of 4001 fp16 tokens, 88 us without, 104 with.
 constexpr int64_t kShortCapped = 512;
 
 // Fewer where there would not be a block of entries for every workgroup.
