@@ -135,10 +135,12 @@ int64_t heads_together(const kh_paged_attention8_args &a, int64_t behind) {
   return n;
 }
 
-// How the entries that sequences share are worked on: not at all (splits 0), or by
-// units of KH_WIDE_ROWS rows of all tokens, in `splits` parts of `each` entries.
+// How the entries that sequences share are worked on: not at all (splits 0), or the
+// first `entries` of them by units of KH_WIDE_ROWS rows of all tokens, in `splits`
+// parts of `each`. Those past the expected length are each sequence's own: what the
+// kernels are told is what the parts were cut from.
 struct SharedPlan {
-  int64_t units, splits, each;
+  int64_t entries, units, splits, each;
   size_t bytes;
 };
 
@@ -164,6 +166,7 @@ SharedPlan shared_plan(const kh_paged_attention8_args &a, size_t workspace_bytes
   if (splits < 1) return p;
   const double saved = static_cast<double>(few - 1) * static_cast<double>(shared * a.cache.kv_heads * 2 * (a.cache.head_dim + 1));
   if (saved < 25e6 + 2.0 * static_cast<double>(splits + 1) * static_cast<double>(part)) return p;
+  p.entries = shared;
   p.each = ceil_div(ceil_div(shared, splits), 64) * 64;
   p.splits = ceil_div(shared, p.each);
   p.bytes = static_cast<size_t>(p.splits + 1) * part;
@@ -304,7 +307,7 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
     if (workspace == nullptr) workspace_bytes = 0;
     const SharedPlan shared = shared_plan(a, workspace_bytes);
     const bool common = shared.splits > 0;
-    const kh_paged_attention_args plain = as_plain(a, common ? a.shared : 0);
+    const kh_paged_attention_args plain = as_plain(a, shared.entries);
     const int64_t group = a.q_heads / c.kv_heads, rows = a.tokens * a.q_heads, d = c.head_dim;
     const bool even = even_pages8(a);
     // What tells who joins which parts comes last.
@@ -314,7 +317,7 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
     // ones: one).
     const bool narrow_only = kh_narrow_only(a.tokens, a.table.seqs, group, a.max_new, narrow_rows_of(KHRT_BF16), 256);
     const bool alone = even && !common && narrow_only;
-    const int64_t together = even ? heads_together(a, common ? a.shared : 0) : 1;
+    const int64_t together = even ? heads_together(a, shared.entries) : 1;
     const AttentionPlan plan = attention_plan(plain, left, {alone ? 2 * KH_GEMM_CUS : most_groups(plain), together, common ? kWholeShared : alone && d <= 128 ? kWholeEven : kWholeBlocks});
     const bool joined = plan.part_bytes + plan.wide_bytes > 0;
     // All rows of parts come first, 16 bytes at a time, then their statistics.
@@ -344,7 +347,7 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
                           static_cast<int32_t>(std::max<int64_t>(plan.splits, 1)), even, a.scale == 0.0f ? 0u : 0xffffffffu,
                           a.scale < 0.0f ? (two_bytes ? 0x80008000u : 0x80000000u) : 0u, kh_div_by(u32(group)), factor},
                          c.k_scale, c.v_scale, u32(c.scale_page_stride), u32(c.scale_head_stride),
-                         common ? static_cast<int32_t>(std::min(a.shared, kCapacity)) : 0, static_cast<int32_t>(shared_blocks),
+                         static_cast<int32_t>(shared.entries), static_cast<int32_t>(shared_blocks),
                          static_cast<int32_t>(std::max<int64_t>(shared.splits, 1)), static_cast<int32_t>(shared.each), shared_o, shared_ml, joins,
                          static_cast<int32_t>(together), static_cast<int32_t>(ceil_div(c.kv_heads, together)), cap_in, std::min(a.cap * 1.44269504088896340736f, most), a.dtype == KHRT_F32 || a.cap > 256.0f || expected_len(a.table, plain.cache) <= kShortCapped};
     const int width = width_of(d);

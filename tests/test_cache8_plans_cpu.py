@@ -1,0 +1,53 @@
+"""How attention over a cache in 8 bits shares a step out, without a GPU: its host
+code with launches that only write down what they were given
+(tests/cpp/cache8_plan_check.cpp)."""
+import json
+import os
+import subprocess
+
+import pytest
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
+
+
+def run(cmd, timeout):
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=timeout)
+    assert r.returncode == 0, r.stdout[-4000:]
+    return r.stdout
+
+
+@pytest.fixture(scope="module")
+def plan_check(tmp_path_factory):
+    exe = str(tmp_path_factory.mktemp("plans") / "cache8_plan_check")
+    src = os.path.join(REPO, "kernel.h_amd", "csrc")
+    run(["g++", "-O1", "-g", "-std=c++20", "-Wall", "-Wextra", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-D__HIP_PLATFORM_AMD__",
+         "-I", os.path.join(REPO, "include"), "-I", os.path.join(src, "include"), "-I", os.path.join(src, "kernels"),
+         "-I", os.path.join(ROCM, "include"), os.path.join(REPO, "tests", "cpp", "cache8_plan_check.cpp"), "-o", exe], 300)
+    return exe
+
+
+@pytest.fixture
+def plan(plan_check):
+    """What a step's first launch is told."""
+    return lambda **kw: json.loads(run([plan_check, *(f"{k}={v}" for k, v in kw.items())], 60))
+
+
+def test_every_entry_is_somebodys(plan_check):
+    """Over a grid of steps: parts of shared entries reach as far as the sequences' own
+    begin, and what the kernels write lies in the workspace."""
+    assert run([plan_check], 300).strip().endswith("cache8_plan_check ok")
+
+
+def test_shared_entries_past_the_expected_length(plan):
+    """max_len below shared: the entries past it are each sequence's own."""
+    p = plan(tokens=64, seqs=64, hq=32, hk=8, d=128, shared=8192, max_len=4096)
+    assert p["shared_blocks"] > 0 and p["shared"] <= p["shared_splits"] * p["shared_each"]
+
+
+def test_the_steps_that_are_run_share_entries(plan):
+    """Those of tests/test_gpu_cache8_plans.py, whose lengths end inside the shared entries."""
+    for max_len in (600, 1499):
+        assert plan(tokens=194, seqs=65, hq=4, hk=4, d=128, width=200, shared=1500, max_len=max_len, max_new=130)["shared"] == max_len
+    for max_len in (600, 1101):
+        assert plan(tokens=64, seqs=64, hq=4, hk=4, d=128, width=200, shared=1500, max_len=max_len)["shared"] == max_len
