@@ -1,6 +1,7 @@
 """How attention over a cache in 8 bits shares a step out, without a GPU: its host
 code with launches that only write down what they were given
 (tests/cpp/cache8_plan_check.cpp)."""
+import itertools
 import json
 import os
 import subprocess
@@ -46,8 +47,13 @@ def test_shared_entries_past_the_expected_length(plan):
 
 
 def test_the_steps_that_are_run_share_entries(plan):
-    """Those of tests/test_gpu_cache8_plans.py, whose lengths end inside the shared entries."""
+    """Those of tests/test_gpu_cache8_plans.py."""
     for max_len in (600, 1499):
         assert plan(tokens=194, seqs=65, hq=4, hk=4, d=128, width=200, shared=1500, max_len=max_len, max_new=130)["shared"] == max_len
     for max_len in (600, 1101):
         assert plan(tokens=64, seqs=64, hq=4, hk=4, d=128, width=200, shared=1500, max_len=max_len)["shared"] == max_len
+    assert plan(tokens=67, seqs=64, hq=4, hk=4, d=128, width=122, shared=1500)["shared"] == 1500
+    assert plan(tokens=285, seqs=150, hq=8, hk=4, d=64, width=69, shared=688, max_new=0)["shared"] == 688
+    for page_size, dtype, (tokens, max_new) in itertools.product((16, 24), (0, 2), ((120, 1), (159, 40))):
+        assert plan(tokens=tokens, seqs=120, hq=4, hk=2, d=128, width=36, page_size=page_size, dtype=dtype, shared=500,
+                    max_new=max_new)["shared"] == 500

@@ -1,9 +1,13 @@
 """Attention over a cache in 8 bits where its launch is shaped by what the caller
-expects and the lengths turn out otherwise."""
+expects and the lengths turn out otherwise, and in steps large enough that shared
+entries are worked on apart (tests/test_cache8_plans_cpu.py checks that they are)."""
+import numpy as np
 import pytest
 
-from cache8test import Step8
-from cachetest import DTYPES
+import kernelh as kh
+from cache8test import Step8, held
+from cachetest import DTYPES, ints_on_gpu, rounded, values_on_gpu
+from khtest import say
 from test_gpu_cache import check_attention
 
 pytestmark = pytest.mark.gpu
@@ -21,3 +25,61 @@ def test_shared_entries_past_the_expected_length(dev, dtype, page_size, window):
     s = Step8(dtype, [1] * 64, lens[:64], 4, 4, 128, seed=page_size + 1, page_size=page_size, shared=1500, window=window)
     for max_len in (600, 1101):
         check_attention(s, max_len=max_len, max_new=1)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_more_sequences_than_lanes_behind_shared_entries(dev, dtype):
+    """A hundred and fifty sequences: single tokens, drafts, chunks, some without new tokens."""
+    g = np.random.default_rng(5)
+    q_lens = [int(x) for x in g.choice([0, 1, 1, 1, 2, 40], 150, p=[0.1, 0.3, 0.2, 0.2, 0.18, 0.02])]
+    lens = [int(x) for x in g.integers(700, 1100, 150)]
+    check_attention(Step8(dtype, q_lens, lens, 8, 4, 64, seed=6, shared=688, before=1, after=2))
+
+
+@pytest.mark.parametrize("starts", ["claimed twice", "descending", "past the last token"])
+def test_starts_that_do_not_ascend_behind_shared_entries(dev, starts):
+    """Whatever the sequences get, the call ends, and tokens of none are left alone."""
+    s = Step8("bf16", [1] * 64, [1501 + 7 * i for i in range(64)], 4, 4, 128, seed=3, before=1, after=2, shared=1500)
+    say(f"starts {starts}")
+    s.starts = {"claimed twice": [1, 60] * 32 + [1], "descending": [60 - i for i in range(65)],
+                "past the last token": [1] * 60 + [65, 1 << 30, 70, 1 << 30, 65]}[starts]
+    for workspace in (None, 0):
+        out, lse = s.run_attention(max_new=1, workspace=workspace)
+        none = {"claimed twice": [0, 60, 65, 66], "descending": list(range(67)), "past the last token": [0]}[starts]
+        assert (out[none] == 7.0).all() and (lse[none] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("page_size,scales_far", [(16, True), (16, False), (24, True)])
+def test_shared_entries_past_4_gb(dev, dtype, page_size, scales_far):
+    """Pages 128 MB apart, their scales behind the rows or elsewhere."""
+    far, pages, hq, hk, d = 1 << 27, 36, 4, 2, 128
+    say(f"far pages of {page_size}, scales far: {scales_far}")
+    g = np.random.default_rng(page_size)
+    bufs = [kh.Buffer(pages * far) for _ in "kv"]
+    near = [kh.Buffer.from_array(np.zeros((pages, hk, page_size), np.uint8)) for _ in "kv"]
+    at = page_size * hk * d
+    cache = kh.PagedCache8(k=bufs[0].ptr, v=bufs[1].ptr, k_scale=bufs[0].ptr + at if scales_far else near[0].ptr,
+                           v_scale=bufs[1].ptr + at if scales_far else near[1].ptr, k_page_stride=far, k_slot_stride=hk * d,
+                           k_head_stride=d, v_page_stride=far, v_slot_stride=hk * d, v_head_stride=d,
+                           scale_page_stride=far if scales_far else hk * page_size, scale_head_stride=page_size, pages=pages,
+                           page_size=page_size, kv_heads=hk, head_dim=d)
+    order, n = g.permutation(pages).astype(np.int32), pages * page_size
+    slots = order[np.arange(n) // page_size].astype(np.int64) * page_size + np.arange(n) % page_size
+    q, k, v = (rounded(g.standard_normal((n, h, d), np.float32), "bf16") for h in (1, hk, hk))
+    dq, dk, dv, dslots = (*(values_on_gpu(x, "bf16") for x in (q, k, v)), ints_on_gpu(slots, np.int64))
+    dqo = values_on_gpu(np.zeros((n, 1, d)), "bf16")
+    kh.synchronize()
+    kh.qk_norm_rope8(kh.QkNormRope8(q=dq.ptr, k=dk.ptr, v=dv.ptr, q_out=dqo.ptr, slots=dslots.ptr, q_stride=d, k_stride=hk * d,
+                                    v_stride=hk * d, q_out_stride=d, cache=cache, tokens=n, q_heads=1, dtype=kh.BF16, eps=0.0))
+    kh.synchronize()
+    lens = [n - i % 60 for i in range(120)]
+    for q_lens in ([1] * 120, [1] * 119 + [40]):
+        s = Step8(dtype, q_lens, [1] * 120, hq, hk, d, page_size=page_size, seed=len(q_lens), shared=0)
+        s.pages, s.table, s.lens, s.shared = pages, np.repeat(order[None], 120, 0), lens, 500
+        for name, x in (("k", k), ("v", v)):
+            codes, scales = np.zeros((n, hk, d), np.uint8), np.zeros((n, hk), np.uint8)
+            codes[slots], scales[slots] = held(x)
+            s.put(name, codes.reshape(pages, page_size, hk, d), scales.reshape(pages, page_size, hk))
+        s.cache8_on_gpu = lambda: (cache, None)
+        check_attention(s, max_new=max(q_lens))
