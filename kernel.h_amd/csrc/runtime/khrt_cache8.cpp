@@ -150,12 +150,18 @@ int64_t shared_units(const kh_paged_attention8_args &a) {
   return ceil_div(a.tokens * (a.q_heads / a.cache.kv_heads), KH_WIDE_ROWS) * a.cache.kv_heads;
 }
 
+// Rows of a step past which its entries are not shared: parts of more take gigabytes,
+// and where sequences have many rows each they read their entries once as it is.
+int64_t most_shared_rows(const kh_paged_attention8_args &a) {
+  return std::min(int64_t(1) << 22, (narrow_rows_of(KHRT_BF16) + 1) * a.table.seqs * a.cache.kv_heads);
+}
+
 SharedPlan shared_plan(const kh_paged_attention8_args &a, size_t workspace_bytes) {
   SharedPlan p{};
   const kh_paged_attention_args plain = as_plain(a, 0);
   const int64_t shared = std::min(a.shared, expected_len(a.table, plain.cache));
   const int64_t rows = a.tokens * a.q_heads, group = a.q_heads / a.cache.kv_heads;
-  if (shared <= 0 || a.table.seqs < 2 || rows > int64_t(1) << 22) return p;
+  if (shared <= 0 || a.table.seqs < 2 || rows > most_shared_rows(a)) return p;
   const size_t part = static_cast<size_t>(rows) * part_row_bytes(plain);
   // What the sequences of few rows need not read, against what parts write and
   // read and the launch that joins them.
@@ -174,10 +180,11 @@ SharedPlan shared_plan(const kh_paged_attention8_args &a, size_t workspace_bytes
 }
 
 // What the shared plan of no smaller step takes more than: its parts' rows are at
-// most those of a unit to a CU, or those of one part.
+// most those of a unit to a CU, or those of one part, and it has no more rows than
+// may share entries.
 size_t shared_workspace(const kh_paged_attention8_args &a) {
   if (a.shared == 0 || a.table.seqs < 2) return 0;
-  const int64_t rows = a.tokens * a.q_heads;
+  const int64_t rows = std::min(a.tokens * a.q_heads, most_shared_rows(a));
   return static_cast<size_t>(rows + std::max<int64_t>(rows, KH_GEMM_CUS * KH_WIDE_ROWS)) * part_row_bytes(as_plain(a, 0));
 }
 

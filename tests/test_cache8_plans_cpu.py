@@ -57,3 +57,20 @@ def test_the_steps_that_are_run_share_entries(plan):
     for page_size, dtype, (tokens, max_new) in itertools.product((16, 24), (0, 2), ((120, 1), (159, 40))):
         assert plan(tokens=tokens, seqs=120, hq=4, hk=2, d=128, width=36, page_size=page_size, dtype=dtype, shared=500,
                     max_new=max_new)["shared"] == 500
+
+
+def test_a_large_step_asks_no_memory_for_parts_it_does_not_make(plan):
+    """Sequences of more than 33 rows a kv head on the whole do not share entries, nor do
+    steps of more than 2^22 rows: a step asks for two parts of so many rows at the most, or
+    for one and a unit of 128 to a CU, beside what parts of other kinds take."""
+    def sizes(**kw):
+        p, without = (plan(hq=32, hk=8, d=128, max_new=0, shared=n, **kw) for n in (8192, 0))
+        return p["shared"] > 0, p["bytes"] - without["bytes"]
+
+    row = (128 + 2) * 4
+    for tokens in (64, 512, 528, 1000, 8192, 200000, 1 << 20):
+        shares, more = sizes(tokens=tokens, seqs=64)
+        assert shares == (tokens * 4 // 33 < 62) and more <= (64 * 33 * 8 + max(64 * 33 * 8, 256 * 128)) * row
+    for tokens in (1 << 17, (1 << 17) + 1, 1 << 20):
+        shares, more = sizes(tokens=tokens, seqs=1 << 17)
+        assert shares == (tokens == 1 << 17) and more <= 2 * (1 << 22) * row
