@@ -125,6 +125,22 @@ constexpr int64_t kWholeShared = 8;
 // chunks of up to 301 of 4001 fp16 tokens, 88 us without, 104 with.
 constexpr int64_t kShortCapped = 512;
 
+// The kernels' two factors of a cap: scores y (queries times keys) become
+// out tanh(y in / (2 log2 e)), in powers of two. in 0: they are not capped.
+struct Cap {
+  float in, out;
+};
+
+// factor: |scale| log2(e). A cap whose factors are past the normal numbers is none: it
+// is above 2^127, or above 2^127 times |scale|, and tanh(x) = x - x^3/3 + .. leaves
+// a y, or a score, below 2^114 as it is.
+Cap cap_of(float cap, float factor) {
+  using Float = std::numeric_limits<float>;
+  const double in = 2.0 * static_cast<double>(factor) / static_cast<double>(cap), out = static_cast<double>(cap) * 1.44269504088896340736;
+  if (!(cap > 0.0f) || in < static_cast<double>(Float::min()) || out > static_cast<double>(Float::max())) return {0.0f, 0.0f};
+  return {static_cast<float>(std::min(in, static_cast<double>(Float::max()))), static_cast<float>(out)};
+}
+
 // Fewer where there would not be a block of entries for every workgroup.
 int64_t heads_together(const kh_paged_attention8_args &a, int64_t behind) {
   const kh_paged_cache8 &c = a.cache;
@@ -342,10 +358,9 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
                         static_cast<int32_t>(c.pages), static_cast<int32_t>(c.page_size), static_cast<int32_t>(c.kv_heads),
                         static_cast<int32_t>(d), kh_div_by(u32(c.page_size))};
     // Scores are masked before the factor: it is above 0, which a scale of 0 makes up
-    // for with queries of 0. tanh(x / cap) takes its argument in powers of two, twice.
-    constexpr float most = std::numeric_limits<float>::max();
+    // for with queries of 0.
     const float factor = a.scale == 0.0f ? 1.0f : std::fabs(in_powers_of_two(a.scale));
-    const float cap_in = a.cap > 0.0f ? std::min(2.0f * (factor / a.cap), most) : 0.0f;
+    const Cap cap = cap_of(a.cap, factor);
     const bool two_bytes = element_bytes(a.dtype) == 2;
     KhAttention8Params p{{cache, device_table(a.table, plain.cache), a.q, a.out, a.lse, a.q_starts, part_o, part_ml, wide_o, wide_ml,
                           a.q_stride, a.out_stride, static_cast<int32_t>(a.tokens), static_cast<int32_t>(a.q_heads),
@@ -356,7 +371,7 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
                          c.k_scale, c.v_scale, u32(c.scale_page_stride), u32(c.scale_head_stride),
                          static_cast<int32_t>(shared.entries), static_cast<int32_t>(shared_blocks),
                          static_cast<int32_t>(std::max<int64_t>(shared.splits, 1)), static_cast<int32_t>(shared.each), shared_o, shared_ml, joins,
-                         static_cast<int32_t>(together), static_cast<int32_t>(ceil_div(c.kv_heads, together)), cap_in, std::min(a.cap * 1.44269504088896340736f, most), a.dtype == KHRT_F32 || a.cap > 256.0f || expected_len(a.table, plain.cache) <= kShortCapped};
+                         static_cast<int32_t>(together), static_cast<int32_t>(ceil_div(c.kv_heads, together)), cap.in, cap.out, a.dtype == KHRT_F32 || a.cap > 256.0f || expected_len(a.table, plain.cache) <= kShortCapped};
     const int width = width_of(d);
     const auto &symbols = wide_blocks + shared_blocks > 0 ? kWide : alone ? kAttention : kOdd;
     const unsigned threads = alone ? 64u * kWaves[width] : 256u;

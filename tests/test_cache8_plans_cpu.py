@@ -3,9 +3,11 @@ code with launches that only write down what they were given
 (tests/cpp/cache8_plan_check.cpp)."""
 import itertools
 import json
+import math
 import os
 import subprocess
 
+import numpy as np
 import pytest
 
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -74,3 +76,24 @@ def test_a_large_step_asks_no_memory_for_parts_it_does_not_make(plan):
     for tokens in (1 << 17, (1 << 17) + 1, 1 << 20):
         shares, more = sizes(tokens=tokens, seqs=1 << 17)
         assert shares == (tokens == 1 << 17) and more <= 2 * (1 << 22) * row
+
+
+@pytest.mark.parametrize("scale", [0.125, 1.0, -3e-20, 1e-30, 100.0, 1e25])
+@pytest.mark.parametrize("cap", [1e-40, 1e-3, 30.0, 1e30, 1e37, 3e37, 2.3e38, 2.4e38, 3e38, 3.4028e38])
+def test_factors_of_caps_hold_their_bits(plan, scale, cap):
+    """cap tanh(x / cap) as two factors in 32 bits, each the formula's but for a few
+    roundings; or no cap, where one of them is not a normal number: then no q . k and no
+    score below 2^114 is off by more than half a step for it. Small caps have their first factor cut to
+    the largest number, where all but a score of 0 is the cap itself."""
+    p = plan(tokens=2, seqs=2, hq=4, hk=2, d=64, scale=scale, cap=cap)
+    scale, cap = float(np.float32(scale)), float(np.float32(cap))
+    top = float(np.finfo(np.float32).max)
+    want_in, want_out = 2 * abs(scale) / math.log(2) / cap, cap / math.log(2)
+    if p["cap_in"] == 0:
+        assert want_in < 2.0 ** -125 or want_out > top * (1 - 2.0 ** -22)
+        # tanh(y) = y - y^3 / 3 + ..
+        assert want_in * 2.0 ** 114 / 2 < 2.0 ** -11 or want_out > top * (1 - 2.0 ** -22)
+        return
+    assert abs(p["cap_in"] / min(want_in, top) - 1) < 2.0 ** -21
+    assert 2.0 ** -126 <= p["cap_in"] and want_out < top * (1 + 2.0 ** -22)
+    assert abs(p["cap_out"] - want_out) <= 2.0 ** -22 * want_out + 2.0 ** -149

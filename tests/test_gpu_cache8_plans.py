@@ -83,3 +83,11 @@ def test_shared_entries_past_4_gb(dev, dtype, page_size, scales_far):
             s.put(name, codes.reshape(pages, page_size, hk, d), scales.reshape(pages, page_size, hk))
         s.cache8_on_gpu = lambda: (cache, None)
         check_attention(s, max_new=max(q_lens))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("cap,scale", [(3e38, 0.125), (2.4e38, 30.0), (3e37, 0.125), (1e37, 1e-3), (1e30, 1e-30)])
+def test_caps_past_every_score(dev, dtype, cap, scale):
+    s = Step8(dtype, [1, 3, 40], [70, 300, 90], 4, 2, 64, seed=9, cap=cap)
+    s.scale = scale
+    check_attention(s)
