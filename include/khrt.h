@@ -616,7 +616,8 @@ KHRT_API int kh_paged_read8(const kh_paged_read8_args *args, void *stream);
 /* kh_paged_attention over a cache in 8 bits, with two additions.
  *
  * cap > 0: the scores are cap tanh(scale q . k / cap). A cap above 2^128 / log2(e), or
- * above 2^127 log2(e) |scale|, is none.
+ * above 2^127 log2(e) |scale|, is none. Capped scores are off by some 2^-21 of their
+ * size; of 16-bit rows of chunks that see more than 512 entries by 2^-23 of the cap.
  *
  * shared > 0: the first `shared` entries of the sequences, as far as each is that
  * long, are the same entries (every sequence's row of the table names pages that

@@ -142,11 +142,14 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) {
 // Scores over the cap, capped: tanh(y cap_in / (2 log2 e)), which cap_out takes back to
 // scores in powers of two. By way of t = 2^(y cap_in) it is 1 - 2 / (t + 1), off by
 // some 2^-23 of the cap. near: what lies below a quarter of the cap comes from the
-// power series (first term left out 2e-9 of the score), 16 instructions a score instead
-// of 5. Few rows have the time for it (64 sequences of 513 to 8192 entries
-// 112 us with either); chunks feel every instruction. Of a chunk's 16-bit rows' weights 2^-23 of a cap up to
-// 256 is nothing (2^-15 of a weight), nor is it of their lse over many entries; rows of
-// fp32, of larger caps or of short sequences take the series there too.
+// power series (first term left out 2e-10 of the score), 16 instructions a score instead
+// of 5. Few rows have the time for it (64 sequences of 513 to 8192 entries 112 us with
+// either); chunks feel every instruction. Of a chunk's 16-bit rows' weights 2^-23 of a
+// cap up to 256 is nothing (2^-15 of a weight), nor is it of their lse over many entries.
+// Rows of fp32, under larger caps or windows of few entries (cap_near), and waves with a
+// row that sees no more than KH_FEW_CAPPED, whose lse is as far off as each of them, take
+// the series there too: what the row sees decides, not what else the step holds (16
+// chunks of up to 301 of 4001 fp16 tokens, windows of 1000, 86 us, all by the series 104).
 template <int N, class X>
 __device__ __forceinline__ void cap(X &y, const KhAttention8Params &p, bool near) {
 #pragma unroll
@@ -1263,9 +1266,10 @@ __device__ __forceinline__ void wide(const KhAttention8Params &p, int block, boo
         const uint64_t present = __builtin_amdgcn_ballot_w64((mark & kThere) != 0);
         const uint64_t odds = mixed(key0) ? __builtin_amdgcn_ballot_w64((mark & kOdd) != 0) : 0;
         if (p.cap_in != 0.0f) [[unlikely]] {
+          const bool near = p.cap_near || low.end <= KH_FEW_CAPPED;
 #pragma unroll
           for (int kt = 0; kt < W::tiles; ++kt) {
-            if (p.cap_near)
+            if (near)
               cap<16>(x[kt], p, true);
             else
               cap<16>(x[kt], p, false);

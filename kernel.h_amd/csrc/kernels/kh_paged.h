@@ -330,6 +330,9 @@ struct KhJoin {
   int32_t head0, spare;
 };
 
+// Entries up to which a row of a chunk counts what is small against the cap in full.
+#define KH_FEW_CAPPED 512
+
 // attention8.hip. The cache's strides are bytes as above, one to an element.
 struct KhAttention8Params : KhAttentionParams {
   const uint8_t *k_scale, *v_scale;  // of slot t of page p and head h: p scale_page + h scale_head + t
@@ -342,7 +345,7 @@ struct KhAttention8Params : KhAttentionParams {
   KhJoin *joins;  // [groups]
   int32_t together, head_groups;  // kv heads that a unit of few rows takes together (the last fewer), and their groups
   float cap_in, cap_out;  // scores y become cap_out tanh(y cap_in / (2 log2 e)); cap_in 0: they do not
-  int32_t cap_near;       // what is small against the cap counts for units of many rows too
+  int32_t cap_near;       // what is small against the cap counts in every unit of many rows
 };
 
 KH_HD int32_t kh_groups_of(const KhAttention8Params &p) { return p.head_groups; }

@@ -120,11 +120,6 @@ constexpr int64_t kWholeEven = 7;
 // this many blocks are not split: a join is another launch.
 constexpr int64_t kWholeShared = 8;
 
-// Up to this many entries to a sequence, capped scores of chunks come from the series
-// near zero too: where a row sees few, its lse is as far off as they are. MI355X, 16
-// chunks of up to 301 of 4001 fp16 tokens, 88 us without, 104 with.
-constexpr int64_t kShortCapped = 512;
-
 // The kernels' two factors of a cap: scores y (queries times keys) become
 // out tanh(y in / (2 log2 e)), in powers of two. in 0: they are not capped.
 struct Cap {
@@ -371,7 +366,7 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
                          c.k_scale, c.v_scale, u32(c.scale_page_stride), u32(c.scale_head_stride),
                          static_cast<int32_t>(shared.entries), static_cast<int32_t>(shared_blocks),
                          static_cast<int32_t>(std::max<int64_t>(shared.splits, 1)), static_cast<int32_t>(shared.each), shared_o, shared_ml, joins,
-                         static_cast<int32_t>(together), static_cast<int32_t>(ceil_div(c.kv_heads, together)), cap.in, cap.out, a.dtype == KHRT_F32 || a.cap > 256.0f || expected_len(a.table, plain.cache) <= kShortCapped};
+                         static_cast<int32_t>(together), static_cast<int32_t>(ceil_div(c.kv_heads, together)), cap.in, cap.out, a.dtype == KHRT_F32 || a.cap > 256.0f || (a.window > 0 && a.window <= KH_FEW_CAPPED)};
     const int width = width_of(d);
     const auto &symbols = wide_blocks + shared_blocks > 0 ? kWide : alone ? kAttention : kOdd;
     const unsigned threads = alone ? 64u * kWaves[width] : 256u;

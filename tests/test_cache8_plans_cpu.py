@@ -54,6 +54,7 @@ def test_the_steps_that_are_run_share_entries(plan):
         assert plan(tokens=194, seqs=65, hq=4, hk=4, d=128, width=200, shared=1500, max_len=max_len, max_new=130)["shared"] == max_len
     for max_len in (600, 1101):
         assert plan(tokens=64, seqs=64, hq=4, hk=4, d=128, width=200, shared=1500, max_len=max_len)["shared"] == max_len
+    assert plan(tokens=41, seqs=41, hq=4, hk=4, d=128, width=120, shared=1500, cap=200)["shared"] == 1500
     assert plan(tokens=67, seqs=64, hq=4, hk=4, d=128, width=122, shared=1500)["shared"] == 1500
     assert plan(tokens=285, seqs=150, hq=8, hk=4, d=64, width=69, shared=688, max_new=0)["shared"] == 688
     for page_size, dtype, (tokens, max_new) in itertools.product((16, 24), (0, 2), ((120, 1), (159, 40))):

@@ -5,10 +5,10 @@ import numpy as np
 import pytest
 
 import kernelh as kh
-from cache8test import Step8, held
+from cache8test import Step8, codes_of, held
 from cachetest import DTYPES, ints_on_gpu, rounded, values_on_gpu
 from khtest import say
-from test_gpu_cache import check_attention
+from test_gpu_cache import check_attention, close
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,55 @@ def test_caps_past_every_score(dev, dtype, cap, scale):
     s = Step8(dtype, [1, 3, 40], [70, 300, 90], 4, 2, 64, seed=9, cap=cap)
     s.scale = scale
     check_attention(s)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("cap", [20.0, 200.0])
+@pytest.mark.parametrize("beside,max_len", [(2000, 0), (2000, 40), (600, 600)])
+def test_small_scores_under_a_cap_beside_long_sequences(dev, dtype, cap, beside, max_len):
+    """A chunk's first row, which sees one entry, has its score for lse, as exact as where
+    the step holds nothing longer: exact before the cap (small whole numbers), and off by
+    some 8 roundings of the series behind it, or where the other form takes over, at a
+    quarter of the cap, by 2^-23 of the cap: 2^-20 of it."""
+    s = Step8(dtype, [40] * 31, [40] * 30 + [beside], 4, 2, 64, cap=cap, seed=beside)
+    whole = s.g.integers(-2, 3, s.k_codes.shape).astype(float)
+    s.put("k", codes_of(whole), np.full(s.k_scales.shape, 127, np.uint8))
+    s.q = s.g.integers(-2, 3, s.q.shape).astype(np.float32)
+    s.scale = 0.125
+    _, lse = s.run_attention(max_len=max_len)
+    first = np.arange(30) * 40  # these tokens see one entry
+    k = whole[s.table[:30, 0], 0]
+    x = s.scale * (s.q.reshape(-1, 4, 64)[first] * np.repeat(k, 2, 1)).sum(-1)
+    y = cap * np.tanh(x / cap)
+    close(lse[first], y, np.abs(y) * 2.0 ** -20, "lse")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_small_scores_under_a_cap_beside_shared_entries(dev, dtype):
+    """A sequence that ends inside the shared entries, its first token after its first entry."""
+    cap = 200.0
+    s = Step8(dtype, [1] * 40 + [1], [1501 + 7 * i for i in range(40)] + [1], 4, 4, 128, cap=cap, seed=41, shared=1500)
+    whole = s.g.integers(-1, 2, s.k_codes.shape).astype(float)
+    s.put("k", codes_of(whole), np.full(s.k_scales.shape, 127, np.uint8))
+    s.q = s.g.integers(-1, 2, s.q.shape).astype(np.float32)
+    s.scale = 0.125
+    _, lse = s.run_attention(max_new=1)
+    x = s.scale * (s.q[-1].reshape(4, 128) * whole[s.table[-1, 0], 0]).sum(-1)
+    y = cap * np.tanh(x / cap)
+    close(lse[-1], y, np.abs(y) * 2.0 ** -20, "lse")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_small_scores_under_a_cap_and_a_window_of_one(dev, dtype):
+    """Every row sees its own entry alone, far from the first."""
+    cap, n = 200.0, 700
+    s = Step8(dtype, [n], [n], 4, 2, 64, cap=cap, seed=42, window=1)
+    whole = s.g.integers(-2, 3, s.k_codes.shape).astype(float)
+    s.put("k", codes_of(whole), np.full(s.k_scales.shape, 127, np.uint8))
+    s.q = s.g.integers(-2, 3, s.q.shape).astype(np.float32)
+    s.scale = 0.125
+    _, lse = s.run_attention()
+    j = np.arange(n)
+    x = s.scale * (s.q.reshape(n, 4, 64) * np.repeat(whole[s.table[0][j // 16], j % 16], 2, 1)).sum(-1)
+    y = cap * np.tanh(x / cap)
+    close(lse, y, np.abs(y) * 2.0 ** -20, "lse")
