@@ -323,6 +323,13 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
     if (int rc = check_attention8(op, a)) return rc;
     if (!aligned(workspace)) return bad(op, "workspace must be 16-byte aligned");
     if (workspace == nullptr) workspace_bytes = 0;
+    const void *const written[] = {a.out, a.lse, workspace_bytes > 0 ? workspace : nullptr};
+    const void *const read[] = {a.q, c.k, c.v, c.k_scale, c.v_scale, a.table.pages, a.table.lens, a.q_starts};
+    for (int i = 0; i < 3; ++i) {
+      if (written[i] == nullptr) continue;
+      if (std::find(std::begin(read), std::end(read), written[i]) != std::end(read) || std::find(written, written + i, written[i]) != written + i)
+        return bad(op, "what is written must not be what is read, or written already");
+    }
     const SharedPlan shared = shared_plan(a, workspace_bytes);
     const bool common = shared.splits > 0;
     const kh_paged_attention_args plain = as_plain(a, shared.entries);

@@ -10,6 +10,10 @@ import subprocess
 import numpy as np
 import pytest
 
+import kernelh as kh
+from test_cache8_cpu import attention
+from test_cache_cpu import refused
+
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
@@ -98,3 +102,18 @@ def test_factors_of_caps_hold_their_bits(plan, scale, cap):
     assert abs(p["cap_in"] / min(want_in, top) - 1) < 2.0 ** -21
     assert 2.0 ** -126 <= p["cap_in"] and want_out < top * (1 + 2.0 ** -22)
     assert abs(p["cap_out"] - want_out) <= 2.0 ** -22 * want_out + 2.0 ** -149
+
+
+@pytest.mark.parametrize("written", ["out", "lse", "workspace"])
+def test_attention_does_not_write_what_it_reads(written):
+    """Equal pointers show that it would."""
+    read = dict(q=16, k=1 << 20, v=2 << 20, k_scale=3 << 20, v_scale=4 << 20, pages=1 << 12, lens=2 << 12, q_starts=1 << 14)
+    others = {"out": dict(lse=64), "lse": dict(out=64), "workspace": dict(out=64, lse=128)}[written]
+    for at in [*read.values(), *others.values()]:
+        kw = dict(q_starts=1 << 14, out=32, lse=48) | others
+        workspace = 1 << 15
+        if written == "workspace":
+            workspace = at
+        else:
+            kw[written] = at
+        refused(lambda: kh.paged_attention8(attention(**kw), workspace, 1 << 20), "paged_attention8")
