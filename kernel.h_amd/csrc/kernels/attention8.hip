@@ -595,9 +595,9 @@ __device__ __forceinline__ void narrow(const KhAttention8Params &p, int block, f
 // A row's 16-byte pieces lie at their number exclusive-or a number of the row's, so
 // that 16 rows of K in a column, and the rows of V that two groups of 16 lanes read
 // across, fill the banks once.
-template <int D, int TILES>
+template <int D>
 struct Ring {
-  static constexpr int tiles = TILES, keys = 16 * TILES, mine = 4 * TILES;  // entries of a block, and of a lane
+  static constexpr int tiles = 2, keys = 16 * tiles, mine = 4 * tiles;  // entries of a block, and of a lane
   static constexpr int pieces = D / 16, rows = 64 / pieces;  // rows that a load brings
   static constexpr int loads = 16 / rows;                    // of a tile
   static constexpr int ops = tiles * loads + 1;              // of a block's rows of K, or V, and their scales
@@ -717,19 +717,13 @@ __device__ __forceinline__ void send(const KhAttention8Params &p, const char *ow
 template <class F>
 __device__ __forceinline__ uint64_t there_of(const char *own, int n) {
   const uint16_t *at = reinterpret_cast<const uint16_t *>(own + F::there_at) + F::tiles * (n % F::ahead);
-  uint64_t there = 0;
-  if constexpr (F::tiles == 4) {
-    const u32x2 w = *reinterpret_cast<const u32x2 *>(at);
-    there = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(w.y) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane(w.x);
-  } else {
-    there = (uint32_t)__builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(at));
-  }
+  const uint32_t there = (uint32_t)__builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(at));
   return n < F::ahead ? there : 0;
 }
 
-template <int D, int TILES, int WAVES>
+template <int D, int WAVES>
 __device__ __forceinline__ void narrow_even(const KhAttention8Params &p, int block, char *lds) {
-  using F = Ring<D, TILES>;
+  using F = Ring<D>;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 15, h = lane >> 4;
   const int d = p.cache.head_dim;
@@ -931,7 +925,7 @@ __device__ __forceinline__ void narrow_even(const KhAttention8Params &p, int blo
             if (odds == 0) continue;
             while (odds != 0) {
               const int in1024 = __builtin_ctzll(odds) / F::pieces;
-              odds &= ~((F::pieces == 64 ? ~uint64_t(0) : (uint64_t(1) << F::pieces) - 1) << (in1024 * F::pieces));
+              odds &= ~(((uint64_t(1) << F::pieces) - 1) << (in1024 * F::pieces));
               const int row = at16 / D + in1024, key = key0 + row;
               if (!(mine && key >= seen.first && key < seen.end)) continue;
 #pragma unroll
@@ -1569,14 +1563,14 @@ __device__ __forceinline__ void settle_shared(KhAttention8Params &p) {
 #define KH_TYPED8(name) KH_PASTE(name, bf16)
 #endif
 
-#define KH_ATTENTION8(D, TILES, WAVES, PER_CU)                                                                          \
+#define KH_ATTENTION8(D, WAVES, PER_CU)                                                                                 \
   extern "C" __global__ void __launch_bounds__(64 * WAVES, PER_CU) KH_TYPED8(attention8_##D)(KhAttention8Params p) { \
-    __shared__ __attribute__((aligned(16))) char lds[WAVES * Ring<D, TILES>::lds];                                   \
-    narrow_even<D, TILES, WAVES>(p, (int)blockIdx.x, lds);                                                           \
+    __shared__ __attribute__((aligned(16))) char lds[WAVES * Ring<D>::lds];                                          \
+    narrow_even<D, WAVES>(p, (int)blockIdx.x, lds);                                                                  \
   }
-KH_ATTENTION8(64, 2, 4, 2)
-KH_ATTENTION8(128, 2, 4, 2)
-KH_ATTENTION8(256, 2, 2, 1)
+KH_ATTENTION8(64, 4, 2)
+KH_ATTENTION8(128, 4, 2)
+KH_ATTENTION8(256, 2, 1)
 #define KH_ATTENTION8_ODD(D, PER_CU)                                                                               \
   extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED8(attention8_odd_##D)(KhAttention8Params p) { \
     __shared__ __attribute__((aligned(16))) float lds[kWaves * kRows * 2 + kRows * 2 + kWaves * kRows * (D + 4)]; \
@@ -1588,22 +1582,22 @@ KH_ATTENTION8_ODD(256, 1)
 // Steps with sequences of many rows or shared entries: their workgroups first. fp32
 // rows of 128, three parts of each, leave registers for one workgroup to a CU: two
 // chunks of 1024 at 4096 entries, 16 heads on 4, 224 us; for two, which spill, 247.
-#define KH_ATTENTION8_WIDE(D, TILES, PER_CU)                                                                       \
+#define KH_ATTENTION8_WIDE(D, PER_CU)                                                                              \
   extern "C" __global__ void __launch_bounds__(256, PER_CU) KH_TYPED8(attention8_wide_##D)(KhAttention8Params p) { \
-    constexpr int kFew = kWaves * Ring<D, TILES>::lds;                                                             \
+    constexpr int kFew = kWaves * Ring<D>::lds;                                                                    \
     __shared__ __attribute__((aligned(16))) char lds[Many<D>::lds > kFew ? Many<D>::lds : kFew];                   \
     settle_shared(p);                                                                                              \
     const int block = (int)blockIdx.x, wide_end = p.shared_blocks + p.wide_blocks;                                 \
     if (block < wide_end)                                                                                          \
       wide<D>(p, block < p.shared_blocks ? block : block - p.shared_blocks, block < p.shared_blocks, lds);         \
     else if (p.even)                                                                                               \
-      narrow_even<D, TILES, kWaves>(p, block - wide_end, lds);                                                     \
+      narrow_even<D, kWaves>(p, block - wide_end, lds);                                                            \
     else                                                                                                           \
       narrow<D>(p, block - wide_end, reinterpret_cast<float *>(lds));                                              \
   }
-KH_ATTENTION8_WIDE(64, 2, 2)
-KH_ATTENTION8_WIDE(128, 2, kParts == 3 ? 1 : 2)
-KH_ATTENTION8_WIDE(256, 2, 1)
+KH_ATTENTION8_WIDE(64, 2)
+KH_ATTENTION8_WIDE(128, kParts == 3 ? 1 : 2)
+KH_ATTENTION8_WIDE(256, 1)
 #define KH_ATTENTION8_JOIN(D)                                                                                   \
   extern "C" __global__ void __launch_bounds__(256) KH_TYPED8(attention8_join_##D)(KhAttention8Params p) {      \
     __shared__ JoinLds lds;                                                                                     \
