@@ -228,7 +228,7 @@ int kh_qk_norm_rope8(const kh_qk_norm_rope8_args *args, void *stream) {
       return bad(op, "output strides must be multiples of 16 bytes and hold a token");
     if ((a.q_out == a.q && a.q_out_stride != a.q_stride) || (a.k_out == a.k && a.k_out_stride != a.k_stride))
       return bad(op, "in place, input and output strides must be the same");
-    for (const void *p : {static_cast<const void *>(c.k), static_cast<const void *>(c.v), static_cast<const void *>(c.k_scale), static_cast<const void *>(c.v_scale)})
+    for (const void *p : std::initializer_list<const void *>{c.k, c.v, c.k_scale, c.v_scale})
       if (p == a.q || p == a.k || p == a.v || p == a.q_out || p == a.k_out) return bad(op, "the cache must not be one of the rows' buffers");
     if (a.q_out == a.k || a.q_out == a.v || a.q_out == a.k_out || (a.k_out != nullptr && (a.k_out == a.q || a.k_out == a.v)))
       return bad(op, "an output must not be another input or output");
@@ -277,7 +277,7 @@ int kh_paged_read8(const kh_paged_read8_args *args, void *stream) {
       if (!aligned(out)) return bad(op, "buffers must be 16-byte aligned");
       if (!stride_ok(is_v ? a.v_out_stride : a.k_out_stride, a.tokens, e, row))
         return bad(op, "output strides must be multiples of 16 bytes and hold a token");
-      for (const void *p : {static_cast<const void *>(c.k), static_cast<const void *>(c.v), static_cast<const void *>(c.k_scale), static_cast<const void *>(c.v_scale), static_cast<const void *>(a.slots)})
+      for (const void *p : std::initializer_list<const void *>{c.k, c.v, c.k_scale, c.v_scale, a.slots})
         if (p == out) return bad(op, "what is written must not be what is read");
     }
     if (a.k_out == a.v_out) return bad(op, "k_out and v_out must not be the same");
@@ -343,37 +343,48 @@ int kh_paged_attention8(const kh_paged_attention8_args *args, void *workspace, s
     const bool narrow_only = kh_narrow_only(a.tokens, a.table.seqs, group, a.max_new, narrow_rows_of(KHRT_BF16), 256);
     const bool alone = even && !common && narrow_only;
     const int64_t together = even ? heads_together(a, shared.entries) : 1;
-    const AttentionPlan plan = attention_plan(plain, left, {alone ? 2 * KH_GEMM_CUS : most_groups(plain), together, common ? kWholeShared : alone && d <= 128 ? kWholeEven : kWholeBlocks});
+    const int64_t whole = common ? kWholeShared : alone && d <= 128 ? kWholeEven : kWholeBlocks;
+    const AttentionPlan plan = attention_plan(plain, left, {alone ? 2 * KH_GEMM_CUS : most_groups(plain), together, whole});
     const bool joined = plan.part_bytes + plan.wide_bytes > 0;
     // All rows of parts come first, 16 bytes at a time, then their statistics.
     float *at = static_cast<float *>(workspace);
     const auto take = [&at](int64_t floats) { return std::exchange(at, floats > 0 ? at + floats : at); };
-    const int64_t narrow_parts = plan.part_bytes > 0 ? plan.groups * 2 * KH_TILE_ROWS * together : 0, wide_parts = plan.wide_bytes > 0 ? plan.splits * rows : 0;
+    const int64_t narrow_parts = plan.part_bytes > 0 ? plan.groups * 2 * KH_TILE_ROWS * together : 0;
+    const int64_t wide_parts = plan.wide_bytes > 0 ? plan.splits * rows : 0;
     const int64_t common_parts = common ? (shared.splits + 1) * rows : 0;
     float *const part_o = take(narrow_parts * d), *const wide_o = take(wide_parts * d), *const shared_o = take(common_parts * d);
     float *const part_ml = take(narrow_parts * 2), *const wide_ml = take(wide_parts * 2), *const shared_ml = take(common_parts * 2);
-    KhJoin *const joins = reinterpret_cast<KhJoin *>(at);
     const int64_t wide_blocks = plan.wide_units * plan.splits, shared_blocks = shared.units * shared.splits;
     const auto u32 = [](int64_t x) { return static_cast<uint32_t>(x); };
-    const KhCache cache{static_cast<const char *>(c.k), static_cast<const char *>(c.v), u32(c.k_page_stride), u32(c.k_slot_stride),
-                        u32(c.k_head_stride), u32(c.v_page_stride), u32(c.v_slot_stride), u32(c.v_head_stride),
-                        static_cast<int32_t>(c.pages), static_cast<int32_t>(c.page_size), static_cast<int32_t>(c.kv_heads),
-                        static_cast<int32_t>(d), kh_div_by(u32(c.page_size))};
+    const auto i32 = [](int64_t x) { return static_cast<int32_t>(x); };
+    KhAttention8Params p{};
+    p.cache = {.k = static_cast<const char *>(c.k), .v = static_cast<const char *>(c.v),
+               .k_page = u32(c.k_page_stride), .k_slot = u32(c.k_slot_stride), .k_head = u32(c.k_head_stride),
+               .v_page = u32(c.v_page_stride), .v_slot = u32(c.v_slot_stride), .v_head = u32(c.v_head_stride),
+               .pages = i32(c.pages), .page_size = i32(c.page_size), .kv_heads = i32(c.kv_heads), .head_dim = i32(d),
+               .by_page = kh_div_by(u32(c.page_size))};
+    p.k_scale = c.k_scale, p.v_scale = c.v_scale;
+    p.scale_page = u32(c.scale_page_stride), p.scale_head = u32(c.scale_head_stride);
+    p.table = device_table(a.table, plain.cache);
+    p.q = a.q, p.out = a.out, p.lse = a.lse, p.q_starts = a.q_starts;
+    p.q_stride = a.q_stride, p.out_stride = a.out_stride;
+    p.tokens = i32(a.tokens), p.q_heads = i32(a.q_heads), p.group = i32(group), p.window = i32(a.window);
+    p.by_group = kh_div_by(u32(group));
+    p.part_o = part_o, p.part_ml = part_ml, p.wide_o = wide_o, p.wide_ml = wide_ml, p.shared_o = shared_o, p.shared_ml = shared_ml;
+    p.joins = reinterpret_cast<KhJoin *>(at);
+    p.groups = i32(plan.groups), p.whole = plan.whole, p.narrow_rows = i32(plan.narrow_rows);
+    p.wide_blocks = i32(wide_blocks), p.wide_splits = i32(std::max<int64_t>(plan.splits, 1));
+    p.shared = i32(shared.entries), p.shared_blocks = i32(shared_blocks);
+    p.shared_splits = i32(std::max<int64_t>(shared.splits, 1)), p.shared_each = i32(shared.each);
+    p.even = even, p.together = i32(together), p.head_groups = i32(ceil_div(c.kv_heads, together));
     // Scores are masked before the factor: it is above 0, which a scale of 0 makes up
     // for with queries of 0.
-    const float factor = a.scale == 0.0f ? 1.0f : std::fabs(in_powers_of_two(a.scale));
-    const Cap cap = cap_of(a.cap, factor);
-    const bool two_bytes = element_bytes(a.dtype) == 2;
-    KhAttention8Params p{{cache, device_table(a.table, plain.cache), a.q, a.out, a.lse, a.q_starts, part_o, part_ml, wide_o, wide_ml,
-                          a.q_stride, a.out_stride, static_cast<int32_t>(a.tokens), static_cast<int32_t>(a.q_heads),
-                          static_cast<int32_t>(group), static_cast<int32_t>(a.window), static_cast<int32_t>(plan.groups), plan.whole,
-                          static_cast<int32_t>(plan.narrow_rows), static_cast<int32_t>(wide_blocks),
-                          static_cast<int32_t>(std::max<int64_t>(plan.splits, 1)), even, a.scale == 0.0f ? 0u : 0xffffffffu,
-                          a.scale < 0.0f ? (two_bytes ? 0x80008000u : 0x80000000u) : 0u, kh_div_by(u32(group)), factor},
-                         c.k_scale, c.v_scale, u32(c.scale_page_stride), u32(c.scale_head_stride),
-                         static_cast<int32_t>(shared.entries), static_cast<int32_t>(shared_blocks),
-                         static_cast<int32_t>(std::max<int64_t>(shared.splits, 1)), static_cast<int32_t>(shared.each), shared_o, shared_ml, joins,
-                         static_cast<int32_t>(together), static_cast<int32_t>(ceil_div(c.kv_heads, together)), cap.in, cap.out, a.dtype == KHRT_F32 || a.cap > 256.0f || (a.window > 0 && a.window <= KH_FEW_CAPPED)};
+    p.scale_log2 = a.scale == 0.0f ? 1.0f : std::fabs(in_powers_of_two(a.scale));
+    p.q_keep = a.scale == 0.0f ? 0u : 0xffffffffu;
+    p.q_sign = a.scale < 0.0f ? (element_bytes(a.dtype) == 2 ? 0x80008000u : 0x80000000u) : 0u;
+    const Cap cap = cap_of(a.cap, p.scale_log2);
+    p.cap_in = cap.in, p.cap_out = cap.out;
+    p.cap_near = a.dtype == KHRT_F32 || a.cap > 256.0f || (a.window > 0 && a.window <= KH_FEW_CAPPED);
     const int width = width_of(d);
     const auto &symbols = wide_blocks + shared_blocks > 0 ? kWide : alone ? kAttention : kOdd;
     const unsigned threads = alone ? 64u * kWaves[width] : 256u;
