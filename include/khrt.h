@@ -616,18 +616,22 @@ KHRT_API int kh_paged_read8(const kh_paged_read8_args *args, void *stream);
 /* kh_paged_attention over a cache in 8 bits, with two additions.
  *
  * cap > 0: the scores are cap tanh(scale q . k / cap). A cap above 2^128 / log2(e), or
- * above 2^127 log2(e) |scale|, is none. Capped scores are off by some 2^-21 of their
- * size; of 16-bit rows of chunks that see more than 512 entries by 2^-23 of the cap.
+ * above 2^127 log2(e) |scale|, is none. Capped scores are off by some 2^-20 of their
+ * size; those of 16-bit rows of chunks that see more than 512 entries by 2^-23 of the
+ * cap, where that is more.
  *
  * shared > 0: the first `shared` entries of the sequences, as far as each is that
  * long, are the same entries (every sequence's row of the table names pages that
  * hold them, the same pages or copies). They may then be read once for all, from
- * sequence 0's pages and as far as it reaches; as max_len and max_new this changes
- * no result but its rounding.
+ * sequence 0's pages and as far as it and max_len reach; as max_len and max_new this
+ * changes no result but its rounding. Where that would not pay (few sequences, chunks of
+ * many rows to a sequence, steps of more than 2^22 rows) or the workspace does not hold
+ * the parts, every sequence reads its own.
  *
  * Products are of bf16 numbers, exactly what the cache holds; queries count in
- * full, the softmax's weights to 8 bits (bf16), 16 (fp16) or 24 (fp32). A NaN
- * in an entry that a token does not see does not reach it.
+ * full, the softmax's weights to 8 bits (bf16), 16 (fp16) or 24 (fp32; to fewer where
+ * the rows of v lie below 1e-30). A NaN in an entry that a token does not see does not
+ * reach it.
  *
  * workspace: as kh_paged_attention's; it also holds what shared entries give each
  * row. A smaller step is one of fewer shared entries too. */

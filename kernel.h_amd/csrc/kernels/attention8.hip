@@ -12,15 +12,16 @@
 // of the matrix units, and 8 bits times 8 bits would need K and V's other operand
 // in e4m3, 4 bits of it.
 //
-// Few rows to a sequence: 16 rows of a wave against blocks of 64 entries (rows past
-// 128 elements: 32), in shares of the step as in paged_attention.hip.
+// Few rows to a sequence: 16 rows of a wave against blocks of entries, in shares of the
+// step as in paged_attention.hip.
 //   S^T = K Q^T     the result's lane l holds row l % 16 and entries 4 (l / 16) + i
 //                   of each 16: a row's softmax crosses lanes twice.
 //   O^T += V^T P^T  P as the lanes hold it, in bf16.
-// In two forms: narrow_even() for pages of whole sixteens (K and V straight to LDS),
-// narrow() for others (K and V in registers). Bound by reading K and V: MI355X, bf16,
+// In two forms: narrow_even() for pages of whole sixteens (K and V straight to LDS, blocks
+// of 32 entries), narrow() for others (K and V in registers, blocks of 64, and of 32 with
+// rows past 128 elements). Bound by reading K and V: MI355X, bf16,
 // 8 kv heads of 128, 64 sequences of 513 to 8192 entries 110 us, 5.2 TB/s, with
-// pages of 24 slots 138; one of 131071 60-67 us, 4.0-4.5 TB/s with the launch of the join
+// pages of 24 slots 138; one of 131071 59-67 us, 4.0-4.6 TB/s with the launch of the join
 // and both kernels' ends; four of 1024, 16 heads of 64 in fp32, 14 us, of which the
 // two launches are ten.
 //
@@ -28,7 +29,7 @@
 // to LDS as bf16: each byte is converted once for 128 rows. Bound by what the waves
 // issue, the softmax's and the conversions' instructions (54% of the time) and the
 // matrix units' (32%) in turn: a chunk of 2048 at 8192 entries, 32 heads on 8 of
-// 128, bf16, 287 to 302 us, 800 to 845 TFLOP/s.
+// 128, bf16, 283 to 305 us, 795 to 855 TFLOP/s.
 //
 // Entries that all sequences share are worked on by wide units whose rows are all
 // tokens of the step; their parts and the sequences' own are joined row by row.

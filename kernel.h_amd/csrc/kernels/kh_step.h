@@ -23,9 +23,9 @@ __device__ __forceinline__ int apart(int h) {
   return h;
 }
 
-// 2^x takes scores times a factor less the row's maximum m (in powers of two) and
-// more kLift:
-// one multiply-add, exact but for its last rounding, while m itself was rounded.
+// 2^x takes scores times a factor less the row's maximum m (in powers of two; in fp16
+// paged_attention more its kLift): one multiply-add, exact but for its last rounding,
+// while m itself was rounded.
 // The largest score is so off by half a step of m: 2^-2 at kFine, whole powers of
 // two further up. Where the wave has such maxima (coarse), the products are
 // rounded as m was before it is taken from them (less), and nothing else is done.

@@ -28,7 +28,7 @@
 // the type's relative step is the same under any scale, so that a power of two loses
 // nothing by it, and what is read back is exact. Rows of k are worked out in 64 bits,
 // the angles' series too, and rounded once: between two numbers of four bits there are
-// ties, which 32 bits take either way (some 20 of 8 million numbers). Infinities and NaN
+// ties, which 32 bits take either way (17 of 8 million numbers). Infinities and NaN
 // become NaN; a row's power is that of its finite elements. A wave's token, part and
 // page are the same in all lanes, and are kept so. The 8192 tokens take 41-44 us, 4.2-4.5
 // TB/s: fewer bytes, but as many rows to work through, each with a maximum across its
@@ -346,7 +346,7 @@ __device__ __forceinline__ void rope(const Params &p) {
 #ifdef KH_CACHE8
     if (!is_q) {
       // In 64 bits: a row is rounded once, to four bits a number. In 32, ties between
-      // two of them go either way: of 8192 tokens' 8 heads of 128 some 20 numbers.
+      // two of them go either way: of 8192 tokens' 8 heads of 128 17 numbers.
       double scale = 1.0;
       if (p.norm) {
         double sq = 0.0;
