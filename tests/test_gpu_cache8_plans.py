@@ -9,6 +9,7 @@ from cache8test import Step8, codes_of, held
 from cachetest import DTYPES, ints_on_gpu, rounded, values_on_gpu
 from khtest import say
 from test_gpu_cache import check_attention, close
+from test_gpu_cache_steps import Graph
 
 pytestmark = pytest.mark.gpu
 
@@ -143,3 +144,32 @@ def test_small_scores_under_a_cap_and_a_window_of_one(dev, dtype):
     x = s.scale * (s.q.reshape(n, 4, 64) * np.repeat(whole[s.table[0][j // 16], j % 16], 2, 1)).sum(-1)
     y = cap * np.tanh(x / cap)
     close(lse, y, np.abs(y) * 2.0 ** -20, "lse")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_captured_call_whose_sequences_grow_past_what_it_expected(dev, dtype):
+    """Captured with an expected length inside the shared entries, and replayed as the
+    lengths go from below it to past the shared entries and back."""
+    full = [1501 + 7 * i for i in range(64)]
+    s = Step8(dtype, [1] * 64, full, 4, 4, 128, seed=50, shared=1500)
+    a, bufs = s.args8(max_len=600, max_new=1)
+    lens = bufs["keep"][1][1]
+    size = kh.paged_attention8_workspace(a)
+    ws, stream = kh.Buffer(size), kh.Stream()
+    kh.synchronize()
+    graph = Graph(stream, lambda: kh.paged_attention8(a, ws, size, stream))
+    for most in (550, 1400, 2000, 601, 3000, 1):
+        s.lens = [min(n, most) for n in full]
+        say(f"captured, lengths up to {most}")
+        lens.copy_from_host(np.array(s.lens, np.int32))
+        for b in (ws, bufs["out"], bufs["lse"]):
+            b.fill(7.0, stream)
+        stream.synchronize()
+        graph.replay()
+        stream.synchronize()
+        out, lse = s.results(bufs)
+        want, bound, y, y_bound = s.attention()
+        close(out, want, bound, "out")
+        close(lse, y, y_bound, "lse")
+    graph.destroy()
+    stream.destroy()
